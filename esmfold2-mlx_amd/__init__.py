@@ -8,6 +8,7 @@ Modules:
   trimul           -- TriMul / TriMulPair: the forward(pair_grid, visibility) module contract
   q8               -- Q8Linear: the quantized_matmul(transpose=True, group 64, bits 8) contract
   esmc             -- EsmcBlock and HipEsmc: the ESMC language model around the 8-bit linear
+  rotary           -- Rotary: rotary positions (layouts, part of a head, long contexts) with the norm of q and k
   trunk            -- PairTransition, TrunkBlock and PairTrunk (the FoldingTrunk drop-in)
   recycle          -- ParcaeLoop (the 6B recycling loop) and its distogram exit signal
   var_hip_trimul   -- the reference-style variant plugin for the TMUs: apply(model)
@@ -23,7 +24,7 @@ Modules:
 
 from . import build, capi  # noqa: F401
 
-__all__ = ["build", "capi", "kernels", "trimul", "q8", "esmc", "trunk", "recycle", "scratch", "var_hip_trimul",
+__all__ = ["build", "capi", "kernels", "trimul", "q8", "esmc", "rotary", "trunk", "recycle", "scratch", "var_hip_trimul",
            "var_hip_trunk", "var_6b_hip_trunks", "var_6b_hip_loop", "var_6b_hip_adaptive", "var_hip_adaptive_loops",
            "variants", "workloads"]
 

@@ -15,6 +15,7 @@ import threading
 from . import build as _build
 
 _vp, _int, _f32, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes); mirrors include/esmfold2_amd.h
 SIGNATURES = {
@@ -51,6 +52,10 @@ SIGNATURES = {
     "esmc_qk_rope": (_int, [_vp, _vp, _vp, _f32, _vp, _vp, _vp, _int, _int, _int, _int, _f32, _vp]),
     "esmc_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _f32, _vp]),
     "esmc_swiglu": (_int, [_vp, _vp, _int, _int, _vp]),
+    "qk_norm_rope": (_int, [_vp] * 4 + [_i64] * 8 + [_vp, _int, _vp, _int, _f32, _vp, _int, _vp, _f32] + [_int] * 9
+                     + [_vp]),
+    "packed_attention_workspace_bytes": (_sz, [_int] * 6),
+    "packed_attention": (_int, [_vp] * 4 + [_i64] * 8 + [_vp, _vp] + [_int] * 7 + [_f32, _int, _vp, _sz, _vp]),
     "esmc_block_workspace_bytes": (_sz, [_int, _int, _int]),
     "esmc_block": (_int, [_vp] * 17 + [_f32, _f32, _f32, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "parcae_step": (_int, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _int, _int, _int, _vp]),

@@ -941,6 +941,110 @@ int esmc_swiglu(const esm_half* x12, esm_half* y, int M, int F, void* stream) {
   return hip_status(esm::launch_esmc_swiglu(H(x12), H(y), (size_t)M, F, (hipStream_t)stream), "esmc_swiglu launch");
 }
 
+// Strides a 16-bit [rows, heads, d] operand may have: whole 16-byte pieces, rows that lie apart, and tile offsets
+// (64 rows) below 2^31 bytes.
+static const char* strides_fault(int64_t st, int64_t sh, int rows, int d) {
+  if (st % 8 != 0 || sh % 8 != 0) return "strides must be multiples of 8";
+  if (sh < 0 || (rows > 1 && (st < d || st > (1 << 23)))) return "row strides must lie between d and 2^23";
+  return nullptr;
+}
+
+int qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_st, int64_t q_sh, int64_t k_st,
+                 int64_t k_sh, int64_t qo_st, int64_t qo_sh, int64_t ko_st, int64_t ko_sh, const float* q_w,
+                 int q_w_heads, const float* k_w, int k_w_heads, float eps, const void* pos, int pos64,
+                 const double* freq, float gain, int T, int H, int Hk, int d, int rot, int norm, int over_row,
+                 int interleaved, int dtype, void* stream) {
+  if (T < 0 || H <= 0 || Hk <= 0 || d <= 0 || rot < 0 || rot > d)
+    return fail(ESM_ERR_SHAPE, "qk_norm_rope: T=%d H=%d Hk=%d d=%d rot=%d", T, H, Hk, d, rot);
+  if (d % 8 != 0 || d > 256 || rot % 16 != 0)
+    return fail(ESM_ERR_UNSUPPORTED, "qk_norm_rope: d=%d rot=%d (d a multiple of 8 up to 256, rot of 16)", d, rot);
+  if (norm < ESM_NORM_NONE || norm > ESM_NORM_LAYER || (dtype != ESM_F16 && dtype != ESM_BF16))
+    return fail(ESM_ERR_UNSUPPORTED, "qk_norm_rope: norm=%d dtype=%d", norm, dtype);
+  if (norm != ESM_NORM_NONE && !(eps >= 0.f)) return fail(ESM_ERR_SHAPE, "qk_norm_rope: eps must be >= 0");
+  if (T >= (1 << 22) || H > (1 << 16) || Hk > (1 << 16))
+    return fail(ESM_ERR_SHAPE, "qk_norm_rope: T=%d H=%d Hk=%d too large", T, H, Hk);
+  const bool row = over_row && norm != ESM_NORM_NONE;
+  if (row && !esm::qk_norm_rope_row_fits(H + Hk, d))
+    return fail(ESM_ERR_UNSUPPORTED, "qk_norm_rope: %d heads of %d are too many for a norm over the row", H + Hk, d);
+  for (const char* why : {strides_fault(q_st, q_sh, T, d), strides_fault(k_st, k_sh, T, d),
+                          strides_fault(qo_st, qo_sh, T, d), strides_fault(ko_st, ko_sh, T, d)})
+    if (why) return fail(ESM_ERR_ALIGN, "qk_norm_rope: %s", why);
+  if (T == 0) return ok();
+  if (!q || !k || !q_out || !k_out || (rot && !freq)) return fail(ESM_ERR_NULL, "qk_norm_rope: NULL pointer");
+  for (const void* x : {q, k, (const void*)q_out, (const void*)k_out, (const void*)q_w, (const void*)k_w})
+    if (!aligned16(x)) return fail(ESM_ERR_ALIGN, "qk_norm_rope: q, k, outputs and weights must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(freq) & 7u) return fail(ESM_ERR_ALIGN, "qk_norm_rope: freq must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(pos) & (pos64 ? 7u : 3u)) return fail(ESM_ERR_ALIGN, "qk_norm_rope: misaligned positions");
+  esm::QkRopeArgs a{};
+  a.q = q, a.k = k, a.qo = q_out, a.ko = k_out;
+  a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh;
+  a.qo_st = qo_st, a.qo_sh = qo_sh, a.ko_st = ko_st, a.ko_sh = ko_sh;
+  a.q_w = q_w, a.k_w = k_w, a.qw_sh = q_w_heads ? d : 0, a.kw_sh = k_w_heads ? d : 0;
+  a.eps = eps, a.freq = freq, a.gain = gain;
+  a.pos32 = pos64 ? nullptr : (const int*)pos;
+  a.pos64 = pos64 ? (const long long*)pos : nullptr;
+  a.T = T, a.H = H, a.Hk = Hk, a.d = d, a.rot = rot, a.norm = norm, a.interleaved = interleaved != 0;
+  return hip_status(esm::launch_qk_norm_rope(a, dtype == ESM_BF16, row, (hipStream_t)stream), "qk_norm_rope launch");
+}
+
+// Workspace of the few-row form: m and l of every (row, split), then O.
+static size_t attention_ml_bytes(int Tq, int H, int splits) { return ((size_t)Tq * H * splits * 8 + 255) / 256 * 256; }
+
+static bool attention_shape(int n, int Tq, int Tk, int H, int Hk, int d) {
+  return n >= 0 && Tq >= 0 && Tk >= 0 && H > 0 && Hk > 0 && H % Hk == 0 && d > 0;
+}
+
+size_t packed_attention_workspace_bytes(int n, int Tq, int Tk, int H, int Hk, int d) {
+  if (!attention_shape(n, Tq, Tk, H, Hk, d) || n == 0 || Tq == 0) return 0;
+  const esm::AttnPlan plan = esm::packed_attention_plan(Tq, Tk, n, Hk, H / Hk, d, cu_count());
+  return plan.splits == 1 ? 0 : attention_ml_bytes(Tq, H, plan.splits) + (size_t)Tq * H * plan.splits * d * 4;
+}
+
+int packed_attention(const void* q, const void* k, const void* v, void* o, int64_t q_st, int64_t q_sh, int64_t k_st,
+                     int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t o_st, int64_t o_sh, const int* cu_q,
+                     const int* cu_k, int n, int Tq, int Tk, int H, int Hk, int d, int causal, float scale, int dtype,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (!attention_shape(n, Tq, Tk, H, Hk, d))
+    return fail(ESM_ERR_SHAPE, "packed_attention: n=%d Tq=%d Tk=%d H=%d Hk=%d d=%d", n, Tq, Tk, H, Hk, d);
+  if (d % 8 != 0 || d > 128) return fail(ESM_ERR_UNSUPPORTED, "packed_attention: d=%d (a multiple of 8 up to 128)", d);
+  if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "packed_attention: dtype=%d", dtype);
+  if (!(scale > 0.f) || std::isinf(scale)) return fail(ESM_ERR_SHAPE, "packed_attention: scale must be positive and finite");
+  for (const char* why : {strides_fault(q_st, q_sh, Tq, d), strides_fault(k_st, k_sh, Tk, d),
+                          strides_fault(v_st, v_sh, Tk, d), strides_fault(o_st, o_sh, Tq, d)})
+    if (why) return fail(ESM_ERR_ALIGN, "packed_attention: %s", why);
+  if (n == 0 || Tq == 0) return ok();
+  const int G = H / Hk;
+  const esm::AttnPlan plan = esm::packed_attention_plan(Tq, Tk, n, Hk, G, d, cu_count());
+  // grids of 256 threads stay below 2^32 threads, row numbers below 2^31
+  if ((long long)Tq * G >= (1LL << 31) - 256 || ((long long)Tq * G / 32 + n) * Hk * plan.splits >= (1LL << 24) ||
+      (plan.splits > 1 && (long long)Tq * H >= (1LL << 25)))
+    return fail(ESM_ERR_SHAPE, "packed_attention: n=%d Tq=%d H=%d too large", n, Tq, H);
+  if (!q || !o || !cu_q || !cu_k || (Tk > 0 && (!k || !v))) return fail(ESM_ERR_NULL, "packed_attention: NULL pointer");
+  for (const void* x : {q, k, v, (const void*)o})
+    if (!aligned16(x)) return fail(ESM_ERR_ALIGN, "packed_attention: q, k, v and o must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3u)
+    return fail(ESM_ERR_ALIGN, "packed_attention: misaligned starts");
+  const size_t need = packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(ESM_ERR_SHAPE, "packed_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+      return fail(ESM_ERR_ALIGN, "packed_attention: workspace must be 256-byte aligned");
+  }
+  esm::PackedAttnArgs a{};
+  a.q = q, a.k = k, a.v = v, a.o = o;
+  a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh, a.o_st = o_st, a.o_sh = o_sh;
+  a.cu_q = cu_q, a.cu_k = cu_k, a.n = n, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = G, a.d = d, a.causal = causal != 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = plan.splits;
+  if (need) {
+    a.part_ml = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + attention_ml_bytes(Tq, H, plan.splits));
+  }
+  return hip_status(esm::launch_packed_attention(a, dtype == ESM_BF16, plan.many, (hipStream_t)stream),
+                    "packed_attention launch");
+}
+
 // The pieces of esmc_block's workspace, each 256-byte aligned: qkv, q, k, v, the attention's output, the
 // residual and its LayerNorm between the halves, the gated FFN rows, and the split-K partials of whichever
 // linear runs.

@@ -146,6 +146,49 @@ struct EsmcAttnArgs {
   float scale_log2;     // scale * log2(e)
 };
 
+// Norm over the head or row in qk_norm_rope.
+enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
+
+struct QkRopeArgs {
+  const void* q;          // [T, H, d], 16-bit; strides in elements
+  const void* k;          // [T, Hk, d]
+  void* qo;               // as q (may be q)
+  void* ko;
+  long long q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh;
+  const float* q_w;       // [d] or [H * d], or nullptr (1)
+  const float* k_w;       // [d] or [Hk * d], or nullptr
+  int qw_sh, kw_sh;       // 0: one weight for every head, d: each its own
+  float eps;
+  const int* pos32;       // [T] positions, or nullptr
+  const long long* pos64; // [T] positions, or nullptr (neither: the row's index)
+  const double* freq;     // [rot / 2] radians per position
+  float gain;             // factor on sine and cosine
+  int T, H, Hk, d, rot;
+  int norm, interleaved;
+  int lph;                // log2 of the lanes per head (set by the launcher)
+};
+
+struct PackedAttnArgs {
+  const void* q;          // [Tq, Hk * G, d], 16-bit; strides in elements
+  const void* k;          // [Tk, Hk, d]
+  const void* v;          // [Tk, Hk, d]
+  void* o;                // [Tq, Hk * G, d]
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
+  const int* cu_q;        // [n + 1] first row of each sequence, then the end of the last
+  const int* cu_k;
+  int n, Tq, Tk, Hk, G, d;
+  int causal;
+  float scale_log2;       // scale * log2(e), > 0
+  int splits;             // of the few-row kernel
+  float* part_ml;         // [Tq, Hk * G, splits, 2] with more than one split
+  float* part_o;          // [Tq, Hk * G, splits, d]
+};
+constexpr int kAttnMaxSplits = 64;
+struct AttnPlan {
+  bool many;              // packed_attention_kernel; else split_attention_kernel with `splits`
+  int splits;
+};
+
 struct ParcaeArgs {
   const float* z;         // [cells, C] recurrent state
   const float* z_init;    // [cells, C]
@@ -229,6 +272,10 @@ hipError_t launch_abs_diff_quantile(const float* x, const float* y, size_t n, fl
 hipError_t launch_esmc_qk_rope(const EsmcRopeArgs& a, hipStream_t s);
 hipError_t launch_esmc_attention(const EsmcAttnArgs& a, hipStream_t s);
 hipError_t launch_esmc_swiglu(const half_t* x12, half_t* y, size_t M, int F, hipStream_t s);
+bool qk_norm_rope_row_fits(int heads, int d);  // whether one workgroup takes a whole row
+hipError_t launch_qk_norm_rope(QkRopeArgs a, bool bf16, bool row, hipStream_t s);
+AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus);
+hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s);
 hipError_t launch_q8_pack(const half_t* s, const half_t* b, uint32_t* sb, int N, int K, hipStream_t st);
 // Bytes of q8_pack_codes' layout: per 32-row block and step of two groups, 4 waves x 64
 // lanes x 16 bytes.

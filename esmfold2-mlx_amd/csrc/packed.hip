@@ -1,0 +1,557 @@
+// Attention over packed sequences of different lengths: softmax(q k^T scale) v within each sequence, query
+// heads in groups of G that share a key head, both ways or causal (the last query sees the last key).
+//
+// The rows a workgroup takes are (query, head of the group) pairs of one sequence and key head, row = query * G +
+// head: the group's heads share every key and value that is staged, and a single new token's heads fill a
+// tile together. A key tile in LDS is used by a wave for 32 QB rows:
+//   S^T[key][row] = K Q^T       (A: K rows from LDS, B: the wave's query fragments, in registers)
+//   p = 2^(S c - m c), l += p   (a lane holds one row: the maximum is over its registers and one exchange)
+//   O^T[d][row] += V^T P^T      (A: V^T by the transposing LDS read, B: p in the accumulator's own key order)
+// in fp32 but for p, which is rounded to the inputs' 16-bit type for the second product (an error of half a
+// step of that type on each p, below the output's own rounding after the sum). m is the running maximum; it, O
+// and l are rescaled only when a row's maximum has grown by more than 2^8 since (p then reaches 2^8 at most).
+//
+// Two kernels share that step: packed_attention_kernel (many rows: four waves of 32 QB rows each over key
+// tiles they share, the next tile in flight) and split_attention_kernel (few rows: 32 rows, keys divided
+// between the four waves and, through fp32 partials joined by a second launch, between workgroups).
+#include "common.h"
+#include "kernels.h"
+
+namespace esm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+
+struct Fp16 {
+  typedef half8 v8;
+  typedef half4 v4;
+  typedef half_t elem;
+  static constexpr uint16_t kExp = 0x7c00, kOne = 0x3c00;
+  static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+struct Bf16 {
+  typedef bf16x8 v8;
+  typedef bf16x4 v4;
+  typedef __bf16 elem;
+  static constexpr uint16_t kExp = 0x7f80, kOne = 0x3f80;
+  static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+constexpr float kGrow = 8.f;  // log2 of what p may reach before its row is rescaled
+
+// LDS rows of HD values, 16-byte pieces swizzled so that the reads below cover the 64 banks once: K fragments
+// read 16 rows at one piece; V's transposing read takes 4 rows x 4 pieces.
+template <int HD>
+DEV int k_piece(int n, int p) { return HD == 64 ? p ^ ((n >> 1) & 7) : p ^ (n & 15); }
+template <int HD>
+DEV int v_piece(int n, int p) { return HD == 64 ? p ^ (((n >> 1) & 1) << 2) : p ^ ((n & 3) << 2); }
+
+// V^T fragment: 4 keys k0 .. k0 + 3 of column n0 + lane % 16 (common.h, ds_read_tr16x4).
+template <class T, int HD>
+DEV typename T::v4 v_read(const char* vs, int k0, int n0, int lane) {
+  const int j = lane & 15, n = k0 + (j >> 2), d = n0 + 4 * (j & 3);
+  return __builtin_bit_cast(typename T::v4, ds_read_tr16x4(vs + n * 2 * HD + 16 * v_piece<HD>(n, d >> 3) + 2 * (d & 7)));
+}
+template <class T, int HD>
+DEV typename T::v8 v_frag(const char* vs, int j, int db, int lane) {  // keys 16 j + 4 h + {0..3, 8..11}, see p
+  const int h = lane >> 5, n0 = 32 * db + 16 * ((lane >> 4) & 1);
+  const typename T::v4 lo = v_read<T, HD>(vs, 16 * j + 4 * h, n0, lane), hi = v_read<T, HD>(vs, 16 * j + 8 + 4 * h, n0, lane);
+  return typename T::v8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// One wave's rows: query fragments, running maximum (of the unscaled scores), sum (this lane's half of the keys)
+// and output. Row r of block qb is column lane % 32 = r of every accumulator.
+template <class T, int HD, int QB>
+struct Rows {
+  typename T::v8 q[QB][HD / 16];
+  f32x16 o[QB][HD / 32];
+  float m[QB], l[QB];
+  int lim[QB];  // last key this row sees, counted within the sequence
+
+  DEV void init() {
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+      m[b] = -INFINITY;
+      l[b] = 0.f;
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[b][d][i] = 0.f;
+    }
+  }
+
+  // Keys key0 .. key0 + 32 NKB - 1 of the sequence from LDS tiles ks, vs. masked: some row sees only a part
+  // of them. later: some of the unseen ones are the sequence's own later keys, whose values may be anything.
+  template <int NKB>
+  DEV void step(const char* ks, const char* vs, int key0, bool masked, bool later, float c, int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    f32x16 s[QB][NKB];
+#pragma unroll
+    for (int b = 0; b < QB; b++)
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[b][kb][i] = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+      for (int k = 0; k < HD / 16; k++) {
+        const int n = 32 * kb + r;
+        const typename T::v8 kf = *reinterpret_cast<const typename T::v8*>(ks + n * 2 * HD + 16 * k_piece<HD>(n, 2 * k + h));
+#pragma unroll
+        for (int b = 0; b < QB; b++) s[b][kb] = T::mfma(kf, q[b][k], s[b][kb]);
+      }
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < QB; b++)
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            s[b][kb][i] = key0 + 32 * kb + acc_row32(i, lane) <= lim[b] ? s[b][kb][i] : -INFINITY;
+    }
+    typename T::v8 pf[QB][2 * NKB];
+#pragma unroll
+    for (int b = 0; b < QB; b++) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[b][kb][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      if (__any((mx - m[b]) * c > kGrow)) {  // (from m = -inf at the first key a row sees)
+        const float mn = fmaxf(m[b], mx), ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f((m[b] - ref) * c);
+        m[b] = mn;
+        l[b] *= alpha;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[b][d][i] *= alpha;
+      }
+      const float mc = m[b] == -INFINITY ? 0.f : m[b] * c;  // no key seen yet
+      float sum = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][kb][i], c, -mc));  // (results below 2^-126 flush)
+          sum += e;
+          pf[b][2 * kb + (i >> 3)][i & 7] = (typename T::elem)e;
+        }
+      l[b] += sum;
+    }
+    if (later && __any(unclean(vs, 32 * NKB, lane))) {
+      apart<NKB>(vs, key0, pf, lane);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * NKB; j++)
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++) {
+        const typename T::v8 vf = v_frag<T, HD>(vs, j, d, lane);
+#pragma unroll
+        for (int b = 0; b < QB; b++) o[b][d] = T::mfma(vf, pf[b][j], o[b][d]);
+      }
+  }
+
+  // Whether this lane's share of the value tile holds an infinity or a NaN.
+  static DEV bool unclean(const char* vs, int keys, int lane) {
+    bool bad = false;
+    for (int i = lane; i < keys * HD / 8; i += 64) {
+      const u16x8 v = *reinterpret_cast<const u16x8*>(vs + 16 * i);
+#pragma unroll
+      for (int e = 0; e < 8; e++) bad = bad || (v[e] & T::kExp) == T::kExp;
+    }
+    return bad;
+  }
+
+  // The second product where later keys' values hold infinities or NaN, which a p of 0 would turn into NaN: the
+  // finite values as ever, and for the others two products of ones count, row by row, the seen keys whose value is
+  // not below +inf, and not above -inf; what such a count touches becomes that infinity (both: NaN).
+  template <int NKB>
+  DEV void apart(const char* vs, int key0, const typename T::v8 (&pf)[QB][2 * NKB], int lane) {
+    const int h = lane >> 5;
+#pragma unroll 1
+    for (int d = 0; d < HD / 32; d++) {
+#pragma unroll
+      for (int b = 0; b < QB; b++) {
+        f32x16 up, down, of = {};
+#pragma unroll
+        for (int i = 0; i < 16; i++) up[i] = down[i] = of[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2 * NKB; j++) {
+          const u16x8 v = __builtin_bit_cast(u16x8, v_frag<T, HD>(vs, j, d, lane));
+          u16x8 fin, pos, neg, seen;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const bool odd = (v[e] & T::kExp) == T::kExp, nan = odd && (v[e] & 0x7fff) != T::kExp;
+            fin[e] = odd ? 0 : v[e];
+            pos[e] = odd && (nan || !(v[e] >> 15)) ? T::kOne : 0;
+            neg[e] = odd && (nan || (v[e] >> 15)) ? T::kOne : 0;
+            seen[e] = key0 + 16 * j + 4 * h + (e & 3) + 8 * (e >> 2) <= lim[b] ? T::kOne : 0;
+          }
+          typedef typename T::v8 v8;
+          of = T::mfma(__builtin_bit_cast(v8, fin), pf[b][j], of);
+          up = T::mfma(__builtin_bit_cast(v8, pos), __builtin_bit_cast(v8, seen), up);
+          down = T::mfma(__builtin_bit_cast(v8, neg), __builtin_bit_cast(v8, seen), down);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          float add = of[i];
+          add += up[i] > 0.f ? INFINITY : 0.f;
+          add -= down[i] > 0.f ? INFINITY : 0.f;
+#pragma unroll
+          for (int dd = 0; dd < HD / 32; dd++) o[b][dd][i] += dd == d ? add : 0.f;
+        }
+      }
+    }
+  }
+};
+
+// Sequence and tile of a work item: item counts the tiles of `unit` rows of all sequences in order. All lanes agree.
+// Starts outside 0 .. total are brought inside, so nothing a caller writes there reaches past the tensors.
+DEV bool find_tile(const int* cu, int n, int total, int G, int unit, int item, int lane, int& seq, int& tile) {
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = i0 + lane;
+    int nt = 0;
+    if (i < n) {
+      const int a = min(max(cu[i], 0), total), b = min(max(cu[i + 1], a), total);
+      nt = ((b - a) * G + unit - 1) / unit;
+    }
+    int sum = nt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o);
+      sum += lane >= o ? up : 0;
+    }
+    const uint64_t past = __ballot(item < sum);
+    if (past) {
+      const int w = __builtin_ctzll(past);
+      seq = i0 + w;
+      tile = item - __builtin_amdgcn_readlane(sum - nt, w);
+      return true;
+    }
+    item -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+struct Span {
+  int q0, nq, k0, nk;  // first row and rows of a sequence, on the query and on the key side
+};
+DEV Span span_of(const PackedAttnArgs& p, int seq) {
+  Span s;
+  const auto side = [&](const int* cu, int total, int& first, int& count) {
+    first = min(max(cu[seq], 0), total);
+    count = min(max(cu[seq + 1], first), total) - first;
+    first = __builtin_amdgcn_readfirstlane(first);
+    count = __builtin_amdgcn_readfirstlane(count);
+  };
+  side(p.cu_q, p.Tq, s.q0, s.nq);
+  side(p.cu_k, p.Tk, s.k0, s.nk);
+  return s;
+}
+
+// A tile of `keys` key rows from key kt of the span on, as a buffer whose range ends with the span's last row:
+// rows past it (another sequence's, or none) load zeros.
+DEV dma_src_t tile_src(const char* base, long long st, int d, int first, int kt, int nk, int keys) {
+  const int rows = min(keys, nk - kt);
+  return dma_src(base + 2 * (st * (long long)(first + kt)), rows > 0 ? (uint32_t)(2 * ((rows - 1) * st + d)) : 0u);
+}
+
+// One wave's DMA of `count` rows (a multiple of the rows of 1 KB), from row n0 of the tile on, into LDS rows at n0.
+template <int HD, bool V>
+DEV void load_rows(dma_src_t src, uint32_t lds, long long st, int d, int n0, int count, int lane) {
+  constexpr int kRow = 2 * HD, kPer = 1024 / kRow, kPieces = HD / 8;
+#pragma unroll
+  for (int i = 0; i < count / kPer; i++) {
+    const int n = n0 + kPer * i + lane / kPieces, lp = lane % kPieces;
+    const int piece = V ? v_piece<HD>(n, lp) : k_piece<HD>(n, lp);
+    dma16(src, lds + kRow * (n0 + kPer * i), 8 * piece < d ? (uint32_t)(2 * st * n + 16 * piece) : kOOB, 0);
+  }
+}
+
+// Query fragments and the limit of row `row` (of the span's nq * G) for every block of the wave.
+template <class T, int HD, int QB>
+DEV void load_queries(Rows<T, HD, QB>& w, const PackedAttnArgs& p, const Span& s, int hk, int row0, int lane) {
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int b = 0; b < QB; b++) {
+    const int row = row0 + 32 * b + r, i = row / p.G, g = row - i * p.G;
+    const bool ok = i < s.nq;
+    const char* src = (const char*)p.q + 2 * ((long long)(s.q0 + (ok ? i : 0)) * p.q_st + (long long)(hk * p.G + g) * p.q_sh);
+#pragma unroll
+    for (int k = 0; k < HD / 16; k++) {
+      w.q[b][k] = typename T::v8{};
+      if (ok && 16 * k + 8 * h < p.d) w.q[b][k] = *reinterpret_cast<const typename T::v8*>(src + 2 * (16 * k + 8 * h));
+    }
+    w.lim[b] = p.causal && ok ? min(s.nk - 1, i + s.nk - s.nq) : s.nk - 1;
+  }
+}
+
+constexpr int kAttnKeys = 64;  // keys per tile of the many-row kernel
+
+template <class T, int HD, int QB>
+__global__ __launch_bounds__(256) void packed_attention_kernel(PackedAttnArgs p) {
+  constexpr int kTile = kAttnKeys * 2 * HD;  // bytes of a K (or V) tile
+  __shared__ __align__(1024) char lds[2][2 * kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // key heads run fastest over the workgroups: the eight XCDs take different heads, each with its own L2, and the
+  // longest tiles of every head start first
+  const int hk = blockIdx.x % p.Hk, item = blockIdx.x / p.Hk;
+  int seq, tile;
+  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, 128 * QB, item, lane, seq, tile)) return;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Span s = span_of(p, seq);
+  const int rows = s.nq * p.G;
+  if (p.causal) tile = (rows + 128 * QB - 1) / (128 * QB) - 1 - tile;
+  const int row0 = 128 * QB * tile + 32 * QB * wave;  // this wave's first row
+
+  Rows<T, HD, QB> w;
+  w.init();
+  load_queries(w, p, s, hk, row0, lane);
+  // keys seen by the workgroup's last row, by this wave's last row, and by its first
+  const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
+  const int end = seen(128 * QB * (tile + 1) - 1);
+  const int wend = row0 < rows ? seen(row0 + 32 * QB - 1) : 0, wfull = seen(row0);
+  const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
+  const char* vb = (const char*)p.v + 2 * (long long)hk * p.v_sh;
+  const auto load = [&](int kt, int buf) {
+    constexpr int kMine = kAttnKeys / 4;
+    const uint32_t at = lds_address(lds[buf]);
+    load_rows<HD, false>(tile_src(kb, p.k_st, p.d, s.k0, kt, s.nk, kAttnKeys), at, p.k_st, p.d, kMine * wave, kMine, lane);
+    load_rows<HD, true>(tile_src(vb, p.v_st, p.d, s.k0, kt, s.nk, kAttnKeys), at + kTile, p.v_st, p.d, kMine * wave, kMine, lane);
+  };
+  if (end > 0) load(0, 0);
+  for (int kt = 0, buf = 0; kt < end; kt += kAttnKeys, buf ^= 1) {
+    wait_vm(0);
+    __syncthreads();  // this tile is in, and every wave has left the other buffer
+    if (kt + kAttnKeys < end) load(kt + kAttnKeys, buf ^ 1);
+    if (kt < wend)
+      w.template step<kAttnKeys / 32>(lds[buf], lds[buf] + kTile, kt, kt + kAttnKeys > wfull, kt + kAttnKeys > wfull && wfull < s.nk, p.scale_log2, lane);
+  }
+
+  const int r = lane & 31;
+#pragma unroll
+  for (int b = 0; b < QB; b++) {
+    const float l = w.l[b] + __shfl_xor(w.l[b], 32);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key is 0
+    const int row = row0 + 32 * b + r, i = row / p.G, g = row - i * p.G;
+    if (row >= rows) continue;
+    char* dst = (char*)p.o + 2 * ((long long)(s.q0 + i) * p.o_st + (long long)(hk * p.G + g) * p.o_sh);
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; i4++) {
+        const int col = 32 * d + acc_row32(4 * i4, lane);
+        typename T::v4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(w.o[b][d][4 * i4 + e] * inv);
+        if (col < p.d) *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
+      }
+  }
+}
+
+// ---- few rows ---------------------------------------------------------------------------------
+// 32 rows per workgroup; its keys are the part of the sequence's that `split` of p.splits takes, in passes of
+// 4 x KW keys, KW to each wave in a private LDS tile. The waves' results are joined through LDS. With more
+// than one split each workgroup leaves (m, l, O) of its part in the workspace and attention_join_kernel sums them.
+template <int HD>
+constexpr int kSplitKeys = HD == 64 ? 64 : 32;  // keys per wave and pass: 64 KB of LDS, two workgroups per CU
+
+// Keys per split: a multiple of a pass, so that no split but the last is ragged.
+DEV int split_keys(int nk, int splits, int pass) { return ((nk + splits - 1) / splits + pass - 1) / pass * pass; }
+
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs p) {
+  constexpr int KW = kSplitKeys<HD>, kTile = KW * 2 * HD, kPass = 4 * KW;
+  __shared__ __align__(1024) char lds[4][2 * kTile];
+  __shared__ float ml[4][2][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int hk = blockIdx.x % p.Hk, split = (blockIdx.x / p.Hk) % p.splits, item = blockIdx.x / p.Hk / p.splits;
+  int seq, tile;
+  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, 32, item, lane, seq, tile)) return;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Span s = span_of(p, seq);
+  const int rows = s.nq * p.G, row0 = 32 * tile;
+  const int part = split_keys(s.nk, p.splits, kPass), first = part * split;
+  const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
+  const int end = min(seen(row0 + 31), first + part), wfull = seen(row0);
+  if (p.splits > 1 && first > 0 && first >= s.nk) return;  // no part of this sequence: the join reads none
+
+  Rows<T, HD, 1> w;
+  w.init();
+  load_queries(w, p, s, hk, row0, lane);
+  const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
+  const char* vb = (const char*)p.v + 2 * (long long)hk * p.v_sh;
+  char *ks = lds[wave], *vs = lds[wave] + kTile;
+  for (int kt = first + KW * wave; kt < end; kt += kPass) {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the last pass's LDS reads are back
+    __asm__ volatile("" ::: "memory");
+    load_rows<HD, false>(tile_src(kb, p.k_st, p.d, s.k0, kt, s.nk, KW), lds_address(ks), p.k_st, p.d, 0, KW, lane);
+    load_rows<HD, true>(tile_src(vb, p.v_st, p.d, s.k0, kt, s.nk, KW), lds_address(vs), p.v_st, p.d, 0, KW, lane);
+    wait_vm(0);
+    w.template step<KW / 32>(ks, vs, kt, kt + KW > wfull, kt + KW > wfull && wfull < s.nk, p.scale_log2, lane);
+  }
+
+  // (m, l, O) of the four waves through LDS; wave i then joins the d quads i, i + 4, .. of every row
+  const float lsum = w.l[0] + __shfl_xor(w.l[0], 32);
+  if (h == 0) {
+    ml[wave][0][r] = w.m[0];
+    ml[wave][1][r] = lsum;
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  __asm__ volatile("" ::: "memory");
+  f32x4* ow = reinterpret_cast<f32x4*>(lds[wave]);
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int i4 = 0; i4 < 4; i4++)
+      ow[(4 * d + i4) * 64 + lane] = f32x4{w.o[0][d][4 * i4], w.o[0][d][4 * i4 + 1], w.o[0][d][4 * i4 + 2], w.o[0][d][4 * i4 + 3]};
+  __syncthreads();
+  const int row = row0 + r, i = row / p.G, g = row - i * p.G;
+  if (row >= rows) return;
+  float M = -INFINITY, L = 0.f, sc[4];
+#pragma unroll
+  for (int v = 0; v < 4; v++) M = fmaxf(M, ml[v][0][r]);
+  const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int v = 0; v < 4; v++) {
+    // (a wave that saw no key has m = -inf and adds 0; an infinite m gives NaN, as its row is)
+    sc[v] = __builtin_amdgcn_exp2f((ml[v][0][r] - ref) * p.scale_log2);
+    L += sc[v] * ml[v][1][r];
+  }
+  const long long q = s.q0 + i;
+  const int head = hk * p.G + g;
+  if (p.splits > 1) {
+    const size_t at = ((size_t)q * (p.G * p.Hk) + head) * p.splits + split;
+    if (wave == 0 && h == 0) {
+      p.part_ml[2 * at] = M;
+      p.part_ml[2 * at + 1] = L;
+    }
+#pragma unroll
+    for (int u = 0; u < HD / 32; u++) {
+      const int qd = wave + 4 * u, col = 32 * (qd >> 2) + acc_row32(4 * (qd & 3), lane);
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < 4; v++) acc += sc[v] * reinterpret_cast<const f32x4*>(lds[v])[qd * 64 + lane];
+      if (col < p.d) *reinterpret_cast<f32x4*>(p.part_o + at * p.d + col) = acc;
+    }
+    return;
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  char* dst = (char*)p.o + 2 * (q * p.o_st + (long long)head * p.o_sh);
+#pragma unroll
+  for (int u = 0; u < HD / 32; u++) {
+    const int qd = wave + 4 * u, col = 32 * (qd >> 2) + acc_row32(4 * (qd & 3), lane);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 4; v++) acc += sc[v] * reinterpret_cast<const f32x4*>(lds[v])[qd * 64 + lane];
+    typename T::v4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
+    if (col < p.d) *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
+  }
+}
+
+// The splits of one (query, head) row: a wave reads their m and l in its lanes, then sums O over them, 4 columns a
+// lane (lanes beyond d / 4 take every other split).
+template <class T, int HD>
+__global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = p.G * p.Hk;
+  const long long at = (long long)blockIdx.x * 4 + wave;
+  if (at >= (long long)p.Tq * H) return;
+  const int q = (int)(at / H), head = (int)(at - (long long)q * H);
+  int seq = -1;  // the sequence of this row, if any
+  for (int i0 = 0; i0 < p.n && seq < 0; i0 += 64) {
+    const int i = i0 + lane;
+    bool in = false;
+    if (i < p.n) {
+      const int a = min(max(p.cu_q[i], 0), p.Tq), b = min(max(p.cu_q[i + 1], a), p.Tq);
+      in = q >= a && q < b;
+    }
+    const uint64_t hit = __ballot(in);
+    if (hit) seq = i0 + __builtin_ctzll(hit);
+  }
+  if (seq < 0) return;  // behind the last sequence: left as it is
+  const Span s = span_of(p, seq);
+  const int part = split_keys(s.nk, p.splits, 4 * kSplitKeys<HD>);
+  const int live = s.nk > 0 ? (s.nk + part - 1) / part : 1;  // splits that wrote (at most 64)
+  const float* pm = p.part_ml + 2 * (size_t)at * p.splits;
+  float m = lane < live ? pm[2 * lane] : -INFINITY, l = lane < live ? pm[2 * lane + 1] : 0.f;
+  float M = m;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+  const float sc = __builtin_amdgcn_exp2f((m - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
+  float L = lane < live ? sc * l : 0.f;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) L += __shfl_xor(L, o);
+  constexpr int kCols = HD / 4, kSide = 64 / kCols;  // lanes across a row, splits at once
+  const int col = 4 * (lane % kCols), side = lane / kCols;
+  const float* po = p.part_o + (size_t)at * p.splits * p.d;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < live; j0 += kSide) {
+    const int j = j0 + side;
+    const float f = __shfl(sc, j & 63);
+    if (j < live && col < p.d) acc += f * *reinterpret_cast<const f32x4*>(po + (size_t)j * p.d + col);
+  }
+#pragma unroll
+  for (int o = kCols; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o);
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  if (side == 0 && col < p.d) {
+    typename T::v4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
+    *reinterpret_cast<typename T::v4*>((char*)p.o + 2 * ((long long)q * p.o_st + (long long)head * p.o_sh + col)) = y;
+  }
+}
+
+template <class T, int HD>
+static hipError_t launch_attention_t(const PackedAttnArgs& a, bool many, hipStream_t s) {
+  if (many) {
+    constexpr int QB = 2;
+    const long long items = (long long)a.Tq * a.G / (128 * QB) + a.n;
+    ESM_LAUNCH((packed_attention_kernel<T, HD, QB>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  const long long items = (long long)a.Tq * a.G / 32 + a.n;
+  ESM_LAUNCH((split_attention_kernel<T, HD>), dim3((unsigned)(items * a.Hk * a.splits)), dim3(256), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  const long long rows = (long long)a.Tq * a.G * a.Hk;
+  ESM_LAUNCH((attention_join_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+// Which kernel and how many splits, from what the host knows: rows, keys, sequences and heads (the lengths are on
+// the device). `cus` compute units.
+AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus) {
+  AttnPlan plan{};
+  const long long tiles = (Tq * G / 256 + 1) * Hk;  // at least this many tiles of 256 rows, if the sequences are long
+  plan.many = tiles >= cus / 2 && Tq / n * G >= 64;
+  plan.splits = 1;
+  if (!plan.many) {
+    const long long small = (Tq * G / 32 + n) * Hk, pass = d <= 64 ? 256 : 128;
+    long long sp = 4 * cus / (small > 0 ? small : 1);
+    // a sequence may hold nearly all keys: its splits are what matters, the others' are empty
+    if (n > 1) sp *= 4;
+    sp = sp < Tk / pass ? sp : Tk / pass;
+    plan.splits = (int)(sp < 1 ? 1 : sp > kAttnMaxSplits ? kAttnMaxSplits : sp);
+  }
+  return plan;
+}
+
+hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s) {
+  if (a.d <= 64) return bf16 ? launch_attention_t<Bf16, 64>(a, many, s) : launch_attention_t<Fp16, 64>(a, many, s);
+  return bf16 ? launch_attention_t<Bf16, 128>(a, many, s) : launch_attention_t<Fp16, 128>(a, many, s);
+}
+
+}  // namespace esm

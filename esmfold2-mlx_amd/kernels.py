@@ -194,6 +194,131 @@ def esmc_attention(q, k, v, sequence_id=None, scale: float | None = None, out=No
     return o
 
 
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def _rows(t, name: str, like=None):
+    """A 16-bit [rows, heads, d] tensor whose heads are contiguous (a view of a wider row, say): the checks that
+    need no shape, and its strides."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise capi.EsmError(-5, f"{name} must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
+    if t.dim() != 3 or t.dtype not in _DTYPES:
+        raise capi.EsmError(-2, f"{name} must be [rows, heads, d] in fp16 or bf16, got {t.dtype} {tuple(t.shape)}")
+    if like is not None and (t.dtype is not like.dtype or t.device != like.device):
+        raise capi.EsmError(-2, f"{name}: {t.dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
+    st, sh, one = t.stride()
+    if one != 1 and t.shape[2] > 1:
+        raise capi.EsmError(-3, f"{name}: the values of a head must be contiguous")
+    # (a stride that nothing is reached by says nothing)
+    return (st if t.shape[0] > 1 else 8 * ((t.shape[1] * t.shape[2] + 7) // 8)), (sh if t.shape[1] > 1 else 0)
+
+
+def _distinct(strides, shape, name: str) -> None:
+    """Refuses an output whose rows or heads share memory."""
+    (st, sh), (T, H, d) = strides, shape
+    if (H > 1 and sh < d) or (T > 1 and H > 1 and min(st, sh) * ((H if st >= sh else T) - 1) + d > max(st, sh)):
+        raise capi.EsmError(-3, f"{name}: rows and heads must not overlap")
+
+
+def _on(device):
+    """A context with the tensors' device current: launches go on its current stream."""
+    return scratch._UNGUARDED if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _aux(t, name: str, dtypes, device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise capi.EsmError(-5, f"{name} must be on {device}")
+    if t.dtype not in dtypes:
+        raise capi.EsmError(-2, f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise capi.EsmError(-3, f"{name} must be contiguous")
+    return t
+
+
+def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: bool = False, norm: str | None = None,
+                 over: str = "head", q_w=None, k_w=None, eps: float = 1e-6, out=None):
+    """Norm and rotation of q [T, H, d] and k [T, Hk, d] (fp16 or bf16, views of wider rows allowed) in one pass ->
+    (q', k'). ``norm``: None, "rms" or "layer", ``over`` each "head" or the whole "row" of heads, with fp32 weights of
+    d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
+    makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
+    0 .. T - 1). ``out`` = (q', k'), which may be (q, k)."""
+    lib = capi.lib()
+    qs, ks = _rows(q, "q"), _rows(k, "k", q)
+    T, H, d = q.shape
+    Hk = k.shape[1]
+    if k.shape[0] != T or k.shape[2] != d:
+        raise capi.EsmError(-2, f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if norm not in _NORMS or over not in ("head", "row"):
+        raise capi.EsmError(-4, f"qk_norm_rope: norm={norm!r} over={over!r}")
+    _aux(freq, "freq", (torch.float64,), q.device)
+    if positions is not None:
+        _aux(positions, "positions", (torch.int32, torch.int64), q.device)
+        if positions.numel() != T:
+            raise capi.EsmError(-2, f"qk_norm_rope: {positions.numel()} positions for {T} rows")
+    w = []
+    for t, n, heads in ((q_w, "q_w", H), (k_w, "k_w", Hk)):
+        if t is not None:
+            _aux(t, n, (torch.float32,), q.device)
+            if t.numel() not in (d, heads * d):
+                raise capi.EsmError(-2, f"qk_norm_rope: {n} has {t.numel()} elements for {heads} heads of {d}")
+        w.append((_ptr(t), int(t is not None and t.numel() != d)))
+    if out is None:
+        qo, ko = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    else:
+        qo, ko = out
+    outs = []
+    for t, n, like in ((qo, "out[0]", q), (ko, "out[1]", k)):
+        outs.append(_rows(t, n, q))
+        if t.shape != like.shape:
+            raise capi.EsmError(-2, f"qk_norm_rope: {n} {tuple(t.shape)}, writes {tuple(like.shape)}")
+        _distinct(outs[-1], t.shape, n)
+    with _on(q.device):
+        capi.check(lib.qk_norm_rope(q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), *qs, *ks, *outs[0],
+                                    *outs[1], *w[0], *w[1], float(eps), _ptr(positions),
+                                    int(positions is not None and positions.dtype == torch.int64), freq.data_ptr(),
+                                    float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], int(over == "row"),
+                                    int(interleaved), _DTYPES[q.dtype], capi.stream_ptr()))
+    return qo, ko
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: float | None = None, out=None):
+    """softmax(q k^T * scale) v within each packed sequence: q [Tq, H, d], k, v [Tk, Hk, d] (fp16 or bf16, views of
+    wider rows allowed; H a multiple of Hk) -> o [Tq, H, d]. ``cu_q``, ``cu_k`` int32 [n + 1] on the device: the first
+    row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
+    the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
+    sequence are not written. The partial results of few rows against many keys live in the shared scratch."""
+    lib = capi.lib()
+    qs, ks, vs = _rows(q, "q"), _rows(k, "k", q), _rows(v, "v", q)
+    Tq, H, d = q.shape
+    Tk, Hk, _ = k.shape
+    if k.shape != v.shape or k.shape[2] != d or Hk == 0 or H % Hk:
+        raise capi.EsmError(-2, f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if cu_k is None:
+        if Tk != Tq:
+            raise capi.EsmError(-2, f"packed_attention: {Tq} query rows and {Tk} key rows need cu_k")
+        cu_k = cu_q
+    for t, n in ((cu_q, "cu_q"), (cu_k, "cu_k")):
+        _aux(t, n, (torch.int32,), q.device)
+    n = cu_q.numel() - 1
+    if n < 0 or cu_k.numel() != n + 1:
+        raise capi.EsmError(-2, f"packed_attention: {cu_q.numel()} and {cu_k.numel()} starts")
+    o = torch.empty(Tq, H, d, dtype=q.dtype, device=q.device) if out is None else out
+    os_ = _rows(o, "out", q)
+    if o.shape != q.shape:
+        raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
+    _distinct(os_, o.shape, "out")
+    with _on(q.device):
+        need = int(lib.packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d))
+        with scratch.guard(q.device, need):
+            ws, wp, stream = scratch.take(need, q.device) if need else (None, None, capi.stream_ptr())
+            capi.check(lib.packed_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_,
+                                            cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, int(causal),
+                                            float(d ** -0.5 if scale is None else scale), _DTYPES[q.dtype], wp, need,
+                                            stream))
+    return o
+
+
 def esmc_swiglu(x12, out=None):
     """[M, 2F] fp16 (rows [x1 | x2]) -> silu(x1) * x2 [M, F] fp16."""
     lib = capi.lib()

@@ -412,6 +412,45 @@ int esmc_attention(const esm_half* q, const esm_half* k, const esm_half* v, cons
 int esmc_swiglu(const esm_half* x12, esm_half* y, int M, int F, void* stream);
 
 /*
+ * Operators of a transformer block over packed rows: sequences of different lengths behind one another, without
+ * padding. dtype: ESM_F16 or ESM_BF16 (all 16-bit tensors of a call). Strides are in elements (st: from row to row, sh:
+ * from head to head, the values of a head contiguous), so that q, k and v may be views of one projection's output;
+ * strides are multiples of 8 and pointers 16-byte aligned.
+ *
+ * qk_norm_rope: q [T, H, d], k [T, Hk, d] -> q_out, k_out (which may be q and k): norm (ESM_NORM_NONE, _RMS:
+ *   x / sqrt(mean x^2 + eps), _LAYER: the same of x - mean x) over each head, or with over_row over all heads of the
+ *   row (q and k apart), times the weights (fp32, [d] or [heads * d] as q_w_heads, k_w_heads say; NULL: 1); then the
+ *   first rot values of each head turn by position * freq[i] (freq [rot / 2] fp64, radians per position), in pairs
+ *   (i, i + rot / 2) or, interleaved, (2i, 2i + 1), with sine and cosine times gain. pos: [T] int32 (pos64: int64), or
+ *   NULL for 0 .. T - 1. fp32 but for the angle (fp64), rounded once. d % 8 == 0, 8 <= d <= 256; rot % 16 == 0,
+ *   rot <= d; T < 2^22; with over_row at most 64 groups of the 64 / (d / 16, rounded up to a power of two) heads that
+ *   a wave takes.
+ * packed_attention: sequence s has the query rows cu_q[s] .. cu_q[s + 1] - 1 and the key rows cu_k[s] ..
+ *   cu_k[s + 1] - 1 (int32 [n + 1] on the device, ascending; values outside 0 .. Tq, 0 .. Tk are brought inside):
+ *   o = softmax(scale q k^T) v within the sequence, query head h with key head h / (H / Hk). causal: query i of nq
+ *   sees the keys 0 .. i + nk - nq of nk. A row that sees no key is 0; rows of no sequence are not written. What
+ *   unseen keys and values hold (infinities, NaN) reaches no output. Scores, softmax and sums are fp32, the
+ *   probabilities rounded to dtype for the second product. d % 8 == 0, d <= 128; scale > 0; row strides from d to 2^23.
+ *   workspace: packed_attention_workspace_bytes(...) bytes, 256-byte aligned (0: none; fp32 partials where a few rows'
+ *   keys are divided between workgroups).
+ */
+#define ESM_F16 0
+#define ESM_BF16 1
+#define ESM_NORM_NONE 0
+#define ESM_NORM_RMS 1
+#define ESM_NORM_LAYER 2
+int qk_norm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_st, int64_t q_sh, int64_t k_st,
+                 int64_t k_sh, int64_t qo_st, int64_t qo_sh, int64_t ko_st, int64_t ko_sh, const float* q_w,
+                 int q_w_heads, const float* k_w, int k_w_heads, float eps, const void* pos, int pos64,
+                 const double* freq, float gain, int T, int H, int Hk, int d, int rot, int norm, int over_row,
+                 int interleaved, int dtype, void* stream);
+size_t packed_attention_workspace_bytes(int n, int Tq, int Tk, int H, int Hk, int d);
+int packed_attention(const void* q, const void* k, const void* v, void* o, int64_t q_st, int64_t q_sh, int64_t k_st,
+                     int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t o_st, int64_t o_sh, const int* cu_q,
+                     const int* cu_k, int n, int Tq, int Tk, int H, int Hk, int d, int causal, float scale, int dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * One whole ESMC block (mlx_esmc.py:84-102) as its eight launches on the stream (one more for each of wqkv, w1
  * whose K is split, and for each linear whose rows are divided between tile forms), from the block's LayerNormed
  * input: x' = x + alpha * wo(attention(wqkv(h))), then x_out = x' + alpha * w2(swiglu(w1(LN2(x')))), then the
