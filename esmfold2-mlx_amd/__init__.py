@@ -7,6 +7,7 @@ Modules:
   kernels          -- one functional wrapper per C entry point (torch tensors in/out)
   trimul           -- TriMul / TriMulPair: the forward(pair_grid, visibility) module contract
   q8               -- Q8Linear: the quantized_matmul(transpose=True, group 64, bits 8) contract
+  f8               -- F8Linear: weights in e4m3 with a scale per 128 x 128 block, on the fp8 matrix cores
   esmc             -- EsmcBlock and HipEsmc: the ESMC language model around the 8-bit linear
   rotary           -- Rotary: rotary positions (layouts, part of a head, long contexts) with the norm of q and k
   trunk            -- PairTransition, TrunkBlock and PairTrunk (the FoldingTrunk drop-in)
@@ -24,7 +25,7 @@ Modules:
 
 from . import build, capi  # noqa: F401
 
-__all__ = ["build", "capi", "kernels", "trimul", "q8", "esmc", "rotary", "trunk", "recycle", "scratch", "var_hip_trimul",
+__all__ = ["build", "capi", "kernels", "trimul", "q8", "f8", "esmc", "rotary", "trunk", "recycle", "scratch", "var_hip_trimul",
            "var_hip_trunk", "var_6b_hip_trunks", "var_6b_hip_loop", "var_6b_hip_adaptive", "var_hip_adaptive_loops",
            "variants", "workloads"]
 

@@ -56,6 +56,13 @@ SIGNATURES = {
                      + [_vp]),
     "packed_attention_workspace_bytes": (_sz, [_int] * 6),
     "packed_attention": (_int, [_vp] * 4 + [_i64] * 8 + [_vp, _vp] + [_int] * 7 + [_f32, _int, _vp, _sz, _vp]),
+    "f8_packed_codes_bytes": (_sz, [_int, _int]),
+    "f8_pack_codes": (_int, [_vp, _vp, _int, _int, _vp]),
+    "f8_quantize_weight": (_int, [_vp, _vp, _vp, _int, _int, _vp]),
+    "f8_linear_workspace_bytes": (_sz, [_int, _int, _int]),
+    "f8_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
+    "f8_linear_partials_bytes": (_sz, [_int, _int, _int]),
+    "f8_linear_partials": (_int, [_vp, _i64, _vp, _vp, _vp, _sz, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "esmc_block_workspace_bytes": (_sz, [_int, _int, _int]),
     "esmc_block": (_int, [_vp] * 17 + [_f32, _f32, _f32, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "parcae_step": (_int, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _int, _int, _int, _vp]),

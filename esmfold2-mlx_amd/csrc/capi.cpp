@@ -1045,6 +1045,104 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
                     "packed_attention launch");
 }
 
+static bool f8_shape(int M, int K, int N) { return M >= 0 && K > 0 && N > 0 && K % 16 == 0 && K <= kQ8MaxK && N % 8 == 0; }
+
+size_t f8_packed_codes_bytes(int N, int K) { return f8_shape(0, K, N) ? esm::f8_packed_size(N, K) : 0; }
+
+int f8_pack_codes(const uint8_t* q, uint8_t* qp, int N, int K, void* stream) {
+  if (!f8_shape(0, K, N)) return fail(ESM_ERR_SHAPE, "f8_pack_codes: K=%d (multiple of 16) N=%d (of 8)", K, N);
+  if (!q || !qp) return fail(ESM_ERR_NULL, "f8_pack_codes: NULL pointer");
+  if (!aligned16(q) || !aligned16(qp)) return fail(ESM_ERR_ALIGN, "f8_pack_codes: codes must be 16-byte aligned");
+  return hip_status(esm::launch_f8_pack(q, qp, N, K, (hipStream_t)stream), "f8_pack_codes launch");
+}
+
+int f8_quantize_weight(const float* w, uint8_t* q, float* s, int N, int K, void* stream) {
+  if (!f8_shape(0, K, N)) return fail(ESM_ERR_SHAPE, "f8_quantize_weight: K=%d (multiple of 16) N=%d (of 8)", K, N);
+  if ((long long)((N + 127) / 128) * ((K + 127) / 128) >= (1LL << 24))
+    return fail(ESM_ERR_SHAPE, "f8_quantize_weight: N=%d K=%d too large", N, K);
+  if (!w || !q || !s) return fail(ESM_ERR_NULL, "f8_quantize_weight: NULL pointer");
+  if (!aligned16(w) || !aligned16(q)) return fail(ESM_ERR_ALIGN, "f8_quantize_weight: w and q must be 16-byte aligned");
+  return hip_status(esm::launch_f8_quantize_weight(w, q, s, N, K, (hipStream_t)stream), "f8_quantize_weight launch");
+}
+
+// f8_linear's workspace: x in e4m3, its scales, then (y rounded from splits) the partials.
+namespace {
+struct F8Ws {
+  esm::F8Plan plan;
+  int Mp;
+  size_t sx, part, total;
+};
+F8Ws f8_layout(int M, int K, int N, bool parts_inside) {
+  F8Ws w{};
+  w.plan = esm::f8_plan(M, K, N, cu_count());
+  w.Mp = round_up(M, 16);
+  if (w.plan.form != esm::kF8Few) {
+    const size_t kb = (size_t)(K + 127) / 128;
+    w.sx = (size_t)w.Mp * kb * 128;
+    w.part = (w.sx + (size_t)w.Mp * kb * 4 + 255) / 256 * 256;
+    w.total = w.part;
+    if (parts_inside && w.plan.splits > 1) w.total += (size_t)w.plan.splits * M * N * 4;
+  }
+  return w;
+}
+
+int f8_run(const char* fn, const void* x, int64_t x_st, const uint8_t* qp, const float* s, void* y, float* parts,
+           size_t parts_bytes, int* splits, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
+           void* stream) {
+  if (splits) *splits = 0;
+  if (!f8_shape(M, K, N)) return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d (multiple of 16) N=%d (of 8)", fn, M, K, N);
+  if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "%s: dtype=%d", fn, dtype);
+  if (M > (1 << 24) || ((long long)M + 63) / 64 * ((N + 127) / 128) >= (1LL << 22))
+    return fail(ESM_ERR_SHAPE, "%s: M=%d N=%d too large", fn, M, N);
+  if (M == 0) return ok();
+  if (!x || !qp || !s || (!y == !parts)) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
+  if (x_st % 8 != 0 || (M > 1 && x_st < K)) return fail(ESM_ERR_ALIGN, "%s: row stride (a multiple of 8, >= K)", fn);
+  if (!aligned16(x) || !aligned16(qp) || !aligned16(y) || !aligned16(parts))
+    return fail(ESM_ERR_ALIGN, "%s: x, codes and outputs must be 16-byte aligned", fn);
+  const F8Ws w = f8_layout(M, K, N, y != nullptr);
+  if (parts && parts_bytes < (size_t)w.plan.splits * M * N * 4)
+    return fail(ESM_ERR_SHAPE, "%s: partials of %zu bytes, %zu needed", fn, parts_bytes, (size_t)w.plan.splits * M * N * 4);
+  if (w.total) {
+    if (!workspace || workspace_bytes < w.total)
+      return fail(ESM_ERR_SHAPE, "%s: workspace of %zu bytes, %zu needed", fn, workspace_bytes, w.total);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+      return fail(ESM_ERR_ALIGN, "%s: workspace must be 256-byte aligned", fn);
+  }
+  char* ws = static_cast<char*>(workspace);
+  esm::F8Args a{};
+  a.x = x, a.x_st = x_st, a.wq = qp, a.sw = s, a.y = y;
+  a.M = M, a.Mp = w.Mp, a.K = K, a.N = N, a.splits = w.plan.splits;
+  if (w.total) {
+    a.xq = reinterpret_cast<uint8_t*>(ws);
+    a.sx = reinterpret_cast<float*>(ws + w.sx);
+  }
+  a.part = parts ? parts : w.plan.splits > 1 ? reinterpret_cast<float*>(ws + w.part) : nullptr;
+  if (splits) *splits = w.plan.splits;
+  return hip_status(esm::launch_f8_linear(a, dtype == ESM_BF16, w.plan.form, (hipStream_t)stream), fn);
+}
+}  // namespace
+
+size_t f8_linear_workspace_bytes(int M, int K, int N) {
+  return f8_shape(M, K, N) && M > 0 ? f8_layout(M, K, N, true).total : 0;
+}
+
+int f8_linear(const void* x, int64_t x_st, const uint8_t* qp, const float* s, void* y, int M, int K, int N, int dtype,
+              void* workspace, size_t workspace_bytes, void* stream) {
+  return f8_run("f8_linear", x, x_st, qp, s, y, nullptr, 0, nullptr, M, K, N, dtype, workspace, workspace_bytes, stream);
+}
+
+size_t f8_linear_partials_bytes(int M, int K, int N) {
+  return f8_shape(M, K, N) && M > 0 ? (size_t)esm::f8_plan(M, K, N, cu_count()).splits * M * N * 4 : 0;
+}
+
+int f8_linear_partials(const void* x, int64_t x_st, const uint8_t* qp, const float* s, float* parts, size_t parts_bytes,
+                       int* splits, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  if (!splits) return fail(ESM_ERR_NULL, "f8_linear_partials: NULL split count");
+  return f8_run("f8_linear_partials", x, x_st, qp, s, nullptr, parts, parts_bytes, splits, M, K, N, dtype, workspace,
+                workspace_bytes, stream);
+}
+
 // The pieces of esmc_block's workspace, each 256-byte aligned: qkv, q, k, v, the attention's output, the
 // residual and its LayerNorm between the halves, the gated FFN rows, and the split-K partials of whichever
 // linear runs.

@@ -1,0 +1,414 @@
+// Linear with weights in e4m3 (one fp32 scale per 128 x 128 block) on the fp8 matrix cores:
+//   r = 448 / max(amax, 2^-96), xq = e4m3(x r), sx = max(amax, 2^-96) / 448   per row of x and 128 columns
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in b} xq[m, k] wq[n, k]
+// The inner sums run in v_mfma_f32_16x16x128_f8f6f4, whose depth is one scale block: each result is taken with
+// its two scales into an fp32 accumulator. Rounded are x (to e4m3, the operator's definition), y, and what the
+// matrix core cuts: it aligns 8 consecutive products to the largest's exponent and drops what lies 13 binary places
+// below (measured; v_mfma_f32_16x16x32_fp8_fp8 does the same at a third of the rate, 1.39 against 4.46 PFLOP/s), about
+// 2^-12 of y, below half a step of fp16; from there on sums are fp32.
+//
+// Both operands are kept in the order of the matrix core's fragments, so every load is 1 KB of consecutive bytes
+// and LDS reads have no bank conflicts:
+//   codes: 64 weight rows x 128 k = 8 KB pieces [N / 64][K / 128][4 j][2][64 lanes][16 bytes]; lane l of fragment j
+//     holds weight row 16 ((l % 16) / 4) + 4 j + l % 4 of the 64, k = 32 (l / 16) + 16 half .. + 15. With the rows
+//     dealt that way the four fragments leave a lane 16 consecutive outputs of one row of x.
+//   x: 16 rows x 128 k = 2 KB pieces [M / 16][K / 128][2][64 lanes][16 bytes], the same k order.
+// Up to 16 rows of x one launch does it all (f8_few_kernel: bound by the codes' bytes); beyond, x goes through
+// f8_quantize_kernel and f8_gemm_kernel, tiles through LDS by loads that write it directly, K split over
+// workgroups where the tiles do not fill the GPU.
+#include <type_traits>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace esm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kF8Top = 448.f, kF8Floor = 0x1p-96f;
+
+// e4m3 x e4m3 -> fp32, 16 x 16 x 128 (a: 16 weight rows, b: 16 rows of x; 32 bytes a lane each). Result: column
+// (row of x) lane % 16, rows 4 (lane / 16) + register.
+DEV f32x4 mfma_f8(i32x8 a, i32x8 b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+
+// Largest magnitude of 8 values as their 16-bit pattern without the sign: NaN above infinity above the rest.
+DEV uint32_t top_bits(u16x8 v) {
+  u16x8 a = v & (uint16_t)0x7fff;
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) m = max(m, (uint32_t)a[e]);
+  return m;
+}
+template <class V8>
+DEV float bits_value(uint32_t b) {
+  V8 v{};
+  u16x8 u = __builtin_bit_cast(u16x8, v);
+  u[0] = (uint16_t)b;
+  return (float)__builtin_bit_cast(V8, u)[0];
+}
+// The factor to e4m3 and the scale back, from a block's largest magnitude (a NaN or infinity makes both rows NaN).
+DEV void f8_scale(float top, float& r, float& s) {
+  top = top < kF8Floor ? kF8Floor : top;
+  r = kF8Top / top;
+  s = top / kF8Top;
+}
+// 8 values times r as 8 codes (round to nearest even; r keeps them within 448).
+template <class V8>
+DEV void f8_codes(V8 v, float r, int& lo, int& hi) {
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32((float)v[0] * r, (float)v[1] * r, 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32((float)v[2] * r, (float)v[3] * r, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32((float)v[4] * r, (float)v[5] * r, 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32((float)v[6] * r, (float)v[7] * r, hi, true);
+}
+
+// ---- x to e4m3 --------------------------------------------------------------------------------
+// A thread takes 16 values, the 8 threads of a row's block share its maximum; a wave covers 8 rows x 128.
+template <class V8>
+__global__ __launch_bounds__(256) void f8_quantize_kernel(const uint16_t* __restrict__ x, long long st, uint8_t* __restrict__ xq,
+                                                          float* __restrict__ sx, int M, int K, int Mp) {
+  const int Kb = (K + 127) / 128, t = threadIdx.x;
+  const int c = t & 7, m = 32 * blockIdx.x + (t >> 3), kb = blockIdx.y, k = 128 * kb + 16 * c;
+  if (m >= Mp) return;
+  u16x8 a{}, b{};
+  if (m < M && k < K) {
+    const u16x8* src = reinterpret_cast<const u16x8*>(x + m * st + k);
+    a = src[0];
+    b = src[1];
+  }
+  uint32_t top = max(top_bits(a), top_bits(b));
+  const auto other = [&](auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  top = max(top, other(std::integral_constant<int, 0xB1>{}));   // quad_perm(1, 0, 3, 2)
+  top = max(top, other(std::integral_constant<int, 0x4E>{}));   // quad_perm(2, 3, 0, 1)
+  top = max(top, other(std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  float r, s;
+  f8_scale(bits_value<V8>(top), r, s);
+  int q[4];
+  f8_codes(__builtin_bit_cast(V8, a), r, q[0], q[1]);
+  f8_codes(__builtin_bit_cast(V8, b), r, q[2], q[3]);
+  uint8_t* dst = xq + ((size_t)(m >> 4) * Kb + kb) * 2048 + (c & 1) * 1024 + (16 * (c >> 1) + (m & 15)) * 16;
+  *reinterpret_cast<i32x4*>(dst) = i32x4{q[0], q[1], q[2], q[3]};
+  if (c == 0) sx[(size_t)kb * Mp + m] = s;
+}
+
+// ---- few rows: everything in one launch ------------------------------------------------------------
+// A workgroup takes 16 NJ weight rows for all (at most 16) rows of x; its 8 waves deal the blocks of 128 k among
+// them, bring x to e4m3 in registers (32 values of one row a lane) and sum through LDS.
+constexpr int kFewWaves = 8;
+template <class V8, int NJ>
+__global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
+  __shared__ float red[kFewWaves][16][16 * NJ];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Kb = (p.K + 127) / 128;
+  const int ng = blockIdx.x / (4 / NJ), j0 = blockIdx.x % (4 / NJ) * NJ;  // 64-row piece, first fragment in it
+  const int m = lane & 15, kl = 32 * (lane >> 4);
+  const uint8_t* wp = p.wq + ((size_t)ng * Kb) * 8192 + j0 * 2048 + lane * 16;
+  const uint16_t* xr = (const uint16_t*)p.x + m * p.x_st;
+  const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
+  f32x4 acc[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < Kb; kb += kFewWaves) {
+    i32x8 w[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(wp + (size_t)kb * 8192 + j * 2048);
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(wp + (size_t)kb * 8192 + j * 2048 + 1024);
+      w[j] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+    u16x8 x[4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int k = 128 * kb + kl + 8 * i;
+      x[i] = u16x8{};
+      if (m < p.M && k < p.K) x[i] = *reinterpret_cast<const u16x8*>(xr + k);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, top_bits(x[i]));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    float r, s;
+    f8_scale(bits_value<V8>(top), r, s);
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) f8_codes(__builtin_bit_cast(V8, x[i]), r, q[2 * i], q[2 * i + 1]);
+    const i32x8 xf = {q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]};
+    s *= sw[kb];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const f32x4 d = mfma_f8(w[j], xf);
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[j][e] = fmaf(s, d[e], acc[j][e]);
+    }
+  }
+  // lane's outputs: row m, weight rows 16 (lane / 16) + 4 (j0 + j) + e of the piece -> column 4 NJ (lane / 16) + 4 j + e
+#pragma unroll
+  for (int j = 0; j < NJ; j++)
+    *reinterpret_cast<f32x4*>(&red[wave][m][4 * NJ * (lane >> 4) + 4 * j]) = acc[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * 16 * NJ; i += 64 * kFewWaves) {
+    const int mm = i / (16 * NJ), c = i % (16 * NJ);
+    float sum = red[0][mm][c];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; w++) sum += red[w][mm][c];
+    const int n = 64 * ng + 16 * (c / (4 * NJ)) + 4 * j0 + c % (4 * NJ);
+    if (mm < p.M && n < p.N) {
+      if (p.part)
+        p.part[(size_t)mm * p.N + n] = sum;
+      else {
+        V8 v{};
+        v[0] = (decltype(+v[0]))sum;
+        ((uint16_t*)p.y)[(size_t)mm * p.N + n] = __builtin_bit_cast(u16x8, v)[0];
+      }
+    }
+  }
+}
+
+// ---- many rows ----------------------------------------------------------------------------------
+// Workgroup tile of 16 MB WM rows of x by 64 WN weight rows, WM x WN waves of 16 MB x 64 each. A step is one
+// block of 128 k: x and weight pieces and each wave's row scales come by direct loads into a ring of S slots.
+template <class V8, int MB, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
+  constexpr int NW = WM * WN, kX = 2048 * MB * WM, kW = 8192 * WN, kScales = 64 * MB;  // bytes a slot
+  constexpr int kSlot = kX + kW + NW * kScales;
+  constexpr int kLoadsX = kX / 1024 / NW, kLoadsW = kW / 1024 / NW, kLoads = kLoadsX + kLoadsW + 1;
+  static_assert(kLoadsX * NW * 1024 == kX && kLoadsW * NW * 1024 == kW, "whole loads per wave");
+  static_assert((S - 2) * kLoads < 64, "loads in flight the counter can tell");
+  __shared__ __align__(1024) char lds[S * kSlot];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN, Kb = (p.K + 127) / 128;
+  // workgroups in groups of 8 row tiles, so that those running together share both operands' pieces in L2
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int tiles = p.mtiles * p.ntiles, split = t / tiles;
+  t -= split * tiles;
+  const int group = t / (8 * p.ntiles), in = t - group * 8 * p.ntiles, gm = min(8, p.mtiles - 8 * group);
+  const int mt = 8 * group + in % gm, nt = in / gm;
+  const int kb0 = (int)((long long)Kb * split / p.splits), kb1 = (int)((long long)Kb * (split + 1) / p.splits);
+  const int mb0 = mt * MB * WM, ng0 = nt * WN, Mb = p.Mp / 16, Ng = (p.N + 63) / 64;
+  const dma_src_t rx = dma_src(p.xq + (size_t)mb0 * Kb * 2048, (uint32_t)min(MB * WM, Mb - mb0) * (uint32_t)Kb * 2048u);
+  const dma_src_t rw = dma_src(p.wq + (size_t)ng0 * Kb * 8192, (uint32_t)min(WN, Ng - ng0) * (uint32_t)Kb * 8192u);
+  const int row0 = 16 * (mb0 + MB * wm);  // this wave's first row
+  const dma_src_t rs = dma_src(p.sx + min(row0, p.Mp), (uint32_t)(4 * max(p.Mp - row0, 0)) + 4u * (uint32_t)p.Mp * (uint32_t)(Kb - 1));
+  const uint32_t base = lds_address(lds);
+  const auto load = [&](int kb, int slot) {
+    const uint32_t at = base + slot * kSlot;
+#pragma unroll
+    for (int i = 0; i < kLoadsX; i++) {
+      const int u = wave * kLoadsX + i;  // KB of the slot: row block u / 2, half u % 2
+      dma16(rx, at + 1024 * u, (uint32_t)((u >> 1) * Kb + kb) * 2048u + 1024u * (u & 1) + 16 * lane, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoadsW; i++) {
+      const int u = wave * kLoadsW + i;
+      dma16(rw, at + kX + 1024 * u, (uint32_t)((u >> 3) * Kb + kb) * 8192u + 1024u * (u & 7) + 16 * lane, 0);
+    }
+    if (lane < 4 * MB) dma16(rs, at + kX + kW + kScales * wave, 4u * (uint32_t)p.Mp * (uint32_t)kb + 16 * lane, 0);
+  };
+  f32x4 acc[MB][4];
+#pragma unroll
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float* sw = p.sw + (size_t)(min(ng0 + wn, Ng - 1) >> 1) * Kb;
+  const int n = kb1 - kb0;
+#pragma unroll
+  for (int i = 0; i < S - 1; i++) load(min(kb0 + i, kb1 - 1), i);  // (past the last block: loaded again, not used)
+  for (int i = 0, slot = 0; i < n; i++, slot = slot + 1 == S ? 0 : slot + 1) {
+    constexpr int kLeft = (S - 2) * kLoads;
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (kLeft & 15) | ((kLeft >> 4) << 14));  // vmcnt(kLeft): this block's loads are in
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+    load(min(kb0 + i + S - 1, kb1 - 1), slot == 0 ? S - 1 : slot - 1);
+    const char* at = lds + slot * kSlot;
+    const float swk = sw[kb0 + i];
+    i32x8 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const char* src = at + kX + 8192 * wn + 2048 * j + 16 * lane;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
+      w[j] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++) {
+      const char* src = at + 2048 * (MB * wm + b) + 16 * lane;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
+      const i32x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const float s = swk * *reinterpret_cast<const float*>(at + kX + kW + kScales * wave + 4 * (16 * b + (lane & 15)));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x4 d = mfma_f8(w[j], x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[b][j][e] = fmaf(s, d[e], acc[b][j][e]);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this slot's reads are back before the next barrier frees it
+    __asm__ volatile("" ::: "memory");
+  }
+  wait_vm(0);  // no load of this workgroup outlives it
+  // lane: row lane % 16 of each block, columns 16 (lane / 16) .. + 15 of the 64
+  const int col = 64 * (ng0 + wn) + 16 * (lane >> 4);
+#pragma unroll
+  for (int b = 0; b < MB; b++) {
+    const int m = row0 + 16 * b + (lane & 15);
+    if (m >= p.M) continue;
+    if (p.part) {
+      float* dst = p.part + ((size_t)split * p.M + m) * p.N + col;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (col + 4 * j < p.N) *reinterpret_cast<f32x4*>(dst + 4 * j) = acc[b][j];
+    } else {
+      uint16_t* dst = (uint16_t*)p.y + (size_t)m * p.N + col;
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        V8 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          v[e] = (decltype(+v[e]))acc[b][j][e];
+          v[4 + e] = (decltype(+v[e]))acc[b][j + 1][e];
+        }
+        if (col + 4 * j < p.N) *reinterpret_cast<V8*>(dst + 4 * j) = v;
+      }
+    }
+  }
+}
+
+// Sum of the splits in their order, one rounding.
+template <class V8>
+__global__ __launch_bounds__(256) void f8_reduce_kernel(const float* __restrict__ part, uint16_t* __restrict__ y, size_t n8, int splits) {
+  for (size_t c = (size_t)blockIdx.x * 256 + threadIdx.x; c < n8; c += (size_t)gridDim.x * 256) {
+    f32x4 a = *reinterpret_cast<const f32x4*>(part + 8 * c), b = *reinterpret_cast<const f32x4*>(part + 8 * c + 4);
+    for (int s = 1; s < splits; s++) {
+      const float* src = part + 8 * (c + s * n8);
+      a += *reinterpret_cast<const f32x4*>(src);
+      b += *reinterpret_cast<const f32x4*>(src + 4);
+    }
+    V8 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      v[e] = (decltype(+v[e]))a[e];
+      v[4 + e] = (decltype(+v[e]))b[e];
+    }
+    *reinterpret_cast<V8*>(y + 8 * c) = v;
+  }
+}
+
+// ---- weights ------------------------------------------------------------------------------------
+// Codes [N, K] into the fragment order, zeros past N and K: a thread writes 16 bytes.
+__global__ __launch_bounds__(256) void f8_pack_kernel(const uint8_t* __restrict__ q, uint8_t* __restrict__ out, int N, int K) {
+  const int Kb = (K + 127) / 128;
+  const size_t total = (size_t)((N + 63) / 64) * Kb * 512;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    const int u = (int)(i % 512), l = u & 63, half = (u >> 6) & 1, j = u >> 7;
+    const size_t piece = i / 512;
+    const int kb = (int)(piece % Kb);
+    const size_t n = 64 * (piece / Kb) + 16 * ((l & 15) >> 2) + 4 * j + (l & 3);
+    const int k = 128 * kb + 32 * (l >> 4) + 16 * half;
+    i32x4 v = {0, 0, 0, 0};
+    if (n < (size_t)N && k < K) v = *reinterpret_cast<const i32x4*>(q + n * K + k);
+    *reinterpret_cast<i32x4*>(out + 16 * i) = v;
+  }
+}
+
+// fp32 weights to codes and scales, a workgroup per 128 x 128 block (the same rule as x's blocks of a row, the
+// scale rounded to fp32 before it divides, as other tools make such weights).
+__global__ __launch_bounds__(256) void f8_quantize_weight_kernel(const float* __restrict__ w, uint8_t* __restrict__ q,
+                                                                 float* __restrict__ sw, int N, int K) {
+  __shared__ uint32_t red[4];
+  const int Kb = (K + 127) / 128, kb = blockIdx.x % Kb, nb = blockIdx.x / Kb, t = threadIdx.x;
+  const int k = 128 * kb + 4 * (t & 31), n0 = 128 * nb + (t >> 5);
+  uint32_t top = 0;
+  for (int i = 0; i < 16; i++) {
+    const int n = n0 + 8 * i;
+    if (n >= N || k >= K) continue;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(w + (size_t)n * K + k);
+#pragma unroll
+    for (int e = 0; e < 4; e++) top = max(top, v[e] & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  if ((t & 63) == 0) red[t >> 6] = top;
+  __syncthreads();
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  float r, s;
+  f8_scale(__builtin_bit_cast(float, top), r, s);
+  if (t == 0) sw[blockIdx.x] = s;
+  for (int i = 0; i < 16; i++) {
+    const int n = n0 + 8 * i;
+    if (n >= N || k >= K) continue;
+    const f32x4 v = *reinterpret_cast<const f32x4*>(w + (size_t)n * K + k);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] / s, v[1] / s, 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] / s, v[3] / s, c, true);
+    *reinterpret_cast<int*>(q + (size_t)n * K + k) = c;
+  }
+}
+
+template <class V8, int MB, int WM, int WN, int S>
+static hipError_t launch_gemm(F8Args a, hipStream_t s) {
+  a.mtiles = (a.M + 16 * MB * WM - 1) / (16 * MB * WM);
+  a.ntiles = (a.N + 64 * WN - 1) / (64 * WN);
+  ESM_LAUNCH((f8_gemm_kernel<V8, MB, WM, WN, S>), dim3((unsigned)((size_t)a.mtiles * a.ntiles * a.splits)), dim3(64 * WM * WN), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class V8>
+static hipError_t launch_f8_t(const F8Args& a, int form, hipStream_t s) {
+  hipError_t e;
+  if (form == kF8Few) {
+    ESM_LAUNCH((f8_few_kernel<V8, 2>), dim3((a.N + 63) / 64 * 2), dim3(64 * kFewWaves), 0, s, a);
+    return hipGetLastError();
+  }
+  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, (a.K + 127) / 128), dim3(256), 0, s, (const uint16_t*)a.x, a.x_st,
+             a.xq, a.sx, a.M, a.K, a.Mp);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (form == kF8Big)
+    e = launch_gemm<V8, 8, 2, 4, 2>(a, s);
+  else
+    e = launch_gemm<V8, 2, 2, 2, 4>(a, s);
+  if (e != hipSuccess || !a.part || !a.y) return e;
+  const size_t n8 = (size_t)a.M * a.N / 8, blocks = (n8 + 255) / 256;
+  ESM_LAUNCH((f8_reduce_kernel<V8>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a.part, (uint16_t*)a.y, n8,
+             a.splits);
+  return hipGetLastError();
+}
+
+hipError_t launch_f8_linear(const F8Args& a, bool bf16, int form, hipStream_t s) {
+  return bf16 ? launch_f8_t<bf16x8>(a, form, s) : launch_f8_t<half8>(a, form, s);
+}
+
+F8Plan f8_plan(int M, int K, int N, int cus) {
+  F8Plan p{kF8Few, 1};
+  if (M <= 16) return p;
+  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
+  if (big >= cus * 3 / 4) {
+    p.form = kF8Big;
+    return p;
+  }
+  p.form = kF8Mid;
+  const long long tiles = (long long)((M + 63) / 64) * ((N + 127) / 128);
+  const int Kb = (K + 127) / 128;
+  long long sp = 2 * cus / tiles;
+  sp = sp < Kb / 4 ? sp : Kb / 4;
+  p.splits = (int)(sp < 1 ? 1 : sp > kF8MaxSplits ? kF8MaxSplits : sp);
+  return p;
+}
+
+hipError_t launch_f8_pack(const uint8_t* q, uint8_t* out, int N, int K, hipStream_t s) {
+  const size_t blocks = ((size_t)((N + 63) / 64) * ((K + 127) / 128) * 512 + 255) / 256;
+  ESM_LAUNCH(f8_pack_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, q, out, N, K);
+  return hipGetLastError();
+}
+
+hipError_t launch_f8_quantize_weight(const float* w, uint8_t* q, float* sw, int N, int K, hipStream_t s) {
+  ESM_LAUNCH(f8_quantize_weight_kernel, dim3((unsigned)((size_t)((N + 127) / 128) * ((K + 127) / 128))), dim3(256), 0, s, w, q, sw, N, K);
+  return hipGetLastError();
+}
+
+}  // namespace esm

@@ -189,6 +189,24 @@ struct AttnPlan {
   int splits;
 };
 
+struct F8Args {
+  const void* x;          // [M, K], 16-bit, rows x_st elements apart
+  long long x_st;
+  const uint8_t* wq;      // codes in fragment order (f8_pack_codes)
+  const float* sw;        // [ceil(N / 128), ceil(K / 128)]
+  void* y;                // [M, N] 16-bit, or nullptr: partials only
+  float* part;            // [splits, M, N] fp32, or nullptr: y straight away (splits 1)
+  uint8_t* xq;            // x in fragment order, Mp rows (more than 16 rows)
+  float* sx;              // [ceil(K / 128), Mp]
+  int M, Mp, K, N;        // Mp: M rounded up to 16
+  int splits, mtiles, ntiles;
+};
+constexpr int kF8MaxSplits = 16;
+enum : int { kF8Few = 0, kF8Mid = 1, kF8Big = 2 };
+struct F8Plan {
+  int form, splits;
+};
+
 struct ParcaeArgs {
   const float* z;         // [cells, C] recurrent state
   const float* z_init;    // [cells, C]
@@ -276,6 +294,11 @@ bool qk_norm_rope_row_fits(int heads, int d);  // whether one workgroup takes a 
 hipError_t launch_qk_norm_rope(QkRopeArgs a, bool bf16, bool row, hipStream_t s);
 AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus);
 hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s);
+F8Plan f8_plan(int M, int K, int N, int cus);
+hipError_t launch_f8_linear(const F8Args& a, bool bf16, int form, hipStream_t s);
+constexpr size_t f8_packed_size(int N, int K) { return (size_t)((N + 63) / 64) * ((K + 127) / 128) * 8192; }
+hipError_t launch_f8_pack(const uint8_t* q, uint8_t* out, int N, int K, hipStream_t s);
+hipError_t launch_f8_quantize_weight(const float* w, uint8_t* q, float* sw, int N, int K, hipStream_t s);
 hipError_t launch_q8_pack(const half_t* s, const half_t* b, uint32_t* sb, int N, int K, hipStream_t st);
 // Bytes of q8_pack_codes' layout: per 32-row block and step of two groups, 4 waves x 64
 // lanes x 16 bytes.

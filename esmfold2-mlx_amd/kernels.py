@@ -626,3 +626,88 @@ def q8_dequant(q, s, b, group: int = 64):
     capi.check(lib.q8_dequant(q.data_ptr(), _dev(s, "s", F16).data_ptr(), _dev(b, "b", F16).data_ptr(),
                               w.data_ptr(), N, K, group, capi.stream_ptr()))
     return w
+
+
+def f8_pack_codes(q):
+    """e4m3 codes [N, K] (uint8 or float8_e4m3fn) in the order ``f8_linear``'s matrix-core fragments take them."""
+    lib = capi.lib()
+    _dev(q, "q")
+    if q.dim() != 2 or q.element_size() != 1:
+        raise capi.EsmError(-2, f"f8_pack_codes: q must be 8-bit codes [N, K], got {q.dtype} {tuple(q.shape)}")
+    N, K = q.shape
+    qp = torch.empty(int(lib.f8_packed_codes_bytes(N, K)), dtype=torch.uint8, device=q.device)
+    with _on(q.device):
+        capi.check(lib.f8_pack_codes(q.data_ptr(), qp.data_ptr(), N, K, capi.stream_ptr()))
+    return qp
+
+
+def f8_quantize_weight(w):
+    """fp32 W [N, K] -> (codes uint8 [N, K] of e4m3, scales fp32 [ceil(N / 128), ceil(K / 128)]), a scale per 128 x
+    128 block: its largest magnitude (at least 2^-96) becomes 448."""
+    lib = capi.lib()
+    _dev(w, "w", torch.float32)
+    if w.dim() != 2:
+        raise capi.EsmError(-2, f"f8_quantize_weight: w must be [N, K], got {tuple(w.shape)}")
+    N, K = w.shape
+    q = torch.empty(N, K, dtype=torch.uint8, device=w.device)
+    s = torch.empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
+    with _on(w.device):
+        capi.check(lib.f8_quantize_weight(w.data_ptr(), q.data_ptr(), s.data_ptr(), N, K, capi.stream_ptr()))
+    return q, s
+
+
+def _f8_operands(x, codes, scales, N, fn):
+    """The checks of ``f8_linear``'s operands on the host: (M, K, row stride of x)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise capi.EsmError(-5, f"{fn}: x must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
+    if x.dim() != 2 or x.dtype not in _DTYPES:
+        raise capi.EsmError(-2, f"{fn}: x must be [rows, K] in fp16 or bf16, got {x.dtype} {tuple(x.shape)}")
+    M, K = x.shape
+    if K > 1 and x.stride(1) != 1:
+        raise capi.EsmError(-3, f"{fn}: the values of a row must be contiguous")
+    _aux(codes, "codes", (torch.uint8,), x.device)
+    _aux(scales, "scales", (torch.float32,), x.device)
+    if codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128):
+        raise capi.EsmError(-2, f"{fn}: {codes.numel()} packed codes and {scales.numel()} scales for [{N}, {K}]")
+    return M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8
+
+
+def f8_linear(x, codes, scales, N: int, out=None):
+    """y = x . W^T on the fp8 matrix cores: x [M, K] fp16 or bf16 (rows may lie apart), brought to e4m3 with a scale
+    per row and 128 columns; W [N, K] as packed e4m3 codes (``f8_pack_codes``) with an fp32 scale per 128 x 128 block;
+    fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch."""
+    lib = capi.lib()
+    M, K, st = _f8_operands(x, codes, scales, N, "f8_linear")
+    if out is None:
+        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    else:
+        y = _out(out, "out", x.dtype, M * N)
+        if y.device != x.device:
+            raise capi.EsmError(-5, f"out must be on {x.device}")
+    with _on(x.device):
+        need = int(lib.f8_linear_workspace_bytes(M, K, N))
+        with scratch.guard(x.device, need):
+            ws, wp, stream = scratch.take(need, x.device) if need else (None, None, capi.stream_ptr())
+            capi.check(lib.f8_linear(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N,
+                                     _DTYPES[x.dtype], wp, need, stream))
+    return y
+
+
+def f8_linear_partials(x, codes, scales, N: int):
+    """``f8_linear`` without the last rounding: (partials [splits, M, N] fp32, splits, scratch generation). Rounded
+    to x's type, their sum in split order is ``f8_linear``'s result. The view lives in the device's shared scratch,
+    valid until its next user (the caller holds ``scratch.guard``)."""
+    lib = capi.lib()
+    M, K, st = _f8_operands(x, codes, scales, N, "f8_linear_partials")
+    splits = ctypes.c_int(0)
+    with _on(x.device), scratch.guard(x.device):
+        nparts = int(lib.f8_linear_partials_bytes(M, K, N))
+        need = int(lib.f8_linear_workspace_bytes(M, K, N))
+        at = (nparts + 255) // 256 * 256
+        buf = scratch.get(at + need, x.device)
+        gen = scratch.generation(x.device)
+        capi.check(lib.f8_linear_partials(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), buf.data_ptr(), nparts,
+                                          ctypes.byref(splits), M, K, N, _DTYPES[x.dtype], buf.data_ptr() + at, need,
+                                          capi.stream_ptr()))
+    n = splits.value
+    return buf[:4 * n * M * N].view(torch.float32).view(n, M, N), n, gen

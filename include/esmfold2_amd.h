@@ -373,6 +373,32 @@ int q8_linear_swiglu_packed_ws(const esm_half* x, const uint8_t* qp, const uint3
                                int N, int group, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Linear with weights in 8-bit floating point (e4m3, one fp32 scale per 128 x 128 block), on the fp8 matrix cores:
+ *   y[m, n] = sum over blocks b of 128 k: sx[m, b] s[n / 128, b] sum_{k in b} xq[m, k] q[n, k]
+ * with x brought to e4m3 by rows and blocks: t = max(max |x|, 2^-96), sx = t / 448, xq = e4m3(x * (448 / t)), in fp32,
+ * to nearest even (a row's block that holds an infinity or a NaN makes the row NaN). Sums are fp32, but that the matrix core aligns 8 consecutive
+ * products to the largest and drops what lies 13 binary places below its exponent (7 2^-13 of that product at most).
+ * x [M, K] fp16 or bf16 (dtype, below), rows x_st elements apart (a multiple of 8, >= K); y [M, N] of the same type;
+ * s [ceil(N / 128), ceil(K / 128)]; K % 16 == 0, K <= 2^20, N % 8 == 0. The codes are taken in the kernel's fragment
+ * order, made once per layer by f8_pack_codes from q [N, K] (f8_packed_codes_bytes bytes). workspace:
+ * f8_linear_workspace_bytes bytes, 256-byte aligned (0 up to 16 rows).
+ * f8_linear_partials writes the fp32 sums of each K range instead, parts [splits, M, N] of
+ * f8_linear_partials_bytes bytes: rounded to x's type, their sum in split order is f8_linear's y (for
+ * esmc_layer_norm_parts). f8_quantize_weight: w [N, K] fp32 -> q [N, K], s, a block's s = max(max |w|, 2^-96) / 448 and
+ * q = e4m3(w / s).
+ */
+size_t f8_packed_codes_bytes(int N, int K);
+int f8_pack_codes(const uint8_t* q, uint8_t* qp, int N, int K, void* stream);
+int f8_quantize_weight(const float* w, uint8_t* q, float* s, int N, int K, void* stream);
+size_t f8_linear_workspace_bytes(int M, int K, int N);
+int f8_linear(const void* x, int64_t x_st, const uint8_t* qp, const float* s, void* y, int M, int K, int N, int dtype,
+              void* workspace, size_t workspace_bytes, void* stream);
+size_t f8_linear_partials_bytes(int M, int K, int N);
+int f8_linear_partials(const void* x, int64_t x_st, const uint8_t* qp, const float* s, float* parts, size_t parts_bytes,
+                       int* splits, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
  * The ESMC transformer block's other kernels (mlx_esmc.py:84-102), around q8_linear.
  *
  * esmc_layer_norm: with y, x_out = x + alpha * y (fp32 residual, y fp16: the scaled

@@ -25,7 +25,7 @@ def test_qk_norm_rope_refusals(lib):
     for kw in (dict(T=-1), dict(H=0), dict(Hk=0), dict(d=0), dict(rot=80), dict(eps=-1.0), dict(eps=math.nan),
                dict(T=1 << 22)):
         assert _rope(lib, **kw) == -2, kw
-    for kw in (dict(d=60), dict(d=264), dict(rot=24), dict(norm=3), dict(dtype=2), dict(H=1030, row=1)):
+    for kw in (dict(d=60, rot=48), dict(d=264), dict(rot=24), dict(norm=3), dict(dtype=2), dict(H=1030, row=1)):
         assert _rope(lib, **kw) == -4, kw
     for kw in (dict(st=60), dict(st=32), dict(sh=4), dict(sh=-64), dict(st=1 << 24), dict(q=ODD), dict(w=ODD),
                dict(freq=ODD)):
@@ -82,3 +82,28 @@ def test_rotary_frequencies(pkg):
     for bad in (dict(head_dim=60), dict(head_dim=264), dict(head_dim=64, rot_dim=24), dict(head_dim=64, rot_dim=80)):
         with pytest.raises(ValueError):
             pkg.rotary.Rotary(device="cpu", **bad)
+
+
+def test_f8_refusals(lib):
+    def linear(M=4, K=256, N=128, st=256, dtype=0, x=P, y=P, ws=None, n=0):
+        return lib.f8_linear(x, st, P, P, y, M, K, N, dtype, ws, n, None)
+
+    assert linear(M=0) == 0
+    for kw in (dict(M=-1), dict(K=0), dict(K=250), dict(N=0), dict(N=100), dict(K=1 << 21, st=1 << 21),
+               dict(M=1 << 23, N=1 << 20)):
+        assert linear(**kw) == -2, kw
+    assert linear(dtype=2) == -4
+    for kw in (dict(st=260), dict(st=128), dict(x=ODD), dict(y=ODD)):
+        assert linear(**kw) == -3, kw
+    assert linear(x=None) == -1 and linear(y=None) == -1
+    need = lib.f8_linear_workspace_bytes(238, 5120, 2560)
+    assert need > 238 * 5120 and lib.f8_linear_workspace_bytes(16, 5120, 2560) == 0
+    assert linear(M=238, K=5120, N=2560, st=5120, ws=P, n=need - 1) == -2
+    assert linear(M=238, K=5120, N=2560, st=5120, ws=ctypes.c_void_p((1 << 20) + 16), n=need) == -3
+    splits = ctypes.c_int(7)
+    assert lib.f8_linear_partials(P, 256, P, P, P, 16, ctypes.byref(splits), 4, 256, 128, 0, None, 0, None) == -2
+    assert splits.value == 0
+    assert lib.f8_linear_partials(P, 256, P, P, P, 1 << 20, None, 4, 256, 128, 0, None, 0, None) == -1
+    assert lib.f8_packed_codes_bytes(65, 129) == 0 and lib.f8_packed_codes_bytes(72, 144) == 2 * 2 * 8192
+    assert lib.f8_pack_codes(None, P, 64, 128, None) == -1 and lib.f8_pack_codes(P, P, 64, 100, None) == -2
+    assert lib.f8_quantize_weight(None, P, P, 64, 128, None) == -1
