@@ -3,7 +3,7 @@
 //
 // The rows a workgroup takes are (query, head of the group) pairs of one sequence and key head, row = query * G +
 // head: the group's heads share every key and value that is staged, and a single new token's heads fill a
-// tile together. A key tile in LDS is used by a wave for 32 QB rows:
+// tile together. A wave holds 32 rows and takes 32 keys from LDS at a time:
 //   S^T[key][row] = K Q^T       (A: K rows from LDS, B: the wave's query fragments, in registers)
 //   p = 2^(S c - m c), l += p   (a lane holds one row: the maximum is over its registers and one exchange)
 //   O^T[d][row] += V^T P^T      (A: V^T by the transposing LDS read, B: p in the accumulator's own key order)
@@ -11,8 +11,8 @@
 // step of that type on each p, below the output's own rounding after the sum). m is the running maximum; it, O
 // and l are rescaled only when a row's maximum has grown by more than 2^8 since (p then reaches 2^8 at most).
 //
-// Two kernels share that step: packed_attention_kernel (many rows: four waves of 32 QB rows each over key
-// tiles they share, the next tile in flight) and split_attention_kernel (few rows: 32 rows, keys divided
+// Two kernels share that step: packed_attention_kernel (many rows: four waves of 32 rows over tiles of 64
+// keys that they share, the next tile in flight) and split_attention_kernel (few rows: 32 rows, keys divided
 // between the four waves and, through fp32 partials joined by a second launch, between workgroups).
 #include "common.h"
 #include "kernels.h"
@@ -28,15 +28,29 @@ struct Fp16 {
   typedef half8 v8;
   typedef half4 v4;
   typedef half_t elem;
-  static constexpr uint16_t kExp = 0x7c00, kOne = 0x3c00;
+  // exponent mask; 1, 128 and 129
+  static constexpr uint16_t kExp = 0x7c00, kOne = 0x3c00, kMany = 0x5800, kBoth = 0x5808;
   static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static DEV float add(v8 v, float s) {  // s + the sum of v, two exact products with 1 at a time
+    const half2v one = {(half_t)1.0f, (half_t)1.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2(half2v{v[i], v[i + 1]}, one, s, false);
+    return s;
+  }
 };
 struct Bf16 {
   typedef bf16x8 v8;
   typedef bf16x4 v4;
   typedef __bf16 elem;
-  static constexpr uint16_t kExp = 0x7f80, kOne = 0x3f80;
+  static constexpr uint16_t kExp = 0x7f80, kOne = 0x3f80, kMany = 0x4300, kBoth = 0x4301;
   static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static DEV float add(v8 v, float s) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    const v2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_fdot2_f32_bf16(v2{v[i], v[i + 1]}, one, s, false);
+    return s;
+  }
 };
 
 constexpr float kGrow = 8.f;  // log2 of what p may reach before its row is rescaled
@@ -62,152 +76,123 @@ DEV typename T::v8 v_frag(const char* vs, int j, int db, int lane) {  // keys 16
 }
 
 // One wave's rows: query fragments, running maximum (of the unscaled scores), sum (this lane's half of the keys)
-// and output. Row r of block qb is column lane % 32 = r of every accumulator.
-template <class T, int HD, int QB>
+// and output. Row r is column lane % 32 = r of every accumulator.
+template <class T, int HD>
 struct Rows {
-  typename T::v8 q[QB][HD / 16];
-  f32x16 o[QB][HD / 32];
-  float m[QB], l[QB];
-  int lim[QB];  // last key this row sees, counted within the sequence
+  typename T::v8 q[HD / 16];
+  f32x16 o[HD / 32];
+  float m, l;
+  int lim;  // last key this row sees, counted within the sequence
 
   DEV void init() {
+    m = -INFINITY;
+    l = 0.f;
+    odd = false;
 #pragma unroll
-    for (int b = 0; b < QB; b++) {
-      m[b] = -INFINITY;
-      l[b] = 0.f;
+    for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-      for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[b][d][i] = 0.f;
-    }
+      for (int i = 0; i < 16; i++) o[d][i] = 0.f;
   }
 
-  // Keys key0 .. key0 + 32 NKB - 1 of the sequence from LDS tiles ks, vs. masked: some row sees only a part
-  // of them. later: some of the unseen ones are the sequence's own later keys, whose values may be anything.
-  template <int NKB>
-  DEV void step(const char* ks, const char* vs, int key0, bool masked, bool later, float c, int lane) {
+  bool odd;  // values taken as 0 by a masked step (``add_odd`` makes up for the seen ones)
+
+  // Keys key0 .. key0 + 32 NKB - 1 of the sequence from LDS rows ks, vs. MASKED: some row sees only a part of them,
+  // and what the others hold must not count: their scores are replaced, and as a p of 0 does not silence an infinity or
+  // a NaN in V, all values that are one are taken as 0.
+  template <int NKB, bool MASKED>
+  DEV void step(const char* ks, const char* vs, int key0, float c, int lane) {
     const int r = lane & 31, h = lane >> 5;
-    f32x16 s[QB][NKB];
+    f32x16 s[NKB];
 #pragma unroll
-    for (int b = 0; b < QB; b++)
+    for (int kb = 0; kb < NKB; kb++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[kb][i] = 0.f;
+      const char* kr = ks + (32 * kb + r) * 2 * HD;
+#pragma unroll
+      for (int k = 0; k < HD / 16; k++)
+        s[kb] = T::mfma(*reinterpret_cast<const typename T::v8*>(kr + 16 * k_piece<HD>(r, 2 * k + h)), q[k], s[kb]);
+    }
+    if (MASKED) {
 #pragma unroll
       for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[b][kb][i] = 0.f;
+        for (int i = 0; i < 16; i++) s[kb][i] = key0 + 32 * kb + acc_row32(i, lane) <= lim ? s[kb][i] : -INFINITY;
+    }
+    float mx = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-      for (int k = 0; k < HD / 16; k++) {
-        const int n = 32 * kb + r;
-        const typename T::v8 kf = *reinterpret_cast<const typename T::v8*>(ks + n * 2 * HD + 16 * k_piece<HD>(n, 2 * k + h));
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kb][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any((mx - m) * c > kGrow)) {  // (from m = -inf at the first key a row sees)
+      const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+      const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-        for (int b = 0; b < QB; b++) s[b][kb] = T::mfma(kf, q[b][k], s[b][kb]);
-      }
-    if (masked) {
+      for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-      for (int b = 0; b < QB; b++)
-#pragma unroll
-        for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-          for (int i = 0; i < 16; i++)
-            s[b][kb][i] = key0 + 32 * kb + acc_row32(i, lane) <= lim[b] ? s[b][kb][i] : -INFINITY;
+        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
     }
-    typename T::v8 pf[QB][2 * NKB];
+    const float mc = MASKED && lim < key0 ? 0.f : m * c;  // (m may be -inf where no key has been seen)
+    typename T::v8 p[2 * NKB];
 #pragma unroll
-    for (int b = 0; b < QB; b++) {
-      float mx = -INFINITY;
+    for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-      for (int kb = 0; kb < NKB; kb++)
+      for (int i = 0; i < 16; i++)  // (results below 2^-126 flush)
+        p[2 * kb + (i >> 3)][i & 7] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -mc));
 #pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[b][kb][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (__any((mx - m[b]) * c > kGrow)) {  // (from m = -inf at the first key a row sees)
-        const float mn = fmaxf(m[b], mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f((m[b] - ref) * c);
-        m[b] = mn;
-        l[b] *= alpha;
-#pragma unroll
-        for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) o[b][d][i] *= alpha;
-      }
-      const float mc = m[b] == -INFINITY ? 0.f : m[b] * c;  // no key seen yet
-      float sum = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[b][kb][i], c, -mc));  // (results below 2^-126 flush)
-          sum += e;
-          pf[b][2 * kb + (i >> 3)][i & 7] = (typename T::elem)e;
-        }
-      l[b] += sum;
-    }
-    if (later && __any(unclean(vs, 32 * NKB, lane))) {
-      apart<NKB>(vs, key0, pf, lane);
-      return;
-    }
+    for (int j = 0; j < 2 * NKB; j++) l = T::add(p[j], l);
 #pragma unroll
     for (int j = 0; j < 2 * NKB; j++)
 #pragma unroll
       for (int d = 0; d < HD / 32; d++) {
-        const typename T::v8 vf = v_frag<T, HD>(vs, j, d, lane);
-#pragma unroll
-        for (int b = 0; b < QB; b++) o[b][d] = T::mfma(vf, pf[b][j], o[b][d]);
+        typename T::v8 v = v_frag<T, HD>(vs, j, d, lane);
+        if (MASKED) v = finite(v);
+        o[d] = T::mfma(v, p[j], o[d]);
       }
   }
 
-  // Whether this lane's share of the value tile holds an infinity or a NaN.
-  static DEV bool unclean(const char* vs, int keys, int lane) {
-    bool bad = false;
-    for (int i = lane; i < keys * HD / 8; i += 64) {
-      const u16x8 v = *reinterpret_cast<const u16x8*>(vs + 16 * i);
+  DEV typename T::v8 finite(typename T::v8 x) {
+    u16x8 v = __builtin_bit_cast(u16x8, x);
 #pragma unroll
-      for (int e = 0; e < 8; e++) bad = bad || (v[e] & T::kExp) == T::kExp;
+    for (int e = 0; e < 8; e++) {
+      const bool bad = (v[e] & T::kExp) == T::kExp;
+      odd = odd || bad;
+      v[e] = bad ? 0 : v[e];
     }
-    return bad;
+    return __builtin_bit_cast(typename T::v8, v);
   }
 
-  // The second product where later keys' values hold infinities or NaN, which a p of 0 would turn into NaN: the
-  // finite values as ever, and for the others two products of ones count, row by row, the seen keys whose value is
-  // not below +inf, and not above -inf; what such a count touches becomes that infinity (both: NaN).
-  template <int NKB>
-  DEV void apart(const char* vs, int key0, const typename T::v8 (&pf)[QB][2 * NKB], int lane) {
-    const int h = lane >> 5;
-#pragma unroll 1
-    for (int d = 0; d < HD / 32; d++) {
+  // What the masked steps' seen infinities and NaN bring, for keys first .. last - 1 (rows of V from `vb`, st elements
+  // apart): a product of ones counts, row by row, the seen values of +inf (by 1), -inf (by 128) and NaN (by both; 16
+  // of each at most, exact), and what it finds becomes that infinity (both: NaN).
+  DEV void add_odd(const char* vb, long long st, int d, int first, int last, int lane) {
+    typedef typename T::v8 v8;
+    const int r = lane & 31, h = lane >> 5;
+    for (int k0 = first; k0 < last; k0 += 16)
 #pragma unroll
-      for (int b = 0; b < QB; b++) {
-        f32x16 up, down, of = {};
+      for (int db = 0; db < HD / 32; db++) {
+        u16x8 v, seen;
 #pragma unroll
-        for (int i = 0; i < 16; i++) up[i] = down[i] = of[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2 * NKB; j++) {
-          const u16x8 v = __builtin_bit_cast(u16x8, v_frag<T, HD>(vs, j, d, lane));
-          u16x8 fin, pos, neg, seen;
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const bool odd = (v[e] & T::kExp) == T::kExp, nan = odd && (v[e] & 0x7fff) != T::kExp;
-            fin[e] = odd ? 0 : v[e];
-            pos[e] = odd && (nan || !(v[e] >> 15)) ? T::kOne : 0;
-            neg[e] = odd && (nan || (v[e] >> 15)) ? T::kOne : 0;
-            seen[e] = key0 + 16 * j + 4 * h + (e & 3) + 8 * (e >> 2) <= lim[b] ? T::kOne : 0;
-          }
-          typedef typename T::v8 v8;
-          of = T::mfma(__builtin_bit_cast(v8, fin), pf[b][j], of);
-          up = T::mfma(__builtin_bit_cast(v8, pos), __builtin_bit_cast(v8, seen), up);
-          down = T::mfma(__builtin_bit_cast(v8, neg), __builtin_bit_cast(v8, seen), down);
+        for (int e = 0; e < 8; e++) {
+          const int key = k0 + 8 * h + e;
+          const uint16_t x = key < last && 32 * db + r < d ? *reinterpret_cast<const uint16_t*>(vb + 2 * (st * key + 32 * db + r)) : 0;
+          const bool bad = (x & T::kExp) == T::kExp, nan = (x & 0x7fff) != T::kExp;
+          v[e] = !bad ? 0 : nan ? T::kBoth : x >> 15 ? T::kMany : T::kOne;
+          seen[e] = key <= lim ? T::kOne : 0;
         }
+        f32x16 n;
+#pragma unroll
+        for (int i = 0; i < 16; i++) n[i] = 0.f;
+        n = T::mfma(__builtin_bit_cast(v8, v), __builtin_bit_cast(v8, seen), n);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          float add = of[i];
-          add += up[i] > 0.f ? INFINITY : 0.f;
-          add -= down[i] > 0.f ? INFINITY : 0.f;
-#pragma unroll
-          for (int dd = 0; dd < HD / 32; dd++) o[b][dd][i] += dd == d ? add : 0.f;
+          const float down = floorf(n[i] * 0.0078125f);
+          o[db][i] += n[i] - 128.f * down > 0.f ? INFINITY : 0.f;
+          o[db][i] -= down > 0.f ? INFINITY : 0.f;
         }
       }
-    }
   }
 };
 
@@ -274,50 +259,50 @@ DEV void load_rows(dma_src_t src, uint32_t lds, long long st, int d, int n0, int
   }
 }
 
-// Query fragments and the limit of row `row` (of the span's nq * G) for every block of the wave.
-template <class T, int HD, int QB>
-DEV void load_queries(Rows<T, HD, QB>& w, const PackedAttnArgs& p, const Span& s, int hk, int row0, int lane) {
-  const int r = lane & 31, h = lane >> 5;
+// Query fragments and the limit of row `row` (of the span's nq * G).
+template <class T, int HD>
+DEV void load_queries(Rows<T, HD>& w, const PackedAttnArgs& p, const Span& s, int hk, int row0, int lane) {
+  const int h = lane >> 5, row = row0 + (lane & 31), i = row / p.G, g = row - i * p.G;
+  const bool ok = i < s.nq;
+  const char* src = (const char*)p.q + 2 * ((long long)(s.q0 + (ok ? i : 0)) * p.q_st + (long long)(hk * p.G + g) * p.q_sh);
 #pragma unroll
-  for (int b = 0; b < QB; b++) {
-    const int row = row0 + 32 * b + r, i = row / p.G, g = row - i * p.G;
-    const bool ok = i < s.nq;
-    const char* src = (const char*)p.q + 2 * ((long long)(s.q0 + (ok ? i : 0)) * p.q_st + (long long)(hk * p.G + g) * p.q_sh);
-#pragma unroll
-    for (int k = 0; k < HD / 16; k++) {
-      w.q[b][k] = typename T::v8{};
-      if (ok && 16 * k + 8 * h < p.d) w.q[b][k] = *reinterpret_cast<const typename T::v8*>(src + 2 * (16 * k + 8 * h));
-    }
-    w.lim[b] = p.causal && ok ? min(s.nk - 1, i + s.nk - s.nq) : s.nk - 1;
+  for (int k = 0; k < HD / 16; k++) {
+    w.q[k] = typename T::v8{};
+    if (ok && 16 * k + 8 * h < p.d) w.q[k] = *reinterpret_cast<const typename T::v8*>(src + 2 * (16 * k + 8 * h));
   }
+  w.lim = p.causal && ok ? min(s.nk - 1, i + s.nk - s.nq) : s.nk - 1;
 }
 
-constexpr int kAttnKeys = 64;  // keys per tile of the many-row kernel
+constexpr int kAttnKeys = 64;   // keys per tile of the many-row kernel
+constexpr int kAttnRows = 128;  // rows per workgroup
 
-template <class T, int HD, int QB>
-__global__ __launch_bounds__(256) void packed_attention_kernel(PackedAttnArgs p) {
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs p) {
   constexpr int kTile = kAttnKeys * 2 * HD;  // bytes of a K (or V) tile
+  // 32-key blocks per step: two share one maximum and its check (16,384 causal rows of 32 heads of 128 2.15 -> 2.09
+  // ms); at 64 columns the registers of one leave room for another wave (a batch of proteins 45.7 -> 42.1 us)
+  constexpr int kStep = HD == 64 ? 1 : 2;
   __shared__ __align__(1024) char lds[2][2 * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // key heads run fastest over the workgroups: the eight XCDs take different heads, each with its own L2, and the
   // longest tiles of every head start first
   const int hk = blockIdx.x % p.Hk, item = blockIdx.x / p.Hk;
   int seq, tile;
-  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, 128 * QB, item, lane, seq, tile)) return;
+  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, kAttnRows, item, lane, seq, tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Span s = span_of(p, seq);
   const int rows = s.nq * p.G;
-  if (p.causal) tile = (rows + 128 * QB - 1) / (128 * QB) - 1 - tile;
-  const int row0 = 128 * QB * tile + 32 * QB * wave;  // this wave's first row
+  if (p.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
+  const int row0 = kAttnRows * tile + 32 * wave;  // this wave's first row
 
-  Rows<T, HD, QB> w;
+  Rows<T, HD> w;
   w.init();
   load_queries(w, p, s, hk, row0, lane);
   // keys seen by the workgroup's last row, by this wave's last row, and by its first
   const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
-  const int end = seen(128 * QB * (tile + 1) - 1);
-  const int wend = row0 < rows ? seen(row0 + 32 * QB - 1) : 0, wfull = seen(row0);
+  const int end = seen(kAttnRows * (tile + 1) - 1);
+  const int wend = row0 < rows ? seen(row0 + 31) : 0;
   const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
   const char* vb = (const char*)p.v + 2 * (long long)hk * p.v_sh;
   const auto load = [&](int kt, int buf) {
@@ -326,34 +311,43 @@ __global__ __launch_bounds__(256) void packed_attention_kernel(PackedAttnArgs p)
     load_rows<HD, false>(tile_src(kb, p.k_st, p.d, s.k0, kt, s.nk, kAttnKeys), at, p.k_st, p.d, kMine * wave, kMine, lane);
     load_rows<HD, true>(tile_src(vb, p.v_st, p.d, s.k0, kt, s.nk, kAttnKeys), at + kTile, p.v_st, p.d, kMine * wave, kMine, lane);
   };
+  // whole tiles that the workgroup's first row sees, then those at the end of what its rows see
+  const int whole = seen(kAttnRows * tile) / kAttnKeys * kAttnKeys;
   if (end > 0) load(0, 0);
-  for (int kt = 0, buf = 0; kt < end; kt += kAttnKeys, buf ^= 1) {
+  int kt = 0, buf = 0;
+  for (; kt < whole; kt += kAttnKeys, buf ^= 1) {
     wait_vm(0);
     __syncthreads();  // this tile is in, and every wave has left the other buffer
     if (kt + kAttnKeys < end) load(kt + kAttnKeys, buf ^ 1);
-    if (kt < wend)
-      w.template step<kAttnKeys / 32>(lds[buf], lds[buf] + kTile, kt, kt + kAttnKeys > wfull, kt + kAttnKeys > wfull && wfull < s.nk, p.scale_log2, lane);
+#pragma unroll
+    for (int u = 0; u < kAttnKeys; u += 32 * kStep)
+      w.template step<kStep, false>(lds[buf] + u * 2 * HD, lds[buf] + kTile + u * 2 * HD, kt + u, p.scale_log2, lane);
   }
+  for (; kt < end; kt += kAttnKeys, buf ^= 1) {
+    wait_vm(0);
+    __syncthreads();
+    if (kt + kAttnKeys < end) load(kt + kAttnKeys, buf ^ 1);
+#pragma unroll 1
+    for (int u = 0; u < kAttnKeys && kt + u < wend; u += 32)
+      w.template step<1, true>(lds[buf] + u * 2 * HD, lds[buf] + kTile + u * 2 * HD, kt + u, p.scale_log2, lane);
+  }
+  if (__any(w.odd)) w.add_odd(vb + 2 * p.v_st * s.k0, p.v_st, p.d, whole, wend, lane);
 
-  const int r = lane & 31;
+  const float l = w.l + __shfl_xor(w.l, 32);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key is 0
+  const int row = row0 + (lane & 31), i = row / p.G, g = row - i * p.G;
+  if (row >= rows) return;
+  char* dst = (char*)p.o + 2 * ((long long)(s.q0 + i) * p.o_st + (long long)(hk * p.G + g) * p.o_sh);
 #pragma unroll
-  for (int b = 0; b < QB; b++) {
-    const float l = w.l[b] + __shfl_xor(w.l[b], 32);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key is 0
-    const int row = row0 + 32 * b + r, i = row / p.G, g = row - i * p.G;
-    if (row >= rows) continue;
-    char* dst = (char*)p.o + 2 * ((long long)(s.q0 + i) * p.o_st + (long long)(hk * p.G + g) * p.o_sh);
+  for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-    for (int d = 0; d < HD / 32; d++)
+    for (int i4 = 0; i4 < 4; i4++) {
+      const int col = 32 * d + acc_row32(4 * i4, lane);
+      typename T::v4 y;
 #pragma unroll
-      for (int i4 = 0; i4 < 4; i4++) {
-        const int col = 32 * d + acc_row32(4 * i4, lane);
-        typename T::v4 y;
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(w.o[b][d][4 * i4 + e] * inv);
-        if (col < p.d) *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
-      }
-  }
+      for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(w.o[d][4 * i4 + e] * inv);
+      if (col < p.d) *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
+    }
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -385,25 +379,39 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   const int end = min(seen(row0 + 31), first + part), wfull = seen(row0);
   if (p.splits > 1 && first > 0 && first >= s.nk) return;  // no part of this sequence: the join reads none
 
-  Rows<T, HD, 1> w;
+  Rows<T, HD> w;
   w.init();
   load_queries(w, p, s, hk, row0, lane);
   const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
   const char* vb = (const char*)p.v + 2 * (long long)hk * p.v_sh;
   char *ks = lds[wave], *vs = lds[wave] + kTile;
-  for (int kt = first + KW * wave; kt < end; kt += kPass) {
+  const auto load = [&](int kt) {
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the last pass's LDS reads are back
     __asm__ volatile("" ::: "memory");
     load_rows<HD, false>(tile_src(kb, p.k_st, p.d, s.k0, kt, s.nk, KW), lds_address(ks), p.k_st, p.d, 0, KW, lane);
     load_rows<HD, true>(tile_src(vb, p.v_st, p.d, s.k0, kt, s.nk, KW), lds_address(vs), p.v_st, p.d, 0, KW, lane);
     wait_vm(0);
-    w.template step<KW / 32>(ks, vs, kt, kt + KW > wfull, kt + KW > wfull && wfull < s.nk, p.scale_log2, lane);
+  };
+  int kt = first + KW * wave;
+  for (; kt < end && kt + KW <= wfull; kt += kPass) {
+    load(kt);
+#pragma unroll
+    for (int u = 0; u < KW; u += 32) w.template step<1, false>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2, lane);
   }
+  const int masked = kt;
+  for (; kt < end; kt += kPass) {
+    load(kt);
+#pragma unroll 1
+    for (int u = 0; u < KW && kt + u < end; u += 32)
+      w.template step<1, true>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2, lane);
+  }
+  if (__any(w.odd))
+    for (kt = masked; kt < end; kt += kPass) w.add_odd(vb + 2 * p.v_st * s.k0, p.v_st, p.d, kt, min(kt + KW, end), lane);
 
   // (m, l, O) of the four waves through LDS; wave i then joins the d quads i, i + 4, .. of every row
-  const float lsum = w.l[0] + __shfl_xor(w.l[0], 32);
+  const float lsum = w.l + __shfl_xor(w.l, 32);
   if (h == 0) {
-    ml[wave][0][r] = w.m[0];
+    ml[wave][0][r] = w.m;
     ml[wave][1][r] = lsum;
   }
   __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -413,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   for (int d = 0; d < HD / 32; d++)
 #pragma unroll
     for (int i4 = 0; i4 < 4; i4++)
-      ow[(4 * d + i4) * 64 + lane] = f32x4{w.o[0][d][4 * i4], w.o[0][d][4 * i4 + 1], w.o[0][d][4 * i4 + 2], w.o[0][d][4 * i4 + 3]};
+      ow[(4 * d + i4) * 64 + lane] = f32x4{w.o[d][4 * i4], w.o[d][4 * i4 + 1], w.o[d][4 * i4 + 2], w.o[d][4 * i4 + 3]};
   __syncthreads();
   const int row = row0 + r, i = row / p.G, g = row - i * p.G;
   if (row >= rows) return;
@@ -517,9 +525,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
 template <class T, int HD>
 static hipError_t launch_attention_t(const PackedAttnArgs& a, bool many, hipStream_t s) {
   if (many) {
-    constexpr int QB = 2;
-    const long long items = (long long)a.Tq * a.G / (128 * QB) + a.n;
-    ESM_LAUNCH((packed_attention_kernel<T, HD, QB>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
+    const long long items = (long long)a.Tq * a.G / kAttnRows + a.n;
+    ESM_LAUNCH((packed_attention_kernel<T, HD>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
     return hipGetLastError();
   }
   const long long items = (long long)a.Tq * a.G / 32 + a.n;
