@@ -19,6 +19,7 @@ from . import kernels
 from .q8 import ScratchParts
 
 BLOCK = 128
+_TYPES = (torch.float16, torch.bfloat16)
 
 
 class F8Linear(nn.Module):
@@ -61,12 +62,15 @@ class F8Linear(nn.Module):
         return self.codes.float() * s.repeat_interleave(BLOCK, 1)[:, :self.in_features]
 
     def _input(self, x: torch.Tensor) -> torch.Tensor:
-        if x.shape[-1] != self.in_features:
-            raise ValueError(f"F8Linear: input of {x.shape[-1]} features, takes {self.in_features}")
-        x2 = x if x.dim() == 2 else x.reshape(-1, self.in_features)
-        if x2.dtype not in (torch.float16, torch.bfloat16):
+        """x as rows the kernel reads where they are, copied only if they must be."""
+        K = self.in_features
+        if x.shape[-1] != K:
+            raise ValueError(f"F8Linear: input of {x.shape[-1]} features, takes {K}")
+        x2 = x if x.dim() == 2 else x.reshape(-1, K)
+        if x2.dtype not in _TYPES:
             x2 = x2.to(torch.float16)
-        if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.stride(0) < self.in_features or x2.data_ptr() % 16:
+        st, one = x2.stride()
+        if one != 1 or st % 8 or st < K or x2.data_ptr() % 16:
             x2 = x2.contiguous()
             if x2.data_ptr() % 16:
                 x2 = x2.clone()
@@ -74,10 +78,11 @@ class F8Linear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x . W^T in x's type (fp16 and bf16 as they are, others through fp16)."""
-        y = kernels.f8_linear(self._input(x), self.codes_packed, self.scales, self.out_features)
+        b = self._buffers
+        y = kernels.f8_linear(self._input(x), b["codes_packed"], b["scales"], self.out_features)
         if x.dim() != 2:
             y = y.reshape(*x.shape[:-1], self.out_features)
-        return y if y.dtype == x.dtype else y.to(x.dtype)
+        return y if y.dtype is x.dtype else y.to(x.dtype)
 
     def partials(self, x: torch.Tensor) -> ScratchParts:
         """(partials [splits, M, N] fp32, splits) in the shared scratch, as ``Q8Linear.partials``: rounded to x's type,

@@ -203,15 +203,16 @@ def _rows(t, name: str, like=None):
     need no shape, and its strides."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise capi.EsmError(-5, f"{name} must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
-    if t.dim() != 3 or t.dtype not in _DTYPES:
-        raise capi.EsmError(-2, f"{name} must be [rows, heads, d] in fp16 or bf16, got {t.dtype} {tuple(t.shape)}")
-    if like is not None and (t.dtype is not like.dtype or t.device != like.device):
-        raise capi.EsmError(-2, f"{name}: {t.dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
-    st, sh, one = t.stride()
-    if one != 1 and t.shape[2] > 1:
+    dtype, shape, strides = t.dtype, t.shape, t.stride()
+    if len(shape) != 3 or dtype not in _DTYPES:
+        raise capi.EsmError(-2, f"{name} must be [rows, heads, d] in fp16 or bf16, got {dtype} {tuple(shape)}")
+    if like is not None and (dtype is not like.dtype or t.get_device() != like.get_device()):
+        raise capi.EsmError(-2, f"{name}: {dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
+    st, sh, one = strides
+    if one != 1 and shape[2] > 1:
         raise capi.EsmError(-3, f"{name}: the values of a head must be contiguous")
     # (a stride that nothing is reached by says nothing)
-    return (st if t.shape[0] > 1 else 8 * ((t.shape[1] * t.shape[2] + 7) // 8)), (sh if t.shape[1] > 1 else 0)
+    return (st if shape[0] > 1 else 8 * ((shape[1] * shape[2] + 7) // 8)), (sh if shape[1] > 1 else 0)
 
 
 def _distinct(strides, shape, name: str) -> None:
@@ -221,9 +222,9 @@ def _distinct(strides, shape, name: str) -> None:
         raise capi.EsmError(-3, f"{name}: rows and heads must not overlap")
 
 
-def _on(device):
-    """A context with the tensors' device current: launches go on its current stream."""
-    return scratch._UNGUARDED if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _elsewhere(t) -> bool:
+    """Whether the tensor's device is not the current one: its call is then made with that device current."""
+    return t.get_device() != torch.cuda.current_device()
 
 
 def _aux(t, name: str, dtypes, device) -> torch.Tensor:
@@ -236,6 +237,20 @@ def _aux(t, name: str, dtypes, device) -> torch.Tensor:
     return t
 
 
+_FP32, _FP64, _INT32, _INTS = (torch.float32,), (torch.float64,), (torch.int32,), (torch.int32, torch.int64)
+
+
+def _weights_of(t, name: str, heads: int, d: int, device):
+    """(pointer, whether every head has its own) of a norm's weight."""
+    if t is None:
+        return None, 0
+    _aux(t, name, _FP32, device)
+    n = t.numel()
+    if n != d and n != heads * d:
+        raise capi.EsmError(-2, f"qk_norm_rope: {name} has {n} elements for {heads} heads of {d}")
+    return t.data_ptr(), int(n != d)
+
+
 def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: bool = False, norm: str | None = None,
                  over: str = "head", q_w=None, k_w=None, eps: float = 1e-6, out=None):
     """Norm and rotation of q [T, H, d] and k [T, Hk, d] (fp16 or bf16, views of wider rows allowed) in one pass ->
@@ -243,42 +258,42 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
     d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
     makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
     0 .. T - 1). ``out`` = (q', k'), which may be (q, k)."""
-    lib = capi.lib()
-    qs, ks = _rows(q, "q"), _rows(k, "k", q)
+    q_st, q_sh = _rows(q, "q")
+    k_st, k_sh = _rows(k, "k", q)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return qk_norm_rope(q, k, freq, positions, gain=gain, interleaved=interleaved, norm=norm, over=over, q_w=q_w,
+                                k_w=k_w, eps=eps, out=out)
     T, H, d = q.shape
-    Hk = k.shape[1]
-    if k.shape[0] != T or k.shape[2] != d:
+    Tk, Hk, dk = k.shape
+    if Tk != T or dk != d:
         raise capi.EsmError(-2, f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
     if norm not in _NORMS or over not in ("head", "row"):
         raise capi.EsmError(-4, f"qk_norm_rope: norm={norm!r} over={over!r}")
-    _aux(freq, "freq", (torch.float64,), q.device)
+    device = q.device
+    _aux(freq, "freq", _FP64, device)
+    pos, pos64 = None, 0
     if positions is not None:
-        _aux(positions, "positions", (torch.int32, torch.int64), q.device)
+        _aux(positions, "positions", _INTS, device)
         if positions.numel() != T:
             raise capi.EsmError(-2, f"qk_norm_rope: {positions.numel()} positions for {T} rows")
-    w = []
-    for t, n, heads in ((q_w, "q_w", H), (k_w, "k_w", Hk)):
-        if t is not None:
-            _aux(t, n, (torch.float32,), q.device)
-            if t.numel() not in (d, heads * d):
-                raise capi.EsmError(-2, f"qk_norm_rope: {n} has {t.numel()} elements for {heads} heads of {d}")
-        w.append((_ptr(t), int(t is not None and t.numel() != d)))
+        pos, pos64 = positions.data_ptr(), int(positions.dtype is torch.int64)
+    qw, qwh = _weights_of(q_w, "q_w", H, d, device)
+    kw, kwh = _weights_of(k_w, "k_w", Hk, d, device)
     if out is None:
-        qo, ko = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+        qo, ko = torch.empty(T, H, d, dtype=q.dtype, device=device), torch.empty(T, Hk, d, dtype=q.dtype, device=device)
+        qo_st, qo_sh, ko_st, ko_sh = H * d, d, Hk * d, d
     else:
         qo, ko = out
-    outs = []
-    for t, n, like in ((qo, "out[0]", q), (ko, "out[1]", k)):
-        outs.append(_rows(t, n, q))
-        if t.shape != like.shape:
-            raise capi.EsmError(-2, f"qk_norm_rope: {n} {tuple(t.shape)}, writes {tuple(like.shape)}")
-        _distinct(outs[-1], t.shape, n)
-    with _on(q.device):
-        capi.check(lib.qk_norm_rope(q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), *qs, *ks, *outs[0],
-                                    *outs[1], *w[0], *w[1], float(eps), _ptr(positions),
-                                    int(positions is not None and positions.dtype == torch.int64), freq.data_ptr(),
-                                    float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], int(over == "row"),
-                                    int(interleaved), _DTYPES[q.dtype], capi.stream_ptr()))
+        for t, n, like in ((qo, "out[0]", q), (ko, "out[1]", k)):
+            if not isinstance(t, torch.Tensor) or t.shape != like.shape:
+                raise capi.EsmError(-2, f"qk_norm_rope: {n} must be {tuple(like.shape)}")
+            _distinct(_rows(t, n, q), t.shape, n)
+        (qo_st, qo_sh), (ko_st, ko_sh) = _rows(qo, "out[0]", q), _rows(ko, "out[1]", q)
+    capi.check(capi.lib().qk_norm_rope(
+        q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
+        qwh, kw, kwh, eps, pos, pos64, freq.data_ptr(), gain, T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
+        bool(interleaved), _DTYPES[q.dtype], capi.stream_ptr()))
     return qo, ko
 
 
@@ -288,34 +303,43 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
     sequence are not written. The partial results of few rows against many keys live in the shared scratch."""
-    lib = capi.lib()
-    qs, ks, vs = _rows(q, "q"), _rows(k, "k", q), _rows(v, "v", q)
+    q_st, q_sh = _rows(q, "q")
+    k_st, k_sh = _rows(k, "k", q)
+    v_st, v_sh = _rows(v, "v", q)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return packed_attention(q, k, v, cu_q, cu_k, causal, scale, out)
     Tq, H, d = q.shape
-    Tk, Hk, _ = k.shape
-    if k.shape != v.shape or k.shape[2] != d or Hk == 0 or H % Hk:
+    Tk, Hk, dk = k.shape
+    if k.shape != v.shape or dk != d or Hk == 0 or H % Hk:
         raise capi.EsmError(-2, f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    device = q.device
+    _aux(cu_q, "cu_q", _INT32, device)
+    n = cu_q.numel() - 1
     if cu_k is None:
         if Tk != Tq:
             raise capi.EsmError(-2, f"packed_attention: {Tq} query rows and {Tk} key rows need cu_k")
         cu_k = cu_q
-    for t, n in ((cu_q, "cu_q"), (cu_k, "cu_k")):
-        _aux(t, n, (torch.int32,), q.device)
-    n = cu_q.numel() - 1
+    else:
+        _aux(cu_k, "cu_k", _INT32, device)
     if n < 0 or cu_k.numel() != n + 1:
         raise capi.EsmError(-2, f"packed_attention: {cu_q.numel()} and {cu_k.numel()} starts")
-    o = torch.empty(Tq, H, d, dtype=q.dtype, device=q.device) if out is None else out
-    os_ = _rows(o, "out", q)
-    if o.shape != q.shape:
-        raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
-    _distinct(os_, o.shape, "out")
-    with _on(q.device):
-        need = int(lib.packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d))
-        with scratch.guard(q.device, need):
-            ws, wp, stream = scratch.take(need, q.device) if need else (None, None, capi.stream_ptr())
-            capi.check(lib.packed_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *qs, *ks, *vs, *os_,
-                                            cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, int(causal),
-                                            float(d ** -0.5 if scale is None else scale), _DTYPES[q.dtype], wp, need,
-                                            stream))
+    if out is None:
+        o, o_st, o_sh = torch.empty(Tq, H, d, dtype=q.dtype, device=device), H * d, d
+    else:
+        o = out
+        o_st, o_sh = _rows(o, "out", q)
+        if o.shape != q.shape:
+            raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
+        _distinct((o_st, o_sh), o.shape, "out")
+    lib = capi.lib()
+    need = lib.packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d)
+    with scratch.guard(device, need):
+        ws, wp, stream = scratch.take(need, device) if need else (None, None, capi.stream_ptr())
+        capi.check(lib.packed_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh,
+                                        v_st, v_sh, o_st, o_sh, cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d,
+                                        bool(causal), d ** -0.5 if scale is None else scale, _DTYPES[q.dtype], wp, need,
+                                        stream))
     return o
 
 
@@ -636,7 +660,7 @@ def f8_pack_codes(q):
         raise capi.EsmError(-2, f"f8_pack_codes: q must be 8-bit codes [N, K], got {q.dtype} {tuple(q.shape)}")
     N, K = q.shape
     qp = torch.empty(int(lib.f8_packed_codes_bytes(N, K)), dtype=torch.uint8, device=q.device)
-    with _on(q.device):
+    with torch.cuda.device(q.device):
         capi.check(lib.f8_pack_codes(q.data_ptr(), qp.data_ptr(), N, K, capi.stream_ptr()))
     return qp
 
@@ -651,7 +675,7 @@ def f8_quantize_weight(w):
     N, K = w.shape
     q = torch.empty(N, K, dtype=torch.uint8, device=w.device)
     s = torch.empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
-    with _on(w.device):
+    with torch.cuda.device(w.device):
         capi.check(lib.f8_quantize_weight(w.data_ptr(), q.data_ptr(), s.data_ptr(), N, K, capi.stream_ptr()))
     return q, s
 
@@ -663,33 +687,37 @@ def _f8_operands(x, codes, scales, N, fn):
     if x.dim() != 2 or x.dtype not in _DTYPES:
         raise capi.EsmError(-2, f"{fn}: x must be [rows, K] in fp16 or bf16, got {x.dtype} {tuple(x.shape)}")
     M, K = x.shape
-    if K > 1 and x.stride(1) != 1:
+    st, one = x.stride()
+    if K > 1 and one != 1:
         raise capi.EsmError(-3, f"{fn}: the values of a row must be contiguous")
-    _aux(codes, "codes", (torch.uint8,), x.device)
-    _aux(scales, "scales", (torch.float32,), x.device)
+    device = x.device
+    _aux(codes, "codes", (torch.uint8,), device)
+    _aux(scales, "scales", _FP32, device)
     if codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128):
         raise capi.EsmError(-2, f"{fn}: {codes.numel()} packed codes and {scales.numel()} scales for [{N}, {K}]")
-    return M, K, x.stride(0) if M > 1 else (K + 7) // 8 * 8
+    return M, K, st if M > 1 else (K + 7) // 8 * 8
 
 
 def f8_linear(x, codes, scales, N: int, out=None):
     """y = x . W^T on the fp8 matrix cores: x [M, K] fp16 or bf16 (rows may lie apart), brought to e4m3 with a scale
     per row and 128 columns; W [N, K] as packed e4m3 codes (``f8_pack_codes``) with an fp32 scale per 128 x 128 block;
     fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch."""
-    lib = capi.lib()
     M, K, st = _f8_operands(x, codes, scales, N, "f8_linear")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return f8_linear(x, codes, scales, N, out)
     if out is None:
         y = torch.empty(M, N, dtype=x.dtype, device=x.device)
     else:
         y = _out(out, "out", x.dtype, M * N)
         if y.device != x.device:
             raise capi.EsmError(-5, f"out must be on {x.device}")
-    with _on(x.device):
-        need = int(lib.f8_linear_workspace_bytes(M, K, N))
-        with scratch.guard(x.device, need):
-            ws, wp, stream = scratch.take(need, x.device) if need else (None, None, capi.stream_ptr())
-            capi.check(lib.f8_linear(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N,
-                                     _DTYPES[x.dtype], wp, need, stream))
+    lib = capi.lib()
+    need = lib.f8_linear_workspace_bytes(M, K, N)
+    with scratch.guard(x.device, need):
+        ws, wp, stream = scratch.take(need, x.device) if need else (None, None, capi.stream_ptr())
+        capi.check(lib.f8_linear(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N,
+                                 _DTYPES[x.dtype], wp, need, stream))
     return y
 
 
@@ -700,7 +728,7 @@ def f8_linear_partials(x, codes, scales, N: int):
     lib = capi.lib()
     M, K, st = _f8_operands(x, codes, scales, N, "f8_linear_partials")
     splits = ctypes.c_int(0)
-    with _on(x.device), scratch.guard(x.device):
+    with torch.cuda.device(x.device), scratch.guard(x.device):
         nparts = int(lib.f8_linear_partials_bytes(M, K, N))
         need = int(lib.f8_linear_workspace_bytes(M, K, N))
         at = (nparts + 255) // 256 * 256

@@ -41,6 +41,7 @@ class _Slot:
     buf: torch.Tensor
     stream: torch.cuda.Stream          # the last stream that called get()
     generation: int = 0
+    raw: int = 0                       # that stream's handle
 
 
 _slots: dict[int, _Slot] = {}
@@ -67,12 +68,16 @@ def guard(device=None, nbytes: int = 1):
 
 
 def _claim(nbytes: int, device):
-    """(the device's buffer, grown if need be, the current stream on it)."""
+    """(the device's buffer, grown if need be, the current stream's handle on it)."""
     idx = _index(device)
     need = max(int(nbytes), 1) + ALIGN
-    stream = torch.cuda.current_stream(idx)
+    raw = torch._C._cuda_getCurrentRawStream(idx)
     with _lock:
         slot = _slots.get(idx)
+        if slot is not None and slot.raw == raw and slot.buf.numel() >= need:  # as the last call left it
+            slot.generation += 1
+            return slot.buf, raw
+        stream = torch.cuda.current_stream(idx)
         moved = slot is not None and slot.stream != stream
         capturing = moved and torch.cuda.is_current_stream_capturing()
         if moved and not capturing:
@@ -82,13 +87,13 @@ def _claim(nbytes: int, device):
             # old buffer is freed here, and record_stream has told the allocator who used it
             size = need if slot is None else max(need, slot.buf.numel() + slot.buf.numel() // 4)
             buf = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", idx))
-            slot = _slots[idx] = _Slot(buf, stream, 0 if slot is None else slot.generation)
+            slot = _slots[idx] = _Slot(buf, stream, 0 if slot is None else slot.generation, raw)
         elif moved:
             if not capturing:
                 slot.buf.record_stream(stream)
-            slot.stream = stream
+            slot.stream, slot.raw = stream, raw
         slot.generation += 1
-        return slot.buf, stream
+        return slot.buf, raw
 
 
 def get(nbytes: int, device=None) -> torch.Tensor:
@@ -102,8 +107,8 @@ def get(nbytes: int, device=None) -> torch.Tensor:
 def take(nbytes: int, device=None):
     """``get`` for one launch: (buffer, 256-byte aligned address in it, raw stream). The caller holds the
     buffer and ``guard(device)`` until its launches are queued."""
-    buf, stream = _claim(nbytes, device)
-    return buf, (buf.data_ptr() + ALIGN - 1) // ALIGN * ALIGN, stream.cuda_stream
+    buf, raw = _claim(nbytes, device)
+    return buf, (buf.data_ptr() + ALIGN - 1) // ALIGN * ALIGN, raw
 
 
 def generation(device=None) -> int:
