@@ -1079,7 +1079,7 @@ F8Ws f8_layout(int M, int K, int N, bool parts_inside) {
   if (w.plan.form != esm::kF8Few) {
     const size_t kb = (size_t)(K + 127) / 128;
     w.sx = (size_t)w.Mp * kb * 128;
-    w.part = (w.sx + (size_t)w.Mp * kb * 4 + 255) / 256 * 256;
+    w.part = (w.sx + (size_t)w.Mp * kb * 4 + 1024 + 255) / 256 * 256;  // (1 KB that a tile's last rows read past)
     w.total = w.part;
     if (parts_inside && w.plan.splits > 1) w.total += (size_t)w.plan.splits * M * N * 4;
   }
@@ -1092,8 +1092,10 @@ int f8_run(const char* fn, const void* x, int64_t x_st, const uint8_t* qp, const
   if (splits) *splits = 0;
   if (!f8_shape(M, K, N)) return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d (multiple of 16) N=%d (of 8)", fn, M, K, N);
   if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "%s: dtype=%d", fn, dtype);
-  if (M > (1 << 24) || ((long long)M + 63) / 64 * ((N + 127) / 128) >= (1LL << 22))
-    return fail(ESM_ERR_SHAPE, "%s: M=%d N=%d too large", fn, M, N);
+  // grids below 2^32 threads, offsets into x's scales below 2^31 bytes
+  if (M > (1 << 24) || ((long long)M + 63) / 64 * ((N + 63) / 64) >= (1LL << 22) ||
+      (long long)round_up(M, 16) * ((K + 127) / 128) * 4 >= (1LL << 31) - 4096)
+    return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d N=%d too large", fn, M, K, N);
   if (M == 0) return ok();
   if (!x || !qp || !s || (!y == !parts)) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
   if (x_st % 8 != 0 || (M > 1 && x_st < K)) return fail(ESM_ERR_ALIGN, "%s: row stride (a multiple of 8, >= K)", fn);
@@ -1118,7 +1120,7 @@ int f8_run(const char* fn, const void* x, int64_t x_st, const uint8_t* qp, const
   }
   a.part = parts ? parts : w.plan.splits > 1 ? reinterpret_cast<float*>(ws + w.part) : nullptr;
   if (splits) *splits = w.plan.splits;
-  return hip_status(esm::launch_f8_linear(a, dtype == ESM_BF16, w.plan.form, (hipStream_t)stream), fn);
+  return hip_status(esm::launch_f8_linear(a, dtype == ESM_BF16, w.plan, (hipStream_t)stream), fn);
 }
 }  // namespace
 

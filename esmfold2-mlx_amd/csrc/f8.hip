@@ -14,8 +14,8 @@
 //     dealt that way the four fragments leave a lane 16 consecutive outputs of one row of x.
 //   x: 16 rows x 128 k = 2 KB pieces [M / 16][K / 128][2][64 lanes][16 bytes], the same k order.
 // Up to 16 rows of x one launch does it all (f8_few_kernel: bound by the codes' bytes); beyond, x goes through
-// f8_quantize_kernel and f8_gemm_kernel, tiles through LDS by loads that write it directly, K split over
-// workgroups where the tiles do not fill the GPU.
+// f8_quantize_kernel, then f8_some_kernel (some hundred rows: no barriers, operands straight to registers) or
+// f8_gemm_kernel (tiles through LDS by loads that write it directly).
 #include <type_traits>
 
 #include "common.h"
@@ -67,86 +67,121 @@ DEV void f8_codes(V8 v, float r, int& lo, int& hi) {
 }
 
 // ---- x to e4m3 --------------------------------------------------------------------------------
-// A thread takes 16 values, the 8 threads of a row's block share its maximum; a wave covers 8 rows x 128.
+// A thread takes 16 values of a row in each of kQuantBlocks blocks, all loaded first; the 8 threads of a row's block
+// share its maximum.
+constexpr int kQuantBlocks = 4;
 template <class V8>
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const uint16_t* __restrict__ x, long long st, uint8_t* __restrict__ xq,
                                                           float* __restrict__ sx, int M, int K, int Mp) {
   const int Kb = (K + 127) / 128, t = threadIdx.x;
-  const int c = t & 7, m = 32 * blockIdx.x + (t >> 3), kb = blockIdx.y, k = 128 * kb + 16 * c;
+  const int c = t & 7, m = 32 * blockIdx.x + (t >> 3), kb0 = kQuantBlocks * blockIdx.y;
   if (m >= Mp) return;
-  u16x8 a{}, b{};
-  if (m < M && k < K) {
-    const u16x8* src = reinterpret_cast<const u16x8*>(x + m * st + k);
-    a = src[0];
-    b = src[1];
+  u16x8 a[kQuantBlocks], b[kQuantBlocks];
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks; i++) {
+    const int k = 128 * (kb0 + i) + 16 * c;
+    a[i] = b[i] = u16x8{};
+    if (m < M && k < K) {
+      const u16x8* src = reinterpret_cast<const u16x8*>(x + m * st + k);
+      a[i] = src[0];
+      b[i] = src[1];
+    }
   }
-  uint32_t top = max(top_bits(a), top_bits(b));
-  const auto other = [&](auto ctrl) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false);
-  };
-  top = max(top, other(std::integral_constant<int, 0xB1>{}));   // quad_perm(1, 0, 3, 2)
-  top = max(top, other(std::integral_constant<int, 0x4E>{}));   // quad_perm(2, 3, 0, 1)
-  top = max(top, other(std::integral_constant<int, 0x141>{}));  // row_half_mirror
-  float r, s;
-  f8_scale(bits_value<V8>(top), r, s);
-  int q[4];
-  f8_codes(__builtin_bit_cast(V8, a), r, q[0], q[1]);
-  f8_codes(__builtin_bit_cast(V8, b), r, q[2], q[3]);
-  uint8_t* dst = xq + ((size_t)(m >> 4) * Kb + kb) * 2048 + (c & 1) * 1024 + (16 * (c >> 1) + (m & 15)) * 16;
-  *reinterpret_cast<i32x4*>(dst) = i32x4{q[0], q[1], q[2], q[3]};
-  if (c == 0) sx[(size_t)kb * Mp + m] = s;
+#pragma unroll
+  for (int i = 0; i < kQuantBlocks; i++) {
+    const int kb = kb0 + i;
+    uint32_t top = max(top_bits(a[i]), top_bits(b[i]));
+    const auto other = [&](auto ctrl) {
+      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false);
+    };
+    top = max(top, other(std::integral_constant<int, 0xB1>{}));   // quad_perm(1, 0, 3, 2)
+    top = max(top, other(std::integral_constant<int, 0x4E>{}));   // quad_perm(2, 3, 0, 1)
+    top = max(top, other(std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    float r, s;
+    f8_scale(bits_value<V8>(top), r, s);
+    int q[4];
+    f8_codes(__builtin_bit_cast(V8, a[i]), r, q[0], q[1]);
+    f8_codes(__builtin_bit_cast(V8, b[i]), r, q[2], q[3]);
+    if (kb >= Kb) break;
+    uint8_t* dst = xq + ((size_t)(m >> 4) * Kb + kb) * 2048 + (c & 1) * 1024 + (16 * (c >> 1) + (m & 15)) * 16;
+    *reinterpret_cast<i32x4*>(dst) = i32x4{q[0], q[1], q[2], q[3]};
+    if (c == 0) sx[(size_t)kb * Mp + m] = s;
+  }
+}
+
+// Fragment at soff + 16 lane of a buffer whose every read is in range.
+DEV i32x4 bload_i4(rsrc_t r, int voff, int soff) {
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+DEV i32x8 bload_frag(rsrc_t r, int voff, int soff) {
+  const i32x4 lo = bload_i4(r, voff, soff), hi = bload_i4(r, voff, soff + 1024);
+  return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 // ---- few rows: everything in one launch ------------------------------------------------------------
 // A workgroup takes 16 NJ weight rows for all (at most 16) rows of x; its 8 waves deal the blocks of 128 k among
-// them, bring x to e4m3 in registers (32 values of one row a lane) and sum through LDS.
+// them (the next block's loads in flight), bring x to e4m3 in registers (32 values of one row a lane) and sum
+// through LDS.
 constexpr int kFewWaves = 8;
 template <class V8, int NJ>
 __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
-  __shared__ float red[kFewWaves][16][16 * NJ];
+  constexpr int kPad = 16 * NJ + 4;  // (16 rows of sums cover the LDS banks)
+  __shared__ __align__(16) float red[kFewWaves][16][kPad];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Kb = (p.K + 127) / 128;
   const int ng = blockIdx.x / (4 / NJ), j0 = blockIdx.x % (4 / NJ) * NJ;  // 64-row piece, first fragment in it
   const int m = lane & 15, kl = 32 * (lane >> 4);
-  const uint8_t* wp = p.wq + ((size_t)ng * Kb) * 8192 + j0 * 2048 + lane * 16;
-  const uint16_t* xr = (const uint16_t*)p.x + m * p.x_st;
+  const rsrc_t rw = make_rsrc(p.wq + (size_t)ng * Kb * 8192 + j0 * 2048);
+  const uint16_t* xr = (const uint16_t*)p.x + (m < p.M ? m : 0) * p.x_st;
   const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
   f32x4 acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < Kb; kb += kFewWaves) {
+  struct Block {
     i32x8 w[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(wp + (size_t)kb * 8192 + j * 2048);
-      const i32x4 hi = *reinterpret_cast<const i32x4*>(wp + (size_t)kb * 8192 + j * 2048 + 1024);
-      w[j] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    }
     u16x8 x[4];
-    uint32_t top = 0;
+    float sw;
+  };
+  const auto load = [&](Block& b, int kb) {
+    kb = min(kb, Kb - 1);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) b.w[j] = bload_frag(rw, 16 * lane, kb * 8192 + 2048 * j);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int k = 128 * kb + kl + 8 * i;
-      x[i] = u16x8{};
-      if (m < p.M && k < p.K) x[i] = *reinterpret_cast<const u16x8*>(xr + k);
+      b.x[i] = u16x8{};
+      if (m < p.M && k < p.K) b.x[i] = *reinterpret_cast<const u16x8*>(xr + k);
     }
+    b.sw = sw[kb];
+  };
+  const auto take = [&](const Block& b) {
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) top = max(top, top_bits(x[i]));
+    for (int i = 0; i < 4; i++) top = max(top, top_bits(b.x[i]));
     top = max(top, (uint32_t)__shfl_xor((int)top, 16));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
     float r, s;
     f8_scale(bits_value<V8>(top), r, s);
     int q[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) f8_codes(__builtin_bit_cast(V8, x[i]), r, q[2 * i], q[2 * i + 1]);
+    for (int i = 0; i < 4; i++) f8_codes(__builtin_bit_cast(V8, b.x[i]), r, q[2 * i], q[2 * i + 1]);
     const i32x8 xf = {q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]};
-    s *= sw[kb];
+    s *= b.sw;
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-      const f32x4 d = mfma_f8(w[j], xf);
+      const f32x4 d = mfma_f8(b.w[j], xf);
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[j][e] = fmaf(s, d[e], acc[j][e]);
     }
+  };
+  Block b0, b1;
+  if (wave < Kb) load(b0, wave);
+  for (int kb = wave; kb < Kb; kb += 2 * kFewWaves) {
+    load(b1, kb + kFewWaves);
+    take(b0);
+    if (kb + kFewWaves >= Kb) break;
+    load(b0, kb + 2 * kFewWaves);
+    take(b1);
   }
   // lane's outputs: row m, weight rows 16 (lane / 16) + 4 (j0 + j) + e of the piece -> column 4 NJ (lane / 16) + 4 j + e
 #pragma unroll
@@ -171,12 +206,99 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
   }
 }
 
+// ---- some rows: no barriers, K divided between the waves ---------------------------------------------
+// A workgroup takes 16 MB rows of x by 64 weight rows; its 8 waves deal the blocks of 128 k among them, read both
+// operands' fragments straight from memory (the next block's in flight) and sum through LDS. Through LDS tiles a
+// step of this size is a chain of latencies (0.47 us at 64 x 128 x 128, whatever its neighbours do).
+constexpr int kSomeWaves = 8, kSomePad = 68;  // (rows of sums 68 floats apart: 16 of them cover the LDS banks)
+template <class V8, int MB>
+__global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
+  __shared__ __align__(16) float red[kSomeWaves][16 * MB * kSomePad];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Kb = (p.K + 127) / 128, Mb = p.Mp / 16;
+  // row tiles run fastest: those that share weights are on one XCD at one time
+  const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, mb0 = (t - ng * p.mtiles) * MB;
+  const rsrc_t rw = make_rsrc(p.wq + (size_t)ng * Kb * 8192), rx = make_rsrc(p.xq + (size_t)mb0 * Kb * 2048);
+  const rsrc_t rs = make_rsrc(p.sx);
+  const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
+  struct Block {
+    i32x8 w[4], x[MB];
+    float s[MB], sw;
+  };
+  const auto load = [&](Block& k, int kb) {
+    kb = min(kb, Kb - 1);
+#pragma unroll
+    for (int j = 0; j < 4; j++) k.w[j] = bload_frag(rw, 16 * lane, kb * 8192 + 2048 * j);
+#pragma unroll
+    for (int b = 0; b < MB; b++) {  // (row blocks past the last: that one again, not stored)
+      const int r = min(b, Mb - 1 - mb0);
+      k.x[b] = bload_frag(rx, 16 * lane, (r * Kb + kb) * 2048);
+      k.s[b] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (lane & 15), 4 * (kb * p.Mp + 16 * (mb0 + r)), 0));
+    }
+    k.sw = sw[kb];
+  };
+  f32x4 acc[MB][4];
+#pragma unroll
+  for (int b = 0; b < MB; b++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const auto take = [&](const Block& k) {
+#pragma unroll
+    for (int b = 0; b < MB; b++) {
+      const float s = k.s[b] * k.sw;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x4 d = mfma_f8(k.w[j], k.x[b]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[b][j][e] = fmaf(s, d[e], acc[b][j][e]);
+      }
+    }
+  };
+  Block k0, k1;
+  if (wave < Kb) load(k0, wave);
+  for (int kb = wave; kb < Kb; kb += 2 * kSomeWaves) {
+    load(k1, kb + kSomeWaves);
+    take(k0);
+    if (kb + kSomeWaves >= Kb) break;
+    load(k0, kb + 2 * kSomeWaves);
+    take(k1);
+  }
+#pragma unroll
+  for (int b = 0; b < MB; b++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      *reinterpret_cast<f32x4*>(&red[wave][(16 * b + (lane & 15)) * kSomePad + 16 * (lane >> 4) + 4 * j]) = acc[b][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MB * 8; i += 64 * kSomeWaves) {  // 8 columns of a row each
+    const int r = i >> 3, c = 8 * (i & 7), m = 16 * mb0 + r, n = 64 * ng + c;
+    if (m >= p.M || n >= p.N) continue;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+    for (int w = 0; w < kSomeWaves; w++) {
+      a += *reinterpret_cast<const f32x4*>(&red[w][r * kSomePad + c]);
+      b += *reinterpret_cast<const f32x4*>(&red[w][r * kSomePad + c + 4]);
+    }
+    if (p.part) {
+      *reinterpret_cast<f32x4*>(p.part + (size_t)m * p.N + n) = a;
+      *reinterpret_cast<f32x4*>(p.part + (size_t)m * p.N + n + 4) = b;
+    } else {
+      V8 v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        v[e] = (decltype(+v[e]))a[e];
+        v[4 + e] = (decltype(+v[e]))b[e];
+      }
+      *reinterpret_cast<V8*>((uint16_t*)p.y + (size_t)m * p.N + n) = v;
+    }
+  }
+}
+
 // ---- many rows ----------------------------------------------------------------------------------
 // Workgroup tile of 16 MB WM rows of x by 64 WN weight rows, WM x WN waves of 16 MB x 64 each. A step is one
 // block of 128 k: x and weight pieces and each wave's row scales come by direct loads into a ring of S slots.
 template <class V8, int MB, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
-  constexpr int NW = WM * WN, kX = 2048 * MB * WM, kW = 8192 * WN, kScales = 64 * MB;  // bytes a slot
+  constexpr int NW = WM * WN, kX = 2048 * MB * WM, kW = 8192 * WN, kScales = 1024;  // bytes a slot
   constexpr int kSlot = kX + kW + NW * kScales;
   constexpr int kLoadsX = kX / 1024 / NW, kLoadsW = kW / 1024 / NW, kLoads = kLoadsX + kLoadsW + 1;
   static_assert(kLoadsX * NW * 1024 == kX && kLoadsW * NW * 1024 == kW, "whole loads per wave");
@@ -190,26 +312,24 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
   t -= split * tiles;
   const int group = t / (8 * p.ntiles), in = t - group * 8 * p.ntiles, gm = min(8, p.mtiles - 8 * group);
   const int mt = 8 * group + in % gm, nt = in / gm;
-  const int kb0 = (int)((long long)Kb * split / p.splits), kb1 = (int)((long long)Kb * (split + 1) / p.splits);
+  const int kb0 = Kb * split / p.splits, kb1 = Kb * (split + 1) / p.splits;  // (below 2^13 x 16)
   const int mb0 = mt * MB * WM, ng0 = nt * WN, Mb = p.Mp / 16, Ng = (p.N + 63) / 64;
-  const dma_src_t rx = dma_src(p.xq + (size_t)mb0 * Kb * 2048, (uint32_t)min(MB * WM, Mb - mb0) * (uint32_t)Kb * 2048u);
-  const dma_src_t rw = dma_src(p.wq + (size_t)ng0 * Kb * 8192, (uint32_t)min(WN, Ng - ng0) * (uint32_t)Kb * 8192u);
   const int row0 = 16 * (mb0 + MB * wm);  // this wave's first row
-  const dma_src_t rs = dma_src(p.sx + min(row0, p.Mp), (uint32_t)(4 * max(p.Mp - row0, 0)) + 4u * (uint32_t)p.Mp * (uint32_t)(Kb - 1));
+  const dma_src_t rx = dma_src(p.xq + (size_t)mb0 * Kb * 2048, kBufRange), rw = dma_src(p.wq + (size_t)ng0 * Kb * 8192, kBufRange);
+  const dma_src_t rs = dma_src(p.sx + min(row0, p.Mp - 16), kBufRange);
   const uint32_t base = lds_address(lds);
-  const auto load = [&](int kb, int slot) {
+  // load number i of this wave's kLoads for a block: pieces of x, pieces of the weights, its rows' scales
+  const auto load = [&](int kb, int slot, int i) {
     const uint32_t at = base + slot * kSlot;
-#pragma unroll
-    for (int i = 0; i < kLoadsX; i++) {
-      const int u = wave * kLoadsX + i;  // KB of the slot: row block u / 2, half u % 2
-      dma16(rx, at + 1024 * u, (uint32_t)((u >> 1) * Kb + kb) * 2048u + 1024u * (u & 1) + 16 * lane, 0);
+    if (i < kLoadsX) {  // (row blocks past the last: that one again, not stored)
+      const int u = wave * kLoadsX + i, r = min(u >> 1, Mb - 1 - mb0);  // KB u of the slot: row block u / 2, half u % 2
+      dma16(rx, at + 1024 * u, 16 * lane, (uint32_t)(r * Kb + kb) * 2048u + 1024u * (u & 1));
+    } else if (i < kLoadsX + kLoadsW) {
+      const int u = wave * kLoadsW + i - kLoadsX, r = min(u >> 3, Ng - 1 - ng0);
+      dma16(rw, at + kX + 1024 * u, 16 * lane, (uint32_t)(r * Kb + kb) * 8192u + 1024u * (u & 7));
+    } else {  // (past the last row: the next block's scales, or the 1 KB behind the last's)
+      dma16(rs, at + kX + kW + kScales * wave, 16 * lane, 4u * (uint32_t)p.Mp * (uint32_t)kb);
     }
-#pragma unroll
-    for (int i = 0; i < kLoadsW; i++) {
-      const int u = wave * kLoadsW + i;
-      dma16(rw, at + kX + 1024 * u, (uint32_t)((u >> 3) * Kb + kb) * 8192u + 1024u * (u & 7) + 16 * lane, 0);
-    }
-    if (lane < 4 * MB) dma16(rs, at + kX + kW + kScales * wave, 4u * (uint32_t)p.Mp * (uint32_t)kb + 16 * lane, 0);
   };
   f32x4 acc[MB][4];
 #pragma unroll
@@ -218,36 +338,68 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
     for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float* sw = p.sw + (size_t)(min(ng0 + wn, Ng - 1) >> 1) * Kb;
   const int n = kb1 - kb0;
+  // This wave's weight scales of 64 blocks, one a lane: a load per block would wait for every tile in flight. (The
+  // empty assembly has the wait here, not at each use.)
+  float sws;
+  const auto load_scales = [&](int i) {
+    sws = i + lane < n ? sw[kb0 + i + lane] : 0.f;
+    __asm__ volatile("" : "+v"(sws));
+  };
+  const auto frag = [&](const char* src) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  load_scales(0);
 #pragma unroll
-  for (int i = 0; i < S - 1; i++) load(min(kb0 + i, kb1 - 1), i);  // (past the last block: loaded again, not used)
+  for (int i = 0; i < S - 1; i++)
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) load(min(kb0 + i, kb1 - 1), i, u);  // (past the last block: loaded again, not used)
   for (int i = 0, slot = 0; i < n; i++, slot = slot + 1 == S ? 0 : slot + 1) {
     constexpr int kLeft = (S - 2) * kLoads;
+    if (i > 0 && (i & 63) == 0) load_scales(i);
     __builtin_amdgcn_s_waitcnt(0x0F70 | (kLeft & 15) | ((kLeft >> 4) << 14));  // vmcnt(kLeft): this block's loads are in
     __asm__ volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
-    load(min(kb0 + i + S - 1, kb1 - 1), slot == 0 ? S - 1 : slot - 1);
+    const int kn = min(kb0 + i + S - 1, kb1 - 1), next = slot == 0 ? S - 1 : slot - 1;
     const char* at = lds + slot * kSlot;
-    const float swk = sw[kb0 + i];
-    i32x8 w[4];
+    const char* xs = at + 2048 * MB * wm + 16 * lane;
+    const float* ss = reinterpret_cast<const float*>(at + kX + kW + kScales * wave) + (lane & 15);
+    const float swk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sws), i & 63));
+    // Loads of a later block are spread over the step: issued at once by all waves they keep every one of them from its
+    // first LDS read until the last is out (72 of 1 KB at 64 bytes a cycle).
+    constexpr int kSpread = (kLoads + (MB < 5 ? MB : 5) - 1) / (MB < 5 ? MB : 5);
+    // The fragment and scale of the next 16 rows are read, and the last 16 rows' results taken into the sums, between
+    // the matrix instructions of these.
+    i32x8 w[4], x = frag(xs), xn;
+    float s = ss[0], sn = 0.f, sp = 0.f;
+    f32x4 d[4], dp[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const char* src = at + kX + 8192 * wn + 2048 * j + 16 * lane;
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
-      w[j] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    }
+    for (int j = 0; j < 4; j++) w[j] = frag(at + kX + 8192 * wn + 2048 * j + 16 * lane);
 #pragma unroll
-    for (int b = 0; b < MB; b++) {
-      const char* src = at + 2048 * (MB * wm + b) + 16 * lane;
-      const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
-      const i32x8 x = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      const float s = swk * *reinterpret_cast<const float*>(at + kX + kW + kScales * wave + 4 * (16 * b + (lane & 15)));
+    for (int b = 0; b <= MB; b++) {
+      if (b + 1 < MB) {
+        xn = frag(xs + 2048 * (b + 1));
+        sn = ss[16 * (b + 1)];
+      }
+#pragma unroll
+      for (int u = kSpread * b; u < kSpread * (b + 1); u++)
+        if (u < kLoads) load(kn, next, u);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const f32x4 d = mfma_f8(w[j], x);
+        if (b < MB) d[j] = mfma_f8(w[j], x);
+        if (b > 0) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[b][j][e] = fmaf(s, d[e], acc[b][j][e]);
+          for (int e = 0; e < 4; e++) acc[b - 1][j][e] = fmaf(sp, dp[j][e], acc[b - 1][j][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int j = 0; j < 4; j++) dp[j] = d[j];
+      x = xn;
+      sp = swk * s;
+      s = sn;
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this slot's reads are back before the next barrier frees it
     __asm__ volatile("" ::: "memory");
@@ -358,20 +510,30 @@ static hipError_t launch_gemm(F8Args a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <class V8, int MB>
+static hipError_t launch_some(F8Args a, hipStream_t s) {
+  a.mtiles = (a.Mp / 16 + MB - 1) / MB;
+  ESM_LAUNCH((f8_some_kernel<V8, MB>), dim3((unsigned)((size_t)a.mtiles * ((a.N + 63) / 64))), dim3(64 * kSomeWaves), 0, s, a);
+  return hipGetLastError();
+}
+
 template <class V8>
-static hipError_t launch_f8_t(const F8Args& a, int form, hipStream_t s) {
+static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) {
   hipError_t e;
   if (form == kF8Few) {
     ESM_LAUNCH((f8_few_kernel<V8, 2>), dim3((a.N + 63) / 64 * 2), dim3(64 * kFewWaves), 0, s, a);
     return hipGetLastError();
   }
-  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, (a.K + 127) / 128), dim3(256), 0, s, (const uint16_t*)a.x, a.x_st,
-             a.xq, a.sx, a.M, a.K, a.Mp);
+  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, ((a.K + 127) / 128 + kQuantBlocks - 1) / kQuantBlocks), dim3(256), 0, s,
+             (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  if (form == kF8Big)
-    e = launch_gemm<V8, 8, 2, 4, 2>(a, s);
-  else
-    e = launch_gemm<V8, 2, 2, 2, 4>(a, s);
+  if (form == kF8Some) return mb == 2 ? launch_some<V8, 2>(a, s) : launch_some<V8, 4>(a, s);
+  switch (mb) {
+    case 2: e = launch_gemm<V8, 2, 2, 4, 2>(a, s); break;
+    case 4: e = launch_gemm<V8, 4, 2, 4, 2>(a, s); break;
+    case 6: e = launch_gemm<V8, 6, 2, 4, 2>(a, s); break;
+    default: e = launch_gemm<V8, 8, 2, 4, 2>(a, s); break;
+  }
   if (e != hipSuccess || !a.part || !a.y) return e;
   const size_t n8 = (size_t)a.M * a.N / 8, blocks = (n8 + 255) / 256;
   ESM_LAUNCH((f8_reduce_kernel<V8>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a.part, (uint16_t*)a.y, n8,
@@ -379,24 +541,37 @@ static hipError_t launch_f8_t(const F8Args& a, int form, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_f8_linear(const F8Args& a, bool bf16, int form, hipStream_t s) {
-  return bf16 ? launch_f8_t<bf16x8>(a, form, s) : launch_f8_t<half8>(a, form, s);
+hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipStream_t s) {
+  return bf16 ? launch_f8_t<bf16x8>(a, plan.form, plan.mb, s) : launch_f8_t<half8>(a, plan.form, plan.mb, s);
 }
 
+// Which form, its row blocks and splits: the lowest of estimated times, from these measurements (us, kernel alone,
+// K = 2560 -> N = 7680 unless said; some: 64 x 64 tiles without barriers; 64, 128, 192, 256: LDS tiles of that many rows):
+//   M = 238   some 13.8, 64 rows 18      M = 512   some 23, 64: 18.6, 128: 22, 256: 32
+//   M = 1000  some 44, 64: 36, 128: 24, 192: 27, 256: 33     M = 1500  128: 44, 192: 31, 256: 33
+//   M = 2000  128: 46, 192: 55, 256: 38    M = 3481  128: 90, 192: 86, 256: 70
+//   5120 -> 2560 at M = 238  some 11.1, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 19, 64 rows in two
+//   splits 21 and 5; at M = 1000  some 31, 64 rows 33, 128 rows in three splits 25 and 6
 F8Plan f8_plan(int M, int K, int N, int cus) {
-  F8Plan p{kF8Few, 1};
+  F8Plan p{kF8Few, 0, 1};
   if (M <= 16) return p;
-  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
-  if (big >= cus * 3 / 4) {
-    p.form = kF8Big;
-    return p;
-  }
-  p.form = kF8Mid;
-  const long long tiles = (long long)((M + 63) / 64) * ((N + 127) / 128);
   const int Kb = (K + 127) / 128;
-  long long sp = 2 * cus / tiles;
-  sp = sp < Kb / 4 ? sp : Kb / 4;
-  p.splits = (int)(sp < 1 ? 1 : sp > kF8MaxSplits ? kF8MaxSplits : sp);
+  const double tiles = (double)((M + 63) / 64) * ((N + 63) / 64);
+  p.form = kF8Some;
+  p.mb = M <= 32 || 2 * tiles < cus ? 2 : 4;
+  double best = 2.5 + 1.2e-3 * Kb * (tiles > cus ? tiles : cus) * cus / 256;
+  const struct { int mb; double step; } forms[] = {{2, 0.78}, {4, 1.0}, {6, 1.25}, {8, 1.55}};  // us a block of k
+  for (const auto& f : forms)
+    for (int sp = 1; sp <= kF8MaxSplits && (sp == 1 || 4 * sp <= Kb); sp++) {
+      const long long wgs = (long long)((M + 32 * f.mb - 1) / (32 * f.mb)) * ((N + 255) / 256) * sp, rounds = (wgs + cus - 1) / cus;
+      if (sp > 1 && rounds > 1) break;  // splits only fill one round
+      double c = rounds * (2.5 + f.step * ((Kb + sp - 1) / sp));
+      if (sp > 1) c += 3.0 + 8.0 * sp * M * N / 4.0e6;  // writing and summing the partials
+      if (c < best) {
+        best = c;
+        p = F8Plan{kF8Tiles, f.mb, sp};
+      }
+    }
   return p;
 }
 

@@ -202,9 +202,11 @@ struct F8Args {
   int splits, mtiles, ntiles;
 };
 constexpr int kF8MaxSplits = 16;
-enum : int { kF8Few = 0, kF8Mid = 1, kF8Big = 2 };
+enum : int { kF8Few = 0, kF8Some = 1, kF8Tiles = 2 };
 struct F8Plan {
-  int form, splits;
+  int form;
+  int mb;                 // 16-row blocks of x per wave
+  int splits;             // of K between workgroups (kF8Tiles)
 };
 
 struct ParcaeArgs {
@@ -295,7 +297,7 @@ hipError_t launch_qk_norm_rope(QkRopeArgs a, bool bf16, bool row, hipStream_t s)
 AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus);
 hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s);
 F8Plan f8_plan(int M, int K, int N, int cus);
-hipError_t launch_f8_linear(const F8Args& a, bool bf16, int form, hipStream_t s);
+hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipStream_t s);
 constexpr size_t f8_packed_size(int N, int K) { return (size_t)((N + 63) / 64) * ((K + 127) / 128) * 8192; }
 hipError_t launch_f8_pack(const uint8_t* q, uint8_t* out, int N, int K, hipStream_t s);
 hipError_t launch_f8_quantize_weight(const float* w, uint8_t* q, float* sw, int N, int K, hipStream_t s);

@@ -41,7 +41,8 @@ def test_against_the_definition(gpu_lib, pkg, K, N, dtype):
         assert bool((buf[:64] == 9.0).all() and (buf[64 + M * N:] == 9.0).all())
 
 
-@pytest.mark.parametrize("M,K,N", [(2049, 272, 8000), (4100, 640, 3584), (1000, 5120, 2560), (3481, 2560, 7680)])
+@pytest.mark.parametrize("M,K,N", [(2049, 272, 8000), (4100, 640, 3584), (1000, 5120, 2560), (3481, 2560, 7680),
+                                   (1000, 10240, 2560), (600, 8192, 1024), (530, 2576, 7688), (1010, 2560, 7680)])
 def test_many_rows(gpu_lib, pkg, M, K, N):
     x, w = _inputs(M, K, N, torch.bfloat16, seed=1)
     lin = pkg.f8.F8Linear.from_float(w)
