@@ -1016,9 +1016,10 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
   const int G = H / Hk;
   const esm::AttnPlan plan = esm::packed_attention_plan(Tq, Tk, n, Hk, G, d, cu_count());
   // grids of 256 threads stay below 2^32 threads, row numbers below 2^31
-  if ((long long)Tq * G >= (1LL << 31) - 256 || ((long long)Tq * G / 32 + n) * Hk * plan.splits >= (1LL << 24) ||
-      (plan.splits > 1 && (long long)Tq * H >= (1LL << 25)))
-    return fail(ESM_ERR_SHAPE, "packed_attention: n=%d Tq=%d H=%d too large", n, Tq, H);
+  if (Tk >= (1 << 30) || (long long)Tq * G >= (1LL << 31) - 256 || ((long long)Tq * G / 32 + n) * Hk >= (1LL << 24) ||
+      (!plan.many && esm::split_attention_items(Tq, Tk, n, G, plan.chunk) * Hk >= (1LL << 24)) ||
+      (plan.splits > 1 && (long long)Tq * H >= (1LL << 24)))
+    return fail(ESM_ERR_SHAPE, "packed_attention: n=%d Tq=%d Tk=%d H=%d too large", n, Tq, Tk, H);
   if (!q || !o || !cu_q || !cu_k || (Tk > 0 && (!k || !v))) return fail(ESM_ERR_NULL, "packed_attention: NULL pointer");
   for (const void* x : {q, k, v, (const void*)o})
     if (!aligned16(x)) return fail(ESM_ERR_ALIGN, "packed_attention: q, k, v and o must be 16-byte aligned");
@@ -1037,6 +1038,7 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
   a.cu_q = cu_q, a.cu_k = cu_k, a.n = n, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = G, a.d = d, a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.splits = plan.splits;
+  a.chunk = plan.chunk;
   if (need) {
     a.part_ml = static_cast<float*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + attention_ml_bytes(Tq, H, plan.splits));

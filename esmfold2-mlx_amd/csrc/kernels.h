@@ -179,15 +179,17 @@ struct PackedAttnArgs {
   int n, Tq, Tk, Hk, G, d;
   int causal;
   float scale_log2;       // scale * log2(e), > 0
-  int splits;             // of the few-row kernel
+  int chunk;              // keys per workgroup of the few-row kernel
+  int splits;             // chunks a sequence may have
   float* part_ml;         // [Tq, Hk * G, splits, 2] with more than one split
-  float* part_o;          // [Tq, Hk * G, splits, d]
+  float* part_o;          // [Tq, Hk * G, splits, d], or nullptr
 };
-constexpr int kAttnMaxSplits = 64;
+constexpr int kAttnMaxSplits = 256;
 struct AttnPlan {
-  bool many;              // packed_attention_kernel; else split_attention_kernel with `splits`
-  int splits;
+  bool many;              // packed_attention_kernel; else split_attention_kernel in chunks
+  int splits, chunk;
 };
+long long split_attention_items(long long Tq, long long Tk, int n, int G, int chunk);
 
 struct F8Args {
   const void* x;          // [M, K], 16-bit, rows x_st elements apart

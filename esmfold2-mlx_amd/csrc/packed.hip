@@ -196,16 +196,22 @@ struct Rows {
   }
 };
 
-// Sequence and tile of a work item: item counts the tiles of `unit` rows of all sequences in order. All lanes agree.
-// Starts outside 0 .. total are brought inside, so nothing a caller writes there reaches past the tensors.
-DEV bool find_tile(const int* cu, int n, int total, int G, int unit, int item, int lane, int& seq, int& tile) {
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + lane;
-    int nt = 0;
-    if (i < n) {
-      const int a = min(max(cu[i], 0), total), b = min(max(cu[i + 1], a), total);
-      nt = ((b - a) * G + unit - 1) / unit;
-    }
+struct Span {
+  int q0, nq, k0, nk;  // first row and rows of a sequence, on the query and on the key side
+};
+
+// Sequence of a work item and the item's number within it: a sequence has as many items as tiles of `unit` rows times
+// chunks of `chunk` keys (at least one; chunk 0: not counted). All lanes agree; the starts are read once, a lane a
+// sequence. Starts outside 0 .. the rows there are are brought inside, so nothing a caller writes there reaches past
+// the tensors.
+DEV bool find_item(const PackedAttnArgs& p, int unit, int chunk, int item, int lane, Span& s, int& at) {
+  for (int i0 = 0; i0 < p.n; i0 += 64) {
+    const int i = min(i0 + lane, p.n - 1);
+    const int a = min(max(p.cu_q[i], 0), p.Tq), b = min(max(p.cu_q[i + 1], a), p.Tq);
+    const int ka = min(max(p.cu_k[i], 0), p.Tk), kb = min(max(p.cu_k[i + 1], ka), p.Tk);
+    int nt = ((b - a) * p.G + unit - 1) / unit;
+    if (chunk) nt *= max(1, (kb - ka + chunk - 1) / chunk);
+    if (i0 + lane >= p.n) nt = 0;
     int sum = nt;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -215,29 +221,16 @@ DEV bool find_tile(const int* cu, int n, int total, int G, int unit, int item, i
     const uint64_t past = __ballot(item < sum);
     if (past) {
       const int w = __builtin_ctzll(past);
-      seq = i0 + w;
-      tile = item - __builtin_amdgcn_readlane(sum - nt, w);
+      at = item - __builtin_amdgcn_readlane(sum - nt, w);
+      s.q0 = __builtin_amdgcn_readlane(a, w);
+      s.nq = __builtin_amdgcn_readlane(b - a, w);
+      s.k0 = __builtin_amdgcn_readlane(ka, w);
+      s.nk = __builtin_amdgcn_readlane(kb - ka, w);
       return true;
     }
     item -= __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
-}
-
-struct Span {
-  int q0, nq, k0, nk;  // first row and rows of a sequence, on the query and on the key side
-};
-DEV Span span_of(const PackedAttnArgs& p, int seq) {
-  Span s;
-  const auto side = [&](const int* cu, int total, int& first, int& count) {
-    first = min(max(cu[seq], 0), total);
-    count = min(max(cu[seq + 1], first), total) - first;
-    first = __builtin_amdgcn_readfirstlane(first);
-    count = __builtin_amdgcn_readfirstlane(count);
-  };
-  side(p.cu_q, p.Tq, s.q0, s.nq);
-  side(p.cu_k, p.Tk, s.k0, s.nk);
-  return s;
 }
 
 // A tile of `keys` key rows from key kt of the span on, as a buffer whose range ends with the span's last row:
@@ -287,11 +280,10 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   // key heads run fastest over the workgroups: the eight XCDs take different heads, each with its own L2, and the
   // longest tiles of every head start first
   const int hk = blockIdx.x % p.Hk, item = blockIdx.x / p.Hk;
-  int seq, tile;
-  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, kAttnRows, item, lane, seq, tile)) return;
-  seq = __builtin_amdgcn_readfirstlane(seq);
+  Span s;
+  int tile;
+  if (!find_item(p, kAttnRows, 0, item, lane, s, tile)) return;
   tile = __builtin_amdgcn_readfirstlane(tile);
-  const Span s = span_of(p, seq);
   const int rows = s.nq * p.G;
   if (p.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
   const int row0 = kAttnRows * tile + 32 * wave;  // this wave's first row
@@ -351,14 +343,12 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
-// 32 rows per workgroup; its keys are the part of the sequence's that `split` of p.splits takes, in passes of
-// 4 x KW keys, KW to each wave in a private LDS tile. The waves' results are joined through LDS. With more
-// than one split each workgroup leaves (m, l, O) of its part in the workspace and attention_join_kernel sums them.
+// 32 rows and one chunk of p.chunk keys (of every sequence the same, so that a long one has many and workgroups
+// are alike) per workgroup, in passes of 4 x KW keys, KW to each wave in a private LDS tile. The waves' results are
+// joined through LDS. Where sequences may have more than one chunk (p.part_o) each workgroup leaves (m, l, O) of
+// its own in the workspace and attention_join_kernel sums them.
 template <int HD>
 constexpr int kSplitKeys = HD == 64 ? 64 : 32;  // keys per wave and pass: 64 KB of LDS, two workgroups per CU
-
-// Keys per split: a multiple of a pass, so that no split but the last is ragged.
-DEV int split_keys(int nk, int splits, int pass) { return ((nk + splits - 1) / splits + pass - 1) / pass * pass; }
 
 template <class T, int HD>
 __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs p) {
@@ -367,17 +357,16 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   __shared__ float ml[4][2][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int hk = blockIdx.x % p.Hk, split = (blockIdx.x / p.Hk) % p.splits, item = blockIdx.x / p.Hk / p.splits;
-  int seq, tile;
-  if (!find_tile(p.cu_q, p.n, p.Tq, p.G, 32, item, lane, seq, tile)) return;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  const Span s = span_of(p, seq);
-  const int rows = s.nq * p.G, row0 = 32 * tile;
-  const int part = split_keys(s.nk, p.splits, kPass), first = part * split;
+  const int hk = blockIdx.x % p.Hk, item = blockIdx.x / p.Hk;
+  Span s;
+  int at;
+  if (!find_item(p, 32, p.chunk, item, lane, s, at)) return;
+  at = __builtin_amdgcn_readfirstlane(at);
+  const int rows = s.nq * p.G, tiles = (rows + 31) / 32, chunk = at / tiles, row0 = 32 * (at - chunk * tiles);
+  const int first = chunk * p.chunk;
   const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
-  const int end = min(seen(row0 + 31), first + part), wfull = seen(row0);
-  if (p.splits > 1 && first > 0 && first >= s.nk) return;  // no part of this sequence: the join reads none
+  const int last = seen(row0 + 31), end = min(last, first + min(p.chunk, s.nk - first)), wfull = seen(row0);
+  if (chunk > 0 && first >= last) return;  // nothing seen: the join reads none
 
   Rows<T, HD> w;
   w.init();
@@ -437,21 +426,11 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   }
   const long long q = s.q0 + i;
   const int head = hk * p.G + g;
-  if (p.splits > 1) {
-    const size_t at = ((size_t)q * (p.G * p.Hk) + head) * p.splits + split;
-    if (wave == 0 && h == 0) {
-      p.part_ml[2 * at] = M;
-      p.part_ml[2 * at + 1] = L;
-    }
-#pragma unroll
-    for (int u = 0; u < HD / 32; u++) {
-      const int qd = wave + 4 * u, col = 32 * (qd >> 2) + acc_row32(4 * (qd & 3), lane);
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int v = 0; v < 4; v++) acc += sc[v] * reinterpret_cast<const f32x4*>(lds[v])[qd * 64 + lane];
-      if (col < p.d) *reinterpret_cast<f32x4*>(p.part_o + at * p.d + col) = acc;
-    }
-    return;
+  const bool part = p.part_o != nullptr;
+  const size_t pat = ((size_t)q * (p.G * p.Hk) + head) * p.splits + chunk;
+  if (part && wave == 0 && h == 0) {
+    p.part_ml[2 * pat] = M;
+    p.part_ml[2 * pat + 1] = L;
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   char* dst = (char*)p.o + 2 * (q * p.o_st + (long long)head * p.o_sh);
@@ -461,63 +440,83 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < 4; v++) acc += sc[v] * reinterpret_cast<const f32x4*>(lds[v])[qd * 64 + lane];
-    typename T::v4 y;
+    if (col >= p.d) continue;
+    if (part) {
+      *reinterpret_cast<f32x4*>(p.part_o + pat * p.d + col) = acc;
+    } else {
+      typename T::v4 y;
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
-    if (col < p.d) *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
+      for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
+      *reinterpret_cast<typename T::v4*>(dst + 2 * col) = y;
+    }
   }
 }
 
-// The splits of one (query, head) row: a wave reads their m and l in its lanes, then sums O over them, 4 columns a
-// lane (lanes beyond d / 4 take every other split).
+// The chunks of one (query, head) row, a workgroup each: a thread takes one chunk's m and l (kAttnMaxSplits of them at
+// most), then groups of d / 4 lanes sum O over every 256 / (HD / 4)-th chunk, joined through LDS.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, H = p.G * p.Hk;
-  const long long at = (long long)blockIdx.x * 4 + wave;
-  if (at >= (long long)p.Tq * H) return;
-  const int q = (int)(at / H), head = (int)(at - (long long)q * H);
-  int seq = -1;  // the sequence of this row, if any
-  for (int i0 = 0; i0 < p.n && seq < 0; i0 += 64) {
-    const int i = i0 + lane;
-    bool in = false;
-    if (i < p.n) {
-      const int a = min(max(p.cu_q[i], 0), p.Tq), b = min(max(p.cu_q[i + 1], a), p.Tq);
-      in = q >= a && q < b;
+  static_assert(kAttnMaxSplits <= 256, "a chunk a thread");
+  __shared__ float weight[256], red[2][4];
+  __shared__ __align__(16) float sums[4][HD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, H = p.G * p.Hk;
+  const int q = blockIdx.x / H, head = blockIdx.x - q * H;
+  Span s;
+  bool found = false;
+  for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
+    const int i = min(i0 + lane, p.n - 1);
+    const int a = min(max(p.cu_q[i], 0), p.Tq), b = min(max(p.cu_q[i + 1], a), p.Tq);
+    const int ka = min(max(p.cu_k[i], 0), p.Tk), kb = min(max(p.cu_k[i + 1], ka), p.Tk);
+    const uint64_t hit = __ballot(q >= a && q < b);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      s = Span{__builtin_amdgcn_readlane(a, w), __builtin_amdgcn_readlane(b - a, w), __builtin_amdgcn_readlane(ka, w),
+               __builtin_amdgcn_readlane(kb - ka, w)};
+      found = true;
     }
-    const uint64_t hit = __ballot(in);
-    if (hit) seq = i0 + __builtin_ctzll(hit);
   }
-  if (seq < 0) return;  // behind the last sequence: left as it is
-  const Span s = span_of(p, seq);
-  const int part = split_keys(s.nk, p.splits, 4 * kSplitKeys<HD>);
-  const int live = s.nk > 0 ? (s.nk + part - 1) / part : 1;  // splits that wrote (at most 64)
-  const float* pm = p.part_ml + 2 * (size_t)at * p.splits;
-  float m = lane < live ? pm[2 * lane] : -INFINITY, l = lane < live ? pm[2 * lane + 1] : 0.f;
+  if (!found) return;  // behind the last sequence: left as it is
+  // chunks that wrote: those that the row's tile sees, or the first
+  const int rows = s.nq * p.G, last = min(((q - s.q0) * p.G + head % p.G) | 31, rows - 1);
+  const int seen = p.causal ? max(min(s.nk, last / p.G + s.nk - s.nq + 1), 0) : s.nk;
+  const int live = max(1, (seen + p.chunk - 1) / p.chunk);
+  const size_t at = (size_t)blockIdx.x * p.splits;
+  const float m = t < live ? p.part_ml[2 * (at + t)] : -INFINITY, l = t < live ? p.part_ml[2 * (at + t) + 1] : 0.f;
   float M = m;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+  if (lane == 0) red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float sc = __builtin_amdgcn_exp2f((m - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
-  float L = lane < live ? sc * l : 0.f;
+  weight[t] = t < live ? sc : 0.f;
+  float L = t < live ? sc * l : 0.f;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) L += __shfl_xor(L, o);
-  constexpr int kCols = HD / 4, kSide = 64 / kCols;  // lanes across a row, splits at once
-  const int col = 4 * (lane % kCols), side = lane / kCols;
-  const float* po = p.part_o + (size_t)at * p.splits * p.d;
+  if (lane == 0) red[1][wave] = L;
+  __syncthreads();
+  L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  constexpr int kCols = HD / 4, kSide = 256 / kCols;  // lanes across a row, chunks at once
+  const int col = 4 * (t % kCols), side = t / kCols;
+  const float* po = p.part_o + at * p.d;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < live; j0 += kSide) {
-    const int j = j0 + side;
-    const float f = __shfl(sc, j & 63);
-    if (j < live && col < p.d) acc += f * *reinterpret_cast<const f32x4*>(po + (size_t)j * p.d + col);
-  }
+#pragma unroll 4
+  for (int j = side; j < live; j += kSide)
+    if (col < p.d) acc += weight[j] * *reinterpret_cast<const f32x4*>(po + (size_t)j * p.d + col);
 #pragma unroll
   for (int o = kCols; o < 64; o <<= 1)
 #pragma unroll
     for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o);
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  if (side == 0 && col < p.d) {
+  if (lane < kCols) *reinterpret_cast<f32x4*>(&sums[wave][col]) = acc;
+  __syncthreads();
+  if (t < kCols && col < p.d) {
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    f32x4 a = *reinterpret_cast<const f32x4*>(&sums[0][col]);
+#pragma unroll
+    for (int v = 1; v < 4; v++) a += *reinterpret_cast<const f32x4*>(&sums[v][col]);
     typename T::v4 y;
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
+    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(a[e] * inv);
     *reinterpret_cast<typename T::v4*>((char*)p.o + 2 * ((long long)q * p.o_st + (long long)head * p.o_sh + col)) = y;
   }
 }
@@ -529,29 +528,44 @@ static hipError_t launch_attention_t(const PackedAttnArgs& a, bool many, hipStre
     ESM_LAUNCH((packed_attention_kernel<T, HD>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
     return hipGetLastError();
   }
-  const long long items = (long long)a.Tq * a.G / 32 + a.n;
-  ESM_LAUNCH((split_attention_kernel<T, HD>), dim3((unsigned)(items * a.Hk * a.splits)), dim3(256), 0, s, a);
+  ESM_LAUNCH((split_attention_kernel<T, HD>), dim3((unsigned)(split_attention_items(a.Tq, a.Tk, a.n, a.G, a.chunk) * a.Hk)),
+             dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  const long long rows = (long long)a.Tq * a.G * a.Hk;
-  ESM_LAUNCH((attention_join_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  if (e != hipSuccess || !a.part_o) return e;
+  ESM_LAUNCH((attention_join_kernel<T, HD>), dim3((unsigned)(a.Tq * a.G * a.Hk)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
-// Which kernel and how many splits, from what the host knows: rows, keys, sequences and heads (the lengths are on
-// the device). `cus` compute units.
+// Work items of the few-row kernel per key head, at most: (tiles, chunks) pairs of all sequences.
+long long split_attention_items(long long Tq, long long Tk, int n, int G, int chunk) {
+  const long long tiles = Tq * G / 32 + n, chunks = Tk / chunk + n;  // of all sequences
+  const long long a = tiles * ((Tk + chunk - 1) / chunk + 1), b = ((Tq * G + 31) / 32) * chunks;  // (one may have all of either)
+  return a < b ? a : b;
+}
+
+// Which kernel and which chunk of keys, from what the host knows: rows, keys, sequences and heads (the lengths are on
+// the device).
 AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus) {
   AttnPlan plan{};
-  const long long tiles = (Tq * G / 256 + 1) * Hk;  // at least this many tiles of 256 rows, if the sequences are long
-  plan.many = tiles >= cus / 2 && Tq / n * G >= 64;
-  plan.splits = 1;
-  if (!plan.many) {
-    const long long small = (Tq * G / 32 + n) * Hk, pass = d <= 64 ? 256 : 128;
-    long long sp = 4 * cus / (small > 0 ? small : 1);
-    // a sequence may hold nearly all keys: its splits are what matters, the others' are empty
-    if (n > 1) sp *= 4;
-    sp = sp < Tk / pass ? sp : Tk / pass;
-    plan.splits = (int)(sp < 1 ? 1 : sp > kAttnMaxSplits ? kAttnMaxSplits : sp);
+  // The many-row kernel where its tiles of 128 rows make some 5/8 of a workgroup per CU (us, many / few rows: 40 heads
+  // of 64, 300 tokens 10.3 / 9.8, 512 tokens 12.3 / 13.6, 1,100 tokens 28 / 38; causal, 32/8 heads of 128, 512 tokens
+  // 19 / 13, 1,024 tokens 29 / 30, 2,048 tokens 57 / 78; 512 new tokens on 8,192 163 / 107), or the sequences are short
+  // on both sides (one of 24 tokens 4.8 / 6.0, 64 of 100 tokens 35 / 136; 64 single tokens on 100 keys 10.5 / 8.6).
+  const long long per = Tq * G / n;
+  plan.many = (Tq * G / 128 * Hk * 8 >= 5 * cus && per >= 64) || (Tk / n <= 128 && per >= 16);
+  const int pass = d <= 64 ? 256 : 128;
+  // as many chunks as make some four workgroups per CU, of two passes at least
+  const long long rows = Tq * G / 32 + 1 < n ? n : Tq * G / 32 + 1;  // row tiles, about
+  long long chunk = (Tk * Hk * ((rows + n - 1) / n) + 4 * cus - 1) / (4 * cus);
+  const long long least = (Tk + kAttnMaxSplits - 1) / kAttnMaxSplits;
+  chunk = chunk < least ? least : chunk;
+  chunk = (chunk + pass - 1) / pass * pass;
+  if (plan.many || chunk < 2 * pass) chunk = chunk < 2 * pass && !plan.many ? 2 * pass : chunk;
+  plan.splits = (int)((Tk + chunk - 1) / chunk);
+  plan.chunk = (int)chunk;
+  if (plan.many || plan.splits <= 1 || rows * Hk >= 2 * cus) {  // one chunk for all
+    plan.splits = 1;
+    plan.chunk = 1 << 30;
   }
   return plan;
 }
