@@ -94,63 +94,129 @@ struct Rows {
       for (int i = 0; i < 16; i++) o[d][i] = 0.f;
   }
 
+  enum { kNone, kEnd, kLater };
   bool odd;  // values taken as 0 by a masked step (``add_odd`` makes up for the seen ones)
 
-  // Keys key0 .. key0 + 32 NKB - 1 of the sequence from LDS rows ks, vs. MASKED: some row sees only a part of them,
-  // and what the others hold must not count: their scores are replaced, and as a p of 0 does not silence an infinity or
-  // a NaN in V, all values that are one are taken as 0.
-  template <int NKB, bool MASKED>
+  // 32 keys key0 .. of the sequence from LDS rows ks, vs, of which some row sees only a part. kEnd: the unseen ones lie
+  // behind the sequence, their rows are zeros. kLater: some are the sequence's own later keys; what they hold must
+  // not count, and as a p of 0 does not silence an infinity or a NaN in V, all values that are one are taken as 0.
+  // kNone: all are seen.
+  template <int MASK>
   DEV void step(const char* ks, const char* vs, int key0, float c, int lane) {
+    constexpr bool MASKED = MASK != kNone;
     const int r = lane & 31, h = lane >> 5;
-    f32x16 s[NKB];
+    f32x16 s;
 #pragma unroll
-    for (int kb = 0; kb < NKB; kb++) {
+    for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i++) s[kb][i] = 0.f;
-      const char* kr = ks + (32 * kb + r) * 2 * HD;
-#pragma unroll
-      for (int k = 0; k < HD / 16; k++)
-        s[kb] = T::mfma(*reinterpret_cast<const typename T::v8*>(kr + 16 * k_piece<HD>(r, 2 * k + h)), q[k], s[kb]);
-    }
+    for (int k = 0; k < HD / 16; k++)
+      s = T::mfma(*reinterpret_cast<const typename T::v8*>(ks + r * 2 * HD + 16 * k_piece<HD>(r, 2 * k + h)), q[k], s);
     if (MASKED) {
 #pragma unroll
-      for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[kb][i] = key0 + 32 * kb + acc_row32(i, lane) <= lim ? s[kb][i] : -INFINITY;
+      for (int i = 0; i < 16; i++) s[i] = key0 + acc_row32(i, lane) <= lim ? s[i] : -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kb][i]);
+    for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any((mx - m) * c > kGrow)) {  // (from m = -inf at the first key a row sees)
-      const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-      const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] *= alpha;
-    }
+    if (__any((mx - m) * c > kGrow)) grow(mx, c);  // (from m = -inf at the first key a row sees)
     const float mc = MASKED && lim < key0 ? 0.f : m * c;  // (m may be -inf where no key has been seen)
-    typename T::v8 p[2 * NKB];
+    typename T::v8 p[2];
 #pragma unroll
-    for (int kb = 0; kb < NKB; kb++)
+    for (int i = 0; i < 16; i++)  // (results below 2^-126 flush)
+      p[i >> 3][i & 7] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(s[i], c, -mc));
 #pragma unroll
-      for (int i = 0; i < 16; i++)  // (results below 2^-126 flush)
-        p[2 * kb + (i >> 3)][i & 7] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -mc));
+    for (int j = 0; j < 2; j++) l = T::add(p[j], l);
 #pragma unroll
-    for (int j = 0; j < 2 * NKB; j++) l = T::add(p[j], l);
-#pragma unroll
-    for (int j = 0; j < 2 * NKB; j++)
+    for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int d = 0; d < HD / 32; d++) {
         typename T::v8 v = v_frag<T, HD>(vs, j, d, lane);
-        if (MASKED) v = finite(v);
+        if (MASK == kLater) v = finite(v);
         o[d] = T::mfma(v, p[j], o[d]);
       }
+  }
+
+  // 64 keys that every row sees, in an order that the scheduler keeps: a fragment is read some matrix instructions
+  // before its own (LDS answers in more than 64 cycles, one takes 32), the maximum of the first 32 keys is taken
+  // between those of the next 32, and the exponentials of the second half between the value products of the first.
+  DEV void step64(const char* ks, const char* vs, float c, int lane) {
+    constexpr int NK = HD / 16, ND = HD / 32;
+    typedef typename T::v8 v8;
+    const int r = lane & 31, h = lane >> 5;
+    const auto key = [&](int kb, int k) {
+      return *reinterpret_cast<const v8*>(ks + (32 * kb + r) * 2 * HD + 16 * k_piece<HD>(r, 2 * k + h));
+    };
+    f32x16 s0, s1;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s0[i] = s1[i] = 0.f;
+    v8 ka[NK], kb[NK], va[ND], vb[ND];
+#pragma unroll
+    for (int k = 0; k < NK; k++) ka[k] = key(0, k);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+      s0 = T::mfma(ka[k], q[k], s0);
+      kb[k] = key(1, k);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+      s1 = T::mfma(kb[k], q[k], s1);
+      if (k < ND) va[k] = v_frag<T, HD>(vs, 0, k, lane);
+      if (k > 0) {  // (its results are there by then)
+#pragma unroll
+        for (int i = 16 * (k - 1) / (NK - 1); i < 16 * k / (NK - 1); i++) mx = fmaxf(mx, s0[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any((mx - m) * c > kGrow)) grow(mx, c);
+    const float mc = m * c;
+    v8 p[4];
+    const auto prob = [&](int i) {  // probabilities 2i, 2i + 1 of 32 (results below 2^-126 flush)
+      const f32x16& s = i < 8 ? s0 : s1;
+      p[i >> 2][2 * (i & 3)] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(s[2 * i & 15], c, -mc));
+      p[i >> 2][2 * (i & 3) + 1] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(s[(2 * i & 15) + 1], c, -mc));
+    };
+#pragma unroll
+    for (int i = 0; i < 8; i++) prob(i);
+    l = T::add(p[0], l);
+    l = T::add(p[1], l);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2 * ND; u++) {  // values of keys 0 .. 31
+      const int j = u / ND, d = u % ND;
+      o[d] = T::mfma(j ? vb[d] : va[d], p[j], o[d]);
+      (j ? va : vb)[d] = v_frag<T, HD>(vs, j + 1, d, lane);
+#pragma unroll
+      for (int i = 8 * u / (2 * ND); i < 8 * (u + 1) / (2 * ND); i++) prob(8 + i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l = T::add(p[2], l);
+    l = T::add(p[3], l);
+#pragma unroll
+    for (int u = 0; u < 2 * ND; u++) {  // and 32 .. 63
+      const int j = u / ND, d = u % ND;
+      o[d] = T::mfma(j ? vb[d] : va[d], p[2 + j], o[d]);
+      if (!j) vb[d] = v_frag<T, HD>(vs, 3, d, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The row's maximum has grown to mx: everything summed so far by the new one.
+  DEV void grow(float mx, float c) {
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[d][i] *= alpha;
   }
 
   DEV typename T::v8 finite(typename T::v8 x) {
@@ -253,7 +319,7 @@ DEV void load_rows(dma_src_t src, uint32_t lds, long long st, int d, int n0, int
 }
 
 // Query fragments and the limit of row `row` (of the span's nq * G).
-template <class T, int HD>
+template <class T, int HD, bool CAUSAL>
 DEV void load_queries(Rows<T, HD>& w, const PackedAttnArgs& p, const Span& s, int hk, int row0, int lane) {
   const int h = lane >> 5, row = row0 + (lane & 31), i = row / p.G, g = row - i * p.G;
   const bool ok = i < s.nq;
@@ -263,18 +329,15 @@ DEV void load_queries(Rows<T, HD>& w, const PackedAttnArgs& p, const Span& s, in
     w.q[k] = typename T::v8{};
     if (ok && 16 * k + 8 * h < p.d) w.q[k] = *reinterpret_cast<const typename T::v8*>(src + 2 * (16 * k + 8 * h));
   }
-  w.lim = p.causal && ok ? min(s.nk - 1, i + s.nk - s.nq) : s.nk - 1;
+  w.lim = CAUSAL && ok ? min(s.nk - 1, i + s.nk - s.nq) : s.nk - 1;
 }
 
 constexpr int kAttnKeys = 64;   // keys per tile of the many-row kernel
 constexpr int kAttnRows = 128;  // rows per workgroup
 
-template <class T, int HD>
+template <class T, int HD, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs p) {
   constexpr int kTile = kAttnKeys * 2 * HD;  // bytes of a K (or V) tile
-  // 32-key blocks per step: two share one maximum and its check (16,384 causal rows of 32 heads of 128 2.15 -> 2.09
-  // ms); at 64 columns the registers of one leave room for another wave (a batch of proteins 45.7 -> 42.1 us)
-  constexpr int kStep = HD == 64 ? 1 : 2;
   __shared__ __align__(1024) char lds[2][2 * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // key heads run fastest over the workgroups: the eight XCDs take different heads, each with its own L2, and the
@@ -285,14 +348,14 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   if (!find_item(p, kAttnRows, 0, item, lane, s, tile)) return;
   tile = __builtin_amdgcn_readfirstlane(tile);
   const int rows = s.nq * p.G;
-  if (p.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
+  if (CAUSAL) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
   const int row0 = kAttnRows * tile + 32 * wave;  // this wave's first row
 
   Rows<T, HD> w;
   w.init();
-  load_queries(w, p, s, hk, row0, lane);
+  load_queries<T, HD, CAUSAL>(w, p, s, hk, row0, lane);
   // keys seen by the workgroup's last row, by this wave's last row, and by its first
-  const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
+  const auto seen = [&](int row) { return CAUSAL ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
   const int end = seen(kAttnRows * (tile + 1) - 1);
   const int wend = row0 < rows ? seen(row0 + 31) : 0;
   const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
@@ -311,19 +374,19 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
     wait_vm(0);
     __syncthreads();  // this tile is in, and every wave has left the other buffer
     if (kt + kAttnKeys < end) load(kt + kAttnKeys, buf ^ 1);
-#pragma unroll
-    for (int u = 0; u < kAttnKeys; u += 32 * kStep)
-      w.template step<kStep, false>(lds[buf] + u * 2 * HD, lds[buf] + kTile + u * 2 * HD, kt + u, p.scale_log2, lane);
+    w.step64(lds[buf], lds[buf] + kTile, p.scale_log2, lane);
   }
   for (; kt < end; kt += kAttnKeys, buf ^= 1) {
     wait_vm(0);
     __syncthreads();
     if (kt + kAttnKeys < end) load(kt + kAttnKeys, buf ^ 1);
 #pragma unroll 1
-    for (int u = 0; u < kAttnKeys && kt + u < wend; u += 32)
-      w.template step<1, true>(lds[buf] + u * 2 * HD, lds[buf] + kTile + u * 2 * HD, kt + u, p.scale_log2, lane);
+    for (int u = 0; u < kAttnKeys && kt + u < wend; u += 32) {
+      const char *ks = lds[buf] + u * 2 * HD, *vs = ks + kTile;
+      w.template step<CAUSAL ? Rows<T, HD>::kLater : Rows<T, HD>::kEnd>(ks, vs, kt + u, p.scale_log2, lane);
+    }
   }
-  if (__any(w.odd)) w.add_odd(vb + 2 * p.v_st * s.k0, p.v_st, p.d, whole, wend, lane);
+  if (CAUSAL && __any(w.odd)) w.add_odd(vb + 2 * p.v_st * s.k0, p.v_st, p.d, whole, wend, lane);
 
   const float l = w.l + __shfl_xor(w.l, 32);
   const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key is 0
@@ -350,7 +413,7 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
 template <int HD>
 constexpr int kSplitKeys = HD == 64 ? 64 : 32;  // keys per wave and pass: 64 KB of LDS, two workgroups per CU
 
-template <class T, int HD>
+template <class T, int HD, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs p) {
   constexpr int KW = kSplitKeys<HD>, kTile = KW * 2 * HD, kPass = 4 * KW;
   __shared__ __align__(1024) char lds[4][2 * kTile];
@@ -364,13 +427,13 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   at = __builtin_amdgcn_readfirstlane(at);
   const int rows = s.nq * p.G, tiles = (rows + 31) / 32, chunk = at / tiles, row0 = 32 * (at - chunk * tiles);
   const int first = chunk * p.chunk;
-  const auto seen = [&](int row) { return p.causal ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
+  const auto seen = [&](int row) { return CAUSAL ? max(min(s.nk, min(row, rows - 1) / p.G + s.nk - s.nq + 1), 0) : s.nk; };
   const int last = seen(row0 + 31), end = min(last, first + min(p.chunk, s.nk - first)), wfull = seen(row0);
   if (chunk > 0 && first >= last) return;  // nothing seen: the join reads none
 
   Rows<T, HD> w;
   w.init();
-  load_queries(w, p, s, hk, row0, lane);
+  load_queries<T, HD, CAUSAL>(w, p, s, hk, row0, lane);
   const char* kb = (const char*)p.k + 2 * (long long)hk * p.k_sh;
   const char* vb = (const char*)p.v + 2 * (long long)hk * p.v_sh;
   char *ks = lds[wave], *vs = lds[wave] + kTile;
@@ -385,16 +448,17 @@ __global__ __launch_bounds__(256, 2) void split_attention_kernel(PackedAttnArgs 
   for (; kt < end && kt + KW <= wfull; kt += kPass) {
     load(kt);
 #pragma unroll
-    for (int u = 0; u < KW; u += 32) w.template step<1, false>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2, lane);
+    for (int u = 0; u < KW; u += 32) w.template step<Rows<T, HD>::kNone>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2, lane);
   }
   const int masked = kt;
   for (; kt < end; kt += kPass) {
     load(kt);
 #pragma unroll 1
     for (int u = 0; u < KW && kt + u < end; u += 32)
-      w.template step<1, true>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2, lane);
+      w.template step<CAUSAL ? Rows<T, HD>::kLater : Rows<T, HD>::kEnd>(ks + u * 2 * HD, vs + u * 2 * HD, kt + u, p.scale_log2,
+                                                                         lane);
   }
-  if (__any(w.odd))
+  if (CAUSAL && __any(w.odd))
     for (kt = masked; kt < end; kt += kPass) w.add_odd(vb + 2 * p.v_st * s.k0, p.v_st, p.d, kt, min(kt + KW, end), lane);
 
   // (m, l, O) of the four waves through LDS; wave i then joins the d quads i, i + 4, .. of every row
@@ -521,14 +585,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
   }
 }
 
-template <class T, int HD>
+template <class T, int HD, bool CAUSAL>
 static hipError_t launch_attention_t(const PackedAttnArgs& a, bool many, hipStream_t s) {
   if (many) {
     const long long items = (long long)a.Tq * a.G / kAttnRows + a.n;
-    ESM_LAUNCH((packed_attention_kernel<T, HD>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
+    ESM_LAUNCH((packed_attention_kernel<T, HD, CAUSAL>), dim3((unsigned)(items * a.Hk)), dim3(256), 0, s, a);
     return hipGetLastError();
   }
-  ESM_LAUNCH((split_attention_kernel<T, HD>), dim3((unsigned)(split_attention_items(a.Tq, a.Tk, a.n, a.G, a.chunk) * a.Hk)),
+  ESM_LAUNCH((split_attention_kernel<T, HD, CAUSAL>), dim3((unsigned)(split_attention_items(a.Tq, a.Tk, a.n, a.G, a.chunk) * a.Hk)),
              dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.part_o) return e;
@@ -570,9 +634,14 @@ AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G,
   return plan;
 }
 
+template <class T>
+static hipError_t launch_attention(const PackedAttnArgs& a, bool many, hipStream_t s) {
+  if (a.d <= 64) return a.causal ? launch_attention_t<T, 64, true>(a, many, s) : launch_attention_t<T, 64, false>(a, many, s);
+  return a.causal ? launch_attention_t<T, 128, true>(a, many, s) : launch_attention_t<T, 128, false>(a, many, s);
+}
+
 hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s) {
-  if (a.d <= 64) return bf16 ? launch_attention_t<Bf16, 64>(a, many, s) : launch_attention_t<Fp16, 64>(a, many, s);
-  return bf16 ? launch_attention_t<Bf16, 128>(a, many, s) : launch_attention_t<Fp16, 128>(a, many, s);
+  return bf16 ? launch_attention<Bf16>(a, many, s) : launch_attention<Fp16>(a, many, s);
 }
 
 }  // namespace esm

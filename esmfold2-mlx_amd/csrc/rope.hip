@@ -213,10 +213,13 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_norm_rope_kernel(QkRopeArg
 
 template <class V8, bool ROW>
 static hipError_t launch_rope_t(const QkRopeArgs& a, int groups, hipStream_t s) {
-  // over the row one workgroup takes all heads; over each head a workgroup takes up to four waves' groups
-  const int nit = ROW ? (groups + kRopeWaves - 1) / kRopeWaves : groups >= 4 && a.T >= 512 ? 2 : 1;
-  const int waves = ROW ? (groups + nit - 1) / nit : groups < 4 * nit ? (groups + nit - 1) / nit : 4;
-  const dim3 grid(a.T, ROW ? 1 : (groups + waves * nit - 1) / (waves * nit)), block(64 * waves);
+  // Over the row one workgroup takes all heads; over each head a workgroup takes up to four waves' groups. With
+  // rows enough to fill the GPU a wave takes several groups for its angles (16,384 rows of 32 + 8 heads of 128: one
+  // group a wave 81, two 74, three 85 us; 3,481 rows of 40 + 40 heads of 64 over the row: 22.8, 20.8, 20.1).
+  const int need = ROW ? (groups + kRopeWaves - 1) / kRopeWaves : 1, want = a.T < 512 ? 1 : ROW ? 3 : 2;
+  const int nit = need > want ? need : want < groups ? want : groups;
+  const int per = (groups + nit - 1) / nit, gy = ROW ? 1 : (per + 3) / 4, waves = (per + gy - 1) / gy;
+  const dim3 grid(a.T, gy), block(64 * waves);
   switch (nit) {
     case 1: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 1>), grid, block, 0, s, a); break;
     case 2: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 2>), grid, block, 0, s, a); break;
