@@ -25,6 +25,7 @@ from torch.nn.modules.module import _has_any_global_hook
 
 from . import kernels
 from .q8 import Q8Linear
+from .rotary import Rotary
 
 EPS = 1e-5
 LINEARS = ("wqkv", "wo", "w1", "w2")
@@ -46,16 +47,17 @@ HF_NORMS = {"ln1_w": "input_layernorm.weight", "ln1_b": "input_layernorm.bias", 
 _LAYER_KEY = re.compile(r"layers\.(\d+)\.([A-Za-z0-9_]+)")
 
 
-def hf_layer(tensors, i: int, device=None) -> tuple[dict, dict]:
+def hf_layer(tensors, i: int, device=None, linear=Q8Linear) -> tuple[dict, dict]:
     """One block from the published HF-named fp32 tensors (``tensors[f"esmc.layers.{i}.{name}"]``):
     (LayerNorm parameters by cache name, {linear: Q8Linear}), each linear quantised on the GPU
-    from fp32 with MLX's affine 8-bit scheme (layer_params, mlx_esmc.py:53-75)."""
+    from fp32 with MLX's affine 8-bit scheme (layer_params, mlx_esmc.py:53-75), or as ``linear``
+    (``F8Linear``) has it."""
     get = lambda name: tensors[f"esmc.layers.{i}.{name}"]  # noqa: E731
     ln = {n: get(h).detach().float() for n, h in HF_NORMS.items()}
     lin = {}
     for n, parts in HF_LINEARS.items():
         w = torch.cat([get(h).detach().float() for h in parts]) if len(parts) > 1 else get(parts[0]).detach().float()
-        lin[n] = Q8Linear.from_float(w, device=device)
+        lin[n] = linear.from_float(w, device=device)
     return ln, lin
 
 
@@ -81,7 +83,7 @@ class EsmcBlock(nn.Module):
                      ("ln2_b", ln2_b)):
             self.register_buffer(n, f(t))
         self.wqkv, self.wo, self.w1, self.w2 = wqkv, wo, w1, w2
-        if w1.out_features % (2 * kernels.SWIGLU_HALF) == 0:
+        if w1.out_features % (2 * kernels.SWIGLU_HALF) == 0 and hasattr(w1, "swiglu_pairs"):
             w1.swiglu_pairs()  # the FFN's SwiGLU runs inside w1's GEMM
         self.D = wo.out_features
         self.F = w2.in_features
@@ -108,7 +110,10 @@ class EsmcBlock(nn.Module):
                    q["w1"], q["w2"], n_heads, device=device)
 
     def params(self) -> dict:
-        """The layer's arrays under the reference's names (inverse of ``from_params``)."""
+        """The layer's arrays under the reference's names (inverse of ``from_params``); they hold ``Q8Linear``'s."""
+        other = [n for n in LINEARS if not isinstance(getattr(self, n), Q8Linear)]
+        if other:
+            raise ValueError(f"the converted-weight layout holds Q8Linear's arrays, not those of {other}")
         p = {n: getattr(self, n).detach().cpu() for n in NORMS}
         for n in LINEARS:
             lin = getattr(self, n)
@@ -165,6 +170,20 @@ class EsmcBlock(nn.Module):
         kernels.esmc_layer_norm(x_mid, next_w, next_b, EPS, y_parts=self.ffn(h2), alpha=1.0 / res_scale, x_out=x_out,
                                 out=out, fp32_out=out.dtype == torch.float32)
 
+    def run_packed(self, x: torch.Tensor, h: torch.Tensor, cu: torch.Tensor, positions: torch.Tensor, rotary: Rotary,
+                   res_scale: float, next_w, next_b, x_out: torch.Tensor, out: torch.Tensor) -> None:
+        """``run`` on packed rows x [T, D] fp32 and h = LN1(x): the sequences that begin at cu [n + 1] (int32, on the
+        device), each attending to itself, with ``positions`` [T] turned by ``rotary``."""
+        T, D = x.shape
+        q, k, v = self.wqkv(h).view(T, 3, self.n_heads, 64).unbind(1)
+        rotary(q, k, positions, norm="layer", over="row", q_w=self.q_ln, k_w=self.k_ln, eps=EPS, out=(q, k))
+        o = kernels.packed_attention(q, k, v, cu).view(T, D)
+        x_mid, h2 = torch.empty_like(x), torch.empty_like(h)
+        kernels.esmc_layer_norm(x, self.ln2_w, self.ln2_b, EPS, y_parts=self.wo.partials(o), alpha=1.0 / res_scale,
+                                x_out=x_mid, out=h2)
+        kernels.esmc_layer_norm(x_mid, next_w, next_b, EPS, y_parts=self.ffn(h2), alpha=1.0 / res_scale, x_out=x_out,
+                                out=out, fp32_out=out.dtype == torch.float32)
+
     def forward(self, x: torch.Tensor, sequence_id=None, res_scale: float = 1.0) -> torch.Tensor:
         """One block on an fp32 residual [B, L, D] (the reference's block_forward, mlx_esmc.py:84-102)."""
         x = x.to(torch.float32).contiguous()
@@ -206,6 +225,7 @@ class HipEsmc(nn.Module):
         self.layers = nn.ModuleList(layers)
         self.n_heads = n_heads
         self.res_scale = math.sqrt(len(layers) / 36)  # mlx_esmc.py:108
+        self._rotary = None  # of the packed form
 
     # ---- construction: the reference's converted-weight cache (mlx_esmc.py:116-148) -------------
     @classmethod
@@ -238,12 +258,15 @@ class HipEsmc(nn.Module):
 
     @classmethod
     def from_hf(cls, tensors, n_layers: int | None = None, n_heads: int = 40, cache=None,
-                device=None) -> "HipEsmc":
+                device=None, linear=Q8Linear) -> "HipEsmc":
         """From the published fp32 checkpoint's HF-named tensors (any mapping, e.g. a dict or a
         lazy shard reader: "esmc.embed_tokens.weight", "esmc.norm.weight",
         "esmc.layers.{i}.…"), every linear quantised to 8 bits on the GPU (the reference's
         from_shards, mlx_esmc.py:116-137). With ``cache`` (a path): load it when it exists,
-        otherwise convert and write it there in the layout ``from_cache`` reads."""
+        otherwise convert and write it there in the layout ``from_cache`` reads. ``linear``: the
+        class of the linears (``F8Linear`` for e4m3; the cache holds ``Q8Linear``'s arrays only)."""
+        if cache is not None and linear is not Q8Linear:
+            raise ValueError("the converted-weight cache holds Q8Linear's arrays")
         if cache is not None and os.path.exists(str(cache)):
             return cls.from_cache(cache, n_heads, device=device)
         if n_layers is None:
@@ -252,7 +275,7 @@ class HipEsmc(nn.Module):
             n_layers = len(idx)
         layers = []
         for i in range(n_layers):
-            ln, lin = hf_layer(tensors, i, device=device)
+            ln, lin = hf_layer(tensors, i, device=device, linear=linear)
             layers.append(EsmcBlock(ln["ln1_w"], ln["ln1_b"], ln["q_ln"], ln["k_ln"], ln["ln2_w"], ln["ln2_b"],
                                     lin["wqkv"], lin["wo"], lin["w1"], lin["w2"], n_heads, device=device))
         esmc = cls(tensors["esmc.embed_tokens.weight"].detach().float(), layers,
@@ -297,6 +320,51 @@ class HipEsmc(nn.Module):
             else:  # the last block's output is only seen through the final norm (weights only)
                 run(states[i], h, sid, self.res_scale, self.norm_w, None, x_last, states[n])
         return hs
+
+    def packed_hidden_states(self, input_ids: torch.Tensor, cu_seqlens: torch.Tensor, positions=None) -> torch.Tensor:
+        """``hidden_states`` of packed sequences: input_ids [T] of all of them, cu_seqlens [n + 1] where each begins
+        and the last ends -> [n_layers + 1, T, D] fp32, each sequence as if alone. ``positions`` [T]: other rotary
+        positions than the places within the sequences (a complex whose chains are sequences of their own but
+        count on). Rows of no sequence hold nothing meaningful."""
+        dev = self.embed.device
+        ids = input_ids.to(dev)
+        if ids.dim() != 1 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError(f"packed ESMC: input_ids {tuple(ids.shape)}, cu_seqlens {tuple(cu_seqlens.shape)}")
+        T, n, D = ids.numel(), len(self.layers), self.embed.shape[1]
+        cu = cu_seqlens.to(device=dev, dtype=torch.int32).contiguous()
+        if positions is None:
+            rows = torch.arange(T, dtype=torch.int32, device=dev)
+            positions = rows - cu[torch.searchsorted(cu[1:].contiguous(), rows, right=True)]
+        else:
+            positions = positions.to(dev).contiguous()
+        if self._rotary is None or self._rotary.freq.device != dev:
+            self._rotary = Rotary(64, device=dev)
+        hs = torch.empty(n + 1, T, D, dtype=torch.float32, device=dev)
+        hs[0] = self.embed[ids]
+        if T == 0:
+            return hs
+        h = kernels.esmc_layer_norm(hs[0], self.layers[0].ln1_w, self.layers[0].ln1_b, EPS)
+        x_last = torch.empty(T, D, dtype=torch.float32, device=dev)
+        states = hs.unbind(0)
+        for i, blk in enumerate(self.layers):
+            run = blk.run_packed if hasattr(blk, "run_packed") else partial(EsmcBlock.run_packed, blk)
+            last = i + 1 == n
+            w, b = (self.norm_w, None) if last else (self.layers[i + 1].ln1_w, self.layers[i + 1].ln1_b)
+            run(states[i], h, cu, positions, self._rotary, self.res_scale, w, b, x_last if last else states[i + 1],
+                states[n] if last else h)
+        return hs
+
+    def packed(self, sequences) -> SimpleNamespace:
+        """The sequences (1-D id tensors of any lengths) in one packed pass: ``hidden_states`` [n_layers + 1, T, D],
+        ``cu_seqlens`` [n + 1] (int32, on the GPU) and ``lengths``; ``hidden_states.split(lengths, 1)`` is each
+        sequence's own."""
+        lengths = [int(s.numel()) for s in sequences]
+        if not lengths or any(s.dim() != 1 for s in sequences):
+            raise ValueError("packed ESMC needs one or more 1-D id tensors")
+        dev = self.embed.device
+        cu = torch.tensor([0] + lengths, dtype=torch.int64).cumsum(0).to(device=dev, dtype=torch.int32)
+        hs = self.packed_hidden_states(torch.cat([s.to(dev) for s in sequences]), cu)
+        return SimpleNamespace(hidden_states=hs, cu_seqlens=cu, lengths=lengths)
 
     def forward(self, input_ids=None, sequence_id=None, output_hidden_states=True, **_):
         return SimpleNamespace(hidden_states=self.hidden_states(input_ids, sequence_id))
