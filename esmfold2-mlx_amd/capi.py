@@ -155,7 +155,7 @@ def stream_ptr(stream=None) -> int:
     import torch
     if stream is not None:
         return stream.cuda_stream
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 class KernelTimes:

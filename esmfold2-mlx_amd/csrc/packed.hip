@@ -14,6 +14,8 @@
 // Two kernels share that step: packed_attention_kernel (many rows: four waves of 32 rows over tiles of 64
 // keys that they share, the next tile in flight) and split_attention_kernel (few rows: 32 rows, keys divided
 // between the four waves and, through fp32 partials joined by a second launch, between workgroups).
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -299,6 +301,59 @@ DEV bool find_item(const PackedAttnArgs& p, int unit, int chunk, int item, int l
   return false;
 }
 
+// Sum over the wave, the same in every lane.
+DEV int wave_sum(int v) {
+  const auto add = [&](auto ctrl) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, false); };
+  add(std::integral_constant<int, 0x128>{});  // row_ror:8, 4, 2, 1
+  add(std::integral_constant<int, 0x124>{});
+  add(std::integral_constant<int, 0x122>{});
+  add(std::integral_constant<int, 0x121>{});
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+
+// find_item for tiles of kAttnRows rows of 2 to 64 sequences, the longest tiles first whichever sequence they are of, so
+// that no long one starts last (prompts of 1 to 4,096 rows 289 -> 244 us): the keys a tile sees fall into 16 levels, and
+// how many tiles of a sequence see at least so many follows from its lengths. `at` counts a sequence's tiles from the
+// one that sees most.
+constexpr int kAttnRows = 128;  // rows per workgroup of the many-row kernel
+template <bool CAUSAL>
+DEV bool find_longest(const PackedAttnArgs& p, int item, int lane, Span& s, int& at) {
+  const int i = min(lane, p.n - 1);
+  const int a = min(max(p.cu_q[i], 0), p.Tq), b = min(max(p.cu_q[i + 1], a), p.Tq);
+  const int ka = min(max(p.cu_k[i], 0), p.Tk), kb = min(max(p.cu_k[i + 1], ka), p.Tk);
+  const int nq = b - a, nk = kb - ka, tiles = lane < p.n ? (nq * p.G + kAttnRows - 1) / kAttnRows : 0;
+  if (item >= wave_sum(tiles)) return false;
+  int most = lane < p.n ? nk : 0;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+  const int level = __builtin_amdgcn_readfirstlane(most / 16 + 1);
+  // tiles of this lane's sequence whose last row sees at least `keys` keys
+  const auto seeing = [&](int keys) {
+    if (keys > nk) return 0;
+    if (!CAUSAL) return tiles;
+    const int first = keys - 1 - nk + nq;  // the first row that does
+    return first <= 0 ? tiles : max(0, tiles - (int)((long long)first * p.G / kAttnRows));
+  };
+  int lv = 0;  // the highest level whose tiles and those above pass the item
+#pragma unroll
+  for (int step = 8; step; step >>= 1)
+    if (wave_sum(seeing((lv + step) * level)) > item) lv += step;
+  const int above = seeing((lv + 1) * level), mine = (lv ? seeing(lv * level) : tiles) - above;
+  item -= wave_sum(above);
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(sum, o);
+    sum += lane >= o ? up : 0;
+  }
+  const int w = __builtin_ctzll(__ballot(item < sum));
+  at = item - __builtin_amdgcn_readlane(sum - mine, w) + __builtin_amdgcn_readlane(above, w);
+  s = Span{__builtin_amdgcn_readlane(a, w), __builtin_amdgcn_readlane(nq, w), __builtin_amdgcn_readlane(ka, w),
+           __builtin_amdgcn_readlane(nk, w)};
+  return true;
+}
+
 // A tile of `keys` key rows from key kt of the span on, as a buffer whose range ends with the span's last row:
 // rows past it (another sequence's, or none) load zeros.
 DEV dma_src_t tile_src(const char* base, long long st, int d, int first, int kt, int nk, int keys) {
@@ -333,7 +388,6 @@ DEV void load_queries(Rows<T, HD>& w, const PackedAttnArgs& p, const Span& s, in
 }
 
 constexpr int kAttnKeys = 64;   // keys per tile of the many-row kernel
-constexpr int kAttnRows = 128;  // rows per workgroup
 
 template <class T, int HD, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs p) {
@@ -345,10 +399,11 @@ __global__ __launch_bounds__(256, 2) void packed_attention_kernel(PackedAttnArgs
   const int hk = blockIdx.x % p.Hk, item = blockIdx.x / p.Hk;
   Span s;
   int tile;
-  if (!find_item(p, kAttnRows, 0, item, lane, s, tile)) return;
+  const bool many = p.n > 1 && p.n <= 64;
+  if (many ? !find_longest<CAUSAL>(p, item, lane, s, tile) : !find_item(p, kAttnRows, 0, item, lane, s, tile)) return;
   tile = __builtin_amdgcn_readfirstlane(tile);
   const int rows = s.nq * p.G;
-  if (CAUSAL) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
+  tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;  // the last see most
   const int row0 = kAttnRows * tile + 32 * wave;  // this wave's first row
 
   Rows<T, HD> w;
@@ -525,6 +580,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
   __shared__ __align__(16) float sums[4][HD];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, H = p.G * p.Hk;
   const int q = blockIdx.x / H, head = blockIdx.x - q * H;
+  // m and l of every chunk there may be and the first chunks' O are read before it is known which were written
+  const size_t at = (size_t)blockIdx.x * p.splits;
+  constexpr int kCols = HD / 4, kSide = 256 / kCols, kAhead = 4;  // lanes across a row, chunks at once, times ahead
+  const int col = 4 * (t % kCols), side = t / kCols;
+  const float* po = p.part_o + at * p.d;
+  const bool may = t < p.splits;
+  const float ml0 = may ? p.part_ml[2 * (at + t)] : 0.f, ml1 = may ? p.part_ml[2 * (at + t) + 1] : 0.f;
+  f32x4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; i++) {
+    const int j = side + kSide * i;
+    ahead[i] = j < p.splits && col < p.d ? *reinterpret_cast<const f32x4*>(po + (size_t)j * p.d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   Span s;
   bool found = false;
   for (int i0 = 0; i0 < p.n && !found; i0 += 64) {
@@ -544,8 +612,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
   const int rows = s.nq * p.G, last = min(((q - s.q0) * p.G + head % p.G) | 31, rows - 1);
   const int seen = p.causal ? max(min(s.nk, last / p.G + s.nk - s.nq + 1), 0) : s.nk;
   const int live = max(1, (seen + p.chunk - 1) / p.chunk);
-  const size_t at = (size_t)blockIdx.x * p.splits;
-  const float m = t < live ? p.part_ml[2 * (at + t)] : -INFINITY, l = t < live ? p.part_ml[2 * (at + t) + 1] : 0.f;
+  const float m = t < live ? ml0 : -INFINITY, l = t < live ? ml1 : 0.f;
   float M = m;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -560,12 +627,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(PackedAttnArgs p) {
   if (lane == 0) red[1][wave] = L;
   __syncthreads();
   L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  constexpr int kCols = HD / 4, kSide = 256 / kCols;  // lanes across a row, chunks at once
-  const int col = 4 * (t % kCols), side = t / kCols;
-  const float* po = p.part_o + at * p.d;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int j = side; j < live; j += kSide)
+#pragma unroll
+  for (int i = 0; i < kAhead; i++)
+    if (side + kSide * i < live) acc += weight[side + kSide * i] * ahead[i];
+  for (int j = side + kSide * kAhead; j < live; j += kSide)
     if (col < p.d) acc += weight[j] * *reinterpret_cast<const f32x4*>(po + (size_t)j * p.d + col);
 #pragma unroll
   for (int o = kCols; o < 64; o <<= 1)

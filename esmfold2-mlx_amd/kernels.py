@@ -198,38 +198,37 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 
 
-def _rows(t, name: str, like=None):
-    """A 16-bit [rows, heads, d] tensor whose heads are contiguous (a view of a wider row, say): the checks that
-    need no shape, and its strides."""
+def _rows(t, name: str, dtype=None, index=None):
+    """A 16-bit [rows, heads, d] tensor whose heads are contiguous (a view of a wider row, say), of the queries' dtype
+    and device where those are given: the checks that need no shape; (shape, row stride, head stride)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise capi.EsmError(-5, f"{name} must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
-    dtype, shape, strides = t.dtype, t.shape, t.stride()
-    if len(shape) != 3 or dtype not in _DTYPES:
-        raise capi.EsmError(-2, f"{name} must be [rows, heads, d] in fp16 or bf16, got {dtype} {tuple(shape)}")
-    if like is not None and (dtype is not like.dtype or t.get_device() != like.get_device()):
-        raise capi.EsmError(-2, f"{name}: {dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype not in _DTYPES:
+        raise capi.EsmError(-2, f"{name} must be [rows, heads, d] in fp16 or bf16, got {t.dtype} {tuple(shape)}")
+    if dtype is not None and (t.dtype is not dtype or t.get_device() != index):
+        raise capi.EsmError(-2, f"{name}: {t.dtype} on {t.device}, the queries are {dtype} on cuda:{index}")
     st, sh, one = strides
-    if one != 1 and shape[2] > 1:
+    T, H, d = shape
+    if one != 1 and d > 1:
         raise capi.EsmError(-3, f"{name}: the values of a head must be contiguous")
     # (a stride that nothing is reached by says nothing)
-    return (st if shape[0] > 1 else 8 * ((shape[1] * shape[2] + 7) // 8)), (sh if shape[1] > 1 else 0)
+    return shape, (st if T > 1 else 8 * ((H * d + 7) // 8)), (sh if H > 1 else 0)
 
 
-def _distinct(strides, shape, name: str) -> None:
-    """Refuses an output whose rows or heads share memory."""
-    (st, sh), (T, H, d) = strides, shape
+def _distinct(t, name: str, dtype, index):
+    """``_rows`` of an output, refused where its rows or heads share memory."""
+    shape, st, sh = _rows(t, name, dtype, index)
+    T, H, d = shape
     if (H > 1 and sh < d) or (T > 1 and H > 1 and min(st, sh) * ((H if st >= sh else T) - 1) + d > max(st, sh)):
         raise capi.EsmError(-3, f"{name}: rows and heads must not overlap")
+    return shape, st, sh
 
 
-def _elsewhere(t) -> bool:
-    """Whether the tensor's device is not the current one: its call is then made with that device current."""
-    return t.get_device() != torch.cuda.current_device()
-
-
-def _aux(t, name: str, dtypes, device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise capi.EsmError(-5, f"{name} must be on {device}")
+def _aux(t, name: str, dtypes, index: int) -> torch.Tensor:
+    """An auxiliary tensor on device ``index``: dtype and contiguity."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index:
+        raise capi.EsmError(-5, f"{name} must be on cuda:{index}")
     if t.dtype not in dtypes:
         raise capi.EsmError(-2, f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
     if not t.is_contiguous():
@@ -237,14 +236,16 @@ def _aux(t, name: str, dtypes, device) -> torch.Tensor:
     return t
 
 
-_FP32, _FP64, _INT32, _INTS = (torch.float32,), (torch.float64,), (torch.int32,), (torch.int32, torch.int64)
+_current = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_FP32, _FP64, _UINT8, _INT32 = (torch.float32,), (torch.float64,), (torch.uint8,), (torch.int32,)
+_INTS = (torch.int32, torch.int64)
 
 
-def _weights_of(t, name: str, heads: int, d: int, device):
+def _weights_of(t, name: str, heads: int, d: int, index: int):
     """(pointer, whether every head has its own) of a norm's weight."""
     if t is None:
         return None, 0
-    _aux(t, name, _FP32, device)
+    _aux(t, name, _FP32, index)
     n = t.numel()
     if n != d and n != heads * d:
         raise capi.EsmError(-2, f"qk_norm_rope: {name} has {n} elements for {heads} heads of {d}")
@@ -258,42 +259,40 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
     d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
     makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
     0 .. T - 1). ``out`` = (q', k'), which may be (q, k)."""
-    q_st, q_sh = _rows(q, "q")
-    k_st, k_sh = _rows(k, "k", q)
-    if _elsewhere(q):
-        with torch.cuda.device(q.device):
+    (T, H, d), q_st, q_sh = _rows(q, "q")
+    dtype, index = q.dtype, q.get_device()
+    (Tk, Hk, dk), k_st, k_sh = _rows(k, "k", dtype, index)
+    if index != _current():
+        with torch.cuda.device(index):
             return qk_norm_rope(q, k, freq, positions, gain=gain, interleaved=interleaved, norm=norm, over=over, q_w=q_w,
                                 k_w=k_w, eps=eps, out=out)
-    T, H, d = q.shape
-    Tk, Hk, dk = k.shape
     if Tk != T or dk != d:
         raise capi.EsmError(-2, f"qk_norm_rope: q {tuple(q.shape)}, k {tuple(k.shape)}")
     if norm not in _NORMS or over not in ("head", "row"):
         raise capi.EsmError(-4, f"qk_norm_rope: norm={norm!r} over={over!r}")
-    device = q.device
-    _aux(freq, "freq", _FP64, device)
+    _aux(freq, "freq", _FP64, index)
     pos, pos64 = None, 0
     if positions is not None:
-        _aux(positions, "positions", _INTS, device)
+        _aux(positions, "positions", _INTS, index)
         if positions.numel() != T:
             raise capi.EsmError(-2, f"qk_norm_rope: {positions.numel()} positions for {T} rows")
         pos, pos64 = positions.data_ptr(), int(positions.dtype is torch.int64)
-    qw, qwh = _weights_of(q_w, "q_w", H, d, device)
-    kw, kwh = _weights_of(k_w, "k_w", Hk, d, device)
+    qw, qwh = _weights_of(q_w, "q_w", H, d, index)
+    kw, kwh = _weights_of(k_w, "k_w", Hk, d, index)
     if out is None:
-        qo, ko = torch.empty(T, H, d, dtype=q.dtype, device=device), torch.empty(T, Hk, d, dtype=q.dtype, device=device)
+        qo, ko = q.new_empty((T, H, d)), q.new_empty((T, Hk, d))
         qo_st, qo_sh, ko_st, ko_sh = H * d, d, Hk * d, d
     else:
         qo, ko = out
         for t, n, like in ((qo, "out[0]", q), (ko, "out[1]", k)):
             if not isinstance(t, torch.Tensor) or t.shape != like.shape:
                 raise capi.EsmError(-2, f"qk_norm_rope: {n} must be {tuple(like.shape)}")
-            _distinct(_rows(t, n, q), t.shape, n)
-        (qo_st, qo_sh), (ko_st, ko_sh) = _rows(qo, "out[0]", q), _rows(ko, "out[1]", q)
+            _distinct(t, n, dtype, index)
+        (_, qo_st, qo_sh), (_, ko_st, ko_sh) = _rows(qo, "out[0]"), _rows(ko, "out[1]")
     capi.check(capi.lib().qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
         qwh, kw, kwh, eps, pos, pos64, freq.data_ptr(), gain, T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
-        bool(interleaved), _DTYPES[q.dtype], capi.stream_ptr()))
+        bool(interleaved), _DTYPES[dtype], capi.stream_ptr()))
     return qo, ko
 
 
@@ -303,43 +302,44 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
     sequence are not written. The partial results of few rows against many keys live in the shared scratch."""
-    q_st, q_sh = _rows(q, "q")
-    k_st, k_sh = _rows(k, "k", q)
-    v_st, v_sh = _rows(v, "v", q)
-    if _elsewhere(q):
-        with torch.cuda.device(q.device):
+    (Tq, H, d), q_st, q_sh = _rows(q, "q")
+    dtype, index = q.dtype, q.get_device()
+    kshape, k_st, k_sh = _rows(k, "k", dtype, index)
+    vshape, v_st, v_sh = _rows(v, "v", dtype, index)
+    if index != _current():
+        with torch.cuda.device(index):
             return packed_attention(q, k, v, cu_q, cu_k, causal, scale, out)
-    Tq, H, d = q.shape
-    Tk, Hk, dk = k.shape
-    if k.shape != v.shape or dk != d or Hk == 0 or H % Hk:
+    Tk, Hk, dk = kshape
+    if kshape != vshape or dk != d or Hk == 0 or H % Hk:
         raise capi.EsmError(-2, f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    device = q.device
-    _aux(cu_q, "cu_q", _INT32, device)
+    _aux(cu_q, "cu_q", _INT32, index)
     n = cu_q.numel() - 1
     if cu_k is None:
         if Tk != Tq:
             raise capi.EsmError(-2, f"packed_attention: {Tq} query rows and {Tk} key rows need cu_k")
         cu_k = cu_q
     else:
-        _aux(cu_k, "cu_k", _INT32, device)
+        _aux(cu_k, "cu_k", _INT32, index)
     if n < 0 or cu_k.numel() != n + 1:
         raise capi.EsmError(-2, f"packed_attention: {cu_q.numel()} and {cu_k.numel()} starts")
     if out is None:
-        o, o_st, o_sh = torch.empty(Tq, H, d, dtype=q.dtype, device=device), H * d, d
+        o, o_st, o_sh = q.new_empty((Tq, H, d)), H * d, d
     else:
         o = out
-        o_st, o_sh = _rows(o, "out", q)
-        if o.shape != q.shape:
+        oshape, o_st, o_sh = _distinct(o, "out", dtype, index)
+        if oshape != q.shape:
             raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
-        _distinct((o_st, o_sh), o.shape, "out")
     lib = capi.lib()
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
+            cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else scale,
+            _DTYPES[dtype])
     need = lib.packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d)
-    with scratch.guard(device, need):
-        ws, wp, stream = scratch.take(need, device) if need else (None, None, capi.stream_ptr())
-        capi.check(lib.packed_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh,
-                                        v_st, v_sh, o_st, o_sh, cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d,
-                                        bool(causal), d ** -0.5 if scale is None else scale, _DTYPES[q.dtype], wp, need,
-                                        stream))
+    if not need:
+        capi.check(lib.packed_attention(*args, None, 0, capi.stream_ptr()))
+        return o
+    with scratch.guard(q.device):
+        ws, wp, stream = scratch.take(need, q.device)
+        capi.check(lib.packed_attention(*args, wp, need, stream))
     return o
 
 
@@ -681,7 +681,7 @@ def f8_quantize_weight(w):
 
 
 def _f8_operands(x, codes, scales, N, fn):
-    """The checks of ``f8_linear``'s operands on the host: (M, K, row stride of x)."""
+    """The checks of ``f8_linear``'s operands on the host: (M, K, row stride of x, device)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise capi.EsmError(-5, f"{fn}: x must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
     if x.dim() != 2 or x.dtype not in _DTYPES:
@@ -690,34 +690,37 @@ def _f8_operands(x, codes, scales, N, fn):
     st, one = x.stride()
     if K > 1 and one != 1:
         raise capi.EsmError(-3, f"{fn}: the values of a row must be contiguous")
-    device = x.device
-    _aux(codes, "codes", (torch.uint8,), device)
-    _aux(scales, "scales", _FP32, device)
+    index = x.get_device()
+    _aux(codes, "codes", _UINT8, index)
+    _aux(scales, "scales", _FP32, index)
     if codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128):
         raise capi.EsmError(-2, f"{fn}: {codes.numel()} packed codes and {scales.numel()} scales for [{N}, {K}]")
-    return M, K, st if M > 1 else (K + 7) // 8 * 8
+    return M, K, st if M > 1 else (K + 7) // 8 * 8, index
 
 
 def f8_linear(x, codes, scales, N: int, out=None):
     """y = x . W^T on the fp8 matrix cores: x [M, K] fp16 or bf16 (rows may lie apart), brought to e4m3 with a scale
     per row and 128 columns; W [N, K] as packed e4m3 codes (``f8_pack_codes``) with an fp32 scale per 128 x 128 block;
     fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch."""
-    M, K, st = _f8_operands(x, codes, scales, N, "f8_linear")
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    M, K, st, index = _f8_operands(x, codes, scales, N, "f8_linear")
+    if index != _current():
+        with torch.cuda.device(index):
             return f8_linear(x, codes, scales, N, out)
     if out is None:
-        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        y = x.new_empty((M, N))
     else:
         y = _out(out, "out", x.dtype, M * N)
-        if y.device != x.device:
+        if y.get_device() != index:
             raise capi.EsmError(-5, f"out must be on {x.device}")
     lib = capi.lib()
+    args = (x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N, _DTYPES[x.dtype])
     need = lib.f8_linear_workspace_bytes(M, K, N)
-    with scratch.guard(x.device, need):
-        ws, wp, stream = scratch.take(need, x.device) if need else (None, None, capi.stream_ptr())
-        capi.check(lib.f8_linear(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N,
-                                 _DTYPES[x.dtype], wp, need, stream))
+    if not need:
+        capi.check(lib.f8_linear(*args, None, 0, capi.stream_ptr()))
+        return y
+    with scratch.guard(x.device):
+        ws, wp, stream = scratch.take(need, x.device)
+        capi.check(lib.f8_linear(*args, wp, need, stream))
     return y
 
 
@@ -726,7 +729,7 @@ def f8_linear_partials(x, codes, scales, N: int):
     to x's type, their sum in split order is ``f8_linear``'s result. The view lives in the device's shared scratch,
     valid until its next user (the caller holds ``scratch.guard``)."""
     lib = capi.lib()
-    M, K, st = _f8_operands(x, codes, scales, N, "f8_linear_partials")
+    M, K, st, _ = _f8_operands(x, codes, scales, N, "f8_linear_partials")
     splits = ctypes.c_int(0)
     with torch.cuda.device(x.device), scratch.guard(x.device):
         nparts = int(lib.f8_linear_partials_bytes(M, K, N))
