@@ -141,7 +141,8 @@ struct Rows {
 
   // 64 keys that every row sees, in an order that the scheduler keeps: a fragment is read some matrix instructions
   // before its own (LDS answers in more than 64 cycles, one takes 32), the maximum of the first 32 keys is taken
-  // between those of the next 32, and the exponentials of the second half between the value products of the first.
+  // between those of the next 32, and the exponentials of the second half between the value products of the first. The
+  // matrix phases go before the other wave's vector work (1,100 tokens of 40 heads of 64 24.9 -> 22.6 us).
   DEV void step64(const char* ks, const char* vs, float c, int lane) {
     constexpr int NK = HD / 16, ND = HD / 32;
     typedef typename T::v8 v8;
@@ -155,6 +156,7 @@ struct Rows {
     v8 ka[NK], kb[NK], va[ND], vb[ND];
 #pragma unroll
     for (int k = 0; k < NK; k++) ka[k] = key(0, k);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < NK; k++) {
@@ -173,6 +175,8 @@ struct Rows {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -188,6 +192,7 @@ struct Rows {
     for (int i = 0; i < 8; i++) prob(i);
     l = T::add(p[0], l);
     l = T::add(p[1], l);
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2 * ND; u++) {  // values of keys 0 .. 31
@@ -207,6 +212,7 @@ struct Rows {
       if (!j) vb[d] = v_frag<T, HD>(vs, 3, d, lane);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   // The row's maximum has grown to mx: everything summed so far by the new one.
