@@ -258,7 +258,7 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
     (q', k'). ``norm``: None, "rms" or "layer", ``over`` each "head" or the whole "row" of heads, with fp32 weights of
     d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
     makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
-    0 .. T - 1). ``out`` = (q', k'), which may be (q, k)."""
+    0 .. T - 1). ``out`` = (q', k'), which may be (q, k) but share no other memory with them."""
     (T, H, d), q_st, q_sh = _rows(q, "q")
     dtype, index = q.dtype, q.get_device()
     (Tk, Hk, dk), k_st, k_sh = _rows(k, "k", dtype, index)
@@ -288,10 +288,12 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
             if not isinstance(t, torch.Tensor) or t.shape != like.shape:
                 raise capi.EsmError(-2, f"qk_norm_rope: {n} must be {tuple(like.shape)}")
             _distinct(t, n, dtype, index)
+        if T and (qo.data_ptr() == k.data_ptr() or ko.data_ptr() == q.data_ptr() or qo.data_ptr() == ko.data_ptr()):
+            raise capi.EsmError(-3, "qk_norm_rope: out may be (q, k), each in its own place")
         (_, qo_st, qo_sh), (_, ko_st, ko_sh) = _rows(qo, "out[0]"), _rows(ko, "out[1]")
     capi.check(capi.lib().qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
-        qwh, kw, kwh, eps, pos, pos64, freq.data_ptr(), gain, T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
+        qwh, kw, kwh, float(eps), pos, pos64, freq.data_ptr(), float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
         bool(interleaved), _DTYPES[dtype], capi.stream_ptr()))
     return qo, ko
 
@@ -301,7 +303,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     wider rows allowed; H a multiple of Hk) -> o [Tq, H, d]. ``cu_q``, ``cu_k`` int32 [n + 1] on the device: the first
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
-    sequence are not written. The partial results of few rows against many keys live in the shared scratch."""
+    sequence are not written. ``out`` may be q, and shares no memory with k and v. The partial results of few rows
+    against many keys live in the shared scratch."""
     (Tq, H, d), q_st, q_sh = _rows(q, "q")
     dtype, index = q.dtype, q.get_device()
     kshape, k_st, k_sh = _rows(k, "k", dtype, index)
@@ -329,9 +332,11 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
         oshape, o_st, o_sh = _distinct(o, "out", dtype, index)
         if oshape != q.shape:
             raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
+        if Tq and Tk and o.data_ptr() in (k.data_ptr(), v.data_ptr()):
+            raise capi.EsmError(-3, "packed_attention: out may be q, not k or v")
     lib = capi.lib()
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
-            cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else scale,
+            cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else float(scale),
             _DTYPES[dtype])
     need = lib.packed_attention_workspace_bytes(n, Tq, Tk, H, Hk, d)
     if not need:
@@ -712,6 +717,8 @@ def f8_linear(x, codes, scales, N: int, out=None):
         y = _out(out, "out", x.dtype, M * N)
         if y.get_device() != index:
             raise capi.EsmError(-5, f"out must be on {x.device}")
+        if M and y.data_ptr() == x.data_ptr():
+            raise capi.EsmError(-3, "f8_linear: out may not be x")
     lib = capi.lib()
     args = (x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N, _DTYPES[x.dtype])
     need = lib.f8_linear_workspace_bytes(M, K, N)
@@ -740,5 +747,5 @@ def f8_linear_partials(x, codes, scales, N: int):
         capi.check(lib.f8_linear_partials(x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), buf.data_ptr(), nparts,
                                           ctypes.byref(splits), M, K, N, _DTYPES[x.dtype], buf.data_ptr() + at, need,
                                           capi.stream_ptr()))
-    n = splits.value
+    n = max(splits.value, 1)  # (no rows: one split of none)
     return buf[:4 * n * M * N].view(torch.float32).view(n, M, N), n, gen

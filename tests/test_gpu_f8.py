@@ -113,8 +113,9 @@ def test_views_types_and_shapes(gpu_lib, pkg, M):
     assert lin(x[:0]).shape == (0, 192) and lin(x.new_zeros(2, 0, 256)).shape == (2, 0, 192)
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 2560, 640), (238, 5120, 2560), (2049, 272, 8000)])
+@pytest.mark.parametrize("M,K,N", [(1, 2560, 640), (238, 5120, 2560), (2049, 272, 8000), (1000, 10240, 2560)])
 def test_partials_sum_to_the_result(gpu_lib, pkg, M, K, N):
+    # (one form of each kind; 1000 rows of a long K are split between workgroups)
     x, w = _inputs(M, K, N, torch.float16, seed=2)
     lin = pkg.f8.F8Linear.from_float(w)
     y = lin(x)
@@ -123,6 +124,8 @@ def test_partials_sum_to_the_result(gpu_lib, pkg, M, K, N):
     for s in range(1, splits):
         acc += parts[s]
     assert torch.equal(acc.half(), y)
+    none, one = lin.partials(x[:0])
+    assert none.shape == (1, 0, N) and one == 1
 
 
 @pytest.mark.parametrize("M", [5, 238])
@@ -145,6 +148,19 @@ def test_graph_and_repeats(gpu_lib, pkg, M):
     del keep
 
 
+def test_codes_that_are_not_numbers(gpu_lib, pkg):
+    # a NaN code makes its own output column NaN, nothing else
+    x, w = _inputs(40, 256, 192, torch.float16)
+    lin = pkg.f8.F8Linear.from_float(w)
+    codes = lin.codes.view(torch.uint8).clone()
+    codes[70, 33] = 0x7f
+    bad = pkg.f8.F8Linear(codes, lin.scales)
+    for rows in (x[:3], x):
+        y, z = lin(rows), bad(rows)
+        cols = [i for i in range(192) if i != 70]
+        assert bool(z[:, 70].isnan().all()) and torch.equal(y[:, cols], z[:, cols])
+
+
 def test_refusals(gpu_lib, pkg):
     K, E = pkg.kernels, pkg.capi.EsmError
     x, w = _inputs(4, 256, 128, torch.float16)
@@ -165,6 +181,8 @@ def test_refusals(gpu_lib, pkg):
     refused(-3, x.t()[:, :4].t()[:, ::2], c, s, 128)
     refused(-2, x, c, s, 128, out=torch.empty(4, 64, dtype=torch.float16, device=DEV))
     refused(-2, x, c, s, 128, out=torch.empty(4, 128, dtype=torch.bfloat16, device=DEV))
+    square = pkg.f8.F8Linear.from_float(torch.zeros(256, 256, device=DEV))
+    refused(-3, x, square.codes_packed, square.scales, 256, out=x)
     refused(-2, x[:, :250].contiguous(), c, s, 128)       # K = 250 rounds to the same pieces: no multiple of 16
     for bad in ((lin.codes[:, :250], s), (lin.codes, s[:, :1]), (lin.codes.float(), s), (lin.codes[:100], s)):
         with pytest.raises(ValueError):

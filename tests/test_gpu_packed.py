@@ -142,6 +142,48 @@ def test_what_unseen_rows_hold_reaches_nothing(gpu_lib, pkg, dtype, many):
     assert bool(got[cq[2] + 50:cq[3], G].isnan().all())
 
 
+@pytest.mark.parametrize("decode", [False, True])
+def test_more_sequences_than_a_wave(gpu_lib, pkg, decode):
+    g = torch.Generator().manual_seed(1)
+    n = 150
+    nq = [1] * n if decode else torch.randint(0, 40, (n,), generator=g).tolist()
+    nk = torch.randint(0, 300, (n,), generator=g).tolist() if decode else None
+    q, k, v, cq, ck = _case(nq, nk, 4, 2, 64, torch.float16, seed=2, tail=3)
+    got = pkg.kernels.packed_attention(q, k, v, _cu(cq), _cu(ck), causal=True)
+    o, bound = O.attention(q, k, v, cq, ck, True, 0.125)
+    _check(got, o, bound)
+
+
+def test_sequences_of_one_length_and_of_many_levels(gpu_lib, pkg):
+    # the order that takes the longest tiles first must visit each tile once: equal lengths, and lengths that differ by
+    # every level, with and without cached keys
+    for nq, nk in (([256] * 9, None), ([16 * i for i in range(1, 33)], None), ([200] * 6, [200 + 300 * i for i in range(6)]),
+                   ([700, 1], [700, 5000])):
+        q, k, v, cq, ck = _case(nq, nk, 16, 2, 64, torch.bfloat16, seed=len(nq))
+        for causal in (False, True):
+            out = torch.full_like(q, math.nan, memory_format=torch.contiguous_format)
+            pkg.kernels.packed_attention(q, k, v, _cu(cq), _cu(ck), causal=causal, out=out)
+            o, bound = O.attention(q[:, 9:10], k[:, 1:], v[:, 1:], cq, ck, causal, 0.125)
+            _check(out[:, 9:10], o, bound)
+            assert bool(torch.isfinite(out).all())
+
+
+def test_offsets_past_32_bits(gpu_lib, pkg):
+    # a cache of 9.4 GB whose last sequences lie beyond 2^32 bytes (and 2^31 elements)
+    rows, Hk, d = 2300000, 8, 128
+    kv = torch.empty(rows, 2 * Hk * d, dtype=torch.bfloat16, device=DEV)
+    nk = [300, 77]
+    kv[-sum(nk):] = torch.randn(sum(nk), 2 * Hk * d, generator=torch.Generator().manual_seed(0)).to(DEV)
+    k, v = (t.unflatten(1, (Hk, d)) for t in kv.split([Hk * d, Hk * d], dim=1))
+    q = torch.randn(130, 16, d, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    first = rows - sum(nk)
+    for nq in ([1, 1], [128, 2], [100, 30]):
+        cq, ck = _starts(nq), [first, first + 300, rows]
+        got = pkg.kernels.packed_attention(q[:cq[-1]], k, v, _cu(cq), _cu(ck), causal=True)
+        o, bound = O.attention(q[:cq[-1], 2:3], k[first:, 1:2], v[first:, 1:2], cq, [0, 300, 377], True, d ** -0.5)
+        _check(got[:, 2:3], o, bound)
+
+
 def test_large_scores_and_equal_ones(gpu_lib, pkg):
     # scores of several thousands, where only the maximum survives, and all equal ones, whose mean is exact to bounds
     q, k, v, cq, ck = _case([90, 40], None, 2, 2, 64, torch.bfloat16, seed=4)
@@ -240,3 +282,6 @@ def test_refusals(gpu_lib, pkg):
         refused(-2, x, x, x, cu, scale=s)
     refused(-2, x, x, x, cu, out=torch.zeros(8, 4, 32, dtype=torch.float16, device=DEV))
     refused(-3, x, x, x, cu, out=torch.zeros(8, 1, 64, dtype=torch.float16, device=DEV).expand(8, 4, 64))
+    y = torch.zeros_like(x)
+    refused(-3, x, y, x, cu, out=y)
+    refused(-3, x, x.clone(), y, cu, out=y)

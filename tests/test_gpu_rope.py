@@ -141,6 +141,9 @@ def test_refusals(gpu_lib, pkg):
     refused(-2, q, q, f, norm="rms", k_w=torch.ones(64, device=DEV, dtype=torch.float16))
     refused(-2, q, q, f, out=(q, q[:, :1]))
     refused(-3, q, q, f, out=(q, q[:1].expand(4, 2, 64)))
+    p = torch.zeros_like(q)
+    refused(-3, q, p, f, out=(p, q))
+    refused(-3, q, p, f, out=(p.clone(), q))
     refused(-3, q[..., 4:36], q[..., 4:36], f[:16])
     w = torch.zeros(1, 520, 256, dtype=torch.float16, device=DEV)
     refused(-4, w, w, f, norm="rms", over="row")
