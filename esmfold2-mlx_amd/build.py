@@ -5,7 +5,9 @@
 The library is compiled for gfx950 only. Every HIP source is compiled with the
 packed-fp32 target feature disabled (-Xclang -target-feature -Xclang
 -packed-fp32-ops): the kernels are written without packed fp32 arithmetic and
-the compiler must not introduce it.
+the compiler must not introduce it. Beside it goes _esm_bind.so, a host-only Python
+module against torch's headers (csrc/bind.cpp): the short way into the library for
+calls whose host steps would cost more than their kernels.
 """
 
 from __future__ import annotations
@@ -21,6 +23,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libesmfold2_amd.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+BIND_NAME = "_esm_bind"
+BIND_PATH = os.path.join(HERE, BIND_NAME + ".so")
+BIND_SOURCE = "bind.cpp"
 SOURCES = ["project.hip", "contract.hip", "epilogue.hip", "q8.hip", "transition.hip", "esmc.hip",
            "recycle.hip", "wide.hip", "stream.hip", "rope.hip", "packed.hip",
            "f8.hip", "capi.cpp"]
@@ -38,7 +43,7 @@ def hipcc() -> str:
 def source_hash() -> str:
     """sha256 over the names and contents of every source and header the library is built from."""
     h = hashlib.sha256()
-    for name in SOURCES + HEADERS:
+    for name in SOURCES + [BIND_SOURCE] + HEADERS:
         h.update(name.encode() + b"\0")
         with open(os.path.join(CSRC, name), "rb") as f:
             h.update(f.read())
@@ -71,9 +76,29 @@ def link_command(objs: list[str], out: str) -> list[str]:
     return [hipcc(), f"--offload-arch={ARCH}", "-shared", *objs, "-o", out]
 
 
+def bind_command(obj: str, src_hash: str) -> list[str]:
+    """hipcc -c of the Python module (host code only)."""
+    import sysconfig
+
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    return [hipcc(), "-O2", "-std=c++17", "-fPIC", "-Wall", "-DUSE_ROCM", f"-DESM_SOURCE_HASH=\"{src_hash}\"",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
+            "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], "-c",
+            os.path.join(CSRC, BIND_SOURCE), "-o", obj]
+
+
+def bind_link_command(obj: str, out: str) -> list[str]:
+    """The module's link: torch's libraries are found loaded when it is imported."""
+    import torch
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    return [cxx, "-shared", obj, "-o", out, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python",
+            "-ltorch_cpu", "-lc10", "-lc10_hip"]
+
+
 def up_to_date() -> bool:
-    """True when the built library exists and was compiled from the current sources (by content)."""
-    return library_hash() == source_hash()
+    """True when the built library and module exist and were compiled from the current sources (by content)."""
+    return library_hash() == source_hash() == library_hash(BIND_PATH)
 
 
 _NOISE = "is not a recognized feature for this target"  # host pass of the fp32 feature flag
@@ -100,13 +125,15 @@ def build(force: bool = True, verbose: bool = False, jobs: int | None = None) ->
         return LIB_PATH
     import tempfile
     h = source_hash()
-    jobs = jobs or max(1, min(len(SOURCES), os.cpu_count() or 1, 16))
+    jobs = jobs or max(1, min(len(SOURCES) + 1, os.cpu_count() or 1, 16))
     with tempfile.TemporaryDirectory(prefix="esm_build_") as tmpdir:
         objs, pending = [], []
         for src in SOURCES:
             obj = os.path.join(tmpdir, src.replace(".", "_") + ".o")
             objs.append(obj)
             pending.append(compile_command(src, obj, h))
+        bind_obj = os.path.join(tmpdir, "bind.o")
+        pending.append(bind_command(bind_obj, h))
         msgs = []
         while pending:
             batch, pending = pending[:jobs], pending[jobs:]
@@ -121,9 +148,16 @@ def build(force: bool = True, verbose: bool = False, jobs: int | None = None) ->
             print("[build]", " ".join(cmd), flush=True)
         msgs.append(_run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                                                  text=True))]))
+        bind_tmp = BIND_PATH + ".tmp"
+        cmd = bind_link_command(bind_obj, bind_tmp)
+        if verbose:
+            print("[build]", " ".join(cmd), flush=True)
+        msgs.append(_run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                                 text=True))]))
     if verbose and any(m.strip() for m in msgs):
         print("\n".join(m for m in msgs if m.strip()), flush=True)
     os.replace(tmp, LIB_PATH)
+    os.replace(bind_tmp, BIND_PATH)
     return LIB_PATH
 
 

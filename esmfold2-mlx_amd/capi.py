@@ -8,6 +8,7 @@ and raises ``EsmError`` with the library's message.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import sys
 import threading
@@ -99,6 +100,11 @@ class EsmError(RuntimeError):
         self.code = code
 
 
+# the native short way of some calls (csrc/bind.cpp), loaded with the library, and the entry points it takes
+bind = None
+_SHORT = ("qk_norm_rope", "packed_attention", "packed_attention_workspace_bytes", "f8_linear",
+          "f8_linear_workspace_bytes")
+
 _lock = threading.Lock()
 _lib = None
 _gpu_ok = False
@@ -123,6 +129,14 @@ def _load() -> ctypes.CDLL:
         fn.restype, fn.argtypes = res, args
     if handle.esm_source_hash().decode() != _build.source_hash():
         raise EsmError(-5, f"{_build.LIB_PATH} does not match its sources after the build")
+    global bind
+    if bind is None:
+        import torch  # noqa: F401  (the module is linked against its libraries)
+        spec = importlib.util.spec_from_file_location(_build.BIND_NAME, _build.BIND_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        bind = mod
+    bind.connect(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SHORT))
     return handle
 
 

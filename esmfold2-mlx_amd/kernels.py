@@ -259,6 +259,11 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
     d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
     makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
     0 .. T - 1). ``out`` = (q', k'), which may be (q, k) but share no other memory with them."""
+    lib = capi.lib()
+    if out is None and norm in _NORMS and (over == "head" or over == "row"):
+        y = capi.bind.qk_norm_rope(q, k, freq, positions, gain, interleaved, _NORMS[norm], over == "row", q_w, k_w, eps)
+        if y is not None:
+            return y
     (T, H, d), q_st, q_sh = _rows(q, "q")
     dtype, index = q.dtype, q.get_device()
     (Tk, Hk, dk), k_st, k_sh = _rows(k, "k", dtype, index)
@@ -291,7 +296,7 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
         if T and (qo.data_ptr() == k.data_ptr() or ko.data_ptr() == q.data_ptr() or qo.data_ptr() == ko.data_ptr()):
             raise capi.EsmError(-3, "qk_norm_rope: out may be (q, k), each in its own place")
         (_, qo_st, qo_sh), (_, ko_st, ko_sh) = _rows(qo, "out[0]"), _rows(ko, "out[1]")
-    capi.check(capi.lib().qk_norm_rope(
+    capi.check(lib.qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
         qwh, kw, kwh, float(eps), pos, pos64, freq.data_ptr(), float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
         bool(interleaved), _DTYPES[dtype], capi.stream_ptr()))
@@ -305,6 +310,15 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
     sequence are not written. ``out`` may be q, and shares no memory with k and v. The partial results of few rows
     against many keys live in the shared scratch."""
+    lib = capi.lib()
+    if out is None:
+        o = capi.bind.packed_attention(q, k, v, cu_q, cu_k, causal, scale, 0, 0)
+        if type(o) is int:  # bytes of workspace
+            with scratch.guard(q.device):
+                ws, wp, _ = scratch.take(o, q.device)
+                o = capi.bind.packed_attention(q, k, v, cu_q, cu_k, causal, scale, wp, o)
+        if o is not None:
+            return o
     (Tq, H, d), q_st, q_sh = _rows(q, "q")
     dtype, index = q.dtype, q.get_device()
     kshape, k_st, k_sh = _rows(k, "k", dtype, index)
@@ -334,7 +348,6 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
             raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
         if Tq and Tk and o.data_ptr() in (k.data_ptr(), v.data_ptr()):
             raise capi.EsmError(-3, "packed_attention: out may be q, not k or v")
-    lib = capi.lib()
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
             cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else float(scale),
             _DTYPES[dtype])
@@ -707,6 +720,15 @@ def f8_linear(x, codes, scales, N: int, out=None):
     """y = x . W^T on the fp8 matrix cores: x [M, K] fp16 or bf16 (rows may lie apart), brought to e4m3 with a scale
     per row and 128 columns; W [N, K] as packed e4m3 codes (``f8_pack_codes``) with an fp32 scale per 128 x 128 block;
     fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch."""
+    lib = capi.lib()
+    if out is None:
+        y = capi.bind.f8_linear(x, codes, scales, N, 0, 0)
+        if type(y) is int:  # bytes of workspace
+            with scratch.guard(x.device):
+                ws, wp, _ = scratch.take(y, x.device)
+                y = capi.bind.f8_linear(x, codes, scales, N, wp, y)
+        if y is not None:
+            return y
     M, K, st, index = _f8_operands(x, codes, scales, N, "f8_linear")
     if index != _current():
         with torch.cuda.device(index):
@@ -719,7 +741,6 @@ def f8_linear(x, codes, scales, N: int, out=None):
             raise capi.EsmError(-5, f"out must be on {x.device}")
         if M and y.data_ptr() == x.data_ptr():
             raise capi.EsmError(-3, "f8_linear: out may not be x")
-    lib = capi.lib()
     args = (x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N, _DTYPES[x.dtype])
     need = lib.f8_linear_workspace_bytes(M, K, N)
     if not need:

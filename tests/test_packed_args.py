@@ -107,3 +107,18 @@ def test_f8_refusals(lib):
     assert lib.f8_packed_codes_bytes(65, 129) == 0 and lib.f8_packed_codes_bytes(72, 144) == 2 * 2 * 8192
     assert lib.f8_pack_codes(None, P, 64, 128, None) == -1 and lib.f8_pack_codes(P, P, 64, 100, None) == -2
     assert lib.f8_quantize_weight(None, P, P, 64, 128, None) == -1
+
+
+def test_short_way_takes_the_ordinary_case_only(pkg, lib):
+    # the native module answers None for whatever it does not take, and the wrappers then refuse with their messages
+    b = pkg.capi.bind
+    assert pkg.build.library_hash(pkg.build.BIND_PATH) == pkg.build.source_hash()
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    assert b.packed_attention(x, x, x, cu, None, False, None, 0, 0) is None          # host tensors
+    assert b.packed_attention(x) is None and b.packed_attention(1, 2, 3, 4, 5, 6, 7, 8, 9) is None
+    assert b.qk_norm_rope(x, x, cu, None, 1.0, False, 0, False, None, None, 1e-6) is None
+    assert b.f8_linear(x[:, 0], cu, cu, 64, 0, 0) is None and b.f8_linear("x", cu, cu, 64, 0, 0) is None
+    with pytest.raises(TypeError):
+        b.connect(1, 2)
+    assert set(pkg.capi._SHORT) <= set(pkg.capi.SIGNATURES)
