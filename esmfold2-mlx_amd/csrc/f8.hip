@@ -521,7 +521,12 @@ template <class V8>
 static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) {
   hipError_t e;
   if (form == kF8Few) {
-    ESM_LAUNCH((f8_few_kernel<V8, 2>), dim3((a.N + 63) / 64 * 2), dim3(64 * kFewWaves), 0, s, a);
+    const dim3 grid((a.N + 63) / 64 * (4 / mb)), block(64 * kFewWaves);
+    switch (mb) {
+      case 4: ESM_LAUNCH((f8_few_kernel<V8, 4>), grid, block, 0, s, a); break;
+      case 2: ESM_LAUNCH((f8_few_kernel<V8, 2>), grid, block, 0, s, a); break;
+      default: ESM_LAUNCH((f8_few_kernel<V8, 1>), grid, block, 0, s, a); break;
+    }
     return hipGetLastError();
   }
   ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, ((a.K + 127) / 128 + kQuantBlocks - 1) / kQuantBlocks), dim3(256), 0, s,
@@ -553,7 +558,14 @@ hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipS
 //   5120 -> 2560 at M = 238  some 11.1, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 19, 64 rows in two
 //   splits 21 and 5; at M = 1000  some 31, 64 rows 33, 128 rows in three splits 25 and 6
 F8Plan f8_plan(int M, int K, int N, int cus) {
-  F8Plan p{kF8Few, 0, 1};
+  // Few rows: the most weight rows a workgroup (16, 32 or 64) that still give more than half the CUs one, as each
+  // workgroup reads x whole and few workgroups in flight leave the codes' loads waiting (us, 64 / 32 / 16 rows, M = 1 to 16:
+  // 2560 -> 10240 5.1 to 6.3 / 6.3 to 9.4 / 8.2 to 12.2, 2560 -> 7680 4.9 to 6.3 / 4.5 to 5.7 / 6.2 to 8.8,
+  // 2560 -> 2560 - / 4.8 to 5.6 / 4.2 to 5.3, 5120 -> 2560 - / 7.2 to 8.3 / 6.8 to 7.9, 8192 -> 8192 12.3 to 16 / 11.5 to 13.2 / 18).
+  // Up to 16 rows, as x brought to e4m3 apart costs 3 us (16 rows of 2560 -> 10240 6.3 against 3 + 4.4, 5120 -> 2560 7.9
+  // against 2.5 + 6.2), and a second block of 16 here 16 us.
+  F8Plan p{kF8Few, 4, 1};
+  while (p.mb > 1 && 16LL * ((N + 63) / 64) * (4 / p.mb) < 9LL * cus) p.mb /= 2;
   if (M <= 16) return p;
   const int Kb = (K + 127) / 128;
   const double tiles = (double)((M + 63) / 64) * ((N + 63) / 64);

@@ -41,6 +41,14 @@ def test_against_the_definition(gpu_lib, pkg, K, N, dtype):
         assert bool((buf[:64] == 9.0).all() and (buf[64 + M * N:] == 9.0).all())
 
 
+@pytest.mark.parametrize("M,K,N", [(1, 272, 8200), (5, 144, 9240), (16, 400, 10240), (16, 2576, 9720), (9, 1040, 4616)])
+def test_few_rows_of_wide_outputs(gpu_lib, pkg, M, K, N):
+    # (16, 32 and 64 weight rows a workgroup; test_against_the_definition has the narrow ones)
+    x, w = _inputs(M, K, N, torch.bfloat16, seed=3)
+    lin = pkg.f8.F8Linear.from_float(w)
+    _check(lin(x), x, lin.codes, lin.scales)
+
+
 @pytest.mark.parametrize("M,K,N", [(2049, 272, 8000), (4100, 640, 3584), (1000, 5120, 2560), (3481, 2560, 7680),
                                    (1000, 10240, 2560), (600, 8192, 1024), (530, 2576, 7688), (1010, 2560, 7680)])
 def test_many_rows(gpu_lib, pkg, M, K, N):
