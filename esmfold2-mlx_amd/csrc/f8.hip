@@ -207,17 +207,21 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
 }
 
 // ---- some rows: no barriers, K divided between the waves ---------------------------------------------
-// A workgroup takes 16 MB rows of x by 64 weight rows; its 8 waves deal the blocks of 128 k among them, read both
-// operands' fragments straight from memory (the next block's in flight) and sum through LDS. Through LDS tiles a
-// step of this size is a chain of latencies (0.47 us at 64 x 128 x 128, whatever its neighbours do).
+// A workgroup takes 16 MB RW rows of x by 64 weight rows; its 8 waves deal the blocks of 128 k among them (RW = 2:
+// four waves to each half of the rows), read both operands' fragments straight from memory (the next block's in
+// flight) and sum through LDS. Through LDS tiles a step of this size is a chain of latencies (0.47 us at
+// 64 x 128 x 128, whatever its neighbours do). One workgroup lies on a CU (240 registers), so 128 rows serve where
+// 64 would need a second round: 238 rows 2560 -> 7680 11.0 -> 9.7 us, 512 rows 5120 -> 2560 18.4 -> 15.7.
 constexpr int kSomeWaves = 8, kSomePad = 68;  // (rows of sums 68 floats apart: 16 of them cover the LDS banks)
-template <class V8, int MB>
+template <class V8, int MB, int RW>
 __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
+  constexpr int KW = kSomeWaves / RW;  // waves that share K; RW tiles of 16 MB rows
   __shared__ __align__(16) float red[kSomeWaves][16 * MB * kSomePad];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rg = wave / KW, kw = wave % KW;
   const int Kb = (p.K + 127) / 128, Mb = p.Mp / 16;
   // row tiles run fastest: those that share weights are on one XCD at one time
-  const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, mb0 = (t - ng * p.mtiles) * MB;
+  const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, mbt = (t - ng * p.mtiles) * MB * RW, mb0 = min(mbt + rg * MB, Mb - 1);
   const rsrc_t rw = make_rsrc(p.wq + (size_t)ng * Kb * 8192), rx = make_rsrc(p.xq + (size_t)mb0 * Kb * 2048);
   const rsrc_t rs = make_rsrc(p.sx);
   const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
@@ -255,12 +259,12 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
     }
   };
   Block k0, k1;
-  if (wave < Kb) load(k0, wave);
-  for (int kb = wave; kb < Kb; kb += 2 * kSomeWaves) {
-    load(k1, kb + kSomeWaves);
+  if (kw < Kb) load(k0, kw);
+  for (int kb = kw; kb < Kb; kb += 2 * KW) {
+    load(k1, kb + KW);
     take(k0);
-    if (kb + kSomeWaves >= Kb) break;
-    load(k0, kb + 2 * kSomeWaves);
+    if (kb + KW >= Kb) break;
+    load(k0, kb + 2 * KW);
     take(k1);
   }
 #pragma unroll
@@ -269,14 +273,15 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
     for (int j = 0; j < 4; j++)
       *reinterpret_cast<f32x4*>(&red[wave][(16 * b + (lane & 15)) * kSomePad + 16 * (lane >> 4) + 4 * j]) = acc[b][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * MB * 8; i += 64 * kSomeWaves) {  // 8 columns of a row each
-    const int r = i >> 3, c = 8 * (i & 7), m = 16 * mb0 + r, n = 64 * ng + c;
+  for (int i = threadIdx.x; i < RW * 16 * MB * 8; i += 64 * kSomeWaves) {  // 8 columns of a row each
+    const int ri = i >> 3, c = 8 * (i & 7), m = 16 * mbt + ri, n = 64 * ng + c;
     if (m >= p.M || n >= p.N) continue;
+    const int g = ri / (16 * MB) * KW, r = ri % (16 * MB);
     f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
 #pragma unroll
-    for (int w = 0; w < kSomeWaves; w++) {
-      a += *reinterpret_cast<const f32x4*>(&red[w][r * kSomePad + c]);
-      b += *reinterpret_cast<const f32x4*>(&red[w][r * kSomePad + c + 4]);
+    for (int w = 0; w < KW; w++) {
+      a += *reinterpret_cast<const f32x4*>(&red[g + w][r * kSomePad + c]);
+      b += *reinterpret_cast<const f32x4*>(&red[g + w][r * kSomePad + c + 4]);
     }
     if (p.part) {
       *reinterpret_cast<f32x4*>(p.part + (size_t)m * p.N + n) = a;
@@ -510,10 +515,10 @@ static hipError_t launch_gemm(F8Args a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <class V8, int MB>
+template <class V8, int MB, int RW>
 static hipError_t launch_some(F8Args a, hipStream_t s) {
-  a.mtiles = (a.Mp / 16 + MB - 1) / MB;
-  ESM_LAUNCH((f8_some_kernel<V8, MB>), dim3((unsigned)((size_t)a.mtiles * ((a.N + 63) / 64))), dim3(64 * kSomeWaves), 0, s, a);
+  a.mtiles = (a.Mp / 16 + MB * RW - 1) / (MB * RW);
+  ESM_LAUNCH((f8_some_kernel<V8, MB, RW>), dim3((unsigned)((size_t)a.mtiles * ((a.N + 63) / 64))), dim3(64 * kSomeWaves), 0, s, a);
   return hipGetLastError();
 }
 
@@ -532,7 +537,7 @@ static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) 
   ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, ((a.K + 127) / 128 + kQuantBlocks - 1) / kQuantBlocks), dim3(256), 0, s,
              (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  if (form == kF8Some) return mb == 2 ? launch_some<V8, 2>(a, s) : launch_some<V8, 4>(a, s);
+  if (form == kF8Some) return mb == 2 ? launch_some<V8, 2, 1>(a, s) : mb == 4 ? launch_some<V8, 4, 1>(a, s) : launch_some<V8, 4, 2>(a, s);
   switch (mb) {
     case 2: e = launch_gemm<V8, 2, 2, 4, 2>(a, s); break;
     case 4: e = launch_gemm<V8, 4, 2, 4, 2>(a, s); break;
@@ -552,10 +557,10 @@ hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipS
 
 // Which form, its row blocks and splits: the lowest of estimated times, from these measurements (us, kernel alone,
 // K = 2560 -> N = 7680 unless said; some: 64 x 64 tiles without barriers; 64, 128, 192, 256: LDS tiles of that many rows):
-//   M = 238   some 13.8, 64 rows 18      M = 512   some 23, 64: 18.6, 128: 22, 256: 32
+//   M = 238   some 9.7, 64 rows 18       M = 512   some 23, 64: 18.6, 128: 22, 256: 32
 //   M = 1000  some 44, 64: 36, 128: 24, 192: 27, 256: 33     M = 1500  128: 44, 192: 31, 256: 33
 //   M = 2000  128: 46, 192: 55, 256: 38    M = 3481  128: 90, 192: 86, 256: 70
-//   5120 -> 2560 at M = 238  some 11.1, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 19, 64 rows in two
+//   5120 -> 2560 at M = 238  some 9.8, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 15.7, 64 rows in two
 //   splits 21 and 5; at M = 1000  some 31, 64 rows 33, 128 rows in three splits 25 and 6
 F8Plan f8_plan(int M, int K, int N, int cus) {
   // Few rows: the most weight rows a workgroup (16, 32 or 64) that still give more than half the CUs one, as each
@@ -572,6 +577,10 @@ F8Plan f8_plan(int M, int K, int N, int cus) {
   p.form = kF8Some;
   p.mb = M <= 32 || 2 * tiles < cus ? 2 : 4;
   double best = 2.5 + 1.2e-3 * Kb * (tiles > cus ? tiles : cus) * cus / 256;
+  if (p.mb == 4 && tiles > cus && (double)((M + 127) / 128) * ((N + 63) / 64) <= cus) {  // 128 rows in one round
+    p.mb = 8;
+    best = 2.5 + 1.5e-3 * Kb * cus;
+  }
   const struct { int mb; double step; } forms[] = {{2, 0.78}, {4, 1.0}, {6, 1.25}, {8, 1.55}};  // us a block of k
   for (const auto& f : forms)
     for (int sp = 1; sp <= kF8MaxSplits && (sp == 1 || 4 * sp <= Kb); sp++) {

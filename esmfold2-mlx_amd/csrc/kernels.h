@@ -207,7 +207,7 @@ constexpr int kF8MaxSplits = 16;
 enum : int { kF8Few = 0, kF8Some = 1, kF8Tiles = 2 };
 struct F8Plan {
   int form;
-  int mb;                 // 16-row blocks: of x per wave; of the weight per workgroup (kF8Few)
+  int mb;                 // 16-row blocks: of the weight per workgroup (kF8Few), of x per workgroup (kF8Some) or wave (kF8Tiles)
   int splits;             // of K between workgroups (kF8Tiles)
 };
 

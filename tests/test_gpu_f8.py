@@ -49,6 +49,16 @@ def test_few_rows_of_wide_outputs(gpu_lib, pkg, M, K, N):
     _check(lin(x), x, lin.codes, lin.scales)
 
 
+@pytest.mark.parametrize("M,K,N", [(238, 2560, 7680), (140, 400, 7800), (197, 144, 8000), (100, 1296, 10248), (500, 640, 2560)])
+def test_some_rows_in_tiles_of_128(gpu_lib, pkg, M, K, N):
+    x, w = _inputs(M, K, N, torch.float16, seed=5)
+    lin = pkg.f8.F8Linear.from_float(w)
+    buf = torch.full((M * N + 128,), 9.0, dtype=x.dtype, device=DEV)
+    y = pkg.kernels.f8_linear(x, lin.codes_packed, lin.scales, N, out=buf[64:64 + M * N].view(M, N))
+    _check(y, x, lin.codes, lin.scales)
+    assert bool((buf[:64] == 9.0).all() and (buf[64 + M * N:] == 9.0).all())
+
+
 @pytest.mark.parametrize("M,K,N", [(2049, 272, 8000), (4100, 640, 3584), (1000, 5120, 2560), (3481, 2560, 7680),
                                    (1000, 10240, 2560), (600, 8192, 1024), (530, 2576, 7688), (1010, 2560, 7680)])
 def test_many_rows(gpu_lib, pkg, M, K, N):
