@@ -309,13 +309,13 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
     sequence are not written. ``out`` may be q, and shares no memory with k and v. The partial results of few rows
-    against many keys live in the shared scratch."""
+    against many keys live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
         o = capi.bind.packed_attention(q, k, v, cu_q, cu_k, causal, scale, 0, 0)
         if type(o) is int:  # bytes of workspace
             with scratch.guard(q.device):
-                ws, wp, _ = scratch.take(o, q.device)
+                ws, wp, _ = scratch.workspace(o, q.device)
                 o = capi.bind.packed_attention(q, k, v, cu_q, cu_k, causal, scale, wp, o)
         if o is not None:
             return o
@@ -356,7 +356,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
         capi.check(lib.packed_attention(*args, None, 0, capi.stream_ptr()))
         return o
     with scratch.guard(q.device):
-        ws, wp, stream = scratch.take(need, q.device)
+        ws, wp, stream = scratch.workspace(need, q.device)
         capi.check(lib.packed_attention(*args, wp, need, stream))
     return o
 
@@ -719,13 +719,13 @@ def _f8_operands(x, codes, scales, N, fn):
 def f8_linear(x, codes, scales, N: int, out=None):
     """y = x . W^T on the fp8 matrix cores: x [M, K] fp16 or bf16 (rows may lie apart), brought to e4m3 with a scale
     per row and 128 columns; W [N, K] as packed e4m3 codes (``f8_pack_codes``) with an fp32 scale per 128 x 128 block;
-    fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch."""
+    fp32 sums. x in e4m3 and split-K partials live in the device's shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
         y = capi.bind.f8_linear(x, codes, scales, N, 0, 0)
         if type(y) is int:  # bytes of workspace
             with scratch.guard(x.device):
-                ws, wp, _ = scratch.take(y, x.device)
+                ws, wp, _ = scratch.workspace(y, x.device)
                 y = capi.bind.f8_linear(x, codes, scales, N, wp, y)
         if y is not None:
             return y
@@ -747,7 +747,7 @@ def f8_linear(x, codes, scales, N: int, out=None):
         capi.check(lib.f8_linear(*args, None, 0, capi.stream_ptr()))
         return y
     with scratch.guard(x.device):
-        ws, wp, stream = scratch.take(need, x.device)
+        ws, wp, stream = scratch.workspace(need, x.device)
         capi.check(lib.f8_linear(*args, wp, need, stream))
     return y
 

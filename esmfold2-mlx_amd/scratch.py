@@ -22,6 +22,9 @@ Rules:
     consumer holds the guard from that check until it is queued).
   * A HIP graph that captured calls keeps the buffers they used alive: ``current`` gives
     the buffer to hold next to the graph.
+  * ``workspace`` is ``take`` for calls whose bytes nobody reads later. Under capture it gives
+    memory of the graph's own instead, so such a graph needs nothing held next to it, and two
+    of them may be replayed at once.
 """
 
 from __future__ import annotations
@@ -109,6 +112,15 @@ def take(nbytes: int, device=None):
     buffer and ``guard(device)`` until its launches are queued."""
     buf, raw = _claim(nbytes, device)
     return buf, (buf.data_ptr() + ALIGN - 1) // ALIGN * ALIGN, raw
+
+
+def workspace(nbytes: int, device=None):
+    """``take`` for a call that leaves nothing there; under HIP-graph capture (of the current device) from the graph's
+    memory pool."""
+    if not torch.cuda.is_current_stream_capturing():
+        return take(nbytes, device)
+    buf = torch.empty(nbytes + ALIGN, dtype=torch.uint8, device=device)
+    return buf, (buf.data_ptr() + ALIGN - 1) // ALIGN * ALIGN, torch._C._cuda_getCurrentRawStream(buf.get_device())
 
 
 def generation(device=None) -> int:

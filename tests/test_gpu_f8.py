@@ -166,6 +166,37 @@ def test_graph_and_repeats(gpu_lib, pkg, M):
     del keep
 
 
+@pytest.mark.parametrize("M,K,N", [(100, 640, 2560), (1000, 10240, 2560)])
+def test_graphs_have_workspaces_of_their_own(gpu_lib, pkg, M, K, N):
+    # (the second with partials of a divided K beside x in e4m3)
+    lins, xs, graphs, outs, refs = [], [], [], [], []
+    for seed in (1, 2):
+        x, w = _inputs(M, K, N, torch.bfloat16, seed=seed)
+        lin = pkg.f8.F8Linear.from_float(w)
+        lins.append(lin), xs.append(x), refs.append(lin(x))
+    before = pkg.scratch.generation(DEV)
+    for lin, x in zip(lins, xs):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(lin(x))
+        graphs.append(graph)
+    assert pkg.scratch.generation(DEV) == before
+    with pkg.scratch.guard(DEV):
+        pkg.scratch.get(pkg.scratch.current(DEV).numel() + 1, DEV).fill_(255)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(10):
+            graphs[0].replay()
+            with torch.cuda.stream(side):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, r) for o, r in zip(outs, refs))
+
+
 def test_codes_that_are_not_numbers(gpu_lib, pkg):
     # a NaN code makes its own output column NaN, nothing else
     x, w = _inputs(40, 256, 192, torch.float16)

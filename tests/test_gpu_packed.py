@@ -252,6 +252,39 @@ def test_graph_and_side_stream(gpu_lib, pkg, nq, nk):
     del keep
 
 
+def test_graphs_have_workspaces_of_their_own(gpu_lib, pkg):
+    # two graphs whose rows have several chunks of keys, replayed at once, after the shared scratch has been given up
+    cases, graphs, outs, refs = [], [], [], []
+    for seed in (1, 2):
+        q, k, v, cq, ck = _case([1] * 8, [6000, 900, 3, 2000, 65, 0, 128, 4100], 8, 2, 128, torch.bfloat16, seed=seed)
+        cases.append((q, k, v, _cu(cq), _cu(ck)))
+        refs.append(pkg.kernels.packed_attention(*cases[-1], causal=True))
+    assert pkg.capi.lib().packed_attention_workspace_bytes(8, 8, cases[0][1].shape[0], 8, 2, 128) > 0
+    before = pkg.scratch.generation(DEV)
+    for c in cases:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(pkg.kernels.packed_attention(*c, causal=True))
+        graphs.append(graph)
+    assert pkg.scratch.generation(DEV) == before
+    with pkg.scratch.guard(DEV):
+        pkg.scratch.get(pkg.scratch.current(DEV).numel() + 1, DEV).fill_(255)
+    other = torch.full((1 << 22,), float("nan"), device=DEV)
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        for o in outs:
+            o.fill_(7.0)
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(10):
+            graphs[0].replay()
+            with torch.cuda.stream(side):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, r) for o, r in zip(outs, refs))
+    assert bool(other.isnan().all())
+
+
 def test_refusals(gpu_lib, pkg):
     K, E = pkg.kernels, pkg.capi.EsmError
     x = torch.zeros(8, 4, 64, dtype=torch.float16, device=DEV)
