@@ -296,6 +296,9 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
         if T and (qo.data_ptr() == k.data_ptr() or ko.data_ptr() == q.data_ptr() or qo.data_ptr() == ko.data_ptr()):
             raise capi.EsmError(-3, "qk_norm_rope: out may be (q, k), each in its own place")
         (_, qo_st, qo_sh), (_, ko_st, ko_sh) = _rows(qo, "out[0]"), _rows(ko, "out[1]")
+        for i, t, same in ((0, q, (qo_st, qo_sh) == (q_st, q_sh)), (1, k, (ko_st, ko_sh) == (k_st, k_sh))):
+            if T and out[i].data_ptr() == t.data_ptr() and not same:
+                raise capi.EsmError(-3, f"qk_norm_rope: out[{i}] over its input must have the input's strides")
     capi.check(lib.qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
         qwh, kw, kwh, float(eps), pos, pos64, freq.data_ptr(), float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
@@ -308,7 +311,7 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     wider rows allowed; H a multiple of Hk) -> o [Tq, H, d]. ``cu_q``, ``cu_k`` int32 [n + 1] on the device: the first
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
-    sequence are not written. ``out`` may be q, and shares no memory with k and v. The partial results of few rows
+    sequence are not written. ``out`` may be q, and shares no other memory with the operands. The partial results of few rows
     against many keys live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
@@ -348,6 +351,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
             raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
         if Tq and Tk and o.data_ptr() in (k.data_ptr(), v.data_ptr()):
             raise capi.EsmError(-3, "packed_attention: out may be q, not k or v")
+        if Tq and o.data_ptr() == q.data_ptr() and (o_st, o_sh) != (q_st, q_sh):
+            raise capi.EsmError(-3, "packed_attention: out over q must have its strides")
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
             cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else float(scale),
             _DTYPES[dtype])

@@ -318,3 +318,5 @@ def test_refusals(gpu_lib, pkg):
     y = torch.zeros_like(x)
     refused(-3, x, y, x, cu, out=y)
     refused(-3, x, x.clone(), y, cu, out=y)
+    buf = torch.zeros(8, 4, 64, dtype=torch.float16, device=DEV)
+    refused(-3, buf[:, :2], x[:, :2], x[:, :2], cu, out=buf.view(-1)[:1024].view(8, 2, 64))  # over q, other strides

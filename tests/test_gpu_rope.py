@@ -145,6 +145,8 @@ def test_refusals(gpu_lib, pkg):
     refused(-3, q, p, f, out=(p, q))
     refused(-3, q, p, f, out=(p.clone(), q))
     refused(-3, q[..., 4:36], q[..., 4:36], f[:16])
+    refused(-3, p[:, :1], q, f, out=(p.view(-1)[:256].view(4, 1, 64), q))    # over q, other strides
+    refused(-3, q, p[:, :1], f, out=(q, p.view(-1)[:256].view(4, 1, 64)))
     w = torch.zeros(1, 520, 256, dtype=torch.float16, device=DEV)
     refused(-4, w, w, f, norm="rms", over="row")
     assert K.qk_norm_rope(q[:0], q[:0], f)[0].shape == (0, 2, 64)
