@@ -175,6 +175,8 @@ class EsmcBlock(nn.Module):
         """``run`` on packed rows x [T, D] fp32 and h = LN1(x): the sequences that begin at cu [n + 1] (int32, on the
         device), each attending to itself, with ``positions`` [T] turned by ``rotary``."""
         T, D = x.shape
+        if not isinstance(self, EsmcBlock) or getattr(self.attention, "__func__", None) is not EsmcBlock.attention:
+            raise ValueError("packed ESMC: a replaced attention takes [B, L, D] rows only (a block may bring a run_packed)")
         q, k, v = self.wqkv(h).view(T, 3, self.n_heads, 64).unbind(1)
         rotary(q, k, positions, norm="layer", over="row", q_w=self.q_ln, k_w=self.k_ln, eps=EPS, out=(q, k))
         o = kernels.packed_attention(q, k, v, cu).view(T, D)
@@ -347,7 +349,7 @@ class HipEsmc(nn.Module):
         x_last = torch.empty(T, D, dtype=torch.float32, device=dev)
         states = hs.unbind(0)
         for i, blk in enumerate(self.layers):
-            run = blk.run_packed if hasattr(blk, "run_packed") else partial(EsmcBlock.run_packed, blk)
+            run = blk.run_packed if hasattr(blk, "run_packed") else partial(EsmcBlock.run_packed, blk)  # (refuses)
             last = i + 1 == n
             w, b = (self.norm_w, None) if last else (self.layers[i + 1].ln1_w, self.layers[i + 1].ln1_b)
             run(states[i], h, cu, positions, self._rotary, self.res_scale, w, b, x_last if last else states[i + 1],

@@ -256,7 +256,7 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
                  over: str = "head", q_w=None, k_w=None, eps: float = 1e-6, out=None):
     """Norm and rotation of q [T, H, d] and k [T, Hk, d] (fp16 or bf16, views of wider rows allowed) in one pass ->
     (q', k'). ``norm``: None, "rms" or "layer", ``over`` each "head" or the whole "row" of heads, with fp32 weights of
-    d or heads * d values (None: 1). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
+    d or heads * d values (None: 1; without a norm not read). ``freq`` [rot / 2] fp64: radians per position of each pair (``rotary.Rotary``
     makes it); pairs (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``. ``positions`` [T] int32 or int64 (None:
     0 .. T - 1). ``out`` = (q', k'), which may be (q, k) but share no other memory with them."""
     lib = capi.lib()

@@ -445,7 +445,7 @@ int esmc_swiglu(const esm_half* x12, esm_half* y, int M, int F, void* stream);
  *
  * qk_norm_rope: q [T, H, d], k [T, Hk, d] -> q_out, k_out (which may be q and k): norm (ESM_NORM_NONE, _RMS:
  *   x / sqrt(mean x^2 + eps), _LAYER: the same of x - mean x) over each head, or with over_row over all heads of the
- *   row (q and k apart), times the weights (fp32, [d] or [heads * d] as q_w_heads, k_w_heads say; NULL: 1); then the
+ *   row (q and k apart), times the weights (fp32, [d] or [heads * d] as q_w_heads, k_w_heads say; NULL: 1; not read without a norm); then the
  *   first rot values of each head turn by position * freq[i] (freq [rot / 2] fp64, radians per position), in pairs
  *   (i, i + rot / 2) or, interleaved, (2i, 2i + 1), with sine and cosine times gain. pos: [T] int32 (pos64: int64), or
  *   NULL for 0 .. T - 1. fp32 but for the angle (fp64), rounded once. d % 8 == 0, 8 <= d <= 256; rot % 16 == 0,

@@ -121,6 +121,32 @@ def test_packed_arguments(gpu_lib, pkg):
     assert model.packed([torch.zeros(0, dtype=torch.int64)]).hidden_states.shape == (2, 0, 128)
 
 
+def test_packed_runs_replaced_parts_or_refuses(gpu_lib, pkg):
+    model, *_ = _model(pkg, 128, 192, 2, 2)
+    ids = [torch.randint(0, 33, (n,), generator=_gen(n)) for n in (30, 7)]
+    want = model.packed(ids).hidden_states
+    blk, calls = model.layers[1], []
+    ffn = blk.ffn
+    blk.ffn = lambda h: (calls.append("ffn"), ffn(h))[1]
+    hook = blk.wqkv.register_forward_hook(lambda *a: calls.append("wqkv"))
+    assert torch.equal(model.packed(ids).hidden_states, want) and calls == ["wqkv", "ffn"]
+    hook.remove()
+    attention = blk.attention
+    blk.attention = lambda *a: attention(*a)
+    with pytest.raises(ValueError):
+        model.packed(ids)
+    del blk.attention
+
+    class Other(torch.nn.Module):  # another module in the block's place, as hidden_states takes it
+        def __init__(self):
+            super().__init__()
+            self.ln1_w, self.ln1_b, self.ffn, self.attention = blk.ln1_w, blk.ln1_b, blk.ffn, blk.attention
+            self.wqkv, self.n_heads = blk.wqkv, blk.n_heads
+    model.layers[1] = Other()
+    with pytest.raises(ValueError):
+        model.packed(ids)
+
+
 def _f8_reference(p, x, H, rs, dense):
     """oe.block_forward with each linear's input brought to e4m3 as the operator does it."""
     D = x.shape[-1]
