@@ -1,6 +1,7 @@
 """Attention over packed sequences against a 64-bit restatement of its definition, with bounds from the arithmetic."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -250,6 +251,35 @@ def test_graph_and_side_stream(gpu_lib, pkg, nq, nk):
         torch.cuda.synchronize()
         assert torch.equal(out, ref) and torch.equal(again, ref)
     del keep
+
+
+def test_two_threads_on_their_own_streams(gpu_lib, pkg):
+    # calls whose chunks of keys meet in the device's one scratch buffer, beside linears that use it too
+    q, k, v, cq, ck = _case([1] * 4, [5000, 70, 0, 2500], 8, 2, 128, torch.float16, seed=3)
+    cuq, cuk = _cu(cq), _cu(ck)
+    x = torch.randn(100, 640, generator=torch.Generator().manual_seed(0)).half().to(DEV)
+    lin = pkg.f8.F8Linear.from_float(torch.randn(2560, 640, generator=torch.Generator().manual_seed(1)))
+    ref, lref = pkg.kernels.packed_attention(q, k, v, cuq, cuk, causal=True), lin(x)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    a = pkg.kernels.packed_attention(q, k, v, cuq, cuk, causal=True)
+                    b = lin(x)
+                    if not (torch.equal(a, ref) and torch.equal(b, lref)):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001  (shown by the assertion)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_graphs_have_workspaces_of_their_own(gpu_lib, pkg):

@@ -57,6 +57,17 @@ def test_stretched_contexts(gpu_lib, pkg, scaling):
         _check(y, O.norm_rope(x, None, pos, rotary.freq, rotary.gain, 128, False, "rms", "head", 1e-6))
 
 
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+def test_positions_before_zero_and_past_32_bits(gpu_lib, pkg, wide):
+    q, k = _inputs(5, 8, 2, 64, torch.bfloat16, seed=9)
+    rotary = pkg.rotary.Rotary(64)
+    far = 2 ** 31 - 1 if wide is torch.int32 else 2 ** 34 + 5
+    pos = torch.tensor([-1, -77, -far, 0, far], dtype=wide)
+    got = rotary(q, k, pos.to(DEV))
+    for y, x in zip(got, (q, k)):
+        _check(y, O.norm_rope(x, None, pos, rotary.freq, rotary.gain, 64, False, None, "head", 1e-6))
+
+
 @pytest.mark.parametrize("T", [1, 2, 513, 2000])
 def test_row_counts_default_positions_and_in_place(gpu_lib, pkg, T):
     q, k = _inputs(T, 32, 4, 64, torch.bfloat16, seed=T)
