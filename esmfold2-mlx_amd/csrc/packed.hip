@@ -274,6 +274,38 @@ struct Span {
   int q0, nq, k0, nk;  // first row and rows of a sequence, on the query and on the key side
 };
 
+// Sum and maximum over the wave, the same in every lane, and the sum of the lanes up to this one, by data-parallel moves
+// (an exchange through LDS answers in some 100 cycles, and six of them in a row stood before a tile's first load).
+template <class F>
+DEV int wave_rows(int v, F f) {  // over each row of 16 lanes
+  const auto with = [&](auto ctrl) { v = f(v, __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)); };
+  with(std::integral_constant<int, 0x128>{});  // row_ror:8, 4, 2, 1
+  with(std::integral_constant<int, 0x124>{});
+  with(std::integral_constant<int, 0x122>{});
+  with(std::integral_constant<int, 0x121>{});
+  return v;
+}
+DEV int wave_sum(int v) {
+  v = wave_rows(v, [](int a, int b) { return a + b; });
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
+}
+DEV int wave_max(int v) {
+  v = wave_rows(v, [](int a, int b) { return max(a, b); });
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+DEV int wave_scan(int v) {
+  const auto add = [&](auto ctrl) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, false); };
+  add(std::integral_constant<int, 0x111>{});  // row_shr:1, 2, 4, 8 (0 from before the row)
+  add(std::integral_constant<int, 0x112>{});
+  add(std::integral_constant<int, 0x114>{});
+  add(std::integral_constant<int, 0x118>{});
+  const int row = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)) >> 4;
+  const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+  return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+
 // Sequence of a work item and the item's number within it: a sequence has as many items as tiles of `unit` rows times
 // chunks of `chunk` keys (at least one; chunk 0: not counted). All lanes agree; the starts are read once, a lane a
 // sequence. Starts outside 0 .. the rows there are are brought inside, so nothing a caller writes there reaches past
@@ -286,12 +318,7 @@ DEV bool find_item(const PackedAttnArgs& p, int unit, int chunk, int item, int l
     int nt = ((b - a) * p.G + unit - 1) / unit;
     if (chunk) nt *= max(1, (kb - ka + chunk - 1) / chunk);
     if (i0 + lane >= p.n) nt = 0;
-    int sum = nt;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(sum, o);
-      sum += lane >= o ? up : 0;
-    }
+    const int sum = wave_scan(nt);
     const uint64_t past = __ballot(item < sum);
     if (past) {
       const int w = __builtin_ctzll(past);
@@ -307,17 +334,6 @@ DEV bool find_item(const PackedAttnArgs& p, int unit, int chunk, int item, int l
   return false;
 }
 
-// Sum over the wave, the same in every lane.
-DEV int wave_sum(int v) {
-  const auto add = [&](auto ctrl) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, false); };
-  add(std::integral_constant<int, 0x128>{});  // row_ror:8, 4, 2, 1
-  add(std::integral_constant<int, 0x124>{});
-  add(std::integral_constant<int, 0x122>{});
-  add(std::integral_constant<int, 0x121>{});
-  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
-         __builtin_amdgcn_readlane(v, 48);
-}
-
 // find_item for tiles of kAttnRows rows of 2 to 64 sequences, the longest tiles first whichever sequence they are of, so
 // that no long one starts last (prompts of 1 to 4,096 rows 289 -> 244 us): the keys a tile sees fall into 16 levels, and
 // how many tiles of a sequence see at least so many follows from its lengths. `at` counts a sequence's tiles from the
@@ -330,10 +346,7 @@ DEV bool find_longest(const PackedAttnArgs& p, int item, int lane, Span& s, int&
   const int ka = min(max(p.cu_k[i], 0), p.Tk), kb = min(max(p.cu_k[i + 1], ka), p.Tk);
   const int nq = b - a, nk = kb - ka, tiles = lane < p.n ? (nq * p.G + kAttnRows - 1) / kAttnRows : 0;
   if (item >= wave_sum(tiles)) return false;
-  int most = lane < p.n ? nk : 0;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
-  const int level = __builtin_amdgcn_readfirstlane(most / 16 + 1);
+  const int level = wave_max(lane < p.n ? nk : 0) / 16 + 1;
   // tiles of this lane's sequence whose last row sees at least `keys` keys
   const auto seeing = [&](int keys) {
     if (keys > nk) return 0;
@@ -347,12 +360,7 @@ DEV bool find_longest(const PackedAttnArgs& p, int item, int lane, Span& s, int&
     if (wave_sum(seeing((lv + step) * level)) > item) lv += step;
   const int above = seeing((lv + 1) * level), mine = (lv ? seeing(lv * level) : tiles) - above;
   item -= wave_sum(above);
-  int sum = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(sum, o);
-    sum += lane >= o ? up : 0;
-  }
+  const int sum = wave_scan(mine);
   const int w = __builtin_ctzll(__ballot(item < sum));
   at = item - __builtin_amdgcn_readlane(sum - mine, w) + __builtin_amdgcn_readlane(above, w);
   s = Span{__builtin_amdgcn_readlane(a, w), __builtin_amdgcn_readlane(nq, w), __builtin_amdgcn_readlane(ka, w),
