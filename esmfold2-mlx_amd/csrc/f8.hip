@@ -210,8 +210,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
 // A workgroup takes 16 MB RW rows of x by 64 weight rows; its 8 waves deal the blocks of 128 k among them (RW = 2:
 // four waves to each half of the rows), read both operands' fragments straight from memory (the next block's in
 // flight) and sum through LDS. Through LDS tiles a step of this size is a chain of latencies (0.47 us at
-// 64 x 128 x 128, whatever its neighbours do). One workgroup lies on a CU (240 registers), so 128 rows serve where
-// 64 would need a second round: 238 rows 2560 -> 7680 11.0 -> 9.7 us, 512 rows 5120 -> 2560 18.4 -> 15.7.
+// 64 x 128 x 128, whatever its neighbours do). One workgroup of 64 rows lies on a CU (240 registers), so 128 rows serve
+// where 64 would need a second round: 238 rows 2560 -> 7680 11.0 -> 9.7 us, 512 rows 5120 -> 2560 18.4 -> 15.7. Bound by L2:
+// 238 rows 5120 -> 2560 in tiles of 48 8.0 us, 14 TB/s of fragments.
 constexpr int kSomeWaves = 8, kSomePad = 68;  // (rows of sums 68 floats apart: 16 of them cover the LDS banks)
 template <class V8, int MB, int RW>
 __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
@@ -539,7 +540,13 @@ static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) 
   ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, ((a.K + 127) / 128 + kQuantBlocks - 1) / kQuantBlocks), dim3(256), 0, s,
              (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  if (form == kF8Some) return mb == 2 ? launch_some<V8, 2, 1>(a, s) : mb == 4 ? launch_some<V8, 4, 1>(a, s) : launch_some<V8, 4, 2>(a, s);
+  if (form == kF8Some) switch (mb) {
+      case 1: return launch_some<V8, 1, 1>(a, s);
+      case 2: return launch_some<V8, 2, 1>(a, s);
+      case 3: return launch_some<V8, 3, 1>(a, s);
+      case 4: return launch_some<V8, 4, 1>(a, s);
+      default: return launch_some<V8, 4, 2>(a, s);
+    }
   switch (mb) {
     case 2: e = launch_gemm<V8, 2, 2, 4, 2>(a, s); break;
     case 4: e = launch_gemm<V8, 4, 2, 4, 2>(a, s); break;
@@ -562,7 +569,7 @@ hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipS
 //   M = 238   some 9.7, 64 rows 18       M = 512   some 23, 64: 18.6, 128: 22, 256: 32
 //   M = 1000  some 44, 64: 36, 128: 24, 192: 27, 256: 33     M = 1500  128: 44, 192: 31, 256: 33
 //   M = 2000  128: 46, 192: 55, 256: 38    M = 3481  128: 90, 192: 86, 256: 70
-//   5120 -> 2560 at M = 238  some 9.8, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 15.7, 64 rows in two
+//   5120 -> 2560 at M = 238  some 8.0, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 15.7, 64 rows in two
 //   splits 21 and 5; at M = 1000  some 31, 64 rows 33, 128 rows in three splits 25 and 6
 F8Plan f8_plan(int M, int K, int N, int cus) {
   // Few rows: the most weight rows a workgroup (16, 32 or 64) that still give more than half the CUs one, as each
@@ -575,13 +582,18 @@ F8Plan f8_plan(int M, int K, int N, int cus) {
   while (p.mb > 1 && 16LL * ((N + 63) / 64) * (4 / p.mb) < 9LL * cus) p.mb /= 2;
   if (M <= 16) return p;
   const int Kb = (K + 127) / 128;
-  const double tiles = (double)((M + 63) / 64) * ((N + 63) / 64);
+  // Some rows: the fewest rows a workgroup (16 to 64) whose tiles fit one to a CU; else 32 if two to a CU take them all
+  // (70 KB of LDS each), else 128 if those fit, else rounds of 64 (us, 16 / 32 / 48 / 64 rows a workgroup: 64 rows
+  // 5120 -> 2560 5.7 / 6.5 / 7.8 / 9.1, 238 rows - / 11.3 / 8.0 / 9.5, 96 rows 2560 -> 7680 - / 7.5 / 5.5 / 6.2, 24 rows
+  // 2560 -> 10240 5.4 / 4.6 / 4.9 / 5.6, 96 rows - / 8.0 / 9.3 / 10.8; 128 rows see f8_some_kernel).
+  const long long pieces = (N + 63) / 64;
+  const auto tiles = [&](int mb) { return ((M + 15) / 16 + mb - 1) / mb * pieces; };
   p.form = kF8Some;
-  p.mb = M <= 32 || 2 * tiles < cus ? 2 : 4;
-  double best = 2.5 + 1.2e-3 * Kb * (tiles > cus ? tiles : cus) * cus / 256;
-  if (p.mb == 4 && tiles > cus && (double)((M + 127) / 128) * ((N + 63) / 64) <= cus) {  // 128 rows in one round
-    p.mb = 8;
-    best = 2.5 + 1.5e-3 * Kb * cus;
+  for (p.mb = 1; p.mb < 5 && tiles(p.mb) > cus;) p.mb++;
+  double best = 2.5 + Kb * (0.03 + 0.045 * p.mb);
+  if (p.mb == 5) {
+    p.mb = tiles(2) <= 2 * cus ? 2 : tiles(8) <= cus ? 8 : 4;
+    best = 2.5 + Kb * (p.mb == 2 ? 0.28 : p.mb == 8 ? 0.38 : 1.2e-3 * (double)tiles(4) * cus / 256);
   }
   const struct { int mb; double step; } forms[] = {{2, 0.78}, {4, 1.0}, {6, 1.25}, {8, 1.55}};  // us a block of k
   for (const auto& f : forms)

@@ -49,8 +49,9 @@ def test_few_rows_of_wide_outputs(gpu_lib, pkg, M, K, N):
     _check(lin(x), x, lin.codes, lin.scales)
 
 
-@pytest.mark.parametrize("M,K,N", [(238, 2560, 7680), (140, 400, 7800), (197, 144, 8000), (100, 1296, 10248), (500, 640, 2560)])
-def test_some_rows_in_tiles_of_128(gpu_lib, pkg, M, K, N):
+@pytest.mark.parametrize("M,K,N", [(238, 2560, 7680), (140, 400, 7800), (197, 144, 8000), (100, 1296, 10248), (500, 640, 2560),
+                                   (96, 2560, 10240), (90, 272, 9000)])
+def test_some_rows_in_tiles_of_128_and_two_to_a_cu(gpu_lib, pkg, M, K, N):
     x, w = _inputs(M, K, N, torch.float16, seed=5)
     lin = pkg.f8.F8Linear.from_float(w)
     buf = torch.full((M * N + 128,), 9.0, dtype=x.dtype, device=DEV)
@@ -65,6 +66,17 @@ def test_many_rows(gpu_lib, pkg, M, K, N):
     x, w = _inputs(M, K, N, torch.bfloat16, seed=1)
     lin = pkg.f8.F8Linear.from_float(w)
     _check(lin(x), x, lin.codes, lin.scales)
+
+
+@pytest.mark.parametrize("M", [17, 40, 96, 97, 130, 238, 250, 330])
+@pytest.mark.parametrize("N", [2560, 7688])
+def test_every_tile_height_of_some_rows(gpu_lib, pkg, M, N):
+    x, w = _inputs(M, 1168, N, torch.bfloat16, seed=7)
+    lin = pkg.f8.F8Linear.from_float(w)
+    buf = torch.full((M * N + 128,), 9.0, dtype=x.dtype, device=DEV)
+    y = pkg.kernels.f8_linear(x, lin.codes_packed, lin.scales, N, out=buf[64:64 + M * N].view(M, N))
+    _check(y, x, lin.codes, lin.scales)
+    assert bool((buf[:64] == 9.0).all() and (buf[64 + M * N:] == 9.0).all())
 
 
 def test_weights_from_float_and_codes(gpu_lib, pkg):
