@@ -582,10 +582,11 @@ F8Plan f8_plan(int M, int K, int N, int cus) {
   while (p.mb > 1 && 16LL * ((N + 63) / 64) * (4 / p.mb) < 9LL * cus) p.mb /= 2;
   if (M <= 16) return p;
   const int Kb = (K + 127) / 128;
-  // Some rows: the fewest rows a workgroup (16 to 64) whose tiles fit one to a CU; else 32 if two to a CU take them all
-  // (70 KB of LDS each), else 128 if those fit, else rounds of 64 (us, 16 / 32 / 48 / 64 rows a workgroup: 64 rows
+  // Some rows: the fewest rows a workgroup (16 to 64) whose tiles fit one to a CU; else 32 where two rounds take them
+  // all, else 128 if those fit, else rounds of 64 (us, 16 / 32 / 48 / 64 rows a workgroup: 64 rows
   // 5120 -> 2560 5.7 / 6.5 / 7.8 / 9.1, 238 rows - / 11.3 / 8.0 / 9.5, 96 rows 2560 -> 7680 - / 7.5 / 5.5 / 6.2, 24 rows
-  // 2560 -> 10240 5.4 / 4.6 / 4.9 / 5.6, 96 rows - / 8.0 / 9.3 / 10.8; 128 rows see f8_some_kernel).
+  // 2560 -> 10240 5.4 / 4.6 / 4.9 / 5.6, 96 rows 9.3 / 8.0 / 9.3 / 10.8 and 9.1 in 128; two of 32 rows on a CU at once would take
+  // 128 registers, which spill: 10.3).
   const long long pieces = (N + 63) / 64;
   const auto tiles = [&](int mb) { return ((M + 15) / 16 + mb - 1) / mb * pieces; };
   p.form = kF8Some;

@@ -51,7 +51,7 @@ def test_few_rows_of_wide_outputs(gpu_lib, pkg, M, K, N):
 
 @pytest.mark.parametrize("M,K,N", [(238, 2560, 7680), (140, 400, 7800), (197, 144, 8000), (100, 1296, 10248), (500, 640, 2560),
                                    (96, 2560, 10240), (90, 272, 9000)])
-def test_some_rows_in_tiles_of_128_and_two_to_a_cu(gpu_lib, pkg, M, K, N):
+def test_some_rows_in_tiles_of_128_and_two_rounds(gpu_lib, pkg, M, K, N):
     x, w = _inputs(M, K, N, torch.float16, seed=5)
     lin = pkg.f8.F8Linear.from_float(w)
     buf = torch.full((M * N + 128,), 9.0, dtype=x.dtype, device=DEV)
