@@ -10,8 +10,10 @@
 // A lane owns 16 values of a head, its 8 pairs, as two 16-byte pieces, so that a rotation stays within the
 // lane; 2^lph lanes make a head and a wave takes 64 / 2^lph heads at a time. Memory bound: what matters is
 // that a wave has its loads in flight before the angles, which depend on the row alone and are used for
-// each of the wave's NIT groups of heads. 16,384 rows of 32 + 8 heads of 128 73 us, 4.6 TB/s; 3,481 rows of 40 + 40
-// heads of 64 over the row 20 us, 3.6 TB/s (two barriers for the row's sums); 8 rows 3.4 us.
+// each of the wave's NIT groups of heads. 16,384 rows of 32 + 8 heads of 128 68 us, 4.9 TB/s; 3,481 rows of 40 + 40
+// heads of 64 over the row 17.7 us, 4.0 TB/s (vector work bounds it beside the bytes); 8 rows 3.4 us.
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -31,56 +33,73 @@ DEV float head_sum(float v, int lph) {
   return v;
 }
 
-// Sums of q's and k's parts over the workgroup.
-DEV void row_sum(float& sq, float& sk, float (*red)[kRopeWaves], int nw) {
-  sq = row16_sum(sq);
-  sk = row16_sum(sk);
-  sq += __shfl_xor(sq, 16);
-  sk += __shfl_xor(sk, 16);
-  sq += __shfl_xor(sq, 32);
-  sk += __shfl_xor(sk, 32);
-  const int w = threadIdx.x >> 6;
-  __syncthreads();  // red is reused by consecutive calls
-  if ((threadIdx.x & 63) == 0) {
-    red[0][w] = sq;
-    red[1][w] = sk;
-  }
-  __syncthreads();
-  sq = red[0][0];
-  sk = red[1][0];
-  for (int i = 1; i < nw; i++) {
-    sq += red[0][i];
-    sk += red[1][i];
-  }
+// Sum over the wave, the same in every lane.
+DEV float wave_total(float v) {
+  v = row16_sum(v);
+  const auto lane = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-template <class V8, bool ROW, int NIT>
+// kFull: the head's lanes are all filled (d = 16 2^lph), and q and k both have weights or neither has: no lane's values
+// or weights are guarded. kPlain: and all turn in the half layout (rot = d). The guards took a third of the instructions,
+// which bound the norm over the row (3,481 rows of 40 + 40 heads of 64 20.2 -> 17.7 us).
+enum : int { kGuarded = 0, kFull = 1, kPlain = 2 };
+template <class V8, bool ROW, int NIT, int FORM>
 __global__ __launch_bounds__(64 * kRopeWaves) void qk_norm_rope_kernel(QkRopeArgs p) {
-  __shared__ float red[2][kRopeWaves];
+  constexpr bool FULL = FORM != kGuarded, PLAIN = FORM == kPlain;
+  __shared__ __align__(16) float red[kRopeWaves][4];
   const size_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const int lph = p.lph, hpw = 64 >> lph;             // heads per wave and pass
   const int c = lane & ((1 << lph) - 1), hl = lane >> lph;
-  const bool turn = 16 * c < p.rot;
+  const bool turn = PLAIN || 16 * c < p.rot;
   // the two pieces of this lane: its pairs' first and second values (half layout), or 16 values in a row
-  const int o1 = turn && !p.interleaved ? 8 * c : 16 * c;
-  const int o2 = turn && !p.interleaved ? o1 + p.rot / 2 : o1 + 8;
-  const bool ok1 = o1 < p.d, ok2 = o2 < p.d;
+  const int o1 = PLAIN || (turn && !p.interleaved) ? 8 * c : 16 * c;
+  const int o2 = PLAIN || (turn && !p.interleaved) ? o1 + p.rot / 2 : o1 + 8;
+  const bool ok1 = FULL || o1 < p.d, ok2 = FULL || o2 < p.d;
   const int g0 = (blockIdx.y * nw + wave) * NIT;      // first group of heads of this wave
 
   V8 x1[NIT], x2[NIT];
-  int head[NIT];
+  int head[NIT], hk[NIT];                             // the lane's head (-1: none), its number among q's or k's
+  bool isk[NIT];
 #pragma unroll
   for (int it = 0; it < NIT; it++) {
-    const int hh = (g0 + it) * hpw + hl;
-    head[it] = hh < p.H + p.Hk ? hh : -1;
-    const bool isk = hh >= p.H;
-    const char* src = (const char*)(isk ? p.k : p.q) +
-                      2 * (row * (size_t)(isk ? p.k_st : p.q_st) + (size_t)(isk ? hh - p.H : hh) * (isk ? p.k_sh : p.q_sh));
-    x1[it] = x2[it] = V8{};
-    if (head[it] >= 0 && ok1) x1[it] = *reinterpret_cast<const V8*>(src + 2 * o1);
-    if (head[it] >= 0 && ok2) x2[it] = *reinterpret_cast<const V8*>(src + 2 * o2);
+    const int hh = (g0 + it) * hpw + hl, last = p.H + p.Hk - 1;
+    head[it] = hh <= last ? hh : -1;
+    isk[it] = hh >= p.H;
+    hk[it] = min(hh, last) - (isk[it] ? p.H : 0);     // (past the last head: that one again, not counted or stored)
+    const char* src = (const char*)(isk[it] ? p.k : p.q) +
+                      2 * (row * (size_t)(isk[it] ? p.k_st : p.q_st) + (size_t)hk[it] * (isk[it] ? p.k_sh : p.q_sh));
+    if constexpr (FULL) {
+      x1[it] = *reinterpret_cast<const V8*>(src + 2 * o1);
+      x2[it] = *reinterpret_cast<const V8*>(src + 2 * o2);
+    } else {
+      x1[it] = x2[it] = V8{};
+      if (ok1) x1[it] = *reinterpret_cast<const V8*>(src + 2 * o1);
+      if (ok2) x2[it] = *reinterpret_cast<const V8*>(src + 2 * o2);
+    }
   }
+
+  // The norm's weights are asked for with the values (16,384 rows of 32 + 8 heads of 128, all turned, 64 -> 62 us); over
+  // the row, where a wave takes three groups, they would take the registers of a second workgroup (20 -> 26 us).
+  f32x4 wt[ROW ? 1 : NIT][4];
+  const bool weighted = p.norm && p.q_w;              // (FULL: k's too)
+  const auto weights = [&](int it) {
+    f32x4* t = wt[ROW ? 0 : it];
+    const float* w = (isk[it] ? p.k_w : p.q_w);
+    if constexpr (!FULL) {
+      t[0] = t[1] = t[2] = t[3] = f32x4{1.f, 1.f, 1.f, 1.f};  // (no weight: 1)
+      if (!p.norm || !w) return;
+    } else if (!weighted) {
+      return;
+    }
+    w += (size_t)hk[it] * (isk[it] ? p.kw_sh : p.qw_sh);
+    if (ok1) t[0] = *reinterpret_cast<const f32x4*>(w + o1), t[1] = *reinterpret_cast<const f32x4*>(w + o1 + 4);
+    if (ok2) t[2] = *reinterpret_cast<const f32x4*>(w + o2), t[3] = *reinterpret_cast<const f32x4*>(w + o2 + 4);
+  };
+  if constexpr (!ROW)
+#pragma unroll
+    for (int it = 0; it < NIT; it++) weights(it);
 
   // sine and cosine of the lane's pairs 8c .. 8c + 7
   float sn[8], cs[8];
@@ -95,92 +114,105 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_norm_rope_kernel(QkRopeArg
     }
   }
 
-  float a[NIT][8], b[NIT][8];
+  // The values stay in 16 bits until they are turned: in fp32 through the sums they would take twice the registers.
+  float off[NIT], rs[NIT];  // y = x rs + off
 #pragma unroll
-  for (int it = 0; it < NIT; it++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      a[it][e] = (float)x1[it][e];
-      b[it][e] = (float)x2[it][e];
-    }
+  for (int it = 0; it < NIT; it++) off[it] = 0.f, rs[it] = 1.f;
   if (p.norm) {
-    float mean[NIT], rstd[NIT];
-    // mean of f over each head, or over q's and k's rows
-    const auto reduce = [&](auto part, float (&out)[NIT]) {
-      if constexpr (ROW) {
+    const bool layer = p.norm == kNormLayer;
+    const auto sum = [&](int it) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) s += (float)x1[it][e] + (float)x2[it][e];  // (pieces past the head hold zeros)
+      return s;
+    };
+    const auto squares = [&](int it, float m) {
+      float s = 0.f, t = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float u = (float)x1[it][e] - m, v = (float)x2[it][e] - m;
+        s = fmaf(u, u, s);
+        t = fmaf(v, v, t);
+      }
+      return (ok1 ? s : 0.f) + (ok2 ? t : 0.f);
+    };
+    if constexpr (ROW) {
+      // Over q's and k's rows with one barrier: each wave's mean and its squares about that, joined, a wave a lane, as
+      //   mean = sum_w n_w mean_w / n,  M2 = sum_w M2_w + n_w (mean_w - mean)^2
+      const auto values_of = [&](int w, int from, int to) {  // how many wave w has of the heads from .. to - 1
+        const int a = w * NIT * hpw;
+        return (float)(max(0, min(a + NIT * hpw, to) - max(a, from)) * p.d);
+      };
+      const float nq = values_of(wave, 0, p.H), nk = values_of(wave, p.H, p.H + p.Hk);
+      float mq = 0.f, mk = 0.f;
+      if (layer) {
         float sq = 0.f, sk = 0.f;
 #pragma unroll
         for (int it = 0; it < NIT; it++) {
-          const float s = part(it);
-          sq += head[it] >= 0 && head[it] < p.H ? s : 0.f;
-          sk += head[it] >= p.H ? s : 0.f;
+          const float s = head[it] >= 0 ? sum(it) : 0.f;
+          sq += isk[it] ? 0.f : s;
+          sk += isk[it] ? s : 0.f;
         }
-        row_sum(sq, sk, red, nw);
-        sq /= (float)(p.H * p.d);
-        sk /= (float)(p.Hk * p.d);
-#pragma unroll
-        for (int it = 0; it < NIT; it++) out[it] = head[it] >= p.H ? sk : sq;
-      } else {
-#pragma unroll
-        for (int it = 0; it < NIT; it++) out[it] = head_sum(part(it), lph) / (float)p.d;
+        mq = wave_total(sq) / fmaxf(nq, 1.f), mk = wave_total(sk) / fmaxf(nk, 1.f);
       }
-    };
-    if (p.norm == kNormLayer) {
-      reduce(
-          [&](int it) {
-            float s = 0.f;
+      float vq = 0.f, vk = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) s += a[it][e] + b[it][e];  // (pieces past the head hold zeros)
-            return s;
-          },
-          mean);
-#pragma unroll
-      for (int it = 0; it < NIT; it++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          a[it][e] -= mean[it];
-          b[it][e] -= mean[it];
-        }
-    }
-    reduce(
-        [&](int it) {
-          float s = 0.f, t = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            s += a[it][e] * a[it][e];
-            t += b[it][e] * b[it][e];
-          }
-          return (ok1 ? s : 0.f) + (ok2 ? t : 0.f);
-        },
-        rstd);
-#pragma unroll
-    for (int it = 0; it < NIT; it++) {
-      if (head[it] < 0) continue;
-      const float r = rsqrtf(rstd[it] + p.eps);
-      const bool isk = head[it] >= p.H;
-      const float* w = isk ? p.k_w : p.q_w;
-      f32x4 wa0 = {1.f, 1.f, 1.f, 1.f}, wa1 = wa0, wb0 = wa0, wb1 = wa0;  // (no weight: 1)
-      if (w) {
-        w += (size_t)(isk ? head[it] - p.H : head[it]) * (isk ? p.kw_sh : p.qw_sh);
-        if (ok1) wa0 = *reinterpret_cast<const f32x4*>(w + o1), wa1 = *reinterpret_cast<const f32x4*>(w + o1 + 4);
-        if (ok2) wb0 = *reinterpret_cast<const f32x4*>(w + o2), wb1 = *reinterpret_cast<const f32x4*>(w + o2 + 4);
+      for (int it = 0; it < NIT; it++) {
+        const float s = head[it] >= 0 ? squares(it, isk[it] ? mk : mq) : 0.f;
+        vq += isk[it] ? 0.f : s;
+        vk += isk[it] ? s : 0.f;
       }
+      vq = wave_total(vq), vk = wave_total(vk);
+      if (lane == 0) *reinterpret_cast<f32x4*>(red[wave]) = f32x4{mq, mk, vq, vk};
+      __syncthreads();
+      const int w = lane & 15;
+      f32x4 part = {0.f, 0.f, 0.f, 0.f};
+      if (w < nw) part = *reinterpret_cast<const f32x4*>(red[w]);
+      const float iq = 1.f / (float)(p.H * p.d), ik = 1.f / (float)(p.Hk * p.d);
+      float aq = 0.f, ak = 0.f;
+      if (layer) {
+        const float cq = values_of(w, 0, p.H), ck = values_of(w, p.H, p.H + p.Hk);
+        aq = row16_sum(cq * part[0]) * iq, ak = row16_sum(ck * part[1]) * ik;
+        part[2] = fmaf(cq * (part[0] - aq), part[0] - aq, part[2]);
+        part[3] = fmaf(ck * (part[1] - ak), part[1] - ak, part[3]);
+      }
+      const float rq = rsqrtf(row16_sum(part[2]) * iq + p.eps), rk = rsqrtf(row16_sum(part[3]) * ik + p.eps);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        a[it][e] = a[it][e] * r * (e < 4 ? wa0[e & 3] : wa1[e & 3]);
-        b[it][e] = b[it][e] * r * (e < 4 ? wb0[e & 3] : wb1[e & 3]);
+      for (int it = 0; it < NIT; it++) rs[it] = isk[it] ? rk : rq, off[it] = -(isk[it] ? ak * rk : aq * rq);
+    } else {
+      const float inv = 1.f / (float)p.d;
+#pragma unroll
+      for (int it = 0; it < NIT; it++) {
+        const float mean = layer ? head_sum(sum(it), lph) * inv : 0.f;
+        rs[it] = rsqrtf(head_sum(squares(it, mean), lph) * inv + p.eps);
+        off[it] = -mean * rs[it];
       }
     }
   }
 #pragma unroll
   for (int it = 0; it < NIT; it++) {
     if (head[it] < 0) continue;
-    V8 y1, y2;
-    if (turn && p.interleaved) {  // pair e: values 2e, 2e + 1 of the 16
+    if constexpr (ROW) weights(it);
+    const f32x4* w = wt[ROW ? 0 : it];
+    float a[8], b[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      a[e] = fmaf((float)x1[it][e], rs[it], off[it]);
+      b[e] = fmaf((float)x2[it][e], rs[it], off[it]);
+    }
+    if (!FULL || weighted) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float u = 2 * e < 8 ? a[it][(2 * e) & 7] : b[it][(2 * e) & 7];
-        const float v = 2 * e < 8 ? a[it][(2 * e + 1) & 7] : b[it][(2 * e + 1) & 7];
+        a[e] *= w[e >> 2][e & 3];
+        b[e] *= w[2 + (e >> 2)][e & 3];
+      }
+    }
+    V8 y1, y2;
+    if (!PLAIN && turn && p.interleaved) {  // pair e: values 2e, 2e + 1 of the 16
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float u = 2 * e < 8 ? a[(2 * e) & 7] : b[(2 * e) & 7];
+        const float v = 2 * e < 8 ? a[(2 * e + 1) & 7] : b[(2 * e + 1) & 7];
         const float ru = u * cs[e] - v * sn[e], rv = v * cs[e] + u * sn[e];
         if (2 * e < 8) {
           y1[(2 * e) & 7] = ru;
@@ -193,39 +225,39 @@ __global__ __launch_bounds__(64 * kRopeWaves) void qk_norm_rope_kernel(QkRopeArg
     } else if (turn) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        y1[e] = a[it][e] * cs[e] - b[it][e] * sn[e];
-        y2[e] = b[it][e] * cs[e] + a[it][e] * sn[e];
+        y1[e] = a[e] * cs[e] - b[e] * sn[e];
+        y2[e] = b[e] * cs[e] + a[e] * sn[e];
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        y1[e] = a[it][e];
-        y2[e] = b[it][e];
+        y1[e] = a[e];
+        y2[e] = b[e];
       }
     }
-    const bool isk = head[it] >= p.H;
-    char* dst = (char*)(isk ? p.ko : p.qo) +
-                2 * (row * (size_t)(isk ? p.ko_st : p.qo_st) +
-                     (size_t)(isk ? head[it] - p.H : head[it]) * (isk ? p.ko_sh : p.qo_sh));
+    char* dst = (char*)(isk[it] ? p.ko : p.qo) +
+                2 * (row * (size_t)(isk[it] ? p.ko_st : p.qo_st) + (size_t)hk[it] * (isk[it] ? p.ko_sh : p.qo_sh));
     if (ok1) *reinterpret_cast<V8*>(dst + 2 * o1) = y1;
     if (ok2) *reinterpret_cast<V8*>(dst + 2 * o2) = y2;
   }
 }
 
-template <class V8, bool ROW>
+template <class V8, bool ROW, int FORM>
 static hipError_t launch_rope_t(const QkRopeArgs& a, int groups, hipStream_t s) {
   // Over the row one workgroup takes all heads; over each head a workgroup takes up to four waves' groups. With
-  // rows enough to fill the GPU a wave takes several groups for its angles (16,384 rows of 32 + 8 heads of 128: one
-  // group a wave 81, two 74, three 85 us; 3,481 rows of 40 + 40 heads of 64 over the row: 22.8, 20.8, 20.1).
-  const int need = ROW ? (groups + kRopeWaves - 1) / kRopeWaves : 1, want = a.T < 512 ? 1 : ROW ? 3 : 2;
+  // rows enough to fill the GPU a wave takes several groups for its angles, three over the row or where that leaves fewer
+  // idle than two (us for 1, 2, 3: 16,384 rows of 32 + 8 heads of 128, half turned 75, 68, 68, all turned 68, 61, 60; of 20 + 4
+  // heads of 80 -, 30, 27; 3,481 rows of 40 + 40 heads of 64 over the row 21.2, 18.8, 17.7).
+  const int need = ROW ? (groups + kRopeWaves - 1) / kRopeWaves : 1;
+  const int want = a.T < 512 ? 1 : ROW || (groups + 2) / 3 * 3 < (groups + 1) / 2 * 2 ? 3 : 2;
   const int nit = need > want ? need : want < groups ? want : groups;
   const int per = (groups + nit - 1) / nit, gy = ROW ? 1 : (per + 3) / 4, waves = (per + gy - 1) / gy;
   const dim3 grid(a.T, gy), block(64 * waves);
   switch (nit) {
-    case 1: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 1>), grid, block, 0, s, a); break;
-    case 2: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 2>), grid, block, 0, s, a); break;
-    case 3: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 3>), grid, block, 0, s, a); break;
-    case 4: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 4>), grid, block, 0, s, a); break;
+    case 1: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 1, FORM>), grid, block, 0, s, a); break;
+    case 2: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 2, FORM>), grid, block, 0, s, a); break;
+    case 3: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 3, FORM>), grid, block, 0, s, a); break;
+    case 4: ESM_LAUNCH((qk_norm_rope_kernel<V8, ROW, 4, FORM>), grid, block, 0, s, a); break;
     default: return hipErrorInvalidValue;  // (heads are bounded by the caller)
   }
   return hipGetLastError();
@@ -242,8 +274,15 @@ bool qk_norm_rope_row_fits(int heads, int d) { return heads <= (64 >> lanes_log2
 hipError_t launch_qk_norm_rope(QkRopeArgs a, bool bf16, bool row, hipStream_t s) {
   a.lph = lanes_log2(a.d);
   const int hpw = 64 >> a.lph, groups = (a.H + a.Hk + hpw - 1) / hpw;
-  if (bf16) return row ? launch_rope_t<bf16x8, true>(a, groups, s) : launch_rope_t<bf16x8, false>(a, groups, s);
-  return row ? launch_rope_t<half8, true>(a, groups, s) : launch_rope_t<half8, false>(a, groups, s);
+  const bool full = a.d == 16 << a.lph && (!a.norm || !a.q_w == !a.k_w), plain = full && a.rot == a.d && !a.interleaved;
+  const auto launch = [&](auto v, auto r) {
+    typedef decltype(v) V8;
+    constexpr bool ROW = decltype(r)::value;
+    if (plain) return launch_rope_t<V8, ROW, kPlain>(a, groups, s);
+    return full ? launch_rope_t<V8, ROW, kFull>(a, groups, s) : launch_rope_t<V8, ROW, kGuarded>(a, groups, s);
+  };
+  if (bf16) return row ? launch(bf16x8{}, std::true_type{}) : launch(bf16x8{}, std::false_type{});
+  return row ? launch(half8{}, std::true_type{}) : launch(half8{}, std::false_type{});
 }
 
 }  // namespace esm

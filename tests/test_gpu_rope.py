@@ -80,6 +80,26 @@ def test_row_counts_default_positions_and_in_place(gpu_lib, pkg, T):
     assert same[0] is q and torch.equal(q, got[0]) and torch.equal(k, got[1])
 
 
+@pytest.mark.parametrize("H,Hk,d,rot,interleaved", [(40, 40, 64, 64, False), (40, 40, 64, 32, True), (7, 3, 128, 128, False),
+                                                    (20, 4, 80, 80, False), (90, 10, 64, 64, False), (1, 1, 128, 128, False)])
+@pytest.mark.parametrize("norm,over", [("rms", "row"), ("layer", "row"), ("layer", "head"), ("rms", "head"), (None, "head")])
+def test_many_rows_in_place_far_from_zero(gpu_lib, pkg, H, Hk, d, rot, interleaved, norm, over):
+    # several groups of heads a wave, waves with heads of both and of neither, means many times the spread, every head
+    # written over its input; with the weights of both, of one and of neither
+    T = 515
+    wq, wk = _weights(H, Hk, d, True)
+    rotary = pkg.rotary.Rotary(d, rot_dim=rot, interleaved=interleaved)
+    pos = torch.arange(T, dtype=torch.int32) * 3
+    for w in ((wq, wk), (wq, None), (None, None)):
+        q, k = _inputs(T, H, Hk, d, torch.float16, seed=d)
+        q, k = q.clone() + 60, k.clone() - 40
+        refs = [O.norm_rope(x, v, pos, rotary.freq, rotary.gain, rot, interleaved, norm, over, 1e-5)
+                for x, v in zip((q, k), w if norm else (None, None))]
+        rotary(q, k, pos.to(DEV), norm=norm, over=over, q_w=w[0], k_w=w[1], eps=1e-5, out=(q, k))
+        for y, ref in zip((q, k), refs):
+            _check(y, ref)
+
+
 def test_rows_of_zeros_and_of_infinities(gpu_lib, pkg):
     q, k = _inputs(3, 4, 4, 64, torch.float16)
     q[0], q[1, 2, 5], k[2, 1, 0] = 0, float("inf"), float("nan")
