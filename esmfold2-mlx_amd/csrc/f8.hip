@@ -67,46 +67,36 @@ DEV void f8_codes(V8 v, float r, int& lo, int& hi) {
 }
 
 // ---- x to e4m3 --------------------------------------------------------------------------------
-// A thread takes 16 values of a row in each of kQuantBlocks blocks, all loaded first; the 8 threads of a row's block
-// share its maximum. Bound by bytes: 8192 x 8192 47 us, 4.4 TB/s; 238 x 5120 2.7 to 3.7 us.
-constexpr int kQuantBlocks = 4;
+// A thread takes 16 values of a row; the 8 threads of a row's block share its maximum. Bound by bytes, small ones by a
+// launch and one latency: 8192 x 8192 47 us, 4.4 TB/s; 3481 x 2560 6.9, 238 x 5120 2.0 to 3.5 (with four blocks a
+// thread 8.1 and 2.7 to 4.3).
 template <class V8>
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const uint16_t* __restrict__ x, long long st, uint8_t* __restrict__ xq,
                                                           float* __restrict__ sx, int M, int K, int Mp) {
   const int Kb = (K + 127) / 128, t = threadIdx.x;
-  const int c = t & 7, m = 32 * blockIdx.x + (t >> 3), kb0 = kQuantBlocks * blockIdx.y;
+  const int c = t & 7, m = 32 * blockIdx.x + (t >> 3), kb = blockIdx.y, k = 128 * kb + 16 * c;
   if (m >= Mp) return;
-  u16x8 a[kQuantBlocks], b[kQuantBlocks];
-#pragma unroll
-  for (int i = 0; i < kQuantBlocks; i++) {
-    const int k = 128 * (kb0 + i) + 16 * c;
-    a[i] = b[i] = u16x8{};
-    if (m < M && k < K) {
-      const u16x8* src = reinterpret_cast<const u16x8*>(x + m * st + k);
-      a[i] = src[0];
-      b[i] = src[1];
-    }
+  u16x8 a = {}, b = {};
+  if (m < M && k < K) {
+    const u16x8* src = reinterpret_cast<const u16x8*>(x + m * st + k);
+    a = src[0];
+    b = src[1];
   }
-#pragma unroll
-  for (int i = 0; i < kQuantBlocks; i++) {
-    const int kb = kb0 + i;
-    uint32_t top = max(top_bits(a[i]), top_bits(b[i]));
-    const auto other = [&](auto ctrl) {
-      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false);
-    };
-    top = max(top, other(std::integral_constant<int, 0xB1>{}));   // quad_perm(1, 0, 3, 2)
-    top = max(top, other(std::integral_constant<int, 0x4E>{}));   // quad_perm(2, 3, 0, 1)
-    top = max(top, other(std::integral_constant<int, 0x141>{}));  // row_half_mirror
-    float r, s;
-    f8_scale(bits_value<V8>(top), r, s);
-    int q[4];
-    f8_codes(__builtin_bit_cast(V8, a[i]), r, q[0], q[1]);
-    f8_codes(__builtin_bit_cast(V8, b[i]), r, q[2], q[3]);
-    if (kb >= Kb) break;
-    uint8_t* dst = xq + ((size_t)(m >> 4) * Kb + kb) * 2048 + (c & 1) * 1024 + (16 * (c >> 1) + (m & 15)) * 16;
-    *reinterpret_cast<i32x4*>(dst) = i32x4{q[0], q[1], q[2], q[3]};
-    if (c == 0) sx[(size_t)kb * Mp + m] = s;
-  }
+  uint32_t top = max(top_bits(a), top_bits(b));
+  const auto other = [&](auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  top = max(top, other(std::integral_constant<int, 0xB1>{}));   // quad_perm(1, 0, 3, 2)
+  top = max(top, other(std::integral_constant<int, 0x4E>{}));   // quad_perm(2, 3, 0, 1)
+  top = max(top, other(std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  float r, s;
+  f8_scale(bits_value<V8>(top), r, s);
+  int q[4];
+  f8_codes(__builtin_bit_cast(V8, a), r, q[0], q[1]);
+  f8_codes(__builtin_bit_cast(V8, b), r, q[2], q[3]);
+  uint8_t* dst = xq + ((size_t)(m >> 4) * Kb + kb) * 2048 + (c & 1) * 1024 + (16 * (c >> 1) + (m & 15)) * 16;
+  *reinterpret_cast<i32x4*>(dst) = i32x4{q[0], q[1], q[2], q[3]};
+  if (c == 0) sx[(size_t)kb * Mp + m] = s;
 }
 
 // Fragment at soff + 16 lane of a buffer whose every read is in range.
@@ -537,7 +527,7 @@ static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) 
     }
     return hipGetLastError();
   }
-  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, ((a.K + 127) / 128 + kQuantBlocks - 1) / kQuantBlocks), dim3(256), 0, s,
+  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, (a.K + 127) / 128), dim3(256), 0, s,
              (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (form == kF8Some) switch (mb) {
