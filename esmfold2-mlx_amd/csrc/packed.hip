@@ -708,7 +708,7 @@ AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G,
   const long long least = (Tk + kAttnMaxSplits - 1) / kAttnMaxSplits;
   chunk = chunk < least ? least : chunk;
   chunk = (chunk + pass - 1) / pass * pass;
-  if (plan.many || chunk < 2 * pass) chunk = chunk < 2 * pass && !plan.many ? 2 * pass : chunk;
+  chunk = chunk < 2 * pass ? 2 * pass : chunk;  // (never 0: there may be no keys at all)
   plan.splits = (int)((Tk + chunk - 1) / chunk);
   plan.chunk = (int)chunk;
   if (plan.many || plan.splits <= 1 || rows * Hk >= 2 * cus) {  // one chunk for all
