@@ -5,7 +5,8 @@
 // head: the group's heads share every key and value that is staged, and a single new token's heads fill a
 // tile together. A wave holds 32 rows and takes 32 keys from LDS at a time:
 //   S^T[key][row] = K Q^T       (A: K rows from LDS, B: the wave's query fragments, in registers)
-//   p = 2^(S c - m c), l += p   (a lane holds one row: the maximum is over its registers and one exchange)
+//   p = 2^(S c - m c), l += p   (a lane holds one row: the maximum is over its registers and one exchange; where
+//                               m c is large, 2^((S - m) c))
 //   O^T[d][row] += V^T P^T      (A: V^T by the transposing LDS read, B: p in the accumulator's own key order)
 // in fp32 but for p, which is rounded to the inputs' 16-bit type for the second product (an error of half a
 // step of that type on each p, below the output's own rounding after the sum). m is the running maximum; it, O
@@ -56,6 +57,7 @@ struct Bf16 {
 };
 
 constexpr float kGrow = 8.f;  // log2 of what p may reach before its row is rescaled
+constexpr float kFar = 1024.f;  // least exponent of a row's maximum that its scores are made relative to
 
 // LDS rows of HD values, 16-byte pieces swizzled so that the reads below cover the 64 banks once: K fragments
 // read 16 rows at one piece; V's transposing read takes 4 rows x 4 pieces.
@@ -122,7 +124,7 @@ struct Rows {
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (__any((mx - m) * c > kGrow)) grow(mx, c);  // (from m = -inf at the first key a row sees)
-    const float mc = MASKED && lim < key0 ? 0.f : m * c;  // (m may be -inf where no key has been seen)
+    const float mc = reference(c, s);
     typename T::v8 p[2];
 #pragma unroll
     for (int i = 0; i < 16; i++)  // (results below 2^-126 flush)
@@ -181,7 +183,7 @@ struct Rows {
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (__any((mx - m) * c > kGrow)) grow(mx, c);
-    const float mc = m * c;
+    const float mc = reference(c, s0, s1);
     v8 p[4];
     const auto prob = [&](int i) {  // probabilities 2i, 2i + 1 of 32 (results below 2^-126 flush)
       const f32x16& s = i < 8 ? s0 : s1;
@@ -213,6 +215,24 @@ struct Rows {
       __builtin_amdgcn_sched_barrier(0);
     }
     __builtin_amdgcn_s_setprio(0);
+  }
+
+  // m c, from which the exponents s c of the scores s are taken with one FMA a score. Its rounding, 2^-24 of its size, goes
+  // into every p as a factor, so where it is large the scores themselves become relative to m (the difference of two
+  // near scores is exact) and 0 is returned. So too where it is not finite: c may carry m past fp32's range, and a row
+  // that has seen no key, or only scores of -inf, has m = -inf; its p are 0.
+  template <class... S>
+  DEV float reference(float c, S&... s) {
+    const float mc = m * c;
+    const bool far = !(fabsf(mc) < kFar);
+    if (!__any(far)) return mc;
+    const float ref = far && m != -INFINITY ? m : 0.f;  // (m = +inf: its row becomes NaN)
+    const auto relative = [&](f32x16& x) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) x[i] -= ref;
+    };
+    (relative(s), ...);
+    return far ? 0.f : mc;
   }
 
   // The row's maximum has grown to mx: everything summed so far by the new one.

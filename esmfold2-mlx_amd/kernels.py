@@ -310,8 +310,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     """softmax(q k^T * scale) v within each packed sequence: q [Tq, H, d], k, v [Tk, Hk, d] (fp16 or bf16, views of
     wider rows allowed; H a multiple of Hk) -> o [Tq, H, d]. ``cu_q``, ``cu_k`` int32 [n + 1] on the device: the first
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
-    the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key are 0; rows of no
-    sequence are not written. ``out`` may be q, and shares no other memory with the operands. The partial results of few rows
+    the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key, or none whose score is
+    above -inf, are 0; rows of no sequence are not written. ``out`` may be q, and shares no other memory with the operands. The partial results of few rows
     against many keys live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
