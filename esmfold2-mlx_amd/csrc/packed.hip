@@ -10,7 +10,10 @@
 //   O^T[d][row] += V^T P^T      (A: V^T by the transposing LDS read, B: p in the accumulator's own key order)
 // in fp32 but for p, which is rounded to the inputs' 16-bit type for the second product (an error of half a
 // step of that type on each p, below the output's own rounding after the sum). m is the running maximum; it, O
-// and l are rescaled only when a row's maximum has grown by more than 2^8 since (p then reaches 2^8 at most).
+// and l are rescaled only when a row's maximum has grown by more than 2^8 since (p then reaches 2^8 at most); in fp16
+// 2^4, as p is kept 2^11 times as large there: fp16 loses bits below 2^-14, and thousands of keys some 2^-20 below one
+// that attends to nothing (a sink) may be the whole output. Half a step holds down to 2^-25 of the row's largest, below
+// that p is off by 2^-36 at most.
 //
 // Two kernels share that step: packed_attention_kernel (many rows: four waves of 32 rows over tiles of 64
 // keys that they share, the next tile in flight) and split_attention_kernel (few rows: 32 rows, keys divided
@@ -31,6 +34,7 @@ struct Fp16 {
   typedef half8 v8;
   typedef half4 v4;
   typedef half_t elem;
+  static constexpr float kGrow = 4.f, kUp = 11.f;  // (p <= 2^15, below fp16's largest)
   // exponent mask; 1, 128 and 129
   static constexpr uint16_t kExp = 0x7c00, kOne = 0x3c00, kMany = 0x5800, kBoth = 0x5808;
   static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -45,6 +49,7 @@ struct Bf16 {
   typedef bf16x8 v8;
   typedef bf16x4 v4;
   typedef __bf16 elem;
+  static constexpr float kGrow = 8.f, kUp = 0.f;  // log2: what p may reach before its row is rescaled, and all p's factor
   static constexpr uint16_t kExp = 0x7f80, kOne = 0x3f80, kMany = 0x4300, kBoth = 0x4301;
   static DEV f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static DEV float add(v8 v, float s) {
@@ -56,7 +61,6 @@ struct Bf16 {
   }
 };
 
-constexpr float kGrow = 8.f;  // log2 of what p may reach before its row is rescaled
 constexpr float kFar = 1024.f;  // least exponent of a row's maximum that its scores are made relative to
 
 // LDS rows of HD values, 16-byte pieces swizzled so that the reads below cover the 64 banks once: K fragments
@@ -123,7 +127,7 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any((mx - m) * c > kGrow)) grow(mx, c);  // (from m = -inf at the first key a row sees)
+    if (__any((mx - m) * c > T::kGrow)) grow(mx, c);  // (from m = -inf at the first key a row sees)
     const float mc = reference(c, s);
     typename T::v8 p[2];
 #pragma unroll
@@ -182,7 +186,7 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < 16; i++) mx = fmaxf(mx, s1[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any((mx - m) * c > kGrow)) grow(mx, c);
+    if (__any((mx - m) * c > T::kGrow)) grow(mx, c);
     const float mc = reference(c, s0, s1);
     v8 p[4];
     const auto prob = [&](int i) {  // probabilities 2i, 2i + 1 of 32 (results below 2^-126 flush)
@@ -217,22 +221,22 @@ struct Rows {
     __builtin_amdgcn_s_setprio(0);
   }
 
-  // m c, from which the exponents s c of the scores s are taken with one FMA a score. Its rounding, 2^-24 of its size, goes
+  // m c less p's own exponent, from which the exponents s c of the scores s are taken with one FMA a score. Its rounding, 2^-24 of its size, goes
   // into every p as a factor, so where it is large the scores themselves become relative to m (the difference of two
-  // near scores is exact) and 0 is returned. So too where it is not finite: c may carry m past fp32's range, and a row
+  // near scores is exact) and m c counts as 0. So too where it is not finite: c may carry m past fp32's range, and a row
   // that has seen no key, or only scores of -inf, has m = -inf; its p are 0.
   template <class... S>
   DEV float reference(float c, S&... s) {
     const float mc = m * c;
     const bool far = !(fabsf(mc) < kFar);
-    if (!__any(far)) return mc;
+    if (!__any(far)) return mc - T::kUp;
     const float ref = far && m != -INFINITY ? m : 0.f;  // (m = +inf: its row becomes NaN)
     const auto relative = [&](f32x16& x) {
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] -= ref;
     };
     (relative(s), ...);
-    return far ? 0.f : mc;
+    return (far ? 0.f : mc) - T::kUp;
   }
 
   // The row's maximum has grown to mx: everything summed so far by the new one.

@@ -455,9 +455,10 @@ int esmc_swiglu(const esm_half* x12, esm_half* y, int M, int F, void* stream);
  *   cu_k[s + 1] - 1 (int32 [n + 1] on the device, ascending; values outside 0 .. Tq, 0 .. Tk are brought inside):
  *   o = softmax(scale q k^T) v within the sequence, query head h with key head h / (H / Hk). causal: query i of nq
  *   sees the keys 0 .. i + nk - nq of nk. A row that sees no key, or none whose score is above -inf, is 0; rows of no
- *   sequence are not written. What unseen keys and values hold (infinities, NaN) reaches no output. Scores, softmax and
- *   sums are fp32, the probabilities rounded to dtype for the second product. d % 8 == 0, d <= 128; scale > 0; row
- *   strides from d to 2^23.
+ *   sequence are not written. What unseen keys and values hold (infinities, NaN) reaches no output; a seen infinity or
+ *   NaN of v makes its column of the row one or the other. Scores, softmax and sums are fp32, the probabilities rounded
+ *   to dtype for the second product (a half step each; in fp16 below 2^-25 of the row's largest 2^-36 of that). d % 8
+ *   == 0, d <= 128; scale > 0; row strides from d to 2^23.
  *   workspace: packed_attention_workspace_bytes(...) bytes, 256-byte aligned (0: none; fp32 partials where a few rows'
  *   keys are divided between workgroups).
  */

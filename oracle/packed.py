@@ -9,17 +9,18 @@ import torch
 
 HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # a rounding, relative to the value
 SMALLEST = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}  # and below the normal range, absolute
+SMALLEST_P = {torch.float16: 2.0 ** -36, torch.bfloat16: 2.0 ** -126}  # the same of a probability, of the row's largest
 
 
 def attention(q, k, v, cu_q, cu_k, causal, scale):
     """(o, bound) in fp64: rows of no sequence NaN; bound on |kernel - o| by arithmetic, element by element.
 
     With u the half step of the type, A = sum_j p_j |v_j| / l and e the relative error of a p:
-      o's rounding u |o|; each p's rounding u (and an absolute one below the type's normal range: at most
-      SMALLEST / l each, l >= 1); e = 2 dS + 2^-21 with dS = scale (d + 2) 2^-24 sum |q| |k| the fp32 score's error,
+      o's rounding u |o|; each p's rounding u (and an absolute one: at most SMALLEST_P / l each, l >= 1, as fp16's p
+      are kept 2^11 times as large and bf16's are 0 below 2^-126); e = 2 dS + 2^-21 with dS = scale (d + 2) 2^-24 sum |q| |k| the fp32 score's error,
       2^-22 |scale s| the exponent argument's (a product and an FMA at the size of m c); sums over nk keys and
       the rescalings: (nk + 64) 2^-24; each of them on the numerator and the sum: twice."""
-    u, tiny = HALF_STEP[q.dtype], SMALLEST[q.dtype]
+    u, tiny, tiny_p = HALF_STEP[q.dtype], SMALLEST[q.dtype], SMALLEST_P[q.dtype]
     q, k, v = (t.detach().cpu().double() for t in (q, k, v))
     Tq, H, d = q.shape
     G = H // k.shape[1]
@@ -45,7 +46,7 @@ def attention(q, k, v, cu_q, cu_k, causal, scale):
                 A = (e / l) @ z[w].abs()
                 ds = scale * (d + 2) * 2.0 ** -24 * float((y[w].abs() @ x[i].abs()).max())
                 rel = 2 * (ds + 2.0 ** -22 * float(sc.abs().max()) + 2.0 ** -21 + (int(w.sum()) + 64) * 2.0 ** -24)
-                bound[a + i, h] = (u * o[a + i, h].abs() + (u + 2 * rel) * A + tiny * z[w].abs().sum(0) + tiny)
+                bound[a + i, h] = (u * o[a + i, h].abs() + (u + 2 * rel) * A + tiny_p * z[w].abs().sum(0) + tiny)
     return o, bound
 
 

@@ -1,5 +1,5 @@
 """Packed attention where sequences, scores and probabilities reach their ends: no keys at all, scores of -inf and of the
-type's lowest value, against the formula."""
+type's lowest value, scores of any size and probabilities far below their row's largest, against the formula."""
 
 import math
 
@@ -217,3 +217,52 @@ def test_far_scores_leave_the_largest_alone(gpu_lib, pkg, nq, nk, H, Hk, d, log2
             o, bound = O.attention(q[:1, h:h + 1] * 0, k[top, e:e + 1] * 0, v[top, e:e + 1], [0, 1], [0, len(top)], False, 1.0)
             err = (got[:, h:h + 1].cpu().double() - o).abs()
             assert float((err / bound).max()) <= 1.0
+
+
+# ---- probabilities far below their row's largest ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nats", [8, 12, 14, 15, 16, 17, 18])
+@pytest.mark.parametrize("nq,nk,H,Hk,d,first", [(1, 16384, 4, 1, 128, 0), (1, 16384, 4, 4, 64, 9000), (1, 3000, 4, 4, 64, 0),
+                                                (600, 4000, 40, 40, 64, 0), (130, 4000, 32, 8, 128, 3000)])
+def test_many_small_probabilities_beside_a_large_one(gpu_lib, pkg, nq, nk, H, Hk, d, first, nats, dtype):
+    # one key far above thousands of equal others: with its values 0 the others' are the whole output, and with all
+    # values 1 the output is 1, as the sum of the probabilities is that of the products
+    g = torch.Generator().manual_seed(nats)
+    q, k = torch.zeros(nq, H, d, dtype=dtype), torch.zeros(nk, Hk, d, dtype=dtype)
+    q[..., 0], k[first, :, 0] = 1, nats
+    v = (1 + 0.5 * torch.randn(nk, Hk, d, generator=g)).to(dtype)
+    v[first] = 0
+    q, k, v = (t.to(DEV) for t in (q, k, v))
+    cq, ck = [0, nq], [0, nk]
+    got = pkg.kernels.packed_attention(q, k, v, _cu(cq), _cu(ck), scale=1.0)
+    o, bound = O.attention(q[:1, :1], k[:, :1], v[:, :1], [0, 1], ck, False, 1.0)
+    y = got[:, :1].cpu().double()
+    worst = float(((y - o).abs() / bound).max())
+    assert worst <= 1.0, f"{nats} nats: error {worst:.2f} of its bound, {float((y - o).abs().max() / o.abs().max()):.4f} of the largest"
+    ones = pkg.kernels.packed_attention(q, k, torch.ones_like(v), _cu(cq), _cu(ck), scale=1.0).double()
+    # numerator and sum are the same sums of the same numbers, each within nk + 64 roundings of 2^-24
+    assert float((ones - 1).abs().max()) <= O.HALF_STEP[dtype] + 2 * (nk + 64) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("step", [0.02, 0.08, 0.3])
+@pytest.mark.parametrize("nq,H,Hk,d", [(2, 4, 1, 128), (600, 40, 40, 64)])
+def test_scores_that_rise_all_the_way(gpu_lib, pkg, nq, H, Hk, d, step, dtype):
+    # the row's maximum moves in every block by less and by more than what it is rescaled for; large values
+    nk = 700
+    q, k = torch.zeros(nq, H, d, dtype=dtype), torch.zeros(nk, Hk, d, dtype=dtype)
+    q[..., :2], k[..., 0] = 1, (step * torch.arange(nk)).to(dtype)[:, None]
+    v = (1000 * torch.randn(nk, Hk, d, generator=torch.Generator().manual_seed(1))).to(dtype)
+    q, k, v = (t.to(DEV) for t in (q, k, v))
+    for causal in (False, True):
+        got = pkg.kernels.packed_attention(q, k, v, _cu([0, nq]), _cu([0, nk]), causal=causal, scale=1.0)
+        rows = sorted({0, nq // 2, nq - 1})
+        for h in (0, H - 1):
+            for i in rows:  # (row by row: a row sees the keys up to its own)
+                n = i + nk - nq + 1 if causal else nk
+                g = h // (H // Hk)
+                o, bound = O.attention(q[i:i + 1, h:h + 1], k[:n, g:g + 1], v[:n, g:g + 1], [0, 1], [0, n], False, 1.0)
+                y = got[i:i + 1, h:h + 1].cpu().double()
+                assert float(((y - o).abs() / bound).max()) <= 1.0
