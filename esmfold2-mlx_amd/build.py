@@ -7,7 +7,8 @@ packed-fp32 target feature disabled (-Xclang -target-feature -Xclang
 -packed-fp32-ops): the kernels are written without packed fp32 arithmetic and
 the compiler must not introduce it. Beside it goes _esm_bind.so, a host-only Python
 module against torch's headers (csrc/bind.cpp): the short way into the library for
-calls whose host steps would cost more than their kernels.
+calls whose host steps would cost more than their kernels. The library needs no torch,
+and does not need the module: where that cannot be built the calls take the longer way.
 """
 
 from __future__ import annotations
@@ -51,16 +52,35 @@ def source_hash() -> str:
 
 
 _TAG = re.compile(rb"ESMSRC:([0-9a-f]{64})")
+_ENV_TAG = re.compile(rb"ESMENV:([0-9a-f]{64})")
+
+
+def _tag(path: str, tag) -> str | None:
+    try:
+        with open(path, "rb") as f:
+            m = tag.search(f.read())
+    except OSError:
+        return None
+    return m.group(1).decode() if m else None
 
 
 def library_hash(path: str = LIB_PATH) -> str | None:
     """The source hash a built library was compiled from (the ESMSRC tag capi.cpp embeds), or None."""
-    try:
-        with open(path, "rb") as f:
-            m = _TAG.search(f.read())
-    except OSError:
-        return None
-    return m.group(1).decode() if m else None
+    return _tag(path, _TAG)
+
+
+def environment() -> str:
+    """sha256 over what the module is compiled against beside its sources: torch's release and C++ ABI, Python's ABI."""
+    import sysconfig
+
+    import torch
+    parts = (torch.__version__, int(torch._C._GLIBCXX_USE_CXX11_ABI), sysconfig.get_config_var("SOABI"))
+    return hashlib.sha256(repr(parts).encode()).hexdigest()
+
+
+def bind_environment(path: str = BIND_PATH) -> str | None:
+    """The environment a built module was compiled in (its ESMENV tag), or None."""
+    return _tag(path, _ENV_TAG)
 
 
 FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall",
@@ -83,7 +103,7 @@ def bind_command(obj: str, src_hash: str) -> list[str]:
     import torch
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     return [hipcc(), "-O2", "-std=c++17", "-fPIC", "-Wall", "-DUSE_ROCM", f"-DESM_SOURCE_HASH=\"{src_hash}\"",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
+            f"-DESM_ENVIRONMENT=\"{environment()}\"", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
             "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], "-c",
             os.path.join(CSRC, BIND_SOURCE), "-o", obj]
 
@@ -97,8 +117,13 @@ def bind_link_command(obj: str, out: str) -> list[str]:
 
 
 def up_to_date() -> bool:
-    """True when the built library and module exist and were compiled from the current sources (by content)."""
-    return library_hash() == source_hash() == library_hash(BIND_PATH)
+    """True when the built library exists and was compiled from the current sources (by content)."""
+    return library_hash() == source_hash()
+
+
+def bind_up_to_date() -> bool:
+    """True when the built module exists and was compiled from the current sources, in this environment."""
+    return library_hash(BIND_PATH) == source_hash() and bind_environment() == environment()
 
 
 _NOISE = "is not a recognized feature for this target"  # host pass of the fp32 feature flag
@@ -118,46 +143,63 @@ def _run(procs) -> str:
     return "\n".join(msgs)
 
 
-def build(force: bool = True, verbose: bool = False, jobs: int | None = None) -> str:
-    """Compile the library (always when ``force``): one hipcc -c per source, up to ``jobs`` at a
-    time, then one link into the in-tree .so. Returns its path."""
-    if not force and up_to_date():
-        return LIB_PATH
+def _start(cmd: list[str], verbose: bool):
+    if verbose:
+        print("[build]", " ".join(cmd), flush=True)
+    return cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _show(msgs, verbose: bool) -> None:
+    if verbose and any(m.strip() for m in msgs):
+        print("\n".join(m for m in msgs if m.strip()), flush=True)
+
+
+def build_library(verbose: bool = False, jobs: int | None = None) -> str:
+    """Compile the library: one hipcc -c per source, up to ``jobs`` at a time, then one link into the in-tree .so."""
     import tempfile
     h = source_hash()
-    jobs = jobs or max(1, min(len(SOURCES) + 1, os.cpu_count() or 1, 16))
+    jobs = jobs or max(1, min(len(SOURCES), os.cpu_count() or 1, 16))
     with tempfile.TemporaryDirectory(prefix="esm_build_") as tmpdir:
-        objs, pending = [], []
-        for src in SOURCES:
-            obj = os.path.join(tmpdir, src.replace(".", "_") + ".o")
-            objs.append(obj)
-            pending.append(compile_command(src, obj, h))
-        bind_obj = os.path.join(tmpdir, "bind.o")
-        pending.append(bind_command(bind_obj, h))
+        objs = [os.path.join(tmpdir, src.replace(".", "_") + ".o") for src in SOURCES]
+        pending = [compile_command(src, obj, h) for src, obj in zip(SOURCES, objs)]
         msgs = []
         while pending:
             batch, pending = pending[:jobs], pending[jobs:]
-            if verbose:
-                for cmd in batch:
-                    print("[build]", " ".join(cmd), flush=True)
-            msgs.append(_run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
-                                                     text=True)) for cmd in batch]))
+            msgs.append(_run([_start(cmd, verbose) for cmd in batch]))
         tmp = LIB_PATH + ".tmp"
-        cmd = link_command(objs, tmp)
-        if verbose:
-            print("[build]", " ".join(cmd), flush=True)
-        msgs.append(_run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
-                                                 text=True))]))
-        bind_tmp = BIND_PATH + ".tmp"
-        cmd = bind_link_command(bind_obj, bind_tmp)
-        if verbose:
-            print("[build]", " ".join(cmd), flush=True)
-        msgs.append(_run([(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
-                                                 text=True))]))
-    if verbose and any(m.strip() for m in msgs):
-        print("\n".join(m for m in msgs if m.strip()), flush=True)
+        msgs.append(_run([_start(link_command(objs, tmp), verbose)]))
+    _show(msgs, verbose)
     os.replace(tmp, LIB_PATH)
-    os.replace(bind_tmp, BIND_PATH)
+    return LIB_PATH
+
+
+def build_bind(verbose: bool = False) -> str:
+    """Compile and link the module. Raises where torch, its headers or Python's are missing, or do not fit."""
+    import tempfile
+    with tempfile.TemporaryDirectory(prefix="esm_build_") as tmpdir:
+        obj, tmp = os.path.join(tmpdir, "bind.o"), BIND_PATH + ".tmp"
+        msgs = [_run([_start(bind_command(obj, source_hash()), verbose)])]
+        msgs.append(_run([_start(bind_link_command(obj, tmp), verbose)]))
+    _show(msgs, verbose)
+    os.replace(tmp, BIND_PATH)
+    return BIND_PATH
+
+
+def try_build_bind(verbose: bool = False) -> bool:
+    """``build_bind``, its failure reported on stderr rather than raised: whether the module is there."""
+    try:
+        build_bind(verbose)
+    except Exception as e:  # noqa: BLE001  (whatever it is, the library stands without the module)
+        print(f"[esmfold2_amd] {BIND_NAME} cannot be built, its calls take the longer way: {e}", file=sys.stderr, flush=True)
+        return False
+    return True
+
+
+def build(force: bool = True, verbose: bool = False, jobs: int | None = None) -> str:
+    """Compile the library (always when ``force``), then the module beside it. Returns the library's path."""
+    if force or not up_to_date():
+        build_library(verbose, jobs)
+        try_build_bind(verbose)
     return LIB_PATH
 
 

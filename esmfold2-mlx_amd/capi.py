@@ -100,6 +100,16 @@ class EsmError(RuntimeError):
         self.code = code
 
 
+class _LongWay:
+    """In the place of the native module where that cannot be built or loaded: every call takes the longer way."""
+
+    @staticmethod
+    def _none(*args):
+        return None
+
+    qk_norm_rope = packed_attention = f8_linear = connect = _none
+
+
 # the native short way of some calls (csrc/bind.cpp), loaded with the library, and the entry points it takes
 bind = None
 _SHORT = ("qk_norm_rope", "packed_attention", "packed_attention_workspace_bytes", "f8_linear",
@@ -131,13 +141,26 @@ def _load() -> ctypes.CDLL:
         raise EsmError(-5, f"{_build.LIB_PATH} does not match its sources after the build")
     global bind
     if bind is None:
+        bind = _load_bind()
+    bind.connect(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SHORT))
+    return handle
+
+
+def _load_bind():
+    """The native module, built first when it is missing or was compiled from other sources or for another torch or
+    Python; ``_LongWay`` where that fails."""
+    try:
         import torch  # noqa: F401  (the module is linked against its libraries)
+        if not (_build.bind_up_to_date() or _build.try_build_bind()):
+            return _LongWay
         spec = importlib.util.spec_from_file_location(_build.BIND_NAME, _build.BIND_PATH)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        bind = mod
-    bind.connect(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SHORT))
-    return handle
+        return mod
+    except ImportError as e:
+        print(f"[esmfold2_amd] {_build.BIND_NAME} cannot be loaded, its calls take the longer way: {e}", file=sys.stderr,
+              flush=True)
+        return _LongWay
 
 
 def lib(reload: bool = False, require_gpu: bool = True) -> ctypes.CDLL:

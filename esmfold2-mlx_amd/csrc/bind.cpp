@@ -249,7 +249,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_esm_bind", nullptr, -1, methods, 
 
 }  // namespace
 
-// Read back by the build to tell whether the module was compiled from the current sources.
-extern "C" __attribute__((used, visibility("default"))) const char esm_bind_tag[] = "ESMSRC:" ESM_SOURCE_HASH;
+// Read back by the build to tell whether the module was compiled from the current sources and in this environment.
+extern "C" __attribute__((used, visibility("default"))) const char esm_bind_tag[] = "ESMSRC:" ESM_SOURCE_HASH " ESMENV:" ESM_ENVIRONMENT;
 
 PyMODINIT_FUNC PyInit__esm_bind(void) { return PyModule_Create(&module); }
