@@ -227,7 +227,7 @@ class HipEsmc(nn.Module):
         self.layers = nn.ModuleList(layers)
         self.n_heads = n_heads
         self.res_scale = math.sqrt(len(layers) / 36)  # mlx_esmc.py:108
-        self._rotary = None  # of the packed form
+        self._rotary = Rotary(64, device=dev)  # of the packed form (made here: a capture refuses its copy from the host)
 
     # ---- construction: the reference's converted-weight cache (mlx_esmc.py:116-148) -------------
     @classmethod
@@ -297,6 +297,12 @@ class HipEsmc(nn.Module):
     def nbytes(self) -> int:
         return sum(b.numel() * b.element_size() for b in self.buffers())
 
+    def _apply(self, *a, **k):
+        super()._apply(*a, **k)
+        if self._rotary.freq.device != self.embed.device:  # (moved by ``cuda``; no buffer, its angles stay fp64)
+            self._rotary = Rotary(64, device=self.embed.device)
+        return self
+
     # nn.Module API the fold calls on its ESMC; the weights stay where they are.
     def to(self, *a, **k):
         return self
@@ -327,7 +333,8 @@ class HipEsmc(nn.Module):
         """``hidden_states`` of packed sequences: input_ids [T] of all of them, cu_seqlens [n + 1] where each begins
         and the last ends -> [n_layers + 1, T, D] fp32, each sequence as if alone. ``positions`` [T]: other rotary
         positions than the places within the sequences (a complex whose chains are sequences of their own but
-        count on). Rows of no sequence hold nothing meaningful."""
+        count on). Rows of no sequence hold nothing meaningful. With every argument on the GPU it may be captured
+        into a HIP graph, its first call too (``packed`` copies its lengths from the host)."""
         dev = self.embed.device
         ids = input_ids.to(dev)
         if ids.dim() != 1 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
@@ -339,8 +346,6 @@ class HipEsmc(nn.Module):
             positions = rows - cu[torch.searchsorted(cu[1:].contiguous(), rows, right=True)]
         else:
             positions = positions.to(dev).contiguous()
-        if self._rotary is None or self._rotary.freq.device != dev:
-            self._rotary = Rotary(64, device=dev)
         hs = torch.empty(n + 1, T, D, dtype=torch.float32, device=dev)
         hs[0] = self.embed[ids]
         if T == 0:
