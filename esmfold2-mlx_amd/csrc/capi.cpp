@@ -1008,7 +1008,8 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
     return fail(ESM_ERR_SHAPE, "packed_attention: n=%d Tq=%d Tk=%d H=%d Hk=%d d=%d", n, Tq, Tk, H, Hk, d);
   if (d % 8 != 0 || d > 128) return fail(ESM_ERR_UNSUPPORTED, "packed_attention: d=%d (a multiple of 8 up to 128)", d);
   if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "packed_attention: dtype=%d", dtype);
-  if (!(scale > 0.f) || std::isinf(scale)) return fail(ESM_ERR_SHAPE, "packed_attention: scale must be positive and finite");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || std::isinf(scale_log2)) return fail(ESM_ERR_SHAPE, "packed_attention: scale must be positive and below 2^127");
   for (const char* why : {strides_fault(q_st, q_sh, Tq, d), strides_fault(k_st, k_sh, Tk, d),
                           strides_fault(v_st, v_sh, Tk, d), strides_fault(o_st, o_sh, Tq, d)})
     if (why) return fail(ESM_ERR_ALIGN, "packed_attention: %s", why);
@@ -1036,7 +1037,7 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
   a.q = q, a.k = k, a.v = v, a.o = o;
   a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh, a.o_st = o_st, a.o_sh = o_sh;
   a.cu_q = cu_q, a.cu_k = cu_k, a.n = n, a.Tq = Tq, a.Tk = Tk, a.Hk = Hk, a.G = G, a.d = d, a.causal = causal != 0;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.splits = plan.splits;
   a.chunk = plan.chunk;
   if (need) {

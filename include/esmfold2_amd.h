@@ -458,7 +458,7 @@ int esmc_swiglu(const esm_half* x12, esm_half* y, int M, int F, void* stream);
  *   sequence are not written. What unseen keys and values hold (infinities, NaN) reaches no output; a seen infinity or
  *   NaN of v makes its column of the row one or the other. Scores, softmax and sums are fp32, the probabilities rounded
  *   to dtype for the second product (a half step each; in fp16 below 2^-25 of the row's largest 2^-36 of that). d % 8
- *   == 0, d <= 128; scale > 0; row strides from d to 2^23.
+ *   == 0, d <= 128; 0 < scale < 2^127; row strides from d to 2^23.
  *   workspace: packed_attention_workspace_bytes(...) bytes, 256-byte aligned (0: none; fp32 partials where a few rows'
  *   keys are divided between workgroups).
  */

@@ -266,3 +266,14 @@ def test_scores_that_rise_all_the_way(gpu_lib, pkg, nq, H, Hk, d, step, dtype):
                 o, bound = O.attention(q[i:i + 1, h:h + 1], k[:n, g:g + 1], v[:n, g:g + 1], [0, 1], [0, n], False, 1.0)
                 y = got[i:i + 1, h:h + 1].cpu().double()
                 assert float(((y - o).abs() / bound).max()) <= 1.0
+
+
+@pytest.mark.parametrize("scale", [1e-37, 1e-42])
+@pytest.mark.parametrize("nq,nk,H,Hk,d", FORMS)
+def test_scales_of_next_to_nothing_leave_the_mean(gpu_lib, pkg, nq, nk, H, Hk, d, scale):
+    # all exponents are 0 to fp32, below its normal range too: the oracle on queries of 0
+    g = torch.Generator().manual_seed(nk)
+    q, k, v = (torch.randn(n, h, d, generator=g).half().to(DEV) for n, h in ((nq, H), (nk, Hk), (nk, Hk)))
+    got = pkg.kernels.packed_attention(q, k, v, _cu([0, nq]), _cu([0, nk]), scale=scale)
+    o, bound = O.attention(q[:1, :1] * 0, k[:, :1], v[:, :1], [0, 1], [0, nk], False, 1.0)
+    assert float(((got[:, :1].cpu().double() - o).abs() / bound).max()) <= 1.0

@@ -1,5 +1,6 @@
 """CPU tests of the packed operators' host plans over sizes of every kind, no keys and no rows among them."""
 
+import ctypes
 import random
 
 import pytest
@@ -16,6 +17,15 @@ def test_attention_without_any_keys_needs_no_workspace(lib, rows, n):
     # a division by a chunk of no keys ended the process here from 16 rows a sequence on
     for H, Hk, d in ((4, 4, 64), (32, 8, 128), (1, 1, 8)):
         assert lib.packed_attention_workspace_bytes(n, rows, 0, H, Hk, d) == 0
+
+
+def test_scales_that_pass_fp32_in_the_exponent_are_refused(lib):
+    # (scale log2(e) was infinite in the kernel, and every row NaN)
+    p, cu = ctypes.c_void_p(1 << 20), ctypes.c_void_p(1 << 20)
+    for scale, rc in ((3e38, -2), (2.4e38, -2), (float("inf"), -2), (1e38, -1)):  # (-1: the next check, of q)
+        got = lib.packed_attention(None, p, p, p, 256, 64, 256, 64, 256, 64, 256, 64, cu, cu, 2, 8, 8, 4, 2, 64, 0, scale, 0,
+                                   None, 0, None)
+        assert got == rc, scale
 
 
 def test_attention_workspace_over_all_sizes(lib):
