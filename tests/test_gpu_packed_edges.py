@@ -277,3 +277,21 @@ def test_scales_of_next_to_nothing_leave_the_mean(gpu_lib, pkg, nq, nk, H, Hk, d
     got = pkg.kernels.packed_attention(q, k, v, _cu([0, nq]), _cu([0, nk]), scale=scale)
     o, bound = O.attention(q[:1, :1] * 0, k[:, :1], v[:, :1], [0, 1], [0, nk], False, 1.0)
     assert float(((got[:, :1].cpu().double() - o).abs() / bound).max()) <= 1.0
+
+
+# ---- the same call again, and over its queries -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,nk,H,Hk,d", [([1, 1], [6000, 4100], 8, 2, 128), ([2, 1, 1], [900, 1, 5000], 4, 4, 64),
+                                          ([300, 420, 65], [300, 420, 65], 40, 40, 64), ([24], [24], 40, 40, 64)])
+def test_repeats_and_outputs_over_the_queries(gpu_lib, pkg, nq, nk, H, Hk, d, dtype):
+    # sums in one order whatever runs beside them; keys divided between workgroups, whose join writes over the queries
+    g = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(sum(n), h, d, generator=g).to(dtype).to(DEV) for n, h in ((nq, H), (nk, Hk), (nk, Hk)))
+    cq, ck = _cu(_starts(nq)), _cu(_starts(nk))
+    ref = pkg.kernels.packed_attention(q, k, v, cq, ck, causal=True)
+    for _ in range(4):
+        assert torch.equal(pkg.kernels.packed_attention(q, k, v, cq, ck, causal=True), ref)
+    over = q.clone()
+    assert pkg.kernels.packed_attention(over, k, v, cq, ck, causal=True, out=over) is over and torch.equal(over, ref)
