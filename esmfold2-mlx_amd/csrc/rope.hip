@@ -11,7 +11,7 @@
 // lane; 2^lph lanes make a head and a wave takes 64 / 2^lph heads at a time. Memory bound: what matters is
 // that a wave has its loads in flight before the angles, which depend on the row alone and are used for
 // each of the wave's NIT groups of heads. 16,384 rows of 32 + 8 heads of 128 68 us, 4.9 TB/s; 3,481 rows of 40 + 40
-// heads of 64 over the row 17.7 us, 4.0 TB/s (vector work bounds it beside the bytes); 8 rows 3.4 us.
+// heads of 64 over the row 17.1 us, 4.2 TB/s (vector work bounds it beside the bytes); 8 rows 3.4 us.
 #include <type_traits>
 
 #include "common.h"
@@ -42,7 +42,7 @@ DEV float wave_total(float v) {
 
 // kFull: the head's lanes are all filled (d = 16 2^lph), and q and k both have weights or neither has: no lane's values
 // or weights are guarded. kPlain: and all turn in the half layout (rot = d). The guards took a third of the instructions,
-// which bound the norm over the row (3,481 rows of 40 + 40 heads of 64 20.2 -> 17.7 us).
+// which bound the norm over the row (3,481 rows of 40 + 40 heads of 64 19.1 -> 17.1 us).
 enum : int { kGuarded = 0, kFull = 1, kPlain = 2 };
 template <class V8, bool ROW, int NIT, int FORM>
 __global__ __launch_bounds__(64 * kRopeWaves) void qk_norm_rope_kernel(QkRopeArgs p) {
@@ -246,8 +246,8 @@ template <class V8, bool ROW, int FORM>
 static hipError_t launch_rope_t(const QkRopeArgs& a, int groups, hipStream_t s) {
   // Over the row one workgroup takes all heads; over each head a workgroup takes up to four waves' groups. With
   // rows enough to fill the GPU a wave takes several groups for its angles, three over the row or where that leaves fewer
-  // idle than two (us for 1, 2, 3: 16,384 rows of 32 + 8 heads of 128, half turned 75, 68, 68, all turned 68, 61, 60; of 20 + 4
-  // heads of 80 -, 30, 27; 3,481 rows of 40 + 40 heads of 64 over the row 21.2, 18.8, 17.7).
+  // idle than two (us for 1, 2, 3: 16,384 rows of 32 + 8 heads of 128, half turned 76, 70, 69, all turned 69, 62, 60; of 20 + 4
+  // heads of 80 29.4, 30.1, 27.5; 3,481 rows of 40 + 40 heads of 64 over the row 20.7, 18.5, 17.1).
   const int need = ROW ? (groups + kRopeWaves - 1) / kRopeWaves : 1;
   const int want = a.T < 512 ? 1 : ROW || (groups + 2) / 3 * 3 < (groups + 1) / 2 * 2 ? 3 : 2;
   const int nit = need > want ? need : want < groups ? want : groups;
