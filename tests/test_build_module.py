@@ -80,3 +80,60 @@ def test_both_ways_give_the_same_bits(gpu_lib, pkg, monkeypatch):
     assert pkg.capi.bind is not pkg.capi._LongWay
     monkeypatch.setattr(pkg.capi, "bind", pkg.capi._LongWay)
     assert all(torch.equal(a, b) for a, b in zip(want, run()))
+
+
+def _outcome(f):
+    """A call's tensors, or the code it is refused with."""
+    from esmfold2_mlx_amd.capi import EsmError
+    try:
+        y = f()
+    except EsmError as e:
+        return e.code
+    return [t.clone() for t in y] if isinstance(y, tuple) else [y]
+
+
+@pytest.mark.gpu
+def test_both_ways_take_and_refuse_the_same_calls(gpu_lib, pkg, monkeypatch):
+    K, dev = pkg.kernels, "cuda"
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    q, kv, cu = r(20, 4, 64).half(), r(20, 2, 64).half(), i32(0, 7, 20)
+    wide, f = r(20, 8, 72).half(), torch.rand(32, generator=g, dtype=torch.float64).to(dev)
+    codes, scales = (lambda m: (m.codes_packed, m.scales))(pkg.f8.F8Linear.from_float(r(128, 256)))
+    x = r(40, 256).bfloat16()
+    attention = [(q, kv, kv, cu), (q, kv, kv, cu, None, True, 0.3), (q, kv, kv, cu, cu), (q, kv, kv, i32(0, 3, 9), i32(0, 20, 20)),
+                 (wide[:, :4, :64], wide[:, 4:6, :64], wide[:, 6:, :64], cu), (q, wide[:, 4:6, 4:68], kv, cu),
+                 (q[:1].expand(20, 4, 64), kv, kv, cu), (q, kv[:, :1].expand(20, 2, 64), kv, cu), (q[:, :3], kv, kv, cu),
+                 (q[:1], kv, kv, i32(0, 1), i32(0, 20)), (q[:, :, :60], kv[:, :, :60], kv[:, :, :60], cu), (q, kv.bfloat16(), kv, cu),
+                 (q, kv[:5], kv[:5], cu), (q, kv, kv, cu.long()), (q, kv, kv, cu[::2]), (q, kv, kv, i32(0), i32(0)), (q, kv, kv, cu, i32(0, 20)),
+                 (q, kv, kv, cu, None, False, 0.0), (q, kv, kv, cu, None, False, float("nan")), (q[:0], kv[:0], kv[:0], i32(0, 0)),
+                 (q.float(), kv, kv, cu), (q.cpu(), kv, kv, cu), (q, kv, kv, cu.cpu()), (q[0], kv, kv, cu)]
+    rope = [((q, kv, f), {}), ((q, kv, f, torch.arange(20, device=dev)), dict(norm="rms", q_w=r(64), k_w=r(64))),
+            ((q, kv, f[:16]), dict(interleaved=True, norm="layer", over="row", q_w=r(256), k_w=r(128))),
+            ((q, kv, f, i32(*range(19))), {}), ((q, kv, f, torch.arange(20.0, device=dev)), {}), ((q, kv, f.float()), {}),
+            ((q, kv, f[:12]), {}), ((wide[:, :4, :64], wide[:, 4:, 8:], f), dict(norm="rms")), ((q, kv[:5], f), {}),
+            ((q, kv, f), dict(norm="rms", q_w=r(63))), ((q, kv, f), dict(q_w=r(63))), ((q, kv, f), dict(norm="rms", eps=-1.0)),
+            ((q, kv, f), dict(norm="none")), ((q, kv, f), dict(over="all")), ((q, kv, f[::2]), {}), ((q, kv, f[:0]), dict(norm="layer")),
+            ((q[..., 4:36], kv[..., 4:36], f[:16]), {}), ((q, kv.bfloat16(), f), {}), ((q, kv, f), dict(norm="rms", q_w=r(64).half()))]
+    linear = [(x, codes, scales, 128), (x[:3], codes, scales, 128), (x[::2], codes, scales, 128), (x[:0], codes, scales, 128),
+              (x.t().contiguous().t(), codes, scales, 128), (x[:, :250], codes, scales, 128), (x[:, :128], codes, scales, 128),
+              (x.float(), codes, scales, 128), (x, codes, scales, 64), (x, codes, scales.half(), 128), (x, codes.cpu(), scales, 128),
+              (x[:1].expand(40, 256), codes, scales, 128), (x[0], codes, scales, 128), (x.half(), codes, scales, 128)]
+
+    def run():
+        return ([_outcome(lambda a=a: K.packed_attention(*a)) for a in attention]
+                + [_outcome(lambda a=a, kw=kw: K.qk_norm_rope(*a, **kw)) for a, kw in rope]
+                + [_outcome(lambda a=a: K.f8_linear(*a)) for a in linear])
+
+    short = run()
+    monkeypatch.setattr(pkg.capi, "bind", pkg.capi._LongWay)
+    long = run()
+    assert {type(a) for a in long} == {int, list}
+    written = {3: 9, 15: 0}  # (rows of no sequence hold what was there: not compared)
+    for i, (a, b) in enumerate(zip(short, long)):
+        if isinstance(a, int) or isinstance(b, int):
+            assert a == b, i
+        else:
+            n = written.get(i)
+            assert [t.shape for t in a] == [t.shape for t in b] and all(torch.equal(s[:n], t[:n]) for s, t in zip(a, b)), i
