@@ -64,6 +64,15 @@ SIGNATURES = {
     "f8_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "f8_linear_partials_bytes": (_sz, [_int, _int, _int]),
     "f8_linear_partials": (_int, [_vp, _i64, _vp, _vp, _vp, _sz, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
+    "add_norm": (_int, [_vp, _int, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _int] + [_i64] * 4 + [_int] * 3 + [_vp]),
+    "f8_rows_bytes": (_sz, [_int, _int]),
+    "f8_rows_scales_bytes": (_sz, [_int, _int]),
+    "linear16_packed_bytes": (_sz, [_int, _int, _int]),
+    "linear16_pack": (_int, [_vp, _vp, _int, _int, _int, _vp]),
+    "linear16_workspace_bytes": (_sz, [_int] * 4),
+    "linear16": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
+    "f8_linear_end_workspace_bytes": (_sz, [_int] * 5),
+    "f8_linear_end": (_int, [_vp, _i64] + [_vp] * 6 + [_i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
     "esmc_block_workspace_bytes": (_sz, [_int, _int, _int]),
     "esmc_block": (_int, [_vp] * 17 + [_f32, _f32, _f32, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "parcae_step": (_int, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _int, _int, _int, _vp]),

@@ -1116,7 +1116,7 @@ int f8_run(const char* fn, const void* x, int64_t x_st, const uint8_t* qp, const
   char* ws = static_cast<char*>(workspace);
   esm::F8Args a{};
   a.x = x, a.x_st = x_st, a.wq = qp, a.sw = s, a.y = y;
-  a.M = M, a.Mp = w.Mp, a.K = K, a.N = N, a.splits = w.plan.splits;
+  a.M = M, a.Mp = w.Mp, a.K = K, a.N = N, a.splits = w.plan.splits, a.pieces = (N + 63) / 64;
   if (w.total) {
     a.xq = reinterpret_cast<uint8_t*>(ws);
     a.sx = reinterpret_cast<float*>(ws + w.sx);
@@ -1146,6 +1146,157 @@ int f8_linear_partials(const void* x, int64_t x_st, const uint8_t* qp, const flo
   if (!splits) return fail(ESM_ERR_NULL, "f8_linear_partials: NULL split count");
   return f8_run("f8_linear_partials", x, x_st, qp, s, nullptr, parts, parts_bytes, splits, M, K, N, dtype, workspace,
                 workspace_bytes, stream);
+}
+
+// ---- the end of a linear: bias, activation or gate, residual ---------------------------------------
+namespace {
+bool linear_shape(int M, int K, int N, int gated, int multiple_k) {
+  return M >= 0 && K > 0 && N > 0 && K % multiple_k == 0 && K <= kQ8MaxK && N % (gated ? 16 : 8) == 0;
+}
+
+// Checks what both linears share and fills in the end; `size`: whether M x 64 pieces outputs give grids below 2^32 threads.
+int linear_end(const char* fn, esm::LinearEnd& e, const float* bias, const void* residual, int64_t r_st, float alpha,
+               int activation, int gated, void* y, int M, int N, int dtype) {
+  if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "%s: dtype=%d", fn, dtype);
+  if (activation < ESM_ACT_NONE || activation > ESM_ACT_SILU) return fail(ESM_ERR_UNSUPPORTED, "%s: activation=%d", fn, activation);
+  if (!std::isfinite(alpha)) return fail(ESM_ERR_SHAPE, "%s: alpha must be finite", fn);
+  const int No = gated ? N / 2 : N;
+  if (M > (1 << 24) || ((long long)M + 63) / 64 * esm::linear_pieces(N, gated) >= (1LL << 22))
+    return fail(ESM_ERR_SHAPE, "%s: M=%d N=%d too large", fn, M, N);
+  if (M == 0) return ESM_OK;
+  if (!y) return fail(ESM_ERR_NULL, "%s: NULL output", fn);
+  if (residual && (r_st % 8 != 0 || (M > 1 && r_st < No)))
+    return fail(ESM_ERR_ALIGN, "%s: residual's row stride (a multiple of 8, >= the outputs)", fn);
+  if (!aligned16(y) || !aligned16(residual) || !aligned16(bias))
+    return fail(ESM_ERR_ALIGN, "%s: bias, residual and output must be 16-byte aligned", fn);
+  e.y = y, e.bias = bias, e.res = residual, e.r_st = M > 1 ? r_st : 0, e.alpha = alpha;
+  e.act = activation, e.gated = gated != 0, e.on = 1, e.No = No, e.Nb = N;
+  return ESM_OK;
+}
+
+int workspace_fault(const char* fn, const void* ws, size_t have, size_t need) {
+  if (!need) return ESM_OK;
+  if (!ws || have < need) return fail(ESM_ERR_SHAPE, "%s: workspace of %zu bytes, %zu needed", fn, have, need);
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return fail(ESM_ERR_ALIGN, "%s: workspace must be 256-byte aligned", fn);
+  return ESM_OK;
+}
+
+// f8_linear_end's workspace: x in e4m3 and its scales unless they are given, then partials of whole pieces.
+F8Ws f8_end_layout(int M, int K, int N, bool gated, bool coded) {
+  F8Ws w{};
+  w.plan = esm::f8_plan(M, K, 64 * esm::linear_pieces(N, gated), cu_count(), gated);
+  w.Mp = round_up(M, 16);
+  if (w.plan.form != esm::kF8Few && !coded) {
+    const size_t kb = (size_t)(K + 127) / 128;
+    w.sx = (size_t)w.Mp * kb * 128;
+    w.part = (w.sx + (size_t)w.Mp * kb * 4 + 1024 + 255) / 256 * 256;
+  }
+  w.total = w.part;
+  if (w.plan.splits > 1) w.total += (size_t)w.plan.splits * M * esm::linear_pieces(N, gated) * 256;
+  return w;
+}
+}  // namespace
+
+size_t f8_rows_bytes(int M, int K) { return M > 0 && K > 0 ? (size_t)round_up(M, 16) * ((K + 127) / 128) * 128 : 0; }
+size_t f8_rows_scales_bytes(int M, int K) {
+  return M > 0 && K > 0 ? (size_t)round_up(M, 16) * ((K + 127) / 128) * 4 + 1024 : 0;  // (1 KB that a tile's last rows read past)
+}
+
+size_t f8_linear_end_workspace_bytes(int M, int K, int N, int gated, int coded) {
+  return linear_shape(M, K, N, gated, 16) && M > 0 ? f8_end_layout(M, K, N, gated, coded).total : 0;
+}
+
+int f8_linear_end(const void* x, int64_t x_st, const uint8_t* xq, const float* sx, const uint8_t* qp, const float* s,
+                  const float* bias, const void* residual, int64_t r_st, float alpha, int activation, int gated, void* y, int M,
+                  int K, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "f8_linear_end";
+  if (!linear_shape(M, K, N, gated, 16) || (gated && N % 64 != 0))
+    return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d (multiple of 16) N=%d (of 8, gated: of 64)", fn, M, K, N);
+  if ((long long)round_up(M < 0 ? 0 : M, 16) * ((K + 127) / 128) * 4 >= (1LL << 31) - 4096)
+    return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d too large", fn, M, K);
+  esm::F8Args a{};
+  const int rc = linear_end(fn, a.end, bias, residual, r_st, alpha, activation, gated, y, M, N, dtype);
+  if (rc != ESM_OK) return rc;
+  if (M == 0) return ok();
+  if (!qp || !s || !x == !xq || (xq && !sx)) return fail(ESM_ERR_NULL, "%s: NULL pointer (x or its codes and scales, not both)", fn);
+  if (x && (x_st % 8 != 0 || (M > 1 && x_st < K))) return fail(ESM_ERR_ALIGN, "%s: row stride (a multiple of 8, >= K)", fn);
+  for (const void* t : {x, (const void*)xq, (const void*)sx, (const void*)qp})
+    if (!aligned16(t)) return fail(ESM_ERR_ALIGN, "%s: x and codes must be 16-byte aligned", fn);
+  const F8Ws w = f8_end_layout(M, K, N, gated, xq != nullptr);
+  const int wrc = workspace_fault(fn, workspace, workspace_bytes, w.total);
+  if (wrc != ESM_OK) return wrc;
+  char* ws = static_cast<char*>(workspace);
+  a.x = x, a.x_st = x_st, a.wq = qp, a.sw = s;
+  a.M = M, a.Mp = w.Mp, a.K = K, a.N = N, a.splits = w.plan.splits, a.pieces = esm::linear_pieces(N, gated);
+  a.coded = xq != nullptr;
+  a.xq = xq ? const_cast<uint8_t*>(xq) : reinterpret_cast<uint8_t*>(ws);
+  a.sx = xq ? const_cast<float*>(sx) : reinterpret_cast<float*>(ws + w.sx);
+  if (w.plan.splits > 1) a.part = reinterpret_cast<float*>(ws + w.part);
+  return hip_status(esm::launch_f8_linear(a, dtype == ESM_BF16, w.plan, (hipStream_t)stream), fn);
+}
+
+size_t linear16_packed_bytes(int N, int K, int gated) {
+  return linear_shape(0, K, N, gated, 8) ? esm::linear16_packed_size(N, K, gated) : 0;
+}
+
+int linear16_pack(const void* w, void* wp, int N, int K, int gated, void* stream) {
+  if (!linear_shape(0, K, N, gated, 8)) return fail(ESM_ERR_SHAPE, "linear16_pack: K=%d N=%d (multiples of 8, gated N of 16)", K, N);
+  if (!w || !wp) return fail(ESM_ERR_NULL, "linear16_pack: NULL pointer");
+  if (!aligned16(w) || !aligned16(wp)) return fail(ESM_ERR_ALIGN, "linear16_pack: weights must be 16-byte aligned");
+  return hip_status(esm::launch_linear16_pack(w, wp, N, K, gated != 0, (hipStream_t)stream), "linear16_pack launch");
+}
+
+size_t linear16_workspace_bytes(int M, int K, int N, int gated) {
+  if (!linear_shape(M, K, N, gated, 8) || M == 0) return 0;
+  const esm::L16Plan plan = esm::linear16_plan(M, K, N, gated != 0, cu_count());
+  return plan.splits > 1 ? (size_t)plan.splits * M * esm::linear_pieces(N, gated) * 256 : 0;
+}
+
+int linear16(const void* x, int64_t x_st, const void* wp, const float* bias, const void* residual, int64_t r_st, float alpha,
+             int activation, int gated, void* y, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
+             void* stream) {
+  const char* fn = "linear16";
+  if (!linear_shape(M, K, N, gated, 8)) return fail(ESM_ERR_SHAPE, "%s: M=%d K=%d N=%d (multiples of 8, gated N of 16)", fn, M, K, N);
+  esm::L16Args a{};
+  const int rc = linear_end(fn, a.end, bias, residual, r_st, alpha, activation, gated, y, M, N, dtype);
+  if (rc != ESM_OK) return rc;
+  if (M == 0) return ok();
+  if (!x || !wp) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
+  if (x_st % 8 != 0 || (M > 1 && (x_st < K || x_st > esm::kL16MaxStride)))
+    return fail(ESM_ERR_ALIGN, "%s: row stride (a multiple of 8, from K to 2^21)", fn);
+  if (!aligned16(x) || !aligned16(wp)) return fail(ESM_ERR_ALIGN, "%s: x and weights must be 16-byte aligned", fn);
+  const esm::L16Plan plan = esm::linear16_plan(M, K, N, gated != 0, cu_count());
+  const int wrc = workspace_fault(fn, workspace, workspace_bytes, linear16_workspace_bytes(M, K, N, gated));
+  if (wrc != ESM_OK) return wrc;
+  a.x = x, a.x_st = M > 1 ? x_st : 0, a.w = wp;
+  a.M = M, a.K = K, a.N = N, a.pieces = esm::linear_pieces(N, gated), a.splits = plan.splits;
+  if (plan.splits > 1) a.part = static_cast<float*>(workspace);
+  return hip_status(esm::launch_linear16(a, dtype == ESM_BF16, plan, (hipStream_t)stream), fn);
+}
+
+int add_norm(const void* x, int x_fp32, const void* y, float alpha, void* s, void* h, uint8_t* hq, float* hs, const float* w,
+             const float* b, float eps, int norm, int64_t x_st, int64_t y_st, int64_t s_st, int64_t h_st, int T, int D,
+             int dtype, void* stream) {
+  const char* fn = "add_norm";
+  if (T < 0 || D <= 0 || D % (hq ? 16 : 8) != 0 || D > esm::kNormMaxD || T > (1 << 24))
+    return fail(ESM_ERR_SHAPE, "%s: T=%d D=%d (a multiple of 8, in e4m3 of 16, up to 32768)", fn, T, D);
+  if ((norm != ESM_NORM_RMS && norm != ESM_NORM_LAYER) || (dtype != ESM_F16 && dtype != ESM_BF16))
+    return fail(ESM_ERR_UNSUPPORTED, "%s: norm=%d dtype=%d", fn, norm, dtype);
+  if (!(eps >= 0.f) || !std::isfinite(alpha)) return fail(ESM_ERR_SHAPE, "%s: eps must be >= 0, alpha finite", fn);
+  if (T == 0) return ok();
+  if (!x || !h == !hq || (hq && !hs)) return fail(ESM_ERR_NULL, "%s: NULL pointer (h or its codes and scales, not both)", fn);
+  for (int64_t st : {x_st, y ? y_st : 0, s ? s_st : 0, h ? h_st : 0})
+    if (st % 8 != 0) return fail(ESM_ERR_ALIGN, "%s: strides must be multiples of 8", fn);
+  if (T > 1 && (x_st < 0 || (y && y_st < 0) || (s && s_st < D) || (h && h_st < D)))
+    return fail(ESM_ERR_ALIGN, "%s: rows of outputs must lie apart", fn);
+  for (const void* t : {x, y, (const void*)s, (const void*)h, (const void*)hq, (const void*)hs, (const void*)w, (const void*)b})
+    if (!aligned16(t)) return fail(ESM_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
+  esm::AddNormArgs a{};
+  a.x = x, a.y = y, a.s = s, a.h = h, a.hq = hq, a.sx = hs, a.w = w, a.b = b;
+  a.x_st = x_st, a.y_st = y_st, a.s_st = s_st, a.h_st = h_st;
+  a.T = T, a.D = D, a.Kb = (D + 127) / 128, a.Mp = round_up(T, 16), a.layer = norm == ESM_NORM_LAYER;
+  a.alpha = alpha, a.eps = eps;
+  return hip_status(esm::launch_add_norm(a, dtype == ESM_BF16, x_fp32 != 0, (hipStream_t)stream), fn);
 }
 
 // The pieces of esmc_block's workspace, each 256-byte aligned: qkv, q, k, v, the attention's output, the

@@ -114,6 +114,22 @@ DEV float row16_sum(float v) {
   return v;
 }
 
+// Sum over the wave, the same in every lane.
+DEV float wave_total(float v) {
+  v = row16_sum(v);
+  const auto lane = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
+// --- e4m3 ----------------------------------------------------------------------------------
+constexpr float kF8Top = 448.f, kF8Floor = 0x1p-96f;  // the largest value; the least maximum a scale is made for
+// The factor to e4m3 and the scale back, from a block's largest magnitude (a NaN or infinity makes all of the block NaN).
+DEV void f8_scale(float top, float& r, float& s) {
+  top = top < kF8Floor ? kF8Floor : top;
+  r = kF8Top / top;
+  s = top / kF8Top;
+}
+
 // --- workgroup order --------------------------------------------------------------------
 // The dispatcher deals workgroup ids round-robin to the 8 XCDs (each with its own L2).
 // This bijection of [0, n) gives each XCD a contiguous run of logical indices, so

@@ -16,10 +16,11 @@
 // Up to 16 rows of x one launch does it all (f8_few_kernel: bound by the codes' bytes); beyond, x goes through
 // f8_quantize_kernel, then f8_some_kernel (some hundred rows: no barriers, operands straight to registers) or
 // f8_gemm_kernel (tiles through LDS by loads that write it directly).
+// The same kernels take x already in e4m3 (add_norm's rows; CODED), and end as linear.h has it, with a bias, an activation or
+// gate and a residual (END): y = r + alpha act(z + bias).
 #include <type_traits>
 
-#include "common.h"
-#include "kernels.h"
+#include "linear.h"
 
 namespace esm {
 
@@ -27,8 +28,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kF8Top = 448.f, kF8Floor = 0x1p-96f;
 
 // e4m3 x e4m3 -> fp32, 16 x 16 x 128 (a: 16 weight rows, b: 16 rows of x; 32 bytes a lane each). Result: column
 // (row of x) lane % 16, rows 4 (lane / 16) + register.
@@ -50,12 +49,6 @@ DEV float bits_value(uint32_t b) {
   u16x8 u = __builtin_bit_cast(u16x8, v);
   u[0] = (uint16_t)b;
   return (float)__builtin_bit_cast(V8, u)[0];
-}
-// The factor to e4m3 and the scale back, from a block's largest magnitude (a NaN or infinity makes both rows NaN).
-DEV void f8_scale(float top, float& r, float& s) {
-  top = top < kF8Floor ? kF8Floor : top;
-  r = kF8Top / top;
-  s = top / kF8Top;
 }
 // 8 values times r as 8 codes (round to nearest even; r keeps them within 448).
 template <class V8>
@@ -108,12 +101,21 @@ DEV i32x8 bload_frag(rsrc_t r, int voff, int soff) {
   return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// The weight scales of a piece: of its even and its odd fragments (gated: the gates' and the up values').
+struct PieceScales {
+  const float *even, *odd;
+};
+DEV PieceScales piece_scales(const F8Args& p, int ng, int Kb) {
+  if (!p.end.gated) return PieceScales{p.sw + (size_t)(ng >> 1) * Kb, p.sw + (size_t)(ng >> 1) * Kb};
+  return PieceScales{p.sw + (size_t)(ng >> 2) * Kb, p.sw + (size_t)((p.end.No + 32 * ng) >> 7) * Kb};
+}
+
 // ---- few rows: everything in one launch ------------------------------------------------------------
 // A workgroup takes 16 NJ weight rows for all (at most 16) rows of x; its 8 waves deal the blocks of 128 k among
 // them (the next block's loads in flight), bring x to e4m3 in registers (32 values of one row a lane) and sum
 // through LDS. Bound by the codes' bytes and a launch's ramp: one row of 2560 -> 10240 5.1 to 6.0 us, 5.1 to 4.4 TB/s.
 constexpr int kFewWaves = 8;
-template <class V8, int NJ>
+template <class V8, int NJ, bool END, bool CODED>
 __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
   constexpr int kPad = 16 * NJ + 4;  // (16 rows of sums cover the LDS banks)
   __shared__ __align__(16) float red[kFewWaves][16][kPad];
@@ -123,45 +125,60 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
   const int m = lane & 15, kl = 32 * (lane >> 4);
   const rsrc_t rw = make_rsrc(p.wq + (size_t)ng * Kb * 8192 + j0 * 2048);
   const uint16_t* xr = (const uint16_t*)p.x + (m < p.M ? m : 0) * p.x_st;
-  const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
+  const PieceScales sw = piece_scales(p, ng, Kb);
+  const rsrc_t rx = make_rsrc(p.xq);
   f32x4 acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Block {
-    i32x8 w[NJ];
+    i32x8 w[NJ], xq;
     u16x8 x[4];
-    float sw;
+    float sw, sw1, sx;
   };
   const auto load = [&](Block& b, int kb) {
     kb = min(kb, Kb - 1);
 #pragma unroll
     for (int j = 0; j < NJ; j++) b.w[j] = bload_frag(rw, 16 * lane, kb * 8192 + 2048 * j);
+    if constexpr (CODED) {  // (rows past the last: whatever is there, not stored)
+      b.xq = bload_frag(rx, 16 * lane, kb * 2048);
+      b.sx = p.sx[(size_t)kb * p.Mp + m];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int k = 128 * kb + kl + 8 * i;
-      b.x[i] = u16x8{};
-      if (m < p.M && k < p.K) b.x[i] = *reinterpret_cast<const u16x8*>(xr + k);
+      for (int i = 0; i < 4; i++) {
+        const int k = 128 * kb + kl + 8 * i;
+        b.x[i] = u16x8{};
+        if (m < p.M && k < p.K) b.x[i] = *reinterpret_cast<const u16x8*>(xr + k);
+      }
     }
-    b.sw = sw[kb];
+    b.sw = sw.even[kb];
+    if (END) b.sw1 = sw.odd[kb];
   };
   const auto take = [&](const Block& b) {
-    uint32_t top = 0;
+    i32x8 xf;
+    float s;
+    if constexpr (CODED) {
+      xf = b.xq;
+      s = b.sx;
+    } else {
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) top = max(top, top_bits(b.x[i]));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    float r, s;
-    f8_scale(bits_value<V8>(top), r, s);
-    int q[8];
+      for (int i = 0; i < 4; i++) top = max(top, top_bits(b.x[i]));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      float r;
+      f8_scale(bits_value<V8>(top), r, s);
+      int q[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) f8_codes(__builtin_bit_cast(V8, b.x[i]), r, q[2 * i], q[2 * i + 1]);
-    const i32x8 xf = {q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]};
+      for (int i = 0; i < 4; i++) f8_codes(__builtin_bit_cast(V8, b.x[i]), r, q[2 * i], q[2 * i + 1]);
+      xf = i32x8{q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7]};
+    }
+    const float s1 = END ? s * b.sw1 : 0.f;
     s *= b.sw;
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
       const f32x4 d = mfma_f8(b.w[j], xf);
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[j][e] = fmaf(s, d[e], acc[j][e]);
+      for (int e = 0; e < 4; e++) acc[j][e] = fmaf(END && (j & 1) ? s1 : s, d[e], acc[j][e]);
     }
   };
   Block b0, b1;
@@ -178,6 +195,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
   for (int j = 0; j < NJ; j++)
     *reinterpret_cast<f32x4*>(&red[wave][m][4 * NJ * (lane >> 4) + 4 * j]) = acc[j];
   __syncthreads();
+  if constexpr (END) {
+    end_few<V8, NJ, kFewWaves, kPad>(p.end, &red[0][0][0], p.M, ng, j0, threadIdx.x, 64 * kFewWaves);
+    return;
+  }
   for (int i = threadIdx.x; i < 16 * 16 * NJ; i += 64 * kFewWaves) {
     const int mm = i / (16 * NJ), c = i % (16 * NJ);
     float sum = red[0][mm][c];
@@ -204,7 +225,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_kernel(F8Args p) {
 // where 64 would need a second round: 238 rows 2560 -> 7680 11.0 -> 9.7 us, 512 rows 5120 -> 2560 18.4 -> 15.7. Bound by L2:
 // 238 rows 5120 -> 2560 in tiles of 48 8.0 us, 14 TB/s of fragments.
 constexpr int kSomeWaves = 8, kSomePad = 68;  // (rows of sums 68 floats apart: 16 of them cover the LDS banks)
-template <class V8, int MB, int RW>
+template <class V8, int MB, int RW, bool END>
 __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
   constexpr int KW = kSomeWaves / RW;  // waves that share K; RW tiles of 16 MB rows
   __shared__ __align__(16) float red[kSomeWaves][16 * MB * kSomePad];
@@ -215,10 +236,10 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
   const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, mbt = (t - ng * p.mtiles) * MB * RW, mb0 = min(mbt + rg * MB, Mb - 1);
   const rsrc_t rw = make_rsrc(p.wq + (size_t)ng * Kb * 8192), rx = make_rsrc(p.xq + (size_t)mb0 * Kb * 2048);
   const rsrc_t rs = make_rsrc(p.sx);
-  const float* sw = p.sw + (size_t)(ng >> 1) * Kb;
+  const PieceScales sw = piece_scales(p, ng, Kb);
   struct Block {
     i32x8 w[4], x[MB];
-    float s[MB], sw;
+    float s[MB], sw, sw1;
   };
   const auto load = [&](Block& k, int kb) {
     kb = min(kb, Kb - 1);
@@ -230,7 +251,8 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
       k.x[b] = bload_frag(rx, 16 * lane, (r * Kb + kb) * 2048);
       k.s[b] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (lane & 15), 4 * (kb * p.Mp + 16 * (mb0 + r)), 0));
     }
-    k.sw = sw[kb];
+    k.sw = sw.even[kb];
+    if (END) k.sw1 = sw.odd[kb];
   };
   f32x4 acc[MB][4];
 #pragma unroll
@@ -240,12 +262,12 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
   const auto take = [&](const Block& k) {
 #pragma unroll
     for (int b = 0; b < MB; b++) {
-      const float s = k.s[b] * k.sw;
+      const float s = k.s[b] * k.sw, s1 = END ? k.s[b] * k.sw1 : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const f32x4 d = mfma_f8(k.w[j], k.x[b]);
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[b][j][e] = fmaf(s, d[e], acc[b][j][e]);
+        for (int e = 0; e < 4; e++) acc[b][j][e] = fmaf(END && (j & 1) ? s1 : s, d[e], acc[b][j][e]);
       }
     }
   };
@@ -264,6 +286,13 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
     for (int j = 0; j < 4; j++)
       *reinterpret_cast<f32x4*>(&red[wave][(16 * b + (lane & 15)) * kSomePad + 16 * (lane >> 4) + 4 * j]) = acc[b][j];
   __syncthreads();
+  if constexpr (END) {
+#pragma unroll
+    for (int g = 0; g < RW; g++)
+      end_lds<V8, kSomePad>(p.end, red[g * KW], KW, 16 * MB * kSomePad, 16 * MB, 16 * (mbt + MB * g), p.M, ng, threadIdx.x,
+                            64 * kSomeWaves);
+    return;
+  }
   for (int i = threadIdx.x; i < RW * 16 * MB * 8; i += 64 * kSomeWaves) {  // 8 columns of a row each
     const int ri = i >> 3, c = 8 * (i & 7), m = 16 * mbt + ri, n = 64 * ng + c;
     if (m >= p.M || n >= p.N) continue;
@@ -294,7 +323,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void f8_some_kernel(F8Args p) {
 // block of 128 k: x and weight pieces and each wave's row scales come by direct loads into a ring of S slots. Bound by
 // the matrix cores' power and the LDS reads that feed them (a wave's 16 MB x 64 reads MB + 4 fragments for 4 MB
 // products): 8192 x 8192 x 8192 435 to 500 us by the clock, 2.5 to 2.2 PFLOP/s; 3481 x 2560 x 7680 72 us, 1.9.
-template <class V8, int MB, int WM, int WN, int S>
+template <class V8, int MB, int WM, int WN, int S, bool END>
 __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
   constexpr int NW = WM * WN, kX = 2048 * MB * WM, kW = 8192 * WN, kScales = 1024;  // bytes a slot
   constexpr int kSlot = kX + kW + NW * kScales;
@@ -311,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
   const int group = t / (8 * p.ntiles), in = t - group * 8 * p.ntiles, gm = min(8, p.mtiles - 8 * group);
   const int mt = 8 * group + in % gm, nt = in / gm;
   const int kb0 = Kb * split / p.splits, kb1 = Kb * (split + 1) / p.splits;  // (below 2^13 x 16)
-  const int mb0 = mt * MB * WM, ng0 = nt * WN, Mb = p.Mp / 16, Ng = (p.N + 63) / 64;
+  const int mb0 = mt * MB * WM, ng0 = nt * WN, Mb = p.Mp / 16, Ng = p.pieces;
   const int row0 = 16 * (mb0 + MB * wm);  // this wave's first row
   const dma_src_t rx = dma_src(p.xq + (size_t)mb0 * Kb * 2048, kBufRange), rw = dma_src(p.wq + (size_t)ng0 * Kb * 8192, kBufRange);
   const dma_src_t rs = dma_src(p.sx + min(row0, p.Mp - 16), kBufRange);
@@ -334,14 +363,18 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
   for (int i = 0; i < MB; i++)
 #pragma unroll
     for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float* sw = p.sw + (size_t)(min(ng0 + wn, Ng - 1) >> 1) * Kb;
+  const PieceScales sw = piece_scales(p, min(ng0 + wn, Ng - 1), Kb);
   const int n = kb1 - kb0;
   // This wave's weight scales of 64 blocks, one a lane: a load per block would wait for every tile in flight. (The
   // empty assembly has the wait here, not at each use.)
-  float sws;
+  float sws, sws1 = 0.f;
   const auto load_scales = [&](int i) {
-    sws = i + lane < n ? sw[kb0 + i + lane] : 0.f;
+    sws = i + lane < n ? sw.even[kb0 + i + lane] : 0.f;
     __asm__ volatile("" : "+v"(sws));
+    if (END) {
+      sws1 = i + lane < n ? sw.odd[kb0 + i + lane] : 0.f;
+      __asm__ volatile("" : "+v"(sws1));
+    }
   };
   const auto frag = [&](const char* src) {
     const i32x4 lo = *reinterpret_cast<const i32x4*>(src), hi = *reinterpret_cast<const i32x4*>(src + 1024);
@@ -364,13 +397,14 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
     const char* xs = at + 2048 * MB * wm + 16 * lane;
     const float* ss = reinterpret_cast<const float*>(at + kX + kW + kScales * wave) + (lane & 15);
     const float swk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sws), i & 63));
+    const float swk1 = END ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sws1), i & 63)) : 0.f;
     // Loads of a later block are spread over the step: issued at once by all waves they keep every one of them from its
     // first LDS read until the last is out (72 of 1 KB at 64 bytes a cycle).
     constexpr int kSpread = (kLoads + (MB < 5 ? MB : 5) - 1) / (MB < 5 ? MB : 5);
     // The fragment and scale of the next 16 rows are read, and the last 16 rows' results taken into the sums, between
     // the matrix instructions of these.
     i32x8 w[4], x = frag(xs), xn;
-    float s = ss[0], sn = 0.f, sp = 0.f;
+    float s = ss[0], sn = 0.f, sp = 0.f, sp1 = 0.f;
     f32x4 d[4], dp[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) w[j] = frag(at + kX + 8192 * wn + 2048 * j + 16 * lane);
@@ -389,7 +423,7 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
         if (b < MB) d[j] = mfma_f8(w[j], x);
         if (b > 0) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) acc[b - 1][j][e] = fmaf(sp, dp[j][e], acc[b - 1][j][e]);
+          for (int e = 0; e < 4; e++) acc[b - 1][j][e] = fmaf(END && (j & 1) ? sp1 : sp, dp[j][e], acc[b - 1][j][e]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -397,12 +431,28 @@ __global__ __launch_bounds__(64 * WM * WN) void f8_gemm_kernel(F8Args p) {
       for (int j = 0; j < 4; j++) dp[j] = d[j];
       x = xn;
       sp = swk * s;
+      if (END) sp1 = swk1 * s;
       s = sn;
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this slot's reads are back before the next barrier frees it
     __asm__ volatile("" ::: "memory");
   }
   wait_vm(0);  // no load of this workgroup outlives it
+  if constexpr (END) {
+    __syncthreads();  // (or lands on what end_tile keeps in LDS)
+    const int ng = ng0 + wn;
+    if (ng >= Ng) return;
+    if (!p.part) {
+      end_tile<V8>(p.end, p.M, row0, ng, lane, acc, lds + 8192 * wave);
+      return;
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++) {
+      const int m = row0 + 16 * b + (lane & 15);
+      if (m < p.M) part16(p.part, (long long)split * p.M + m, Ng, ng, lane >> 4, acc[b]);
+    }
+    return;
+  }
   // lane: row lane % 16 of each block, columns 16 (lane / 16) .. + 15 of the 64
   const int col = 64 * (ng0 + wn) + 16 * (lane >> 4);
 #pragma unroll
@@ -500,50 +550,62 @@ __global__ __launch_bounds__(256) void f8_quantize_weight_kernel(const float* __
   }
 }
 
-template <class V8, int MB, int WM, int WN, int S>
+template <class V8, bool END, int MB, int WM, int WN, int S>
 static hipError_t launch_gemm(F8Args a, hipStream_t s) {
   a.mtiles = (a.M + 16 * MB * WM - 1) / (16 * MB * WM);
-  a.ntiles = (a.N + 64 * WN - 1) / (64 * WN);
-  ESM_LAUNCH((f8_gemm_kernel<V8, MB, WM, WN, S>), dim3((unsigned)((size_t)a.mtiles * a.ntiles * a.splits)), dim3(64 * WM * WN), 0, s, a);
+  a.ntiles = (a.pieces + WN - 1) / WN;
+  ESM_LAUNCH((f8_gemm_kernel<V8, MB, WM, WN, S, END>), dim3((unsigned)((size_t)a.mtiles * a.ntiles * a.splits)), dim3(64 * WM * WN), 0,
+             s, a);
   return hipGetLastError();
 }
 
-template <class V8, int MB, int RW>
+template <class V8, bool END, int MB, int RW>
 static hipError_t launch_some(F8Args a, hipStream_t s) {
   a.mtiles = (a.Mp / 16 + MB * RW - 1) / (MB * RW);
-  ESM_LAUNCH((f8_some_kernel<V8, MB, RW>), dim3((unsigned)((size_t)a.mtiles * ((a.N + 63) / 64))), dim3(64 * kSomeWaves), 0, s, a);
+  ESM_LAUNCH((f8_some_kernel<V8, MB, RW, END>), dim3((unsigned)((size_t)a.mtiles * a.pieces)), dim3(64 * kSomeWaves), 0, s, a);
   return hipGetLastError();
 }
 
-template <class V8>
+template <class V8, bool END, bool CODED>
+static hipError_t launch_few(const F8Args& a, int mb, hipStream_t s) {
+  const dim3 grid(a.pieces * (4 / mb)), block(64 * kFewWaves);
+  switch (mb) {
+    case 4: ESM_LAUNCH((f8_few_kernel<V8, 4, END, CODED>), grid, block, 0, s, a); break;
+    case 2: ESM_LAUNCH((f8_few_kernel<V8, 2, END, CODED>), grid, block, 0, s, a); break;
+    default: ESM_LAUNCH((f8_few_kernel<V8, 1, END, CODED>), grid, block, 0, s, a); break;
+  }
+  return hipGetLastError();
+}
+
+template <class V8, bool END>
 static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) {
   hipError_t e;
   if (form == kF8Few) {
-    const dim3 grid((a.N + 63) / 64 * (4 / mb)), block(64 * kFewWaves);
-    switch (mb) {
-      case 4: ESM_LAUNCH((f8_few_kernel<V8, 4>), grid, block, 0, s, a); break;
-      case 2: ESM_LAUNCH((f8_few_kernel<V8, 2>), grid, block, 0, s, a); break;
-      default: ESM_LAUNCH((f8_few_kernel<V8, 1>), grid, block, 0, s, a); break;
-    }
-    return hipGetLastError();
+    if constexpr (END)
+      if (a.coded) return launch_few<V8, true, true>(a, mb, s);
+    return launch_few<V8, END, false>(a, mb, s);
   }
-  ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, (a.K + 127) / 128), dim3(256), 0, s,
-             (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (!a.coded) {
+    ESM_LAUNCH((f8_quantize_kernel<V8>), dim3((a.Mp + 31) / 32, (a.K + 127) / 128), dim3(256), 0, s,
+               (const uint16_t*)a.x, a.x_st, a.xq, a.sx, a.M, a.K, a.Mp);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   if (form == kF8Some) switch (mb) {
-      case 1: return launch_some<V8, 1, 1>(a, s);
-      case 2: return launch_some<V8, 2, 1>(a, s);
-      case 3: return launch_some<V8, 3, 1>(a, s);
-      case 4: return launch_some<V8, 4, 1>(a, s);
-      default: return launch_some<V8, 4, 2>(a, s);
+      case 1: return launch_some<V8, END, 1, 1>(a, s);
+      case 2: return launch_some<V8, END, 2, 1>(a, s);
+      case 3: return launch_some<V8, END, 3, 1>(a, s);
+      case 4: return launch_some<V8, END, 4, 1>(a, s);
+      default: return launch_some<V8, END, 4, 2>(a, s);
     }
   switch (mb) {
-    case 2: e = launch_gemm<V8, 2, 2, 4, 2>(a, s); break;
-    case 4: e = launch_gemm<V8, 4, 2, 4, 2>(a, s); break;
-    case 6: e = launch_gemm<V8, 6, 2, 4, 2>(a, s); break;
-    default: e = launch_gemm<V8, 8, 2, 4, 2>(a, s); break;
+    case 2: e = launch_gemm<V8, END, 2, 2, 4, 2>(a, s); break;
+    case 4: e = launch_gemm<V8, END, 4, 2, 4, 2>(a, s); break;
+    case 6: e = launch_gemm<V8, END, 6, 2, 4, 2>(a, s); break;
+    default: e = launch_gemm<V8, END, 8, 2, 4, 2>(a, s); break;
   }
-  if (e != hipSuccess || !a.part || !a.y) return e;
+  if (e != hipSuccess || !a.part) return e;
+  if constexpr (END) return launch_linear_join<V8>(a.part, a.end, a.M, a.pieces, a.splits, s);
+  if (!a.y) return e;
   const size_t n8 = (size_t)a.M * a.N / 8, blocks = (n8 + 255) / 256;
   ESM_LAUNCH((f8_reduce_kernel<V8>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a.part, (uint16_t*)a.y, n8,
              a.splits);
@@ -551,7 +613,8 @@ static hipError_t launch_f8_t(const F8Args& a, int form, int mb, hipStream_t s) 
 }
 
 hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipStream_t s) {
-  return bf16 ? launch_f8_t<bf16x8>(a, plan.form, plan.mb, s) : launch_f8_t<half8>(a, plan.form, plan.mb, s);
+  if (a.end.on) return bf16 ? launch_f8_t<bf16x8, true>(a, plan.form, plan.mb, s) : launch_f8_t<half8, true>(a, plan.form, plan.mb, s);
+  return bf16 ? launch_f8_t<bf16x8, false>(a, plan.form, plan.mb, s) : launch_f8_t<half8, false>(a, plan.form, plan.mb, s);
 }
 
 // Which form, its row blocks and splits: the lowest of estimated times, from these measurements (us, kernel alone,
@@ -561,7 +624,7 @@ hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipS
 //   M = 2000  128: 46, 192: 55, 256: 38    M = 3481  128: 90, 192: 86, 256: 70
 //   5120 -> 2560 at M = 238  some 8.0, LDS tiles with K split 15 and 4 for the sum; at M = 512  some 15.7, 64 rows in two
 //   splits 21 and 5; at M = 1000  some 31, 64 rows 33, 128 rows in three splits 25 and 6
-F8Plan f8_plan(int M, int K, int N, int cus) {
+F8Plan f8_plan(int M, int K, int N, int cus, bool gated) {
   // Few rows: the most weight rows a workgroup (16, 32 or 64) that still give more than half the CUs one, as each
   // workgroup reads x whole and few workgroups in flight leave the codes' loads waiting (us, 64 / 32 / 16 rows, M = 1 to 16:
   // 2560 -> 10240 5.1 to 6.3 / 6.3 to 9.4 / 8.2 to 12.2, 2560 -> 7680 4.9 to 6.3 / 4.5 to 5.7 / 6.2 to 8.8,
@@ -569,7 +632,8 @@ F8Plan f8_plan(int M, int K, int N, int cus) {
   // Up to 16 rows, as x brought to e4m3 apart costs 3 us (16 rows of 2560 -> 10240 6.3 against 3 + 4.4, 5120 -> 2560 7.9
   // against 2.5 + 6.2), and a second block of 16 here 16 us.
   F8Plan p{kF8Few, 4, 1};
-  while (p.mb > 1 && 16LL * ((N + 63) / 64) * (4 / p.mb) < 9LL * cus) p.mb /= 2;
+  const int least = gated ? 2 : 1;  // (a gate and its up value in one workgroup)
+  while (p.mb > least && 16LL * ((N + 63) / 64) * (4 / p.mb) < 9LL * cus) p.mb /= 2;
   if (M <= 16) return p;
   const int Kb = (K + 127) / 128;
   // Some rows: the fewest rows a workgroup (16 to 64) whose tiles fit one to a CU; else 32 where two rounds take them

@@ -191,6 +191,18 @@ struct AttnPlan {
 };
 long long split_attention_items(long long Tq, long long Tk, int n, int G, int chunk);
 
+// The end of a linear (linear.h): y = r + alpha act(z + bias), or r + alpha act(g) u of gated weights.
+enum : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+struct LinearEnd {
+  void* y;                // [M, No] 16-bit
+  const float* bias;      // [Nb] or nullptr
+  const void* res;        // [M, No] 16-bit, rows r_st elements apart, or nullptr (may be y)
+  long long r_st;
+  float alpha;
+  int act, gated, on;     // on: this end, else y as it is
+  int No, Nb;             // outputs of a row; biases (gated: 2 No, gate then up)
+};
+
 struct F8Args {
   const void* x;          // [M, K], 16-bit, rows x_st elements apart
   long long x_st;
@@ -202,6 +214,9 @@ struct F8Args {
   float* sx;              // [ceil(K / 128), Mp]
   int M, Mp, K, N;        // Mp: M rounded up to 16
   int splits, mtiles, ntiles;
+  int pieces;             // of 64 packed weight rows
+  int coded;              // xq and sx are given (add_norm's): x is not read
+  LinearEnd end;
 };
 constexpr int kF8MaxSplits = 16;
 enum : int { kF8Few = 0, kF8Some = 1, kF8Tiles = 2 };
@@ -268,6 +283,45 @@ constexpr int kCellTile = 64;
 constexpr int kEpiUnit = 32;
 constexpr int kEpiWaves = 8;
 
+struct L16Args {
+  const void* x;          // [M, K], 16-bit, rows x_st elements apart
+  long long x_st;
+  const void* w;          // fragment order (linear16_pack)
+  float* part;            // [splits, M, 64 pieces] fp32, or nullptr
+  int M, K, N, pieces;
+  int splits, mtiles, ntiles;
+  LinearEnd end;
+};
+constexpr long long kL16MaxStride = 1 << 21;  // of x's rows: 256 of them lie within 2^30 bytes
+constexpr int kL16MaxSplits = 16;
+enum : int { kL16Few = 0, kL16Some = 1, kL16Tiles = 2 };
+struct L16Plan {
+  int form;
+  int mb;                 // as F8Plan's
+  int splits;
+};
+constexpr size_t linear16_packed_size(int N, int K, bool gated) {
+  return (size_t)(gated ? (N / 2 + 31) / 32 : (N + 63) / 64) * ((K + 63) / 64) * 8192;
+}
+
+// Residual and norm (dtype: the 16-bit type of y and h; x and s fp32 or that type).
+constexpr int kNormMaxD = 32768;
+struct AddNormArgs {
+  const void* x;
+  const void* y;          // or nullptr
+  void* s;                // x + alpha y, or nullptr
+  void* h;                // 16-bit rows, or nullptr with
+  uint8_t* hq;            // e4m3 in the e4m3 linear's order and
+  float* sx;              // its scales [Kb][Mp]
+  const float* w;         // [D] or nullptr
+  const float* b;
+  long long x_st, y_st, s_st, h_st;  // elements from row to row
+  long long T;
+  int D, Kb, Mp, layer;
+  float alpha, eps;
+  int waves, rows;        // waves per row, rows per workgroup (set by the launcher)
+};
+
 // Each launcher returns the hipError_t of the launch.
 hipError_t launch_project(const ProjectArgs& a, int grid, hipStream_t s);
 hipError_t launch_contract(const ContractArgs& a, hipStream_t s);
@@ -298,7 +352,12 @@ bool qk_norm_rope_row_fits(int heads, int d);  // whether one workgroup takes a 
 hipError_t launch_qk_norm_rope(QkRopeArgs a, bool bf16, bool row, hipStream_t s);
 AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G, int d, int cus);
 hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s);
-F8Plan f8_plan(int M, int K, int N, int cus);
+hipError_t launch_linear16_pack(const void* w, void* out, int N, int K, bool gated, hipStream_t s);
+L16Plan linear16_plan(int M, int K, int N, bool gated, int cus);
+hipError_t launch_linear16(const L16Args& a, bool bf16, const L16Plan& plan, hipStream_t s);
+constexpr int linear_pieces(int N, bool gated) { return gated ? (N / 2 + 31) / 32 : (N + 63) / 64; }
+hipError_t launch_add_norm(const AddNormArgs& a, bool bf16, bool x32, hipStream_t s);
+F8Plan f8_plan(int M, int K, int N, int cus, bool gated = false);
 hipError_t launch_f8_linear(const F8Args& a, bool bf16, const F8Plan& plan, hipStream_t s);
 constexpr size_t f8_packed_size(int N, int K) { return (size_t)((N + 63) / 64) * ((K + 127) / 128) * 8192; }
 hipError_t launch_f8_pack(const uint8_t* q, uint8_t* out, int N, int K, hipStream_t s);

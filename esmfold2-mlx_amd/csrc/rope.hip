@@ -33,13 +33,6 @@ DEV float head_sum(float v, int lph) {
   return v;
 }
 
-// Sum over the wave, the same in every lane.
-DEV float wave_total(float v) {
-  v = row16_sum(v);
-  const auto lane = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
-  return (lane(0) + lane(16)) + (lane(32) + lane(48));
-}
-
 // kFull: the head's lanes are all filled (d = 16 2^lph), and q and k both have weights or neither has: no lane's values
 // or weights are guarded. kPlain: and all turn in the half layout (rot = d). The guards took a third of the instructions,
 // which bound the norm over the row (3,481 rows of 40 + 40 heads of 64 19.1 -> 17.1 us).

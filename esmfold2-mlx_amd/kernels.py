@@ -775,3 +775,187 @@ def f8_linear_partials(x, codes, scales, N: int):
                                           capi.stream_ptr()))
     n = max(splits.value, 1)  # (no rows: one split of none)
     return buf[:4 * n * M * N].view(torch.float32).view(n, M, N), n, gen
+
+
+# ---- around the packed rows' attention and linears -------------------------------------------------
+_NORM_KINDS = {"rms": 1, "layer": 2}
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_STREAMS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _matrix(t, name: str, dtypes, index: int | None = None, shape=None):
+    """A [rows, values] operand, the values of a row contiguous: (row stride, device)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise capi.EsmError(-5, f"{name} must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
+    at = t.get_device()
+    if index is not None and at != index:
+        raise capi.EsmError(-5, f"{name} must be on cuda:{index}")
+    if t.dim() != 2 or t.dtype not in dtypes or (shape is not None and t.shape != shape):
+        want = "" if shape is None else f" {tuple(shape)}"
+        raise capi.EsmError(-2, f"{name} must be [rows, values]{want} in {' or '.join(map(str, dtypes))}, got {t.dtype} {tuple(t.shape)}")
+    st, one = t.stride()
+    if t.shape[1] > 1 and one != 1:
+        raise capi.EsmError(-3, f"{name}: the values of a row must be contiguous")
+    return (st if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8), at
+
+
+def _vector(t, name: str, n: int, index: int):
+    """Device pointer of an fp32 [n] parameter (None: none)."""
+    if t is None:
+        return None
+    _aux(t, name, _FP32, index)
+    if t.numel() != n:
+        raise capi.EsmError(-2, f"{name} has {t.numel()} values, {n} are read")
+    return t.data_ptr()
+
+
+def _add_norm(fn, x, y, w, b, alpha, norm, eps, dtype, sum_out, out, f8):
+    lib = capi.lib()
+    x_st, index = _matrix(x, "x", _STREAMS)
+    if index != _current():
+        with torch.cuda.device(index):
+            return _add_norm(fn, x, y, w, b, alpha, norm, eps, dtype, sum_out, out, f8)
+    T, D = x.shape
+    if dtype is None:
+        dtype = y.dtype if isinstance(y, torch.Tensor) else out.dtype if isinstance(out, torch.Tensor) else x.dtype
+    if dtype not in _DTYPES or (x.dtype is not dtype and x.dtype is not torch.float32) or norm not in _NORM_KINDS:
+        raise capi.EsmError(-4, f"{fn}: x in {x.dtype}, h in {dtype}, norm={norm!r} (x in fp32 or h's 16-bit type)")
+    y_st = s_st = h_st = 0
+    s = x
+    if y is not None:
+        y_st, _ = _matrix(y, "y", (dtype,), index, x.shape)
+        s = x.new_empty((T, D)) if sum_out is None else sum_out
+        s_st, _ = _matrix(s, "sum_out", (x.dtype,), index, x.shape)
+        if T and (s.data_ptr() == y.data_ptr() or (s.data_ptr() == x.data_ptr() and s_st != x_st)):
+            raise capi.EsmError(-3, f"{fn}: sum_out may be x with its strides, and share no memory with y")
+    elif sum_out is not None or alpha != 1.0:
+        raise capi.EsmError(-2, f"{fn}: sum_out and alpha go with y")
+    wp, bp = _vector(w, "w", D, index), _vector(b, "b", D, index)
+    hq = hs = None
+    if f8:
+        hq = torch.empty(int(lib.f8_rows_bytes(T, D)), dtype=torch.uint8, device=x.device)
+        hs = torch.empty(int(lib.f8_rows_scales_bytes(T, D)) // 4, dtype=torch.float32, device=x.device)
+        h = (hq, hs)
+    else:
+        h = torch.empty((T, D), dtype=dtype, device=x.device) if out is None else out
+        h_st, _ = _matrix(h, "out", (dtype,), index, x.shape)
+        if T and any(t is not None and h.data_ptr() == t.data_ptr() for t in (x, y, s)):
+            raise capi.EsmError(-3, f"{fn}: out shares no memory with x, y or sum_out")
+    capi.check(lib.add_norm(x.data_ptr(), x.dtype is torch.float32, _ptr(y), float(alpha), None if y is None else s.data_ptr(),
+                            None if f8 else h.data_ptr(), _ptr(hq), _ptr(hs), wp, bp, float(eps), _NORM_KINDS[norm], x_st,
+                            y_st, s_st, h_st, T, D, _DTYPES[dtype], capi.stream_ptr()))
+    return s, h
+
+
+def add_norm(x, y=None, w=None, b=None, *, alpha: float = 1.0, norm: str = "rms", eps: float = 1e-6, dtype=None,
+             sum_out=None, out=None):
+    """(s, h): s = x + alpha * y (x itself without ``y``) and h = the norm of s, "rms" or "layer", times ``w``, plus ``b``
+    (fp32 [D]; None: 1 and 0), one pass. x [T, D] in fp32 or in h's type, y and h fp16 or bf16 (``dtype``: h's, else y's or
+    x's); rows may lie apart. fp32 throughout, the norm of s as it is before its rounding to x's type. ``sum_out`` may be
+    x; ``out`` shares no memory with the operands. D a multiple of 8 up to 32768."""
+    return _add_norm("add_norm", x, y, w, b, alpha, norm, eps, dtype, sum_out, out, False)
+
+
+def add_norm_f8(x, y=None, w=None, b=None, *, alpha: float = 1.0, norm: str = "rms", eps: float = 1e-6, dtype=None,
+                sum_out=None):
+    """``add_norm`` with h in e4m3, brought there from fp32 by ``f8_linear``'s rule: (s, (codes, scales)) in the order its
+    matrix cores take (``f8.F8Rows`` gives them back). D a multiple of 16."""
+    return _add_norm("add_norm_f8", x, y, w, b, alpha, norm, eps, dtype, sum_out, None, True)
+
+
+def _linear_end(fn, M: int, No: int, Nb: int, bias, activation, residual, out, dtype, index: int, x):
+    """The checks of a linear's end: (bias, residual, its stride, activation, y)."""
+    if activation not in _ACTIVATIONS:
+        raise capi.EsmError(-4, f"{fn}: activation={activation!r}")
+    bp = _vector(bias, "bias", Nb, index)
+    r_st = 0
+    if residual is not None:
+        r_st, _ = _matrix(residual, "residual", (dtype,), index, (M, No))
+    if out is None:
+        y = torch.empty((M, No), dtype=dtype, device=torch.device("cuda", index))
+    else:
+        y = _out(out, "out", dtype, M * No)
+        if y.get_device() != index:
+            raise capi.EsmError(-5, f"out must be on cuda:{index}")
+        if M and x is not None and y.data_ptr() == x.data_ptr():
+            raise capi.EsmError(-3, f"{fn}: out may be the residual, not x")
+        if M > 1 and residual is not None and y.data_ptr() == residual.data_ptr() and r_st != No:
+            raise capi.EsmError(-3, f"{fn}: out over the residual must have its strides")
+    return bp, _ptr(residual), r_st, _ACTIVATIONS[activation], y
+
+
+def linear16_pack(w, gated: bool = False):
+    """A weight [N, K] (fp16 or bf16) in the order ``linear16``'s matrix-core fragments take it, as bytes."""
+    lib = capi.lib()
+    if not isinstance(w, torch.Tensor) or w.dtype not in _DTYPES or w.dim() != 2:
+        raise capi.EsmError(-2, "linear16_pack: w must be [N, K] in fp16 or bf16")
+    _dev(w, "w")
+    N, K = w.shape
+    wp = torch.empty(int(lib.linear16_packed_bytes(N, K, gated)), dtype=torch.uint8, device=w.device)
+    with torch.cuda.device(w.device):
+        capi.check(lib.linear16_pack(w.data_ptr(), wp.data_ptr(), N, K, gated, capi.stream_ptr()))
+    return wp
+
+
+def linear16(x, packed, N: int, bias=None, *, gated: bool = False, activation: str | None = None, residual=None,
+             alpha: float = 1.0, out=None):
+    """y = residual + alpha * act(x . W^T + bias), or with ``gated`` residual + alpha * act(g) u of the two halves of the
+    N outputs: x [M, K] fp16 or bf16 (rows may lie apart), W [N, K] of its type as ``linear16_pack`` has it, ``bias`` [N]
+    fp32, ``activation`` None, "relu", "gelu", "gelu_tanh" or "silu", ``residual`` of y's type. fp32 sums, one rounding.
+    ``out`` (contiguous) may be the residual. Split-K partials live in the shared scratch (``scratch.workspace``)."""
+    lib = capi.lib()
+    x_st, index = _matrix(x, "x", tuple(_DTYPES))
+    if index != _current():
+        with torch.cuda.device(index):
+            return linear16(x, packed, N, bias, gated=gated, activation=activation, residual=residual, alpha=alpha, out=out)
+    M, K = x.shape
+    _aux(packed, "packed", _UINT8, index)
+    if not packed.numel() or packed.numel() != lib.linear16_packed_bytes(N, K, gated):
+        raise capi.EsmError(-2, f"linear16: {packed.numel()} packed bytes for [{N}, {K}]")
+    bp, rp, r_st, act, y = _linear_end("linear16", M, N // 2 if gated else N, N, bias, activation, residual, out, x.dtype, index, x)
+    args = (x.data_ptr(), x_st, packed.data_ptr(), bp, rp, r_st, float(alpha), act, gated, y.data_ptr(), M, K, N, _DTYPES[x.dtype])
+    need = lib.linear16_workspace_bytes(M, K, N, gated)
+    if not need:
+        capi.check(lib.linear16(*args, None, 0, capi.stream_ptr()))
+        return y
+    with scratch.guard(x.device):
+        ws, wp, stream = scratch.workspace(need, x.device)
+        capi.check(lib.linear16(*args, wp, need, stream))
+    return y
+
+
+def f8_linear_end(x, codes, scales, N: int, bias=None, *, gated: bool = False, activation: str | None = None, residual=None,
+                  alpha: float = 1.0, rows=None, dtype=None, out=None):
+    """``f8_linear`` with the end of ``linear16``. In x's place may stand ``rows`` = (codes, scales, M, K) of
+    ``add_norm_f8`` (x None), then with ``dtype`` as y's type."""
+    lib = capi.lib()
+    if rows is None:
+        M, K, x_st, index = _f8_operands(x, codes, scales, N, "f8_linear_end")
+        dtype, device, xq, sx = x.dtype, x.device, None, None
+    else:
+        xq, sx, M, K = rows
+        if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
+            raise capi.EsmError(-5, "rows must be CUDA(HIP) tensors; the HIP path has no CPU fallback")
+        index, device, x_st = xq.get_device(), xq.device, 0
+        for t, n, kinds in ((xq, "rows' codes", _UINT8), (sx, "rows' scales", _FP32), (codes, "codes", _UINT8), (scales, "scales", _FP32)):
+            _aux(t, n, kinds, index)
+        if dtype not in _DTYPES:
+            raise capi.EsmError(-2, f"f8_linear_end: dtype={dtype}")
+        if (xq.numel() < lib.f8_rows_bytes(M, K) or 4 * sx.numel() < lib.f8_rows_scales_bytes(M, K)
+                or codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128)):
+            raise capi.EsmError(-2, f"f8_linear_end: {codes.numel()} packed codes and {scales.numel()} scales for [{N}, {K}]")
+    if index != _current():
+        with torch.cuda.device(index):
+            return f8_linear_end(x, codes, scales, N, bias, gated=gated, activation=activation, residual=residual, alpha=alpha,
+                                 rows=rows, dtype=dtype, out=out)
+    bp, rp, r_st, act, y = _linear_end("f8_linear_end", M, N // 2 if gated else N, N, bias, activation, residual, out, dtype, index, x)
+    args = (_ptr(x), x_st, _ptr(xq), _ptr(sx), codes.data_ptr(), scales.data_ptr(), bp, rp, r_st, float(alpha), act, gated,
+            y.data_ptr(), M, K, N, _DTYPES[dtype])
+    need = lib.f8_linear_end_workspace_bytes(M, K, N, gated, xq is not None)
+    if not need:
+        capi.check(lib.f8_linear_end(*args, None, 0, capi.stream_ptr()))
+        return y
+    with scratch.guard(device):
+        ws, wp, stream = scratch.workspace(need, device)
+        capi.check(lib.f8_linear_end(*args, wp, need, stream))
+    return y

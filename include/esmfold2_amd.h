@@ -479,6 +479,44 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Around the packed rows' attention and linears (no reference counterpart). dtype: the 16-bit type of every 16-bit tensor.
+ *
+ * add_norm: s = x + alpha y (y NULL: x), written to s unless NULL (s may be x with x's stride); h = s / sqrt(mean s^2 +
+ *   eps) w (ESM_NORM_RMS) or (s - mean) / sqrt(var + eps) w + b (ESM_NORM_LAYER; a b is added in either). x and s [T, D] in
+ *   fp32 (x_fp32) or 16 bits, y 16 bits, w and b [D] fp32 or NULL (1 and 0). fp32 throughout; the norm takes s before it is
+ *   rounded to x's type. Out: h [T, D] in 16 bits, or (h NULL) hq and hs: h in e4m3 as f8_linear brings its x to it, from
+ *   the fp32 values, in the order f8_linear_end takes: f8_rows_bytes(T, D) and f8_rows_scales_bytes(T, D) bytes. Rows
+ *   x_st, y_st, s_st, h_st elements apart (multiples of 8). D % 8 == 0 (e4m3: 16), D <= 32768; T <= 2^24.
+ * linear16: y = r + alpha act(x W^T + bias) (residual NULL: no r), x [M, K] and W [N, K] in 16 bits, W by linear16_pack, bias
+ *   [N] fp32 or NULL, fp32 sums, one rounding; gated: W = [gate; up], y = r + alpha act(g) u with N / 2 outputs. gelu is z
+ *   P(z) with the normal distribution's P, ESM_ACT_GELU_TANH its usual form with a tanh. residual [M, outputs] in 16 bits (rows
+ *   r_st apart, may be y where r_st is the outputs), y contiguous. K % 8 == 0, N % 8 == 0 (gated: 16), x_st <= 2^21.
+ * f8_linear_end: the same on e4m3 weights (f8_pack_codes; gated: rows in linear16's order, see F8Linear, N % 64 == 0) with
+ *   x [M, K] in 16 bits brought to e4m3 as f8_linear does, or (x NULL) add_norm's codes and scales of M rows.
+ * Workspaces as their sizes say, 256-byte aligned (0: none).
+ */
+#define ESM_ACT_NONE 0
+#define ESM_ACT_RELU 1
+#define ESM_ACT_GELU 2
+#define ESM_ACT_GELU_TANH 3
+#define ESM_ACT_SILU 4
+int add_norm(const void* x, int x_fp32, const void* y, float alpha, void* s, void* h, uint8_t* hq, float* hs, const float* w,
+             const float* b, float eps, int norm, int64_t x_st, int64_t y_st, int64_t s_st, int64_t h_st, int T, int D,
+             int dtype, void* stream);
+size_t f8_rows_bytes(int M, int K);
+size_t f8_rows_scales_bytes(int M, int K);
+size_t linear16_packed_bytes(int N, int K, int gated);
+int linear16_pack(const void* w, void* wp, int N, int K, int gated, void* stream);
+size_t linear16_workspace_bytes(int M, int K, int N, int gated);
+int linear16(const void* x, int64_t x_st, const void* wp, const float* bias, const void* residual, int64_t r_st, float alpha,
+             int activation, int gated, void* y, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
+             void* stream);
+size_t f8_linear_end_workspace_bytes(int M, int K, int N, int gated, int coded);
+int f8_linear_end(const void* x, int64_t x_st, const uint8_t* xq, const float* sx, const uint8_t* qp, const float* s,
+                  const float* bias, const void* residual, int64_t r_st, float alpha, int activation, int gated, void* y, int M,
+                  int K, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * One whole ESMC block (mlx_esmc.py:84-102) as its eight launches on the stream (one more for each of wqkv, w1
  * whose K is split, and for each linear whose rows are divided between tile forms), from the block's LayerNormed
  * input: x' = x + alpha * wo(attention(wqkv(h))), then x_out = x' + alpha * w2(swiglu(w1(LN2(x')))), then the
