@@ -298,7 +298,7 @@ def run(state):
         cache, at = state["cache"], (state["cu"], state["lens"], state["table"])
         if kind == "write":
             cache.append(state["k"], state["v"], *at)
-            return cache.read(*at)
+            return cache.read(*at, rows=state["k"].shape[0])
         return cache.attend(state["q"], *at, causal=case["causal"])
     if kind in ("norm", "norm8"):
         s, h = _add_norm(state, case)
