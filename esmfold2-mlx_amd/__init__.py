@@ -10,6 +10,7 @@ Modules:
   f8               -- F8Linear: weights in e4m3 with a scale per 128 x 128 block, on the fp8 matrix cores
   linear           -- Linear16: weights in 16 bits, with bias, activation or gate and residual at its end
   norm             -- AddNorm: the residual's addition and the norm of the sum, in 16 bits or in e4m3 for F8Linear
+  cache4           -- Cache4: keys and values in 4 bits, in pages, and the attention on them
   esmc             -- EsmcBlock and HipEsmc: the ESMC language model around the 8-bit linear
   rotary           -- Rotary: rotary positions (layouts, part of a head, long contexts) with the norm of q and k
   trunk            -- PairTransition, TrunkBlock and PairTrunk (the FoldingTrunk drop-in)
@@ -27,7 +28,7 @@ Modules:
 
 from . import build, capi  # noqa: F401
 
-__all__ = ["build", "capi", "kernels", "trimul", "q8", "f8", "linear", "norm", "esmc", "rotary", "trunk", "recycle", "scratch", "var_hip_trimul",
+__all__ = ["build", "capi", "kernels", "trimul", "q8", "f8", "linear", "norm", "cache4", "esmc", "rotary", "trunk", "recycle", "scratch", "var_hip_trimul",
            "var_hip_trunk", "var_6b_hip_trunks", "var_6b_hip_loop", "var_6b_hip_adaptive", "var_hip_adaptive_loops",
            "variants", "workloads"]
 

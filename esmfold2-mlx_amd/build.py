@@ -29,7 +29,7 @@ BIND_PATH = os.path.join(HERE, BIND_NAME + ".so")
 BIND_SOURCE = "bind.cpp"
 SOURCES = ["project.hip", "contract.hip", "epilogue.hip", "q8.hip", "transition.hip", "esmc.hip",
            "recycle.hip", "wide.hip", "stream.hip", "rope.hip", "packed.hip",
-           "f8.hip", "norm.hip", "linear.hip", "capi.cpp"]
+           "f8.hip", "norm.hip", "linear.hip", "cache4.hip", "capi.cpp"]
 HEADERS = ["common.h", "kernels.h", "linear.h", os.path.join("..", "..", "include", "esmfold2_amd.h")]
 ARCH = "gfx950"
 

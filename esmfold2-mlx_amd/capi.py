@@ -73,6 +73,11 @@ SIGNATURES = {
     "linear16": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
     "f8_linear_end_workspace_bytes": (_sz, [_int] * 5),
     "f8_linear_end": (_int, [_vp, _i64] + [_vp] * 6 + [_i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
+    "cache4_bytes": (_sz, [_int] * 3),
+    "cache4_append": (_int, [_vp, _vp] + [_i64] * 4 + [_vp] * 4 + [_int] * 7 + [_vp]),
+    "cache4_read": (_int, [_vp] * 6 + [_int] * 7 + [_vp]),
+    "cache4_attention_workspace_bytes": (_sz, [_int] * 6),
+    "cache4_attention": (_int, [_vp, _vp] + [_i64] * 4 + [_vp] * 4 + [_int] * 8 + [_f32, _int, _vp, _sz, _vp]),
     "esmc_block_workspace_bytes": (_sz, [_int, _int, _int]),
     "esmc_block": (_int, [_vp] * 17 + [_f32, _f32, _f32, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _sz, _vp]),
     "parcae_step": (_int, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _int, _int, _int, _vp]),

@@ -1,0 +1,708 @@
+// Keys and values in 4 bits, in pages of 64 keys, and the attention that reads them.
+//
+// x ~ s (c - z) per key (or value) and group of 64 values of a head: s the least bf16 value, 2^-96 or more, of which 15 reach
+// over the group's range and 120 to its farthest value from zero; z = rint(-min / s), c = clamp(rint(x / s) + z, 0, 15). A
+// group that holds a NaN or an infinity reads as NaN (s is).
+//
+// The matrix cores take codes as they are: in bf16 0x4180 | c << 3 is 16 + c, in fp16 0x4c00 | c << 6, one instruction for
+// two codes and a shift. Products with 16 + c and with -(16 + z) cancel in fp32, and s multiplies what comes out (keys) or the
+// probability that goes in (values):
+//   S^T[key][row] = sum_g s_kg (sum_d (16 + c_kd) q_d - (16 + z_kg) Q_g),  Q_g = sum_d q_d
+//   O^T[d][row]  += sum_k (16 + c_kd) P_kg - (16 + z_kg) P_kg,             P_kg = p_k s_kg, rounded
+// both by v_mfma_f32_16x16x32: a wave holds 16 rows of queries (or RT times 16), a row a lane (lane % 16) of every
+// accumulator, and takes 32 keys at a time. P is bf16 whatever the type (its range is p's times the values'); for fp16 it is
+// kept as the sum of two bf16 values, 16 bits of it. No operand passes through LDS: the cache lies in the order the matrix
+// cores take (Dp = 64 or 128, the head size filled up; a page and head's pieces behind one another):
+//   key codes   [4 blocks of 16 keys][64 lanes][Dp / 8 bytes]: lane 16 g + key % 16, dword t: dims 32 t + 8 g + {0 .. 7}, the
+//               dword's nibble i dim 2 i, nibble 4 + i dim 2 i + 1
+//   key steps   [4 blocks][Dp / 64 groups][16 keys] words s << 16 | 16 + z (in the type's own 16 bits)
+//   value codes [2 blocks of 32 keys][Dp / 64][64 lanes][16 bytes]: lane 16 g + dim % 16; a byte is one key's dims 32 p +
+//               lane % 16 (low) and 16 more (high), 8 bytes a pair p; key 16 b + 4 g + e of the block is slot 4 b + e, whose
+//               byte is {0, 2, 1, 3}[slot % 4] of the dword
+//   value steps [2 blocks][groups][32 slots] s (bf16), then the same of -(16 + z) (bf16), slot 8 g + 4 b + e
+#include <type_traits>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace esm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+
+// Bytes of a page and head, and of its parts.
+template <int HD>
+struct Page {
+  static constexpr int kGroups = HD / 64;
+  static constexpr int kKeyCodes = 64 * HD / 2, kKeySteps = 64 * kGroups * 4;
+  static constexpr int kValCodes = kKeyCodes, kValSteps = kKeySteps;
+  static constexpr int kKeyStepsAt = kKeyCodes, kValCodesAt = kKeyStepsAt + kKeySteps, kValStepsAt = kValCodesAt + kValCodes;
+  static constexpr int kBytes = kValStepsAt + kValSteps;
+};
+static_assert(Page<64>::kBytes == cache4_page_bytes(64) && Page<128>::kBytes == cache4_page_bytes(128), "a page's size");
+
+DEV uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint32_t, v) >> 16; }  // (of values that bf16 holds)
+
+// ---- writing ------------------------------------------------------------------------------------
+// Step and zero of a group from its least and largest value and a NaN's presence: s = NaN then.
+DEV void four_bit_step(float lo, float hi, bool bad, float& s, float& z) {
+  const float far = fmaxf(fabsf(lo), fabsf(hi)), range = hi - lo;
+  s = fmaxf(fmaxf(range / 15.f, far / 120.f), 0x1p-96f);
+  uint32_t b = __builtin_bit_cast(uint32_t, s) & 0xffff0000u;
+  const float t = __builtin_bit_cast(float, b);
+  if (15.f * t < range || 120.f * t < far) b += 0x10000u;
+  s = __builtin_bit_cast(float, b);
+  z = rintf(-lo / s);
+  if (bad) s = __builtin_bit_cast(float, 0x7fc00000u), z = 0.f;
+}
+
+// The row's place in the cache: sequence, its page and the slot in it; false where there is none.
+struct Slot {
+  int page, key;
+};
+DEV bool find_slot(const Cache4Args& p, int row, int lane, Slot& s) {
+  for (int i0 = 0; i0 < p.n; i0 += 64) {
+    const int i = min(i0 + lane, p.n - 1);
+    const int a = min(max(p.cu[i], 0), p.T), b = min(max(p.cu[i + 1], a), p.T);
+    const uint64_t hit = __ballot(row >= a && row < b);
+    if (!hit) continue;
+    const int w = __builtin_ctzll(hit), seq = i0 + w;
+    const long long pos = (long long)p.lens[seq] - __builtin_amdgcn_readlane(b, w) + row;
+    if (pos < 0 || pos >= (long long)p.width * kCache4Page) return false;
+    s.page = p.table[(size_t)seq * p.width + (pos >> 6)];
+    s.key = (int)(pos & 63);
+    return s.page >= 0 && s.page < p.pages;
+  }
+  return false;
+}
+
+// A wave takes a row's keys or values of a head: 8 lanes a group of 64 values, a lane 8 of them.
+template <class V8, int HD>
+__global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
+  typedef Page<HD> P;
+  constexpr int kLanes = HD / 8, kPer = 64 / kLanes;  // lanes of a head, heads of a wave
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x;
+  Slot at;
+  if (!find_slot(p, row, lane, at)) return;
+  const int c = lane % kLanes, item = (blockIdx.y * 4 + wave) * kPer + lane / kLanes;  // keys' heads, then values'
+  const bool val = item >= p.Hk, live = item < 2 * p.Hk;
+  const int h = live ? item - (val ? p.Hk : 0) : 0;
+  V8 x{};
+  const bool in = live && 8 * c < p.d;
+  if (in) x = *reinterpret_cast<const V8*>((const uint16_t*)(val ? p.v : p.k) + (long long)row * (val ? p.v_st : p.k_st) +
+                                           (long long)h * (val ? p.v_sh : p.k_sh) + 8 * c);
+  float v[8], lo = INFINITY, hi = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    v[e] = (float)x[e];
+    bad = bad || !(fabsf(v[e]) < INFINITY);
+    lo = fminf(lo, v[e]);
+    hi = fmaxf(hi, v[e]);
+  }
+  if (!in) lo = INFINITY, hi = -INFINITY;
+  const auto over = [&](auto ctrl) {
+    const float a = dpp_f32<decltype(ctrl)::value>(lo), b = dpp_f32<decltype(ctrl)::value>(hi);
+    const int n = __builtin_amdgcn_update_dpp(0, (int)bad, decltype(ctrl)::value, 0xf, 0xf, false);
+    lo = fminf(lo, a), hi = fmaxf(hi, b), bad = bad || n;
+  };
+  over(std::integral_constant<int, 0xB1>{});   // quad_perm(1, 0, 3, 2)
+  over(std::integral_constant<int, 0x4E>{});   // quad_perm(2, 3, 0, 1)
+  over(std::integral_constant<int, 0x141>{});  // row_half_mirror: 8 lanes, a group
+  if (!live) return;
+  float s, z;
+  if (lo > hi) lo = hi = 0.f;  // (a group past the head's values)
+  four_bit_step(lo, hi, bad, s, z);
+  uint32_t code[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) code[e] = bad || !in ? 0 : (uint32_t)fminf(fmaxf(rintf(v[e] / s) + z, 0.f), 15.f);
+  char* page = (char*)p.data + ((size_t)at.page * p.Hk + h) * P::kBytes;
+  const int g = c >> 3;  // group
+  if (!val) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w |= code[e] << (4 * (e >> 1) + 16 * (e & 1));
+    const int blk = at.key >> 4, ln = 16 * (c & 3) + (at.key & 15), t = c >> 2;  // dims 8 c = 32 t + 8 (c % 4)
+    *reinterpret_cast<uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t) = w;
+    if ((c & 7) == 0) {
+      const uint32_t zb = std::is_same<V8, bf16x8>::value ? bf16_bits(16.f + z)
+                                                          : (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(16.f + z));
+      *reinterpret_cast<uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (at.key & 15)) * 4) =
+          (__builtin_bit_cast(uint32_t, s) & 0xffff0000u) | zb;
+    }
+  } else {
+    // dims 8 c ..: half (c / 2) % 2 of the 32 of pair p = c / 4 -- a lane holds low nibbles (c / 2 even) or high ones
+    uint32_t mine[2] = {0, 0}, theirs[2];
+#pragma unroll
+    for (int e = 0; e < 8; e++) mine[e >> 2] |= code[e] << (8 * (e & 3));
+    // the lane two further holds the high nibbles of this one's bytes
+    theirs[0] = __shfl_down(mine[0], 2);
+    theirs[1] = __shfl_down(mine[1], 2);
+    const int blk = at.key >> 5, k = at.key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
+    if (((c >> 1) & 1) == 0) {
+      const int pair = c >> 2, byte = (slot & 4) + ((0x3120 >> (4 * (slot & 3))) & 3);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int dim = 8 * (c & 1) + e;  // of the pair's low 16
+        page[P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + byte] =
+            (uint8_t)(((mine[e >> 2] >> (8 * (e & 3))) & 15) | (((theirs[e >> 2] >> (8 * (e & 3))) & 15) << 4));
+      }
+    }
+    if ((c & 7) == 0) {
+      uint16_t* st = reinterpret_cast<uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
+      st[0] = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
+      st[2 * P::kGroups * 32] = (uint16_t)bf16_bits(-(16.f + z));
+    }
+  }
+}
+
+// What a row's place holds, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
+template <class V8, int HD>
+__global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Args p) {
+  typedef Page<HD> P;
+  constexpr int kLanes = HD / 8, kPer = 64 / kLanes;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x;
+  Slot at{0, 0};
+  const bool there = find_slot(p, row, lane, at);
+  const int c = lane % kLanes, item = (blockIdx.y * 4 + wave) * kPer + lane / kLanes;
+  const bool val = item >= p.Hk;
+  if (item >= 2 * p.Hk || 8 * c >= p.d) return;
+  const int h = item - (val ? p.Hk : 0), g = c >> 3;
+  V8* dst = reinterpret_cast<V8*>((uint16_t*)(val ? p.vo : p.ko) + ((size_t)row * p.Hk + h) * p.d + 8 * c);
+  if (!there) {
+    *dst = V8{};
+    return;
+  }
+  const char* page = (const char*)p.data + ((size_t)at.page * p.Hk + h) * P::kBytes;
+  float s, z;
+  uint32_t code[8];
+  if (!val) {
+    const int blk = at.key >> 4, ln = 16 * (c & 3) + (at.key & 15), t = c >> 2;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t);
+#pragma unroll
+    for (int e = 0; e < 8; e++) code[e] = (w >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
+    const uint32_t st = *reinterpret_cast<const uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (at.key & 15)) * 4);
+    s = __builtin_bit_cast(float, st & 0xffff0000u);
+    z = std::is_same<V8, bf16x8>::value ? __builtin_bit_cast(float, st << 16) - 16.f
+                                        : (float)__builtin_bit_cast(half_t, (uint16_t)st) - 16.f;
+  } else {
+    const int blk = at.key >> 5, k = at.key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
+    const int pair = c >> 2, byte = (slot & 4) + ((0x3120 >> (4 * (slot & 3))) & 3);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int dim = 8 * (c & 1) + e;
+      const uint8_t b = page[P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + byte];
+      code[e] = (b >> (2 * (c & 2))) & 15;
+    }
+    const uint16_t* st = reinterpret_cast<const uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
+    s = __builtin_bit_cast(float, (uint32_t)st[0] << 16);
+    z = -__builtin_bit_cast(float, (uint32_t)st[2 * P::kGroups * 32] << 16) - 16.f;
+  }
+  V8 y;
+#pragma unroll
+  for (int e = 0; e < 8; e++) y[e] = (decltype(+y[e]))(s * ((float)code[e] - z));
+  *dst = y;
+}
+
+// ---- attention --------------------------------------------------------------------------------------
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+struct F16Keys {
+  typedef half8 v8;
+  typedef half4 v4;
+  typedef half_t elem;
+  static constexpr uint32_t kMask = 0x03c003c0u, kMagic = 0x4c004c00u;
+  static constexpr int kUp = 6;      // a code's place in the 16 bits
+  static constexpr bool kSplit = true;
+  static DEV f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static DEV float zero_of(uint32_t w) { return (float)__builtin_bit_cast(half_t, (uint16_t)w); }
+};
+struct B16Keys {
+  typedef bf16x8 v8;
+  typedef bf16x4 v4;
+  typedef __bf16 elem;
+  static constexpr uint32_t kMask = 0x00780078u, kMagic = 0x41804180u;
+  static constexpr int kUp = 3;
+  static constexpr bool kSplit = false;
+  static DEV f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static DEV float zero_of(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+};
+DEV f32x4 mfma_b16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// The two codes at bits AT of each half of w, as 16 + c in 16 bits.
+template <int AT, int UP, uint32_t MASK, uint32_t MAGIC>
+DEV uint32_t two_codes(uint32_t w) {
+  return ((AT > UP ? w >> (AT > UP ? AT - UP : 0) : w << (UP > AT ? UP - AT : 0)) & MASK) | MAGIC;
+}
+template <class T>
+DEV typename T::v8 key_codes(uint32_t w) {
+  return __builtin_bit_cast(typename T::v8,
+                            u32x4{two_codes<0, T::kUp, T::kMask, T::kMagic>(w), two_codes<4, T::kUp, T::kMask, T::kMagic>(w),
+                                  two_codes<8, T::kUp, T::kMask, T::kMagic>(w), two_codes<12, T::kUp, T::kMask, T::kMagic>(w)});
+}
+template <bool HIGH>
+DEV bf16x8 value_codes(uint32_t a, uint32_t b) {  // slots 0 .. 3 and 4 .. 7 of the pair's low or high dims
+  constexpr uint32_t M = B16Keys::kMask, G = B16Keys::kMagic;
+  constexpr int A = HIGH ? 4 : 0;
+  return __builtin_bit_cast(bf16x8, u32x4{two_codes<A, 3, M, G>(a), two_codes<A + 8, 3, M, G>(a), two_codes<A, 3, M, G>(b),
+                                          two_codes<A + 8, 3, M, G>(b)});
+}
+
+// Largest and sum over the four lanes that hold a row (those of one lane % 16).
+DEV float row_max4(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+DEV float row_sum4(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// A work item is a (sequence, tile of 16 RT rows, chunk of keys) of one key head; chunks are as many whole passes of 256 keys
+// as spread all sequences' keys over p.target workgroups of a head. Each workgroup, and the join, finds the same from the
+// lengths on the device, so that lengths may change between two replays of one graph.
+constexpr int kPass = 4 * kCache4Page;  // keys of a workgroup's pass, a page a wave
+struct Item {
+  int seq, q0, nq, nk, tile, chunk, chunks, keys, slot;  // keys: of a chunk; slot: where its partials go
+};
+template <bool BY_ROW>  // what: the item's number, or a row of q (then tile, chunk and slot are the caller's to find)
+DEV bool find_item4(const Cache4Args& p, int rows, int what, int lane, Item& it) {
+  const int most = p.width * kCache4Page;
+  const auto spans = [&](int i0, int& a, int& nq, int& nk, int& tiles) {
+    const int i = min(i0 + lane, p.n - 1);
+    a = min(max(p.cu[i], 0), p.T);
+    nq = min(max(p.cu[i + 1], a), p.T) - a;
+    nk = min(max(p.lens[i], 0), most);
+    tiles = i0 + lane < p.n ? (nq * p.G + rows - 1) / rows : 0;
+  };
+  int a, nq, nk, tiles;
+  it.keys = 1 << 30;
+  spans(0, a, nq, nk, tiles);
+  if (p.divide) {
+    float passes = 0.f;  // (whole numbers below 2^24, or so many that a few do not count)
+    for (int i0 = 0;;) {
+      passes += wave_total((float)tiles * (float)((nk + kPass - 1) / kPass));
+      if ((i0 += 64) >= p.n) break;
+      spans(i0, a, nq, nk, tiles);
+    }
+    // (at least a 256th of the longest there may be: kCache4MaxChunks)
+    it.keys = kPass * max(max(1, (int)ceilf(passes / (float)p.target)), (most + kPass * kCache4MaxChunks - 1) / (kPass * kCache4MaxChunks));
+    if (p.n > 64) spans(0, a, nq, nk, tiles);
+  }
+  int before = 0;
+  for (int i0 = 0;;) {
+    const int chunks = max(1, (nk + it.keys - 1) / it.keys), items = tiles * chunks, sum = wave_scan(items);
+    const uint64_t hit = __ballot(BY_ROW ? i0 + lane < p.n && what >= a && what < a + nq : what < before + sum);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, w); };
+      it.seq = i0 + w, it.q0 = of(a), it.nq = of(nq), it.nk = of(nk), it.chunks = of(chunks);
+      it.slot = before + of(sum - items);
+      if (!BY_ROW) {
+        const int at = what - it.slot;
+        it.tile = at / it.chunks, it.chunk = at - it.tile * it.chunks;
+        it.slot = what;
+        return at >= 0 && it.tile < of(tiles);  // (starts that do not ascend: nothing outside)
+      }
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    if ((i0 += 64) >= p.n) return false;
+    spans(i0, a, nq, nk, tiles);
+  }
+}
+
+constexpr float kFar4 = 1024.f;   // least exponent of a row's maximum that its scores are made relative to
+constexpr float kGrow4 = 8.f;     // log2: what p may reach before its row is rescaled
+
+template <class T, int HD, int RT>
+struct Rows4 {
+  typedef typename T::v8 v8;
+  static constexpr int G = HD / 64;
+  v8 q[RT][HD / 32];
+  float qs[RT][G];       // sums of a group's query values
+  f32x4 o[RT][HD / 16];  // lane: row lane % 16, dims 16 i + 4 (lane / 16) + e
+  float m[RT], l[RT];    // running maximum of the unscaled scores, this lane's part of the sum
+  int lim[RT];           // last key the row sees
+
+  // 32 keys' operands of this lane.
+  struct Keys {
+    uint32_t kc[2][HD / 32], vc[HD / 16];
+    u32x4 ks[2][G], vs[G], vz[G];
+  };
+  static DEV void load_keys(Keys& k, const char* page, int half, int lane) {
+    typedef Page<HD> P;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const char* src = page + ((2 * half + b) * 64 + lane) * (HD / 8);
+      if constexpr (HD == 128) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+        for (int t = 0; t < 4; t++) k.kc[b][t] = v[t];
+      } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(src);
+        k.kc[b][0] = v[0], k.kc[b][1] = v[1];
+      }
+#pragma unroll
+      for (int i = 0; i < G; i++)
+        k.ks[b][i] = *reinterpret_cast<const u32x4*>(page + P::kKeyStepsAt + (((2 * half + b) * G + i) * 16 + 4 * g) * 4);
+    }
+  }
+  static DEV void load_values(Keys& k, const char* page, int half, int lane) {
+    typedef Page<HD> P;
+    const int g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(page + P::kValCodesAt + ((half * G + i) * 64 + lane) * 16);
+#pragma unroll
+      for (int t = 0; t < 4; t++) k.vc[4 * i + t] = v[t];
+      const char* st = page + P::kValStepsAt + (half * G + i) * 64 + 16 * g;
+      k.vs[i] = *reinterpret_cast<const u32x4*>(st);
+      k.vz[i] = *reinterpret_cast<const u32x4*>(st + 128 * G);
+    }
+  }
+
+  DEV void grow(int r, float mx, float c) {
+    const float mn = fmaxf(m[r], mx), ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f((m[r] - ref) * c);
+    m[r] = mn;
+    l[r] *= alpha;
+#pragma unroll
+    for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[r][i][e] *= alpha;
+  }
+
+  // The 32 keys from key0 of the sequence on; MASKED: some row may not see some of them. Unseen keys may hold anything. The
+  // registers of keys, then of values, take the next 32 keys' (`next`, `half`) as soon as they have been read.
+  template <bool MASKED>
+  DEV void step(Keys& k, int key0, float c, int lane, const char* next, int half) {
+    const int g = lane >> 4;
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      if (b) __builtin_amdgcn_sched_barrier(0);
+      f32x4 acc[RT][G];
+#pragma unroll
+      for (int t = 0; t < HD / 32; t++) {
+        const v8 kc = key_codes<T>(k.kc[b][t]);
+#pragma unroll
+        for (int r = 0; r < RT; r++) acc[r][t >> 1] = T::mfma(kc, q[r][t], t & 1 ? acc[r][t >> 1] : f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+#pragma unroll
+      for (int r = 0; r < RT; r++) s[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < G; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t w = k.ks[b][i][e];
+          const float st = __builtin_bit_cast(float, w & 0xffff0000u), z = T::zero_of(w);
+#pragma unroll
+          for (int r = 0; r < RT; r++) s[r][b][e] = fmaf(st, fmaf(-z, qs[r][i], acc[r][i][e]), s[r][b][e]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(k, next, half, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    if (MASKED) {
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          s[r][j >> 2][j & 3] = key0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim[r] ? s[r][j >> 2][j & 3] : -INFINITY;
+    }
+    float p[RT][8];
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, s[r][j >> 2][j & 3]);
+      if (__any((mx - m[r]) * c > kGrow4)) grow(r, row_max4(mx), c);
+      const float mc = m[r] * c;
+      const bool far = !(fabsf(mc) < kFar4);
+      float ref = 0.f, base = mc;
+      if (__any(far)) {  // (see packed.hip: large exponents, and rows that have seen nothing)
+        ref = far && m[r] != -INFINITY ? m[r] : 0.f;
+        base = far ? 0.f : mc;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3] - ref, c, -base));
+        sum += p[r][j];
+      }
+      l[r] += sum;
+    }
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8 hi[RT], lo[RT];
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const uint32_t w = k.vs[i][j >> 1];
+          const float st = __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16);
+          float v = p[r][j] * st;
+          if (MASKED) v = key0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim[r] ? v : 0.f;
+          hi[r][j] = (__bf16)v;
+          if (T::kSplit) lo[r][j] = (__bf16)(v - (float)hi[r][j]);
+        }
+      const bf16x8 z = __builtin_bit_cast(bf16x8, k.vz[i]);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const uint32_t a = k.vc[4 * i + 2 * (u >> 1)], b = k.vc[4 * i + 2 * (u >> 1) + 1];
+        const bf16x8 v = u & 1 ? value_codes<true>(a, b) : value_codes<false>(a, b);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          f32x4& acc = o[r][4 * i + u];
+          acc = mfma_b16(v, hi[r], acc);
+          acc = mfma_b16(z, hi[r], acc);
+          if (T::kSplit) {
+            acc = mfma_b16(v, lo[r], acc);
+            acc = mfma_b16(z, lo[r], acc);
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(k, next, half, lane);
+  }
+};
+
+// A workgroup takes 16 RT rows (query, head of the group; row = query G + head) of a sequence and key head and one chunk of
+// its keys, a page a wave in turn, the next 32 keys' operands in flight; the waves' results are joined through LDS.
+template <class T, int HD, int RT>
+__global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void cache4_attention_kernel(Cache4Args p) {
+  typedef Page<HD> P;
+  typedef Rows4<T, HD, RT> R;
+  constexpr int kRows = 16 * RT;
+  __shared__ __align__(16) f32x4 lds[4][RT][HD / 16][64];
+  __shared__ float ml[4][2][kRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x % p.Hk;
+  Item it;
+  if (!find_item4<false>(p, kRows, blockIdx.x / p.Hk, lane, it)) return;
+  const int rows = it.nq * p.G, row0 = kRows * it.tile;
+  R w;
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const int row = row0 + 16 * r + (lane & 15), i = row / p.G, h = row - i * p.G;
+    const bool ok = row < rows;
+    const char* src = (const char*)p.q + 2 * ((long long)(it.q0 + (ok ? i : 0)) * p.q_st + (long long)(hk * p.G + h) * p.q_sh);
+#pragma unroll
+    for (int t = 0; t < HD / 32; t++) {
+      const int c = 32 * t + 8 * (lane >> 4);
+      w.q[r][t] = typename T::v8{};
+      if (ok && c < p.d) w.q[r][t] = *reinterpret_cast<const typename T::v8*>(src + 2 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < R::G; u++) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) t += (float)w.q[r][2 * u + j][e];
+      w.qs[r][u] = row_sum4(t);
+    }
+    w.m[r] = -INFINITY;
+    w.l[r] = 0.f;
+    w.lim[r] = p.causal && ok ? min(it.nk - 1, i + it.nk - it.nq) : it.nk - 1;
+#pragma unroll
+    for (int u = 0; u < HD / 16; u++) w.o[r][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // keys seen by the tile's first row and by its last
+  const auto seen = [&](int row) { return p.causal ? max(min(it.nk, min(row, rows - 1) / p.G + it.nk - it.nq + 1), 0) : it.nk; };
+  const int whole = seen(row0), first = it.chunk * it.keys, last = min(seen(row0 + kRows - 1), min(first + min(it.keys, it.nk), it.nk));
+  const int page0 = first / kCache4Page + wave, pages = (last + kCache4Page - 1) / kCache4Page;  // of this chunk, this wave's first
+  const int* table = p.table + (size_t)it.seq * p.width;
+  const char* base = (const char*)p.data + (size_t)hk * P::kBytes;
+  // this wave's pages of 64 turns, one a lane
+  int ids = -1;
+  const auto page_of = [&](int turn) {
+    if ((turn & 63) == 0) {
+      const int i = page0 + 4 * (turn + lane);
+      ids = i < pages ? table[i] : -1;
+    }
+    return __builtin_amdgcn_readlane(ids, turn & 63);
+  };
+  const auto at = [&](int id) { return base + (size_t)(id >= 0 && id < p.pages ? id : 0) * p.Hk * P::kBytes; };
+  if (page0 < pages) {
+    typename R::Keys k;
+    int id = page_of(0);
+    const char* page = at(id);
+    R::load_keys(k, page, 0, lane);
+    R::load_values(k, page, 0, lane);
+    bool good = id >= 0 && id < p.pages;  // (a page of no cache: not seen)
+    for (int u = 0, pg = page0; pg < pages; u++) {  // halves of pages
+      const int half = u & 1, key0 = kCache4Page * pg + 32 * half;
+      const bool seen = good;
+      if (half) {
+        pg += 4;
+        id = pg < pages ? page_of((u + 1) >> 1) : id;  // (behind the last page: that one again, not used)
+        page = at(id);
+        good = id >= 0 && id < p.pages;
+      }
+      if (seen && key0 + 32 <= whole) {
+        w.template step<false>(k, key0, p.scale_log2, lane, page, half ^ 1);
+      } else if (seen) {
+        w.template step<true>(k, key0, p.scale_log2, lane, page, half ^ 1);
+      } else {
+        R::load_keys(k, page, half ^ 1, lane);
+        R::load_values(k, page, half ^ 1, lane);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; r++) {
+    const float l = row_sum4(w.l[r]);
+    if (lane < 16) ml[wave][0][16 * r + lane] = w.m[r], ml[wave][1][16 * r + lane] = l;
+#pragma unroll
+    for (int u = 0; u < HD / 16; u++) lds[wave][r][u][lane] = w.o[r][u];
+  }
+  __syncthreads();
+  const bool part = it.chunks > 1;
+  const size_t slot = (size_t)it.slot * p.Hk + hk;
+#pragma unroll 1
+  for (int u = wave; u < RT * (HD / 16); u += 4) {  // 16 rows x 16 dims
+    const int r = u / (HD / 16), db = u - r * (HD / 16), rr = 16 * r + (lane & 15), row = row0 + rr;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 4; v++) M = fmaxf(M, ml[v][0][rr]);
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+      const float sc = __builtin_amdgcn_exp2f((ml[v][0][rr] - ref) * p.scale_log2);
+      L = fmaf(sc, ml[v][1][rr], L);
+      const f32x4 x = lds[v][r][db][lane];
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[e] = fmaf(sc, x[e], acc[e]);
+    }
+    if (row >= rows) continue;
+    const int col = 16 * db + 4 * (lane >> 4), i = row / p.G, h = row - i * p.G;
+    if (part) {
+      if (db == 0 && lane < 16) {
+        p.part_ml[2 * (slot * kRows + rr)] = M;
+        p.part_ml[2 * (slot * kRows + rr) + 1] = L;
+      }
+      *reinterpret_cast<f32x4*>(p.part_o + (slot * kRows + rr) * HD + col) = acc;
+    } else if (col < p.d) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      typename T::v4 y;
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = (typename T::elem)(acc[e] * inv);
+      *reinterpret_cast<typename T::v4*>((char*)p.o + 2 * ((long long)(it.q0 + i) * p.o_st + (long long)(hk * p.G + h) * p.o_sh + col)) = y;
+    }
+  }
+}
+
+// The chunks of one (query, head) row: a thread takes one chunk's m and l, then groups of HD / 4 lanes sum O over every
+// 1024 / HD-th chunk, joined through LDS.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args p, int rows) {
+  __shared__ float weight[256], red[2][4];
+  __shared__ __align__(16) float sums[4][HD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, H = p.G * p.Hk;
+  const int q = blockIdx.x / H, head = blockIdx.x - q * H, hk = head / p.G;
+  Item it;
+  if (!find_item4<true>(p, rows, q, lane, it) || it.chunks == 1) return;
+  const int row = (q - it.q0) * p.G + head - hk * p.G, tile = row / rows, rr = row - tile * rows;
+  const size_t slot0 = (size_t)it.slot + (size_t)tile * it.chunks;
+  if (it.slot < 0 || slot0 + it.chunks > (size_t)p.items) return;  // (starts that do not ascend)
+  const auto at = [&](int j) { return ((slot0 + j) * p.Hk + hk) * rows + rr; };
+  const bool live = t < it.chunks;  // (kCache4MaxChunks of them at most)
+  const float m = live ? p.part_ml[2 * at(t)] : -INFINITY, l = live ? p.part_ml[2 * at(t) + 1] : 0.f;
+  float M = m;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+  if (lane == 0) red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float sc = __builtin_amdgcn_exp2f((m - (M == -INFINITY ? 0.f : M)) * p.scale_log2);
+  weight[t] = live ? sc : 0.f;
+  const float L4 = wave_total(live ? sc * l : 0.f);
+  if (lane == 0) red[1][wave] = L4;
+  __syncthreads();
+  const float L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  constexpr int kCols = HD / 4, kSide = 256 / kCols;
+  const int col = 4 * (t % kCols), side = t / kCols;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int j = side; j < it.chunks; j += kSide) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at(j) * HD + col);
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] = fmaf(weight[j], x[e], acc[e]);
+  }
+#pragma unroll
+  for (int o = kCols; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o);
+  if (lane < kCols) *reinterpret_cast<f32x4*>(&sums[wave][col]) = acc;
+  __syncthreads();
+  if (t < kCols && col < p.d) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    typename T::v4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (typename T::elem)((sums[0][col + e] + sums[1][col + e] + sums[2][col + e] + sums[3][col + e]) * inv);
+    *reinterpret_cast<typename T::v4*>((char*)p.o + 2 * ((long long)q * p.o_st + (long long)head * p.o_sh + col)) = y;
+  }
+}
+
+// Rows of a tile by the mean rows of a sequence; keys divided unless the table holds few or the tiles alone fill the GPU
+// many times over.
+Cache4Plan cache4_plan(long long T, int n, int width, int Hk, int G, int cus) {
+  Cache4Plan plan{};
+  const long long per = T * G / n;
+  plan.rt = per <= 16 ? 1 : per <= 32 ? 2 : 4;
+  const long long tiles = T * G / (16 * plan.rt) + n;
+  plan.divide = width > 2 * kPass / kCache4Page && tiles * Hk < 64LL * cus;
+  plan.target = (int)((4LL * cus + Hk - 1) / Hk);
+  if (plan.target > kCache4MaxChunks) plan.target = kCache4MaxChunks;
+  plan.items = tiles + (plan.divide ? plan.target : 0);
+  return plan;
+}
+
+template <class T, int HD, int RT>
+static hipError_t launch_cache4_t(const Cache4Args& a, const Cache4Plan& plan, hipStream_t s) {
+  ESM_LAUNCH((cache4_attention_kernel<T, HD, RT>), dim3((unsigned)(plan.items * a.Hk)), dim3(256), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.divide) return e;
+  ESM_LAUNCH((cache4_join_kernel<T, HD>), dim3((unsigned)(a.T * a.G * a.Hk)), dim3(256), 0, s, a, 16 * RT);
+  return hipGetLastError();
+}
+template <class T, int HD>
+static hipError_t launch_cache4_hd(const Cache4Args& a, const Cache4Plan& plan, hipStream_t s) {
+  switch (plan.rt) {
+    case 1: return launch_cache4_t<T, HD, 1>(a, plan, s);
+    case 2: return launch_cache4_t<T, HD, 2>(a, plan, s);
+    default: return launch_cache4_t<T, HD, 4>(a, plan, s);
+  }
+}
+
+hipError_t launch_cache4_attention(const Cache4Args& a, bool bf16, const Cache4Plan& plan, hipStream_t s) {
+  if (bf16) return a.d <= 64 ? launch_cache4_hd<B16Keys, 64>(a, plan, s) : launch_cache4_hd<B16Keys, 128>(a, plan, s);
+  return a.d <= 64 ? launch_cache4_hd<F16Keys, 64>(a, plan, s) : launch_cache4_hd<F16Keys, 128>(a, plan, s);
+}
+
+template <class V8, int HD>
+static hipError_t launch_write_t(const Cache4Args& a, bool read, hipStream_t s) {
+  const int per = 4 * (64 / (HD / 8));  // heads of a workgroup, keys' and values'
+  const dim3 grid(a.T, (2 * a.Hk + per - 1) / per);
+  if (read) {
+    ESM_LAUNCH((cache4_read_kernel<V8, HD>), grid, dim3(256), 0, s, a);
+  } else {
+    ESM_LAUNCH((cache4_write_kernel<V8, HD>), grid, dim3(256), 0, s, a);
+  }
+  return hipGetLastError();
+}
+static hipError_t launch_rows4(const Cache4Args& a, bool bf16, bool read, hipStream_t s) {
+  if (bf16) return a.d <= 64 ? launch_write_t<bf16x8, 64>(a, read, s) : launch_write_t<bf16x8, 128>(a, read, s);
+  return a.d <= 64 ? launch_write_t<half8, 64>(a, read, s) : launch_write_t<half8, 128>(a, read, s);
+}
+hipError_t launch_cache4_write(const Cache4Args& a, bool bf16, hipStream_t s) { return launch_rows4(a, bf16, false, s); }
+hipError_t launch_cache4_read(const Cache4Args& a, bool bf16, hipStream_t s) { return launch_rows4(a, bf16, true, s); }
+
+}  // namespace esm

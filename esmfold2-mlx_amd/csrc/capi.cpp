@@ -1148,6 +1148,110 @@ int f8_linear_partials(const void* x, int64_t x_st, const uint8_t* qp, const flo
                 workspace_bytes, stream);
 }
 
+namespace {
+int workspace_fault(const char* fn, const void* ws, size_t have, size_t need) {
+  if (!need) return ESM_OK;
+  if (!ws || have < need) return fail(ESM_ERR_SHAPE, "%s: workspace of %zu bytes, %zu needed", fn, have, need);
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return fail(ESM_ERR_ALIGN, "%s: workspace must be 256-byte aligned", fn);
+  return ESM_OK;
+}
+}  // namespace
+
+// ---- keys and values in 4 bits ----------------------------------------------------------------------
+namespace {
+// What the cache's calls share: sizes, the caller's starts, lengths and table.
+int cache4_args(const char* fn, esm::Cache4Args& a, const void* data, const int* cu, const int* lens, const int* table, int n,
+                int T, int Hk, int d, int pages, int width, int dtype) {
+  if (n < 0 || T < 0 || Hk <= 0 || d <= 0 || pages < 0 || width < 0)
+    return fail(ESM_ERR_SHAPE, "%s: n=%d T=%d Hk=%d d=%d pages=%d width=%d", fn, n, T, Hk, d, pages, width);
+  if (d % 8 != 0 || d > 128) return fail(ESM_ERR_UNSUPPORTED, "%s: d=%d (a multiple of 8 up to 128)", fn, d);
+  if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "%s: dtype=%d", fn, dtype);
+  if (T >= (1 << 24) || n >= (1 << 24) || Hk > (1 << 16) || width >= (1 << 23) || (long long)T * Hk >= (1LL << 31))
+    return fail(ESM_ERR_SHAPE, "%s: n=%d T=%d Hk=%d width=%d too large", fn, n, T, Hk, width);
+  if (n == 0 || T == 0) return ESM_OK;
+  if (!cu || !lens || (width > 0 && !table) || (pages > 0 && !data)) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
+  if (!aligned16(data)) return fail(ESM_ERR_ALIGN, "%s: the cache must be 16-byte aligned", fn);
+  if ((reinterpret_cast<uintptr_t>(cu) | reinterpret_cast<uintptr_t>(lens) | reinterpret_cast<uintptr_t>(table)) & 3u)
+    return fail(ESM_ERR_ALIGN, "%s: misaligned starts, lengths or table", fn);
+  a.data = const_cast<void*>(data);
+  a.cu = cu, a.lens = lens, a.table = table;
+  a.n = n, a.T = T, a.Hk = Hk, a.d = d, a.pages = pages, a.width = pages > 0 ? width : 0;  // (no page: no key anywhere)
+  return ESM_OK;
+}
+bool attn4_shape(int n, int T, int width, int H, int Hk, int d) {
+  return n > 0 && T > 0 && width >= 0 && width < (1 << 23) && Hk > 0 && H > 0 && H % Hk == 0 && d > 0 && d <= 128;
+}
+size_t attn4_ml_bytes(const esm::Cache4Plan& plan, int Hk) { return (size_t)plan.items * Hk * 16 * plan.rt * 8; }
+}  // namespace
+
+size_t cache4_bytes(int pages, int Hk, int d) {
+  return pages > 0 && Hk > 0 && d > 0 && d <= 128 ? (size_t)pages * Hk * esm::cache4_page_bytes(d <= 64 ? 64 : 128) : 0;
+}
+
+int cache4_append(const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, void* data,
+                  const int* cu, const int* lens, const int* table, int n, int T, int Hk, int d, int pages, int width,
+                  int dtype, void* stream) {
+  esm::Cache4Args a{};
+  const int rc = cache4_args("cache4_append", a, data, cu, lens, table, n, T, Hk, d, pages, width, dtype);
+  if (rc != ESM_OK) return rc;
+  for (const char* why : {strides_fault(k_st, k_sh, T, d), strides_fault(v_st, v_sh, T, d)})
+    if (why) return fail(ESM_ERR_ALIGN, "cache4_append: %s", why);
+  if (n == 0 || T == 0) return ok();
+  if (!k || !v) return fail(ESM_ERR_NULL, "cache4_append: NULL pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(ESM_ERR_ALIGN, "cache4_append: k and v must be 16-byte aligned");
+  a.k = k, a.v = v, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  return hip_status(esm::launch_cache4_write(a, dtype == ESM_BF16, (hipStream_t)stream), "cache4_append launch");
+}
+
+int cache4_read(void* k, void* v, const void* data, const int* cu, const int* lens, const int* table, int n, int T, int Hk, int d,
+                int pages, int width, int dtype, void* stream) {
+  esm::Cache4Args a{};
+  const int rc = cache4_args("cache4_read", a, data, cu, lens, table, n, T, Hk, d, pages, width, dtype);
+  if (rc != ESM_OK) return rc;
+  if (n == 0 || T == 0) return ok();
+  if (!k || !v) return fail(ESM_ERR_NULL, "cache4_read: NULL pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(ESM_ERR_ALIGN, "cache4_read: k and v must be 16-byte aligned");
+  a.ko = k, a.vo = v;
+  return hip_status(esm::launch_cache4_read(a, dtype == ESM_BF16, (hipStream_t)stream), "cache4_read launch");
+}
+
+size_t cache4_attention_workspace_bytes(int n, int T, int width, int H, int Hk, int d) {
+  if (!attn4_shape(n, T, width, H, Hk, d)) return 0;
+  const esm::Cache4Plan plan = esm::cache4_plan(T, n, width, Hk, H / Hk, cu_count());
+  return plan.divide ? attn4_ml_bytes(plan, Hk) + (size_t)plan.items * Hk * 16 * plan.rt * (d <= 64 ? 64 : 128) * 4 : 0;
+}
+
+int cache4_attention(const void* q, void* o, int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh, const void* data,
+                     const int* cu, const int* lens, const int* table, int n, int T, int H, int Hk, int d, int pages, int width,
+                     int causal, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "cache4_attention";
+  if (H <= 0 || Hk <= 0 || H % Hk != 0) return fail(ESM_ERR_SHAPE, "%s: H=%d Hk=%d", fn, H, Hk);
+  esm::Cache4Args a{};
+  const int rc = cache4_args(fn, a, data, cu, lens, table, n, T, Hk, d, pages, width, dtype);
+  if (rc != ESM_OK) return rc;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || std::isinf(scale_log2)) return fail(ESM_ERR_SHAPE, "%s: scale must be positive and below 2^127", fn);
+  for (const char* why : {strides_fault(q_st, q_sh, T, d), strides_fault(o_st, o_sh, T, d)})
+    if (why) return fail(ESM_ERR_ALIGN, "%s: %s", fn, why);
+  if (n == 0 || T == 0) return ok();
+  const esm::Cache4Plan plan = esm::cache4_plan(T, n, width, Hk, H / Hk, cu_count());
+  // grids of 256 threads stay below 2^32 threads
+  if (plan.items * Hk >= (1LL << 24) || (long long)T * H >= (plan.divide ? 1LL << 24 : 1LL << 31))
+    return fail(ESM_ERR_SHAPE, "%s: n=%d T=%d H=%d too large", fn, n, T, H);
+  if (!q || !o) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
+  if (!aligned16(q) || !aligned16(o)) return fail(ESM_ERR_ALIGN, "%s: q and o must be 16-byte aligned", fn);
+  const int wrc = workspace_fault(fn, workspace, workspace_bytes, cache4_attention_workspace_bytes(n, T, width, H, Hk, d));
+  if (wrc != ESM_OK) return wrc;
+  a.q = q, a.o = o, a.q_st = q_st, a.q_sh = q_sh, a.o_st = o_st, a.o_sh = o_sh;
+  a.G = H / Hk, a.causal = causal != 0, a.scale_log2 = scale_log2;
+  a.divide = plan.divide, a.target = plan.target, a.items = plan.items;
+  if (plan.divide) {
+    a.part_ml = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + attn4_ml_bytes(plan, Hk));
+  }
+  return hip_status(esm::launch_cache4_attention(a, dtype == ESM_BF16, plan, (hipStream_t)stream), "cache4_attention launch");
+}
+
 // ---- the end of a linear: bias, activation or gate, residual ---------------------------------------
 namespace {
 bool linear_shape(int M, int K, int N, int gated, int multiple_k) {
@@ -1171,13 +1275,6 @@ int linear_end(const char* fn, esm::LinearEnd& e, const float* bias, const void*
     return fail(ESM_ERR_ALIGN, "%s: bias, residual and output must be 16-byte aligned", fn);
   e.y = y, e.bias = bias, e.res = residual, e.r_st = M > 1 ? r_st : 0, e.alpha = alpha;
   e.act = activation, e.gated = gated != 0, e.on = 1, e.No = No, e.Nb = N;
-  return ESM_OK;
-}
-
-int workspace_fault(const char* fn, const void* ws, size_t have, size_t need) {
-  if (!need) return ESM_OK;
-  if (!ws || have < need) return fail(ESM_ERR_SHAPE, "%s: workspace of %zu bytes, %zu needed", fn, have, need);
-  if (reinterpret_cast<uintptr_t>(ws) & 255u) return fail(ESM_ERR_ALIGN, "%s: workspace must be 256-byte aligned", fn);
   return ESM_OK;
 }
 

@@ -322,6 +322,35 @@ struct AddNormArgs {
   int waves, rows;        // waves per row, rows per workgroup (set by the launcher)
 };
 
+// Keys and values in 4 bits (cache4.hip).
+constexpr int kCache4Page = 64;      // keys of a page
+constexpr int kCache4MaxChunks = 256;  // of one sequence's keys
+// Bytes of a page's head: 64 keys and values of hd (64 or 128) 4-bit codes and 4 bytes for 64 of them.
+constexpr int cache4_page_bytes(int hd) { return 2 * 64 * (hd / 2 + hd / 64 * 4); }
+struct Cache4Args {
+  const void *k, *v;      // rows to write
+  void *ko, *vo;          // rows read back, [T, Hk, d]
+  const void* q;
+  void* o;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh;
+  void* data;             // [pages][Hk][cache4_page_bytes]
+  const int *cu, *lens, *table;  // [n + 1], [n], [n, width]
+  int n, T, Hk, G, d, pages, width, causal;
+  float scale_log2;
+  int divide, target;     // whether keys are divided between workgroups; over how many of a key head
+  long long items;        // partials of a key head there is room for
+  float *part_ml, *part_o;
+};
+struct Cache4Plan {
+  int rt;                 // 16-row tiles of a workgroup
+  int divide, target;
+  long long items;        // (sequence, tile, chunk) of a key head at most
+};
+Cache4Plan cache4_plan(long long T, int n, int width, int Hk, int G, int cus);
+hipError_t launch_cache4_write(const Cache4Args& a, bool bf16, hipStream_t s);
+hipError_t launch_cache4_read(const Cache4Args& a, bool bf16, hipStream_t s);
+hipError_t launch_cache4_attention(const Cache4Args& a, bool bf16, const Cache4Plan& plan, hipStream_t s);
+
 // Each launcher returns the hipError_t of the launch.
 hipError_t launch_project(const ProjectArgs& a, int grid, hipStream_t s);
 hipError_t launch_contract(const ContractArgs& a, hipStream_t s);

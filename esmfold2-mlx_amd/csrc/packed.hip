@@ -299,38 +299,6 @@ struct Span {
   int q0, nq, k0, nk;  // first row and rows of a sequence, on the query and on the key side
 };
 
-// Sum and maximum over the wave, the same in every lane, and the sum of the lanes up to this one, by data-parallel moves
-// (an exchange through LDS answers in some 100 cycles, and six of them in a row stood before a tile's first load).
-template <class F>
-DEV int wave_rows(int v, F f) {  // over each row of 16 lanes
-  const auto with = [&](auto ctrl) { v = f(v, __builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, false)); };
-  with(std::integral_constant<int, 0x128>{});  // row_ror:8, 4, 2, 1
-  with(std::integral_constant<int, 0x124>{});
-  with(std::integral_constant<int, 0x122>{});
-  with(std::integral_constant<int, 0x121>{});
-  return v;
-}
-DEV int wave_sum(int v) {
-  v = wave_rows(v, [](int a, int b) { return a + b; });
-  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
-         __builtin_amdgcn_readlane(v, 48);
-}
-DEV int wave_max(int v) {
-  v = wave_rows(v, [](int a, int b) { return max(a, b); });
-  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
-}
-DEV int wave_scan(int v) {
-  const auto add = [&](auto ctrl) { v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, 0xf, 0xf, false); };
-  add(std::integral_constant<int, 0x111>{});  // row_shr:1, 2, 4, 8 (0 from before the row)
-  add(std::integral_constant<int, 0x112>{});
-  add(std::integral_constant<int, 0x114>{});
-  add(std::integral_constant<int, 0x118>{});
-  const int row = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)) >> 4;
-  const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
-  return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
-}
-
 // Sequence of a work item and the item's number within it: a sequence has as many items as tiles of `unit` rows times
 // chunks of `chunk` keys (at least one; chunk 0: not counted). All lanes agree; the starts are read once, a lane a
 // sequence. Starts outside 0 .. the rows there are are brought inside, so nothing a caller writes there reaches past

@@ -959,3 +959,93 @@ def f8_linear_end(x, codes, scales, N: int, bias=None, *, gated: bool = False, a
         ws, wp, stream = scratch.workspace(need, device)
         capi.check(lib.f8_linear_end(*args, wp, need, stream))
     return y
+
+
+# ---- keys and values in 4 bits ---------------------------------------------------------------------
+def _cache4(fn, data, heads: int, d: int, T: int, cu, lens, table, index: int):
+    """The checks of what the cache's calls share: (their last arguments but dtype, pages)."""
+    lib = capi.lib()
+    _aux(data, "data", _UINT8, index)
+    _aux(cu, "cu", _INT32, index)
+    _aux(lens, "lens", _INT32, index)
+    _aux(table, "table", _INT32, index)
+    n = lens.numel()
+    each = int(lib.cache4_bytes(1, heads, d))
+    if cu.numel() != n + 1 or table.dim() != 2 or table.shape[0] != n:
+        raise capi.EsmError(-2, f"{fn}: {cu.numel()} starts, {n} lengths, table {tuple(table.shape)}")
+    if not each or data.numel() % each:
+        raise capi.EsmError(-2, f"{fn}: a cache of {data.numel()} bytes for {heads} heads of {d}")
+    return n, data.numel() // each, table.shape[1]
+
+
+def cache4_append(data, k, v, cu, lens, table):
+    """Rows k, v [T, Hk, d] (fp16 or bf16, views of wider rows allowed) into a cache in 4 bits (``cache4.Cache4``): sequence
+    i's rows cu[i] .. cu[i + 1] - 1 become the last of its lens[i] keys, key j in page table[i, j // 64] (int32 on the device).
+    Rows whose place lies outside the table or the cache are left out."""
+    lib = capi.lib()
+    (T, Hk, d), k_st, k_sh = _rows(k, "k")
+    dtype, index = k.dtype, k.get_device()
+    vshape, v_st, v_sh = _rows(v, "v", dtype, index)
+    if index != _current():
+        with torch.cuda.device(index):
+            return cache4_append(data, k, v, cu, lens, table)
+    if vshape != k.shape:
+        raise capi.EsmError(-2, f"cache4_append: k {tuple(k.shape)}, v {tuple(v.shape)}")
+    n, pages, width = _cache4("cache4_append", data, Hk, d, T, cu, lens, table, index)
+    capi.check(lib.cache4_append(k.data_ptr(), v.data_ptr(), k_st, k_sh, v_st, v_sh, data.data_ptr(), cu.data_ptr(),
+                                 lens.data_ptr(), table.data_ptr(), n, T, Hk, d, pages, width, _DTYPES[dtype], capi.stream_ptr()))
+
+
+def cache4_read(data, T: int, heads: int, d: int, dtype, cu, lens, table):
+    """(k, v) [T, heads, d] in ``dtype``, the cache's own: what the places of ``cache4_append``'s rows hold (rows without a
+    place: 0)."""
+    lib = capi.lib()
+    if not isinstance(data, torch.Tensor) or not data.is_cuda:
+        raise capi.EsmError(-5, "data must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
+    index = data.get_device()
+    if index != _current():
+        with torch.cuda.device(index):
+            return cache4_read(data, T, heads, d, dtype, cu, lens, table)
+    n, pages, width = _cache4("cache4_read", data, heads, d, T, cu, lens, table, index)
+    if dtype not in _DTYPES:
+        raise capi.EsmError(-2, f"cache4_read: dtype={dtype}")
+    k, v = (torch.empty((T, heads, d), dtype=dtype, device=data.device) for _ in range(2))
+    capi.check(lib.cache4_read(k.data_ptr(), v.data_ptr(), data.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), n,
+                               T, heads, d, pages, width, _DTYPES[dtype], capi.stream_ptr()))
+    return k, v
+
+
+def cache4_attention(data, q, heads: int, cu, lens, table, causal: bool = True, scale: float | None = None, out=None):
+    """softmax(q k^T * scale) v over keys and values held in 4 bits (``cache4.Cache4`` of q's type, ``heads`` key heads): q [T,
+    H, d] -> o [T, H, d]. Sequence i has the query rows cu[i] .. cu[i + 1] - 1 and the first lens[i] keys of its pages
+    table[i]; ``causal``: its last row sees the last key. Rows that see no key are 0, rows of no sequence are not written,
+    keys in pages outside the cache are not seen. ``out`` may be q. Where keys are divided between workgroups the partial
+    results live in the shared scratch (``scratch.workspace``)."""
+    lib = capi.lib()
+    (T, H, d), q_st, q_sh = _rows(q, "q")
+    dtype, index = q.dtype, q.get_device()
+    if index != _current():
+        with torch.cuda.device(index):
+            return cache4_attention(data, q, heads, cu, lens, table, causal, scale, out)
+    if heads <= 0 or H % heads:
+        raise capi.EsmError(-2, f"cache4_attention: {H} query heads, {heads} key heads")
+    n, pages, width = _cache4("cache4_attention", data, heads, d, T, cu, lens, table, index)
+    if out is None:
+        o, o_st, o_sh = q.new_empty((T, H, d)), H * d, d
+    else:
+        o = out
+        oshape, o_st, o_sh = _distinct(o, "out", dtype, index)
+        if oshape != q.shape:
+            raise capi.EsmError(-2, f"cache4_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
+        if T and o.data_ptr() == q.data_ptr() and (o_st, o_sh) != (q_st, q_sh):
+            raise capi.EsmError(-3, "cache4_attention: out over q must have its strides")
+    args = (q.data_ptr(), o.data_ptr(), q_st, q_sh, o_st, o_sh, data.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), n,
+            T, H, heads, d, pages, width, bool(causal), d ** -0.5 if scale is None else float(scale), _DTYPES[dtype])
+    need = lib.cache4_attention_workspace_bytes(n, T, width, H, heads, d)
+    if not need:
+        capi.check(lib.cache4_attention(*args, None, 0, capi.stream_ptr()))
+        return o
+    with scratch.guard(q.device):
+        ws, wp, stream = scratch.workspace(need, q.device)
+        capi.check(lib.cache4_attention(*args, wp, need, stream))
+    return o

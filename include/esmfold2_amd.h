@@ -517,6 +517,36 @@ int f8_linear_end(const void* x, int64_t x_st, const uint8_t* xq, const float* s
                   int K, int N, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Keys and values in 4 bits, in pages of 64 keys, and the attention that reads them (no reference counterpart).
+ *
+ * A value stands as s (c - z), c in 0 .. 15, with s and z per key (or value), head and 64 values: s the least bf16 value, 2^-96
+ * or more, of which 15 reach over the 64 values' range and 120 to the farthest from zero, z = rint(-min / s), c = clamp(rint(x
+ * / s) + z, 0, 15); 64 values with a NaN or an infinity among them read as NaN. data: cache4_bytes(pages, Hk, d) bytes, 16-byte
+ * aligned, zeroed or written before they are read. The layout is the kernels' own and depends on dtype.
+ * Sequence i has the rows cu[i] .. cu[i + 1] - 1 of a call (int32 [n + 1], ascending; brought inside 0 .. T), which are the
+ * last of its lens[i] keys (int32 [n]); its key j lies in page table[i][j / 64] (int32 [n, width]). All of them on the device.
+ *
+ * cache4_append: writes k and v [T, Hk, d] to their places. Rows whose place lies outside the table or the pages are left out.
+ * cache4_read: what is held in those places, [T, Hk, d] contiguous, rounded once to dtype; rows without a place are 0.
+ * cache4_attention: o = softmax(scale q k^T) v over the sequence's keys, q and o [T, H, d], query head h with key head h / (H /
+ *   Hk); causal: row i of nq sees the keys 0 .. i + nk - nq of nk. lens beyond the table are brought inside; keys in pages
+ *   outside 0 .. pages - 1 are not seen. Rows that see no key are 0, rows of no sequence are not written, what unseen places
+ *   hold reaches no output. Scores and sums are fp32; probability times step is rounded to bf16 (fp16: to 16 bits) for the
+ *   second product. |q| < 2^110.
+ * d % 8 == 0, d <= 128; strides as packed_attention's. Workspace 256-byte aligned (0: none).
+ */
+size_t cache4_bytes(int pages, int Hk, int d);
+int cache4_append(const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, void* data,
+                  const int* cu, const int* lens, const int* table, int n, int T, int Hk, int d, int pages, int width,
+                  int dtype, void* stream);
+int cache4_read(void* k, void* v, const void* data, const int* cu, const int* lens, const int* table, int n, int T, int Hk, int d,
+                int pages, int width, int dtype, void* stream);
+size_t cache4_attention_workspace_bytes(int n, int T, int width, int H, int Hk, int d);
+int cache4_attention(const void* q, void* o, int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh, const void* data,
+                     const int* cu, const int* lens, const int* table, int n, int T, int H, int Hk, int d, int pages, int width,
+                     int causal, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * One whole ESMC block (mlx_esmc.py:84-102) as its eight launches on the stream (one more for each of wqkv, w1
  * whose K is split, and for each linear whose rows are divided between tile forms), from the block's LayerNormed
  * input: x' = x + alpha * wo(attention(wqkv(h))), then x_out = x' + alpha * w2(swiglu(w1(LN2(x')))), then the
