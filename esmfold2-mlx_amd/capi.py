@@ -122,12 +122,15 @@ class _LongWay:
         return None
 
     qk_norm_rope = packed_attention = f8_linear = connect = _none
+    add_norm = linear16 = f8_linear_rows = cache4_append = cache4_read = cache4_attention = _none
 
 
 # the native short way of some calls (csrc/bind.cpp), loaded with the library, and the entry points it takes
 bind = None
 _SHORT = ("qk_norm_rope", "packed_attention", "packed_attention_workspace_bytes", "f8_linear",
-          "f8_linear_workspace_bytes")
+          "f8_linear_workspace_bytes", "add_norm", "f8_rows_bytes", "f8_rows_scales_bytes", "linear16", "linear16_workspace_bytes",
+          "linear16_packed_bytes", "f8_linear_end", "f8_linear_end_workspace_bytes", "cache4_bytes", "cache4_append", "cache4_read",
+          "cache4_attention", "cache4_attention_workspace_bytes")
 
 _lock = threading.Lock()
 _lib = None

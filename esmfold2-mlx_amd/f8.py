@@ -30,8 +30,9 @@ class F8Rows:
     """Rows [..., K] in e4m3, with a scale per row and 128 columns, in the order ``F8Linear`` takes (``kernels.add_norm_f8``)."""
 
     def __init__(self, packed: torch.Tensor, packed_scales: torch.Tensor, shape, features: int, dtype: torch.dtype):
-        self.packed, self.packed_scales, self.shape = packed, packed_scales, torch.Size(shape)
-        self.rows, self.features, self.dtype = self.shape.numel(), features, dtype  # dtype: of a linear's outputs
+        self.packed, self.packed_scales, self.shape = packed, packed_scales, shape
+        self.rows = shape[0] if len(shape) == 1 else torch.Size(shape).numel()
+        self.features, self.dtype = features, dtype  # dtype: of a linear's outputs
 
     @property
     def codes(self) -> torch.Tensor:

@@ -811,6 +811,10 @@ def _vector(t, name: str, n: int, index: int):
 
 def _add_norm(fn, x, y, w, b, alpha, norm, eps, dtype, sum_out, out, f8):
     lib = capi.lib()
+    if y is not None and out is None and sum_out is None and norm in _NORM_KINDS and (dtype is None or dtype is getattr(y, "dtype", None)):
+        r = capi.bind.add_norm(x, y, w, b, alpha, _NORM_KINDS[norm], eps, f8)
+        if r is not None:
+            return r
     x_st, index = _matrix(x, "x", _STREAMS)
     if index != _current():
         with torch.cuda.device(index):
@@ -904,6 +908,15 @@ def linear16(x, packed, N: int, bias=None, *, gated: bool = False, activation: s
     fp32, ``activation`` None, "relu", "gelu", "gelu_tanh" or "silu", ``residual`` of y's type. fp32 sums, one rounding.
     ``out`` (contiguous) may be the residual. Split-K partials live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
+    act = _ACTIVATIONS.get(activation)
+    if out is None and act is not None:
+        y = capi.bind.linear16(x, packed, N, bias, gated, act, residual, alpha, 0, 0)
+        if type(y) is int:  # bytes of workspace
+            with scratch.guard(x.device):
+                ws, wp, _ = scratch.workspace(y, x.device)
+                y = capi.bind.linear16(x, packed, N, bias, gated, act, residual, alpha, wp, y)
+        if y is not None:
+            return y
     x_st, index = _matrix(x, "x", tuple(_DTYPES))
     if index != _current():
         with torch.cuda.device(index):
@@ -934,6 +947,16 @@ def f8_linear_end(x, codes, scales, N: int, bias=None, *, gated: bool = False, a
         dtype, device, xq, sx = x.dtype, x.device, None, None
     else:
         xq, sx, M, K = rows
+        act = _ACTIVATIONS.get(activation)
+        if out is None and act is not None and dtype in _DTYPES:
+            a = (xq, sx, M, K, dtype is torch.bfloat16, codes, scales, N, bias, gated, act, residual, alpha)
+            y = capi.bind.f8_linear_rows(*a, 0, 0)
+            if type(y) is int:  # bytes of workspace
+                with scratch.guard(xq.device):
+                    ws, wp, _ = scratch.workspace(y, xq.device)
+                    y = capi.bind.f8_linear_rows(*a, wp, y)
+            if y is not None:
+                return y
         if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
             raise capi.EsmError(-5, "rows must be CUDA(HIP) tensors; the HIP path has no CPU fallback")
         index, device, x_st = xq.get_device(), xq.device, 0
@@ -983,6 +1006,8 @@ def cache4_append(data, k, v, cu, lens, table):
     i's rows cu[i] .. cu[i + 1] - 1 become the last of its lens[i] keys, key j in page table[i, j // 64] (int32 on the device).
     Rows whose place lies outside the table or the cache are left out."""
     lib = capi.lib()
+    if capi.bind.cache4_append(data, k, v, cu, lens, table):
+        return
     (T, Hk, d), k_st, k_sh = _rows(k, "k")
     dtype, index = k.dtype, k.get_device()
     vshape, v_st, v_sh = _rows(v, "v", dtype, index)
@@ -1000,6 +1025,10 @@ def cache4_read(data, T: int, heads: int, d: int, dtype, cu, lens, table):
     """(k, v) [T, heads, d] in ``dtype``, the cache's own: what the places of ``cache4_append``'s rows hold (rows without a
     place: 0)."""
     lib = capi.lib()
+    if dtype in _DTYPES:
+        y = capi.bind.cache4_read(data, T, heads, d, dtype is torch.bfloat16, cu, lens, table)
+        if y is not None:
+            return y
     if not isinstance(data, torch.Tensor) or not data.is_cuda:
         raise capi.EsmError(-5, "data must be a CUDA(HIP) tensor; the HIP path has no CPU fallback")
     index = data.get_device()
@@ -1022,6 +1051,14 @@ def cache4_attention(data, q, heads: int, cu, lens, table, causal: bool = True, 
     keys in pages outside the cache are not seen. ``out`` may be q. Where keys are divided between workgroups the partial
     results live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
+    if out is None:
+        o = capi.bind.cache4_attention(data, q, heads, cu, lens, table, causal, scale, 0, 0)
+        if type(o) is int:  # bytes of workspace
+            with scratch.guard(q.device):
+                ws, wp, _ = scratch.workspace(o, q.device)
+                o = capi.bind.cache4_attention(data, q, heads, cu, lens, table, causal, scale, wp, o)
+        if o is not None:
+            return o
     (T, H, d), q_st, q_sh = _rows(q, "q")
     dtype, index = q.dtype, q.get_device()
     if index != _current():

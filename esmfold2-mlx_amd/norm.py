@@ -29,19 +29,20 @@ class AddNorm(nn.Module):
                 sum_out=None, out=None):
         """(s, h): s = x + alpha * y in x's type (x itself without y) and its norm. x [..., D] fp32 or 16-bit, y and h fp16 or
         bf16 (``dtype``: h's, else y's or x's). ``f8``: h as ``F8Rows``. ``sum_out`` may be x."""
-        D = self.weight.numel()
-        if x.shape[-1] != D:
-            raise ValueError(f"AddNorm: rows of {x.shape[-1]} values, made for {D}")
+        w, b = self._buffers["weight"], self._buffers["bias"]
         shape = x.shape
-        if x.dim() != 2:  # (views of whole rows; a copy would lose what is written to it)
-            flat = lambda t: None if t is None else t.view(-1, D)  # noqa: E731
-            x, y, sum_out, out = x.reshape(-1, D), None if y is None else y.reshape(-1, D), flat(sum_out), flat(out)
-        kw = dict(alpha=alpha, norm=self.norm, eps=self.eps, dtype=dtype, sum_out=sum_out)
+        D = shape[-1]
+        if D != w.numel():
+            raise ValueError(f"AddNorm: rows of {D} values, made for {w.numel()}")
+        if f8 and out is not None:
+            raise ValueError("AddNorm: rows in e4m3 have no out")
+        flat = len(shape) == 2
+        if not flat:  # (views of whole rows; a copy would lose what is written to it)
+            view = lambda t: None if t is None else t.view(-1, D)  # noqa: E731
+            x, y, sum_out, out = x.reshape(-1, D), None if y is None else y.reshape(-1, D), view(sum_out), view(out)
+        s, h = kernels._add_norm("add_norm", x, y, w, b, alpha, self.norm, self.eps, dtype, sum_out, out, f8)
         if f8:
-            if out is not None:
-                raise ValueError("AddNorm: rows in e4m3 have no out")
-            s, (codes, scales) = kernels.add_norm_f8(x, y, self.weight, self.bias, **kw)
-            kind = dtype or (x.dtype if y is None else y.dtype)
-            return s.view(shape), F8Rows(codes, scales, shape[:-1], D, kind)
-        s, h = kernels.add_norm(x, y, self.weight, self.bias, out=out, **kw)
-        return s.view(shape), h.view(shape)
+            h = F8Rows(*h, shape[:-1], D, dtype or (x.dtype if y is None else y.dtype))
+        if flat:
+            return s, h
+        return s.view(shape), h if f8 else h.view(shape)
