@@ -231,23 +231,31 @@ struct B16Keys {
   static DEV float zero_of(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 };
 DEV f32x4 mfma_b16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-// The two codes at bits AT of each half of w, as 16 + c in 16 bits.
-template <int AT, int UP, uint32_t MASK, uint32_t MAGIC>
-DEV uint32_t two_codes(uint32_t w) {
-  return ((AT > UP ? w >> (AT > UP ? AT - UP : 0) : w << (UP > AT ? UP - AT : 0)) & MASK) | MAGIC;
-}
-template <class T>
-DEV typename T::v8 key_codes(uint32_t w) {
-  return __builtin_bit_cast(typename T::v8,
-                            u32x4{two_codes<0, T::kUp, T::kMask, T::kMagic>(w), two_codes<4, T::kUp, T::kMask, T::kMagic>(w),
-                                  two_codes<8, T::kUp, T::kMask, T::kMagic>(w), two_codes<12, T::kUp, T::kMask, T::kMagic>(w)});
+// Mask and exponent that make 16 + c of a code, in registers of their own (hidden from the compiler, which would otherwise
+// write them into a v_and and a v_or instead of one v_and_or).
+template <uint32_t MASK, uint32_t MAGIC>
+struct Unpack {
+  uint32_t mask, magic;
+  DEV Unpack() : mask(MASK), magic(MAGIC) {
+    __asm__ volatile("" : "+s"(mask));
+    __asm__ volatile("" : "+v"(magic));
+  }
+  // The two codes at bits AT of each half of w; UP: a code's place in the 16 bits.
+  template <int AT, int UP>
+  DEV uint32_t two(uint32_t w) const {
+    return ((AT > UP ? w >> (AT > UP ? AT - UP : 0) : w << (UP > AT ? UP - AT : 0)) & mask) | magic;
+  }
+};
+typedef Unpack<B16Keys::kMask, B16Keys::kMagic> UnpackB;
+template <class T, class U>
+DEV typename T::v8 key_codes(const U& u, uint32_t w) {
+  return __builtin_bit_cast(typename T::v8, u32x4{u.template two<0, T::kUp>(w), u.template two<4, T::kUp>(w), u.template two<8, T::kUp>(w),
+                                                  u.template two<12, T::kUp>(w)});
 }
 template <bool HIGH>
-DEV bf16x8 value_codes(uint32_t a, uint32_t b) {  // slots 0 .. 3 and 4 .. 7 of the pair's low or high dims
-  constexpr uint32_t M = B16Keys::kMask, G = B16Keys::kMagic;
+DEV bf16x8 value_codes(const UnpackB& u, uint32_t a, uint32_t b) {  // slots 0 .. 3 and 4 .. 7 of the pair's low or high dims
   constexpr int A = HIGH ? 4 : 0;
-  return __builtin_bit_cast(bf16x8, u32x4{two_codes<A, 3, M, G>(a), two_codes<A + 8, 3, M, G>(a), two_codes<A, 3, M, G>(b),
-                                          two_codes<A + 8, 3, M, G>(b)});
+  return __builtin_bit_cast(bf16x8, u32x4{u.two<A, 3>(a), u.two<A + 8, 3>(a), u.two<A, 3>(b), u.two<A + 8, 3>(b)});
 }
 
 // Largest and sum over the four lanes that hold a row (those of one lane % 16).
@@ -287,8 +295,8 @@ DEV bool find_item4(const Cache4Args& p, int rows, int what, int lane, Item& it)
       if ((i0 += 64) >= p.n) break;
       spans(i0, a, nq, nk, tiles);
     }
-    // (at least a 256th of the longest there may be: kCache4MaxChunks)
-    it.keys = kPass * max(max(1, (int)ceilf(passes / (float)p.target)), (most + kPass * kCache4MaxChunks - 1) / (kPass * kCache4MaxChunks));
+    // (two passes at least, and a 256th of the longest there may be: kCache4MaxChunks)
+    it.keys = kPass * max(max(2, (int)ceilf(passes / (float)p.target)), (most + kPass * kCache4MaxChunks - 1) / (kPass * kCache4MaxChunks));
     if (p.n > 64) spans(0, a, nq, nk, tiles);
   }
   int before = 0;
@@ -325,6 +333,8 @@ struct Rows4 {
   float qs[RT][G];       // sums of a group's query values
   f32x4 o[RT][HD / 16];  // lane: row lane % 16, dims 16 i + 4 (lane / 16) + e
   float m[RT], l[RT];    // running maximum of the unscaled scores, this lane's part of the sum
+  Unpack<T::kMask, T::kMagic> ku;
+  UnpackB vu;
   int lim[RT];           // last key the row sees
 
   // 32 keys' operands of this lane.
@@ -388,7 +398,7 @@ struct Rows4 {
       f32x4 acc[RT][G];
 #pragma unroll
       for (int t = 0; t < HD / 32; t++) {
-        const v8 kc = key_codes<T>(k.kc[b][t]);
+        const v8 kc = key_codes<T>(ku, k.kc[b][t]);
 #pragma unroll
         for (int r = 0; r < RT; r++) acc[r][t >> 1] = T::mfma(kc, q[r][t], t & 1 ? acc[r][t >> 1] : f32x4{0.f, 0.f, 0.f, 0.f});
       }
@@ -423,15 +433,17 @@ struct Rows4 {
       if (__any((mx - m[r]) * c > kGrow4)) grow(r, row_max4(mx), c);
       const float mc = m[r] * c;
       const bool far = !(fabsf(mc) < kFar4);
-      float ref = 0.f, base = mc;
+      float base = mc;
       if (__any(far)) {  // (see packed.hip: large exponents, and rows that have seen nothing)
-        ref = far && m[r] != -INFINITY ? m[r] : 0.f;
+        const float ref = far && m[r] != -INFINITY ? m[r] : 0.f;
         base = far ? 0.f : mc;
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[r][j >> 2][j & 3] -= ref;
       }
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3] - ref, c, -base));
+        p[r][j] = __builtin_amdgcn_exp2f(fmaf(s[r][j >> 2][j & 3], c, -base));
         sum += p[r][j];
       }
       l[r] += sum;
@@ -455,7 +467,7 @@ struct Rows4 {
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const uint32_t a = k.vc[4 * i + 2 * (u >> 1)], b = k.vc[4 * i + 2 * (u >> 1) + 1];
-        const bf16x8 v = u & 1 ? value_codes<true>(a, b) : value_codes<false>(a, b);
+        const bf16x8 v = u & 1 ? value_codes<true>(vu, a, b) : value_codes<false>(vu, a, b);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
           f32x4& acc = o[r][4 * i + u];
@@ -476,7 +488,7 @@ struct Rows4 {
 // A workgroup takes 16 RT rows (query, head of the group; row = query G + head) of a sequence and key head and one chunk of
 // its keys, a page a wave in turn, the next 32 keys' operands in flight; the waves' results are joined through LDS.
 template <class T, int HD, int RT>
-__global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void cache4_attention_kernel(Cache4Args p) {
+__global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(Cache4Args p) {
   typedef Page<HD> P;
   typedef Rows4<T, HD, RT> R;
   constexpr int kRows = 16 * RT;
@@ -537,22 +549,32 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void cache4_attention_kernel(
     R::load_keys(k, page, 0, lane);
     R::load_values(k, page, 0, lane);
     bool good = id >= 0 && id < p.pages;  // (a page of no cache: not seen)
-    for (int u = 0, pg = page0; pg < pages; u++) {  // halves of pages
-      const int half = u & 1, key0 = kCache4Page * pg + 32 * half;
-      const bool seen = good;
-      if (half) {
+    int u = 0, pg = page0;                // halves of pages
+    // to the next half: what its step takes, and where the one behind it lies (behind the last page: that one again, not used)
+    const auto next = [&](bool& seen, int& key0) {
+      seen = good;
+      key0 = kCache4Page * pg + 32 * (u & 1);
+      if (u & 1) {
         pg += 4;
-        id = pg < pages ? page_of((u + 1) >> 1) : id;  // (behind the last page: that one again, not used)
+        id = pg < pages ? page_of((u + 1) >> 1) : id;
         page = at(id);
         good = id >= 0 && id < p.pages;
       }
-      if (seen && key0 + 32 <= whole) {
-        w.template step<false>(k, key0, p.scale_log2, lane, page, half ^ 1);
-      } else if (seen) {
-        w.template step<true>(k, key0, p.scale_log2, lane, page, half ^ 1);
+      u++;
+    };
+    bool seen;
+    int key0;
+    while (pg < pages && good && kCache4Page * pg + 32 * (u & 1) + 32 <= whole) {  // every row sees all 32
+      next(seen, key0);
+      w.template step<false>(k, key0, p.scale_log2, lane, page, u & 1);
+    }
+    while (pg < pages) {
+      next(seen, key0);
+      if (seen) {
+        w.template step<true>(k, key0, p.scale_log2, lane, page, u & 1);
       } else {
-        R::load_keys(k, page, half ^ 1, lane);
-        R::load_values(k, page, half ^ 1, lane);
+        R::load_keys(k, page, u & 1, lane);
+        R::load_values(k, page, u & 1, lane);
       }
     }
   }
@@ -656,10 +678,10 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args p, int rows
 Cache4Plan cache4_plan(long long T, int n, int width, int Hk, int G, int cus) {
   Cache4Plan plan{};
   const long long per = T * G / n;
-  plan.rt = per <= 16 ? 1 : per <= 32 ? 2 : 4;
+  plan.rt = per <= 64 ? 1 : 2;
   const long long tiles = T * G / (16 * plan.rt) + n;
-  plan.divide = width > 2 * kPass / kCache4Page && tiles * Hk < 64LL * cus;
-  plan.target = (int)((4LL * cus + Hk - 1) / Hk);
+  plan.divide = width > 2 * kPass / kCache4Page && T * G / (16 * plan.rt) * Hk < 2LL * cus;
+  plan.target = (int)((8LL * cus + Hk - 1) / Hk);
   if (plan.target > kCache4MaxChunks) plan.target = kCache4MaxChunks;
   plan.items = tiles + (plan.divide ? plan.target : 0);
   return plan;
@@ -677,8 +699,7 @@ template <class T, int HD>
 static hipError_t launch_cache4_hd(const Cache4Args& a, const Cache4Plan& plan, hipStream_t s) {
   switch (plan.rt) {
     case 1: return launch_cache4_t<T, HD, 1>(a, plan, s);
-    case 2: return launch_cache4_t<T, HD, 2>(a, plan, s);
-    default: return launch_cache4_t<T, HD, 4>(a, plan, s);
+    default: return launch_cache4_t<T, HD, 2>(a, plan, s);
   }
 }
 
