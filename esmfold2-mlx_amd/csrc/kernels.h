@@ -297,7 +297,7 @@ constexpr int kL16MaxSplits = 16;
 enum : int { kL16Few = 0, kL16Some = 1, kL16Tiles = 2 };
 struct L16Plan {
   int form;
-  int mb;                 // as F8Plan's
+  int mb;                 // kL16Few: fragments of a piece, kL16Some: 16-row blocks per workgroup, kL16Tiles: which tile
   int splits;
 };
 constexpr size_t linear16_packed_size(int N, int K, bool gated) {

@@ -6,8 +6,8 @@
 // 8 (l / 16) .. + 7, zeros past N and K. Dealt that way four fragments leave a lane 16 consecutive packed rows for one row of
 // x: in a gated linear the gates and the up values of 8 outputs.
 //
-// Three forms, as the e4m3 linear's: up to 16 rows of x the weights' bytes bound it and 8 waves divide K (few); some
-// hundred rows run without barriers, both operands straight to registers (some); many go through tiles in LDS (tiles).
+// Up to 16 rows of x the weights' bytes bound it and 8 waves divide K (few); small products run without barriers, both
+// operands straight to registers (some); the rest goes through tiles in LDS, of 64 x 128 to 256 x 256 outputs.
 #include <type_traits>
 
 #include "linear.h"
@@ -43,6 +43,7 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_few_kernel(L16Args p)
     V8 w[kSteps][NJ], x[kSteps];
   };
   const auto load = [&](Block& b, int kb) {
+    kb = min(kb, blocks - 1);  // (past the last: that one again, not used)
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
 #pragma unroll
@@ -63,11 +64,15 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_few_kernel(L16Args p)
   Block b0, b1;
   if (wave < blocks) load(b0, wave);
   for (int kb = wave; kb < blocks; kb += 2 * kL16Waves) {
-    if (kb + kL16Waves < blocks) load(b1, kb + kL16Waves);
+    load(b1, kb + kL16Waves);
+    __builtin_amdgcn_sched_barrier(0);
     take(b0);
+    __builtin_amdgcn_sched_barrier(0);
     if (kb + kL16Waves >= blocks) break;
-    if (kb + 2 * kL16Waves < blocks) load(b0, kb + 2 * kL16Waves);
+    load(b0, kb + 2 * kL16Waves);
+    __builtin_amdgcn_sched_barrier(0);
     take(b1);
+    __builtin_amdgcn_sched_barrier(0);
   }
   // lane's sums: row m, packed rows 16 (lane / 16) + 4 (j0 + j) + e -> column 4 NJ (lane / 16) + 4 j + e
 #pragma unroll
@@ -77,23 +82,22 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_few_kernel(L16Args p)
 }
 
 // ---- some rows --------------------------------------------------------------------------------------
-// A workgroup takes 16 MB RW rows of x by a piece of 64 packed weight rows; its 8 waves deal the blocks of 64 k among them
-// (RW = 2: four waves to each half of the rows), the next block's fragments in flight, and sum through LDS.
+// A workgroup takes 16 MB rows of x by a piece of 64 packed weight rows; its 8 waves deal the blocks of 64 k among them, the
+// next block's fragments in flight, and sum through LDS.
 constexpr int kL16Pad = 68;
-template <class V8, int MB, int RW>
+template <class V8, int MB>
 __global__ __launch_bounds__(64 * kL16Waves) void linear16_some_kernel(L16Args p) {
-  constexpr int KW = kL16Waves / RW;
   __shared__ __align__(16) float red[kL16Waves][16 * MB * kL16Pad];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rg = wave / KW, kw = wave % KW, Kb = (p.K + 63) / 64;
-  const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, row0 = (t - ng * p.mtiles) * 16 * MB * RW;
-  const int first = min(row0 + 16 * MB * rg, p.M - 1);  // (rows past the last: that one again, not stored)
+  const int Kb = (p.K + 63) / 64;
+  // row tiles run fastest: those that share weights are on one XCD at one time
+  const int t = xcd_remap(blockIdx.x, gridDim.x), ng = t / p.mtiles, row0 = (t - ng * p.mtiles) * 16 * MB;
   const rsrc_t rw = make_rsrc((const char*)p.w + (size_t)ng * Kb * 8192);
-  const rsrc_t rx = make_rsrc((const uint16_t*)p.x + first * p.x_st);
+  const rsrc_t rx = make_rsrc((const uint16_t*)p.x + row0 * p.x_st);
   uint32_t xo[MB];
 #pragma unroll
   for (int b = 0; b < MB; b++) {
-    const int r = min(16 * b + (lane & 15), p.M - 1 - first);
+    const int r = min(16 * b + (lane & 15), p.M - 1 - row0);  // (rows past the last: that one again, not stored)
     xo[b] = (uint32_t)(2 * (r * p.x_st + 8 * (lane >> 4)));
   }
   struct Block {
@@ -124,13 +128,18 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_some_kernel(L16Args p
         for (int j = 0; j < 4; j++) acc[b][j] = mfma_l16(k.w[i][j], k.x[i][b], acc[b][j]);
   };
   Block k0, k1;
-  if (kw < Kb) load(k0, kw);
-  for (int kb = kw; kb < Kb; kb += 2 * KW) {
-    load(k1, kb + KW);
+  if (wave < Kb) load(k0, wave);
+  for (int kb = wave; kb < Kb; kb += 2 * kL16Waves) {
+    // (the compiler would sink the next block's loads behind this block's products, and each wave wait for its own)
+    load(k1, kb + kL16Waves);
+    __builtin_amdgcn_sched_barrier(0);
     take(k0);
-    if (kb + KW >= Kb) break;
-    load(k0, kb + 2 * KW);
+    __builtin_amdgcn_sched_barrier(0);
+    if (kb + kL16Waves >= Kb) break;
+    load(k0, kb + 2 * kL16Waves);
+    __builtin_amdgcn_sched_barrier(0);
     take(k1);
+    __builtin_amdgcn_sched_barrier(0);
   }
 #pragma unroll
   for (int b = 0; b < MB; b++)
@@ -138,15 +147,12 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_some_kernel(L16Args p
     for (int j = 0; j < 4; j++)
       *reinterpret_cast<f32x4*>(&red[wave][(16 * b + (lane & 15)) * kL16Pad + 16 * (lane >> 4) + 4 * j]) = acc[b][j];
   __syncthreads();
-#pragma unroll
-  for (int g = 0; g < RW; g++)
-    end_lds<V8, kL16Pad>(p.end, red[g * KW], KW, 16 * MB * kL16Pad, 16 * MB, row0 + 16 * MB * g, p.M, ng, threadIdx.x,
-                         64 * kL16Waves);
+  end_lds<V8, kL16Pad>(p.end, red[0], kL16Waves, 16 * MB * kL16Pad, 16 * MB, row0, p.M, ng, threadIdx.x, 64 * kL16Waves);
 }
 
-// ---- many rows ----------------------------------------------------------------------------------
+// ---- tiles of up to 192 rows ----------------------------------------------------------------------
 // Workgroup tile of 16 MB WM rows of x by WN pieces of weights, WM x WN waves of 16 MB x 64 each. A step is 64 k: both
-// operands come by direct loads into a ring of S slots. Rows of x land 128 bytes a row, 16-byte chunk c of row r at c ^
+// operands come by direct loads into a ring of S slots, S - 1 steps ahead. Rows of x land 128 bytes a row, 16-byte chunk c of row r at c ^
 // (r % 8), so that a load takes whole lines of memory and a fragment's rows lie in different banks.
 template <class V8, int MB, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void linear16_tiles_kernel(L16Args p) {
@@ -254,6 +260,130 @@ __global__ __launch_bounds__(64 * WM * WN) void linear16_tiles_kernel(L16Args p)
   }
 }
 
+// ---- tiles of 256 x 256 ---------------------------------------------------------------------------
+// The same in steps of 32 k, of which LDS holds four where it holds two of 64. Rows of x land 64 bytes a row, 16-byte chunk c of row r at c ^
+// (r / 4 % 4), so that a fragment's 16 rows cover the banks. A step's first fragments are read at the end of the step before
+// it, behind the products, as the barrier between them stands for the slot after the next: with the slot itself the
+// waves would leave each barrier only to wait for LDS.
+template <class V8, int MB, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN) void linear16_large_kernel(L16Args p) {
+  constexpr int NW = WM * WN, kX = 1024 * MB * WM, kW = 4096 * WN, kSlot = kX + kW;  // bytes a slot
+  constexpr int kLoadsX = kX / 1024 / NW, kLoadsW = kW / 1024 / NW, kLoads = kLoadsX + kLoadsW;
+  constexpr int R = MB % 4 == 0 ? 4 : MB % 3 == 0 ? 3 : 2;  // fragments of x in registers, R - 1 of them ahead
+  static_assert(kLoadsX * NW * 1024 == kX && kLoadsW * NW * 1024 == kW, "whole loads per wave");
+  static_assert(S >= 4 && (S - 2) * kLoads < 64, "a slot behind the next; loads in flight the counter can tell");
+  static_assert(S * kSlot >= 8192 * NW, "end_tile's part of LDS");
+  __shared__ __align__(1024) char lds[S * kSlot];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN, Ks = 2 * ((p.K + 63) / 64);  // (weights are whole 64s, zeros past K)
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int tiles = p.mtiles * p.ntiles, split = t / tiles;
+  t -= split * tiles;
+  const int group = t / (8 * p.ntiles), in = t - group * 8 * p.ntiles, gm = min(8, p.mtiles - 8 * group);
+  const int mt = 8 * group + in % gm, nt = in / gm;
+  const int k0 = Ks * split / p.splits, k1 = Ks * (split + 1) / p.splits;
+  const int m0 = mt * 16 * MB * WM, ng0 = nt * WN, row0 = m0 + 16 * MB * wm;
+  const dma_src_t rx = dma_src((const uint16_t*)p.x + m0 * p.x_st, kBufRange);
+  const dma_src_t rw = dma_src((const char*)p.w + (size_t)ng0 * Ks * 4096, kBufRange);
+  const uint32_t base = lds_address(lds);
+  // where this lane reads x from: row lane / 4 of a load's 16, the chunk that lands at place lane % 4 of it
+  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t xo[kLoadsX];
+#pragma unroll
+  for (int i = 0; i < kLoadsX; i++) {
+    const int r = min(16 * (wave * kLoadsX + i) + (lane >> 2), p.M - 1 - m0);  // (rows past the last: that one again)
+    xo[i] = (uint32_t)(2 * (r * p.x_st + 8 * chunk));
+  }
+  const auto load = [&](int k, int slot, int i) {
+    const uint32_t at = base + slot * kSlot;
+    if (i < kLoadsX) {
+      dma16(rx, at + 1024 * (wave * kLoadsX + i), 32 * k + 8 * chunk < p.K ? xo[i < kLoadsX ? i : 0] : kOOB, 64u * (uint32_t)k);
+    } else {
+      const int u = wave * kLoadsW + i - kLoadsX, r = min(u >> 2, p.pieces - 1 - ng0);
+      dma16(rw, at + kX + 1024 * u, 16 * lane, (uint32_t)(r * Ks + k) * 4096u + 1024u * (u & 3));
+    }
+  };
+  f32x4 acc[MB][4];
+#pragma unroll
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int n = k1 - k0;
+#pragma unroll
+  for (int i = 0; i < S - 1; i++)
+#pragma unroll
+    for (int u = 0; u < kLoads; u++) load(min(k0 + i, k1 - 1), i, u);  // (past the last step: loaded again, not used)
+  const int mine = kX + 4096 * wn + 16 * lane, rows = 1024 * MB * wm + 64 * (lane & 15) + 16 * ((lane >> 4) ^ ((lane >> 2) & 3));
+  const auto weight = [&](int slot, int j) { return *reinterpret_cast<const V8*>(lds + slot * kSlot + mine + 1024 * j); };
+  const auto row = [&](int slot, int b) { return *reinterpret_cast<const V8*>(lds + slot * kSlot + rows + 1024 * b); };
+  V8 wa[4], wb[4], x[R];
+  constexpr int kLeft = (S - 3) * kLoads;
+  const auto settle = [&]() {  // the loads of all slots but the last S - 3 asked for are in, every wave's
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (kLeft & 15) | ((kLeft >> 4) << 14));
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+  };
+  // One step from slot: its weights are in w, the first R - 1 fragments of x in x; the next step's go to nw and x.
+  const auto step = [&](int i, int slot, V8 (&w)[4], V8 (&nw)[4]) {
+    settle();
+    const int kn = min(k0 + i + S - 1, k1 - 1), last = slot == 0 ? S - 1 : slot - 1, next = slot + 1 == S ? 0 : slot + 1;
+    constexpr int kSpread = (kLoads + MB - 1) / MB;
+#pragma unroll
+    for (int b = 0; b < MB; b++) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[b][j] = mfma_l16(w[j], x[b % R], acc[b][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      const int f = b + R - 1;  // the fragment to read now
+      x[f % R] = f < MB ? row(slot, f) : row(next, f - MB);
+      if (MB >= 4 ? b >= MB - 4 : true) {
+        constexpr int kPer = MB >= 4 ? 1 : 4 / MB;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+          const int jj = (MB >= 4 ? b - (MB - 4) : b * kPer) + j;
+          nw[jj] = weight(next, jj);
+        }
+      }
+#pragma unroll
+      for (int l = kSpread * b; l < kSpread * (b + 1); l++)
+        if (l < kLoads) load(kn, last, l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // before the first step: slot 0 is in
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (((S - 2) * kLoads) & 15) | ((((S - 2) * kLoads) >> 4) << 14));
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __asm__ volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 4; j++) wa[j] = weight(0, j);
+#pragma unroll
+  for (int b = 0; b < R - 1; b++) x[b] = row(0, b);
+  int slot = 0;
+  const auto after = [&]() { slot = slot + 1 == S ? 0 : slot + 1; };
+  int i = 0;
+  for (; i + 1 < n; i += 2) {  // (the weights' registers change places)
+    step(i, slot, wa, wb);
+    after();
+    step(i + 1, slot, wb, wa);
+    after();
+  }
+  if (i < n) step(i, slot, wa, wb);
+  wait_vm(0);  // no load of this workgroup outlives it, or lands on what end_tile keeps in LDS
+  __syncthreads();
+  const int ng = ng0 + wn;
+  if (ng >= p.pieces) return;
+  if (p.part) {
+#pragma unroll
+    for (int b = 0; b < MB; b++) {
+      const int m = row0 + 16 * b + (lane & 15);
+      if (m < p.M) part16(p.part, (long long)split * p.M + m, p.pieces, ng, lane >> 4, acc[b]);
+    }
+  } else {
+    end_tile<V8>(p.end, p.M, row0, ng, lane, acc, lds + 8192 * wave);
+  }
+}
+
 // ---- weights ------------------------------------------------------------------------------------
 // [N, K] into the fragment order, a thread 16 bytes; gated: fragments 0 and 2 of a piece from the first half of the rows, 1
 // and 3 from the second.
@@ -278,17 +408,25 @@ template <class V8, int MB, int WM, int WN, int S>
 static hipError_t launch_tiles16(L16Args a, hipStream_t s) {
   a.mtiles = (a.M + 16 * MB * WM - 1) / (16 * MB * WM);
   a.ntiles = (a.pieces + WN - 1) / WN;
-  ESM_LAUNCH((linear16_tiles_kernel<V8, MB, WM, WN, S>), dim3((unsigned)((size_t)a.mtiles * a.ntiles * a.splits)), dim3(64 * WM * WN),
-             0, s, a);
+  const dim3 grid((unsigned)((size_t)a.mtiles * a.ntiles * a.splits)), block(64 * WM * WN);
+  if constexpr (MB == 8) {
+    ESM_LAUNCH((linear16_large_kernel<V8, MB, WM, WN, S>), grid, block, 0, s, a);
+  } else {
+    ESM_LAUNCH((linear16_tiles_kernel<V8, MB, WM, WN, S>), grid, block, 0, s, a);
+  }
   return hipGetLastError();
 }
 
-template <class V8, int MB, int RW>
+template <class V8, int MB>
 static hipError_t launch_some16(L16Args a, hipStream_t s) {
-  a.mtiles = (a.M + 16 * MB * RW - 1) / (16 * MB * RW);
-  ESM_LAUNCH((linear16_some_kernel<V8, MB, RW>), dim3((unsigned)((size_t)a.mtiles * a.pieces)), dim3(64 * kL16Waves), 0, s, a);
+  a.mtiles = (a.M + 16 * MB - 1) / (16 * MB);
+  ESM_LAUNCH((linear16_some_kernel<V8, MB>), dim3((unsigned)((size_t)a.mtiles * a.pieces)), dim3(64 * kL16Waves), 0, s, a);
   return hipGetLastError();
 }
+
+// The tiles: rows, pieces of 64 packed weight rows, workgroups on a CU; us per workgroup and per 64 k of it.
+static const struct L16Tile { int rows, pieces, per_cu; double start, step; } kL16Tile[] = {
+    {64, 2, 2, 2.5, 0.41}, {64, 4, 1, 2.5, 0.58}, {128, 2, 1, 2.5, 0.60}, {128, 4, 1, 3.5, 0.76}, {192, 4, 1, 4.0, 1.15}, {256, 4, 1, 4.5, 1.47}};
 
 template <class V8>
 static hipError_t launch_linear16_t(const L16Args& a, int form, int mb, hipStream_t s) {
@@ -301,19 +439,15 @@ static hipError_t launch_linear16_t(const L16Args& a, int form, int mb, hipStrea
     }
     return hipGetLastError();
   }
-  if (form == kL16Some) switch (mb) {
-      case 1: return launch_some16<V8, 1, 1>(a, s);
-      case 2: return launch_some16<V8, 2, 1>(a, s);
-      case 3: return launch_some16<V8, 3, 1>(a, s);
-      case 4: return launch_some16<V8, 4, 1>(a, s);
-      default: return launch_some16<V8, 4, 2>(a, s);
-    }
+  if (form == kL16Some) return mb == 1 ? launch_some16<V8, 1>(a, s) : launch_some16<V8, 3>(a, s);
   hipError_t e;
-  switch (mb) {
-    case 2: e = launch_tiles16<V8, 2, 2, 4, 2>(a, s); break;
-    case 4: e = launch_tiles16<V8, 4, 2, 4, 2>(a, s); break;
-    case 6: e = launch_tiles16<V8, 6, 2, 4, 2>(a, s); break;
-    default: e = launch_tiles16<V8, 8, 2, 4, 2>(a, s); break;
+  switch (mb) {  // (kL16Tile's order)
+    case 0: e = launch_tiles16<V8, 2, 2, 2, 3>(a, s); break;
+    case 1: e = launch_tiles16<V8, 2, 2, 4, 4>(a, s); break;
+    case 2: e = launch_tiles16<V8, 4, 2, 2, 5>(a, s); break;
+    case 3: e = launch_tiles16<V8, 4, 2, 4, 3>(a, s); break;
+    case 4: e = launch_tiles16<V8, 6, 2, 4, 2>(a, s); break;
+    default: e = launch_tiles16<V8, 8, 2, 4, 4>(a, s); break;
   }
   if (e != hipSuccess || !a.part) return e;
   return launch_linear_join<V8>(a.part, a.end, a.M, a.pieces, a.splits, s);
@@ -323,34 +457,39 @@ hipError_t launch_linear16(const L16Args& a, bool bf16, const L16Plan& plan, hip
   return bf16 ? launch_linear16_t<bf16x8>(a, plan.form, plan.mb, s) : launch_linear16_t<half8>(a, plan.form, plan.mb, s);
 }
 
-// Which form: as the e4m3 linear's plan.
+// Which form: the lowest of estimated times, from measurements of the kernels alone (us; rows, K -> N):
+//   some, 16 rows a workgroup  24, 2560 -> 7680 9.8; 64, 5120 -> 2560 13.6     48 rows  238, 2560 -> 2560 14.2; 238, 5120 -> 2560 23.7
+//   64 x 128   238, 2560 -> 7680 19.3; 300 30.2; 512, 5120 -> 2560 in three splits 22.8 and 4.6 for the join
+//   64 x 256   1000, 2560 -> 2560 24.7; 512, 2560 -> 7680 32.6       128 x 128  512, 2560 -> 7680 29.0; 700, 4096 -> 4096 37.4
+//   128 x 256  2000, 5120 -> 2560 60.3; 1000, 10240 -> 2560 in three splits 56.1 and 6.9
+//   192 x 256  3481, 2560 -> 2560 48.7; 1500, 2560 -> 7680 62.2      256 x 256  3481, 2560 -> 7680 129; 8192, 8192 -> 8192 794
 L16Plan linear16_plan(int M, int K, int N, bool gated, int cus) {
   const long long pieces = linear_pieces(N, gated);
+  // Few rows: the most weight rows a workgroup (16, 32, 64) that still give more than half the CUs one (one row, 2560 -> 2560 4.1 /
+  // 4.6 / 6.4, 16 rows, 2560 -> 10240 15.8 / 15.5 / 12.7, 4096 -> 4096 9.2 / 11.0 / 14.8).
   L16Plan p{kL16Few, 4, 1};
   const int least = gated ? 2 : 1;  // (a gate and its up value in one workgroup)
   while (p.mb > least && 16LL * pieces * (4 / p.mb) < 9LL * cus) p.mb /= 2;
   if (M <= 16) return p;
   const int Kb = (K + 63) / 64;
-  const auto tiles = [&](int mb) { return ((M + 15) / 16 + mb - 1) / mb * pieces; };
-  p.form = kL16Some;
-  for (p.mb = 1; p.mb < 5 && tiles(p.mb) > cus;) p.mb++;
-  double best = 2.5 + Kb * (0.03 + 0.045 * p.mb);
-  if (p.mb == 5) {
-    p.mb = tiles(2) <= 2 * cus ? 2 : tiles(8) <= cus ? 8 : 4;
-    best = 2.5 + Kb * (p.mb == 2 ? 0.28 : p.mb == 8 ? 0.38 : 1.2e-3 * (double)tiles(4) * cus / 256);
+  double best = 1e30;
+  for (int mb : {1, 3}) {
+    if ((M + 16LL * mb - 1) / (16 * mb) * pieces > cus) continue;  // (a second round takes as long as the first)
+    const double c = 2.6 + (Kb + 7) / 8 * (0.5 + 0.6 * mb);
+    if (c < best) best = c, p = L16Plan{kL16Some, mb, 1};
   }
-  const struct { int mb; double step; } forms[] = {{2, 0.78}, {4, 1.0}, {6, 1.25}, {8, 1.55}};  // us a block of k
-  for (const auto& f : forms)
+  for (int i = 0; i < (int)(sizeof kL16Tile / sizeof kL16Tile[0]); i++) {
+    const L16Tile& t = kL16Tile[i];
     for (int sp = 1; sp <= kL16MaxSplits && (sp == 1 || 4 * sp <= Kb); sp++) {
-      const long long wgs = (long long)((M + 32 * f.mb - 1) / (32 * f.mb)) * ((pieces + 3) / 4) * sp, rounds = (wgs + cus - 1) / cus;
-      if (sp > 1 && rounds > 1) break;  // splits only fill one round
-      double c = rounds * (2.5 + f.step * ((Kb + sp - 1) / sp));
-      if (sp > 1) c += 3.0 + 8.0 * sp * M * 64.0 * pieces / 4.0e6;  // writing and summing the partials
-      if (c < best) {
-        best = c;
-        p = L16Plan{kL16Tiles, f.mb, sp};
-      }
+      const long long wgs = (M + t.rows - 1) / t.rows * ((pieces + t.pieces - 1) / t.pieces) * sp, each = (long long)cus * t.per_cu;
+      if (sp > 1 && wgs > each) break;  // splits only fill one round
+      // two on a CU take 1.6 times as long as one
+      const double rounds = wgs <= cus ? 1 : (double)((wgs + each - 1) / each) * (t.per_cu == 2 ? 1.6 : 1);
+      double c = rounds * (t.start + t.step * ((Kb + sp - 1) / sp));
+      if (sp > 1) c += 3.5 + 1.5e-6 * sp * M * 64.0 * pieces;  // writing and summing the partials
+      if (c < best) best = c, p = L16Plan{kL16Tiles, i, sp};
     }
+  }
   return p;
 }
 
