@@ -46,63 +46,125 @@ static_assert(Page<64>::kBytes == cache4_page_bytes(64) && Page<128>::kBytes == 
 DEV uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint32_t, v) >> 16; }  // (of values that bf16 holds)
 
 // ---- writing ------------------------------------------------------------------------------------
-// Step and zero of a group from its least and largest value and a NaN's presence: s = NaN then.
-DEV void four_bit_step(float lo, float hi, bool bad, float& s, float& z) {
+// rint(x / s) from inv, about 1 / s: without a division, of which eight a lane bound the writing (26 us for 8,287 rows). x has at
+// most 11 binary places and s 8, so x / s lies on k + 1/2 or 2^-12 from it at least, and x inv is off by less than 2^-16: only
+// ties can go the wrong way, and those are told by x - t s = s / 2, which is exact, and go to the even one.
+DEV float whole_steps(float x, float s, float inv) {
+  float t = rintf(x * inv);
+  const float rest = fmaf(-t, s, x);
+  if (fabsf(rest) == 0.5f * s) t = 2.f * rintf(0.5f * (t + (rest > 0.f ? 0.5f : -0.5f)));
+  return t;
+}
+// Step and zero of a group from its least and largest value; bad: it holds a NaN or an infinity, s is NaN then.
+DEV void four_bit_step(float lo, float hi, bool bad, float& s, float& inv, float& z) {
   const float far = fmaxf(fabsf(lo), fabsf(hi)), range = hi - lo;
-  s = fmaxf(fmaxf(range / 15.f, far / 120.f), 0x1p-96f);
-  uint32_t b = __builtin_bit_cast(uint32_t, s) & 0xffff0000u;
-  const float t = __builtin_bit_cast(float, b);
-  if (15.f * t < range || 120.f * t < far) b += 0x10000u;
+  const auto reaches = [&](float t) { return 15.f * t >= range && 120.f * t >= far && t >= 0x1p-96f; };
+  uint32_t b = __builtin_bit_cast(uint32_t, fmaxf(fmaxf(range * (1.f / 15.f), far * (1.f / 120.f)), 0x1p-96f)) & 0xffff0000u;
+  if (reaches(__builtin_bit_cast(float, b - 0x10000u))) b -= 0x10000u;  // (the products may be off by a step of fp32 either way)
+  else if (!reaches(__builtin_bit_cast(float, b))) b += 0x10000u;
   s = __builtin_bit_cast(float, b);
-  z = rintf(-lo / s);
+  inv = __builtin_amdgcn_rcpf(s);
+  z = whole_steps(-lo, s, inv);
   if (bad) s = __builtin_bit_cast(float, 0x7fc00000u), z = 0.f;
 }
 
-// The row's place in the cache: sequence, its page and the slot in it; false where there is none.
-struct Slot {
-  int page, key;
+// Four keys of a sequence that lie behind one another in a page, their slot a multiple of 4 (those at the ends of the call's
+// rows may be of other calls): key k's row is row + k for from <= k < to. page: -1 where it is none of the cache's, or the
+// rows stand before the sequence's first place or behind its table, or in no sequence.
+struct Four {
+  int row, from, to, page, key;
 };
-DEV bool find_slot(const Cache4Args& p, int row, int lane, Slot& s) {
+// Groups there may be of T rows in n sequences: a sequence's first and last may be incomplete, so may those of no sequence.
+static long long four_groups(long long T, int n) { return T / 4 + 2LL * n + 4; }
+DEV bool find_four(const Cache4Args& p, int what, int lane, Four& f) {
+  int before = 0, end = 0, start = 0;
   for (int i0 = 0; i0 < p.n; i0 += 64) {
     const int i = min(i0 + lane, p.n - 1);
-    const int a = min(max(p.cu[i], 0), p.T), b = min(max(p.cu[i + 1], a), p.T);
-    const uint64_t hit = __ballot(row >= a && row < b);
-    if (!hit) continue;
-    const int w = __builtin_ctzll(hit), seq = i0 + w;
-    const long long pos = (long long)p.lens[seq] - __builtin_amdgcn_readlane(b, w) + row;
-    if (pos < 0 || pos >= (long long)p.width * kCache4Page) return false;
-    s.page = p.table[(size_t)seq * p.width + (pos >> 6)];
-    s.key = (int)(pos & 63);
-    return s.page >= 0 && s.page < p.pages;
+    const int a = min(max(p.cu[i], 0), p.T), nq = min(max(p.cu[i + 1], a), p.T) - a;
+    const long long first = (long long)p.lens[i] - nq, lead = first & 3;  // (may be negative)
+    const int groups = i0 + lane < p.n && nq > 0 ? (int)((lead + nq + 3) >> 2) : 0, sum = wave_scan(groups);
+    const uint64_t hit = __ballot(what < before + sum);
+    if (hit) {
+      const int w = __builtin_ctzll(hit), seq = i0 + w;
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, w); };
+      const int g = what - before - of(sum - groups), nqw = of(nq), leadw = of((int)lead);
+      const long long pos = (((long long)of((int)(first >> 32)) << 32) | (uint32_t)of((int)first)) - leadw + 4LL * g;
+      f.row = of(a) - leadw + 4 * g;
+      f.from = max(0, leadw - 4 * g);
+      f.to = min(4, leadw + nqw - 4 * g);
+      f.page = -1;
+      f.key = (int)(pos & 63);
+      if (pos >= 0 && pos < (long long)p.width * kCache4Page) f.page = p.table[(size_t)seq * p.width + (pos >> 6)];
+      if (f.page < 0 || f.page >= p.pages) f.page = -1;
+      return g >= 0 && f.row + f.from >= 0 && f.row + f.to <= p.T;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+    if (i0 == 0) start = __builtin_amdgcn_readlane(a, 0);
+    end = __builtin_amdgcn_readlane(a + nq, 63);
   }
-  return false;
+  // rows of no sequence: behind the last, then before the first
+  int g = what - before;
+  f.page = -1, f.key = 0, f.from = 0;
+  f.row = end + 4 * g;
+  f.to = min(4, p.T - f.row);
+  if (f.to > 0) return g >= 0;
+  f.row = 4 * (g - (p.T - end + 3) / 4);
+  f.to = min(4, start - f.row);
+  return f.row >= 0 && f.to > 0;
 }
 
-// A wave takes a row's keys or values of a head: 8 lanes a group of 64 values, a lane 8 of them.
+// A wave takes four keys (or their values) of 64 / (HD / 2) heads: HD / 8 lanes a key, a lane 8 of its values.
+template <int HD>
+struct FourLanes {
+  static constexpr int kLanes = HD / 8, kHeads = 64 / (4 * kLanes);
+  int c, k, item;  // 8 values of key k of an item (the keys' heads, then the values')
+  DEV FourLanes(int lane) : c(lane % kLanes), k(lane / kLanes & 3), item((blockIdx.y * 4 + (threadIdx.x >> 6)) * kHeads + lane / (4 * kLanes)) {}
+  // The wave's next item, of those that the blocks of one group of keys deal among them; `first`: the item of its lane 0.
+  DEV bool next(int items) {
+    item += 4 * gridDim.y * kHeads;
+    return __builtin_amdgcn_readfirstlane(item) < items;
+  }
+  // Bytes of 8 dims (a, b: 4 each) of one key a lane, to two dims (x, y) of the four keys a lane, 2 k and 2 k + 1 of the 8, in
+  // the order of a value dword (keys 0, 2, 1, 3); and back. Exchanges with the lanes of keys k ^ 2 and k ^ 1.
+  DEV void gather(uint32_t a, uint32_t b, uint32_t& x, uint32_t& y) const {
+    const bool up = k & 2, odd = k & 1;
+    const uint32_t v = __shfl_xor(up ? a : b, 2 * kLanes);
+    const uint32_t m = up ? v : a, n = up ? b : v;  // four dims of keys k % 2 and k % 2 + 2
+    const uint32_t lo = (m & 0xffff) | (n << 16), hi = (m >> 16) | (n & 0xffff0000u);
+    const uint32_t w = __shfl_xor(odd ? lo : hi, kLanes);
+    const uint32_t r = odd ? w : lo, q = odd ? hi : w;  // two dims of keys 0 and 2, of 1 and 3
+    x = __builtin_amdgcn_perm(q, r, 0x06040200u);
+    y = __builtin_amdgcn_perm(q, r, 0x07050301u);
+  }
+  DEV void scatter(uint32_t x, uint32_t y, uint32_t& a, uint32_t& b) const {
+    const bool up = k & 2, odd = k & 1;
+    const uint32_t r = __builtin_amdgcn_perm(y, x, 0x05010400u), q = __builtin_amdgcn_perm(y, x, 0x07030602u);
+    const uint32_t w = __shfl_xor(odd ? r : q, kLanes);
+    const uint32_t lo = odd ? w : r, hi = odd ? q : w;
+    const uint32_t m = (lo & 0xffff) | (hi << 16), n = (lo >> 16) | (hi & 0xffff0000u);
+    const uint32_t v = __shfl_xor(up ? m : n, 2 * kLanes);
+    a = up ? v : m;
+    b = up ? n : v;
+  }
+};
+DEV uint32_t two_lanes_on(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x102, 0xf, 0xf, false); }  // row_shl:2
+
+// One item of a wave: x, the lane's 8 values, to its place.
 template <class V8, int HD>
-__global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
+DEV void hold_four(const Cache4Args& p, const Four& f, const FourLanes<HD>& at, V8 x, bool there) {
   typedef Page<HD> P;
-  constexpr int kLanes = HD / 8, kPer = 64 / kLanes;  // lanes of a head, heads of a wave
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x;
-  Slot at;
-  if (!find_slot(p, row, lane, at)) return;
-  const int c = lane % kLanes, item = (blockIdx.y * 4 + wave) * kPer + lane / kLanes;  // keys' heads, then values'
-  const bool val = item >= p.Hk, live = item < 2 * p.Hk;
-  const int h = live ? item - (val ? p.Hk : 0) : 0;
-  V8 x{};
-  const bool in = live && 8 * c < p.d;
-  if (in) x = *reinterpret_cast<const V8*>((const uint16_t*)(val ? p.v : p.k) + (long long)row * (val ? p.v_st : p.k_st) +
-                                           (long long)h * (val ? p.v_sh : p.k_sh) + 8 * c);
-  float v[8], lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
+  const int c = at.c;
+  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, mine = live && there, in = mine && 8 * c < p.d;
+  const int h = live ? at.item - (val ? p.Hk : 0) : 0, key = f.key + at.k;
+  float v[8], lo = INFINITY, hi = -INFINITY, none = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     v[e] = (float)x[e];
-    bad = bad || !(fabsf(v[e]) < INFINITY);
+    none = fmaf(v[e], 0.f, none);  // (NaN of a NaN or an infinity)
     lo = fminf(lo, v[e]);
     hi = fmaxf(hi, v[e]);
   }
+  bool bad = !(none == 0.f);
   if (!in) lo = INFINITY, hi = -INFINITY;
   const auto over = [&](auto ctrl) {
     const float a = dpp_f32<decltype(ctrl)::value>(lo), b = dpp_f32<decltype(ctrl)::value>(hi);
@@ -112,46 +174,50 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
   over(std::integral_constant<int, 0xB1>{});   // quad_perm(1, 0, 3, 2)
   over(std::integral_constant<int, 0x4E>{});   // quad_perm(2, 3, 0, 1)
   over(std::integral_constant<int, 0x141>{});  // row_half_mirror: 8 lanes, a group
-  if (!live) return;
-  float s, z;
+  float s, inv, z;
   if (lo > hi) lo = hi = 0.f;  // (a group past the head's values)
-  four_bit_step(lo, hi, bad, s, z);
+  four_bit_step(lo, hi, bad, s, inv, z);
   uint32_t code[8];
 #pragma unroll
-  for (int e = 0; e < 8; e++) code[e] = bad || !in ? 0 : (uint32_t)fminf(fmaxf(rintf(v[e] / s) + z, 0.f), 15.f);
-  char* page = (char*)p.data + ((size_t)at.page * p.Hk + h) * P::kBytes;
+  for (int e = 0; e < 8; e++) code[e] = bad || !in ? 0 : (uint32_t)fminf(fmaxf(whole_steps(v[e], s, inv) + z, 0.f), 15.f);
+  char* page = (char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes;
   const int g = c >> 3;  // group
+  // values: a lane of low nibbles (c / 2 even) joins the high ones of the lane two further, its bytes are 8 dims of a pair
+  uint32_t bytes[2] = {0, 0}, x4, y4;
+#pragma unroll
+  for (int e = 0; e < 8; e++) bytes[e >> 2] |= code[e] << (8 * (e & 3));
+  bytes[0] |= two_lanes_on(bytes[0]) << 4;
+  bytes[1] |= two_lanes_on(bytes[1]) << 4;
+  at.gather(bytes[0], bytes[1], x4, y4);
+  if (!live) return;
   if (!val) {
+    if (!mine) return;
     uint32_t w = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) w |= code[e] << (4 * (e >> 1) + 16 * (e & 1));
-    const int blk = at.key >> 4, ln = 16 * (c & 3) + (at.key & 15), t = c >> 2;  // dims 8 c = 32 t + 8 (c % 4)
+    const int blk = key >> 4, ln = 16 * (c & 3) + (key & 15), t = c >> 2;  // dims 8 c = 32 t + 8 (c % 4)
     *reinterpret_cast<uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t) = w;
     if ((c & 7) == 0) {
       const uint32_t zb = std::is_same<V8, bf16x8>::value ? bf16_bits(16.f + z)
                                                           : (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(16.f + z));
-      *reinterpret_cast<uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (at.key & 15)) * 4) =
+      *reinterpret_cast<uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (key & 15)) * 4) =
           (__builtin_bit_cast(uint32_t, s) & 0xffff0000u) | zb;
     }
   } else {
-    // dims 8 c ..: half (c / 2) % 2 of the 32 of pair p = c / 4 -- a lane holds low nibbles (c / 2 even) or high ones
-    uint32_t mine[2] = {0, 0}, theirs[2];
+    const int blk = key >> 5, k = key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);  // (slot % 4 is at.k)
+    if (!(c & 2)) {
+      const int pair = c >> 2, dim = 8 * (c & 1);  // of the pair's low 16
+      char* dst = page + P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + (slot & 4);
+      if (f.from == 0 && f.to == 4) {
+        *reinterpret_cast<uint32_t*>(dst + 16 * (2 * at.k)) = x4;
+        *reinterpret_cast<uint32_t*>(dst + 16 * (2 * at.k + 1)) = y4;
+      } else if (mine) {
+        const int byte = (0x3120 >> (4 * at.k)) & 3;
 #pragma unroll
-    for (int e = 0; e < 8; e++) mine[e >> 2] |= code[e] << (8 * (e & 3));
-    // the lane two further holds the high nibbles of this one's bytes
-    theirs[0] = __shfl_down(mine[0], 2);
-    theirs[1] = __shfl_down(mine[1], 2);
-    const int blk = at.key >> 5, k = at.key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
-    if (((c >> 1) & 1) == 0) {
-      const int pair = c >> 2, byte = (slot & 4) + ((0x3120 >> (4 * (slot & 3))) & 3);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int dim = 8 * (c & 1) + e;  // of the pair's low 16
-        page[P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + byte] =
-            (uint8_t)(((mine[e >> 2] >> (8 * (e & 3))) & 15) | (((theirs[e >> 2] >> (8 * (e & 3))) & 15) << 4));
+        for (int e = 0; e < 8; e++) dst[16 * e + byte] = (char)(bytes[e >> 2] >> (8 * (e & 3)));
       }
     }
-    if ((c & 7) == 0) {
+    if ((c & 7) == 0 && mine) {
       uint16_t* st = reinterpret_cast<uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
       st[0] = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
       st[2 * P::kGroups * 32] = (uint16_t)bf16_bits(-(16.f + z));
@@ -159,53 +225,87 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
   }
 }
 
-// What a row's place holds, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
+// Bound by a wave's latencies (starts, table, rows): with rows enough to fill the GPU one workgroup takes all heads of its four
+// keys, the next one's values asked for before this one's work.
 template <class V8, int HD>
-__global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Args p) {
+__global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
+  const int lane = threadIdx.x & 63;
+  Four f;
+  if (!find_four(p, blockIdx.x, lane, f) || f.page < 0) return;
+  FourLanes<HD> at(lane);
+  const bool there = at.k >= f.from && at.k < f.to;
+  const auto load = [&]() {
+    const bool val = at.item >= p.Hk;
+    V8 x{};
+    if (there && at.item < 2 * p.Hk && 8 * at.c < p.d)
+      x = *reinterpret_cast<const V8*>((const uint16_t*)(val ? p.v : p.k) + (long long)(f.row + at.k) * (val ? p.v_st : p.k_st) +
+                                       (long long)(at.item - (val ? p.Hk : 0)) * (val ? p.v_sh : p.k_sh) + 8 * at.c);
+    return x;
+  };
+  V8 x = load();
+  for (bool more = true; more;) {
+    const FourLanes<HD> now = at;
+    const V8 y = x;
+    more = at.next(2 * p.Hk);
+    if (more) x = load();  // (the next item's, before this one's work)
+    hold_four<V8, HD>(p, f, now, y, there);
+  }
+}
+
+template <class V8, int HD>
+DEV void give_four(const Cache4Args& p, const Four& f, const FourLanes<HD>& at, bool there) {
   typedef Page<HD> P;
-  constexpr int kLanes = HD / 8, kPer = 64 / kLanes;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x;
-  Slot at{0, 0};
-  const bool there = find_slot(p, row, lane, at);
-  const int c = lane % kLanes, item = (blockIdx.y * 4 + wave) * kPer + lane / kLanes;
-  const bool val = item >= p.Hk;
-  if (item >= 2 * p.Hk || 8 * c >= p.d) return;
-  const int h = item - (val ? p.Hk : 0), g = c >> 3;
-  V8* dst = reinterpret_cast<V8*>((uint16_t*)(val ? p.vo : p.ko) + ((size_t)row * p.Hk + h) * p.d + 8 * c);
-  if (!there) {
-    *dst = V8{};
+  const int c = at.c, g = c >> 3, key = f.key + at.k;
+  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, mine = live && there && 8 * c < p.d;
+  const int h = live ? at.item - (val ? p.Hk : 0) : 0;
+  V8* dst = reinterpret_cast<V8*>((uint16_t*)(val ? p.vo : p.ko) + ((size_t)(mine ? f.row + at.k : 0) * p.Hk + h) * p.d + (mine ? 8 * c : 0));
+  if (f.page < 0) {
+    if (mine) *dst = V8{};
     return;
   }
-  const char* page = (const char*)p.data + ((size_t)at.page * p.Hk + h) * P::kBytes;
+  const char* page = (const char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes;
   float s, z;
   uint32_t code[8];
-  if (!val) {
-    const int blk = at.key >> 4, ln = 16 * (c & 3) + (at.key & 15), t = c >> 2;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t);
+  if (val) {  // (a head's lanes exchange their bytes)
+    const int blk = key >> 5, k = key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
+    const int pair = c >> 2, dim = 8 * (c & 1);
+    const char* src = page + P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + (slot & 4);
+    uint32_t bytes[2];
+    at.scatter(*reinterpret_cast<const uint32_t*>(src + 16 * (2 * at.k)), *reinterpret_cast<const uint32_t*>(src + 16 * (2 * at.k + 1)),
+               bytes[0], bytes[1]);  // (the lanes of high nibbles read the same bytes)
 #pragma unroll
-    for (int e = 0; e < 8; e++) code[e] = (w >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
-    const uint32_t st = *reinterpret_cast<const uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (at.key & 15)) * 4);
-    s = __builtin_bit_cast(float, st & 0xffff0000u);
-    z = std::is_same<V8, bf16x8>::value ? __builtin_bit_cast(float, st << 16) - 16.f
-                                        : (float)__builtin_bit_cast(half_t, (uint16_t)st) - 16.f;
-  } else {
-    const int blk = at.key >> 5, k = at.key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
-    const int pair = c >> 2, byte = (slot & 4) + ((0x3120 >> (4 * (slot & 3))) & 3);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int dim = 8 * (c & 1) + e;
-      const uint8_t b = page[P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + byte];
-      code[e] = (b >> (2 * (c & 2))) & 15;
-    }
+    for (int e = 0; e < 8; e++) code[e] = (bytes[e >> 2] >> (8 * (e & 3) + 2 * (c & 2))) & 15;
     const uint16_t* st = reinterpret_cast<const uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
     s = __builtin_bit_cast(float, (uint32_t)st[0] << 16);
     z = -__builtin_bit_cast(float, (uint32_t)st[2 * P::kGroups * 32] << 16) - 16.f;
+  } else {
+    const int blk = key >> 4, ln = 16 * (c & 3) + (key & 15), t = c >> 2;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t);
+#pragma unroll
+    for (int e = 0; e < 8; e++) code[e] = (w >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
+    const uint32_t st = *reinterpret_cast<const uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (key & 15)) * 4);
+    s = __builtin_bit_cast(float, st & 0xffff0000u);
+    z = std::is_same<V8, bf16x8>::value ? __builtin_bit_cast(float, st << 16) - 16.f
+                                        : (float)__builtin_bit_cast(half_t, (uint16_t)st) - 16.f;
   }
+  if (!mine) return;
   V8 y;
 #pragma unroll
   for (int e = 0; e < 8; e++) y[e] = (decltype(+y[e]))(s * ((float)code[e] - z));
   *dst = y;
+}
+
+// What the rows' places hold, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
+template <class V8, int HD>
+__global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Args p) {
+  const int lane = threadIdx.x & 63;
+  Four f;
+  if (!find_four(p, blockIdx.x, lane, f)) return;
+  FourLanes<HD> at(lane);
+  const bool there = at.k >= f.from && at.k < f.to;
+  do {
+    give_four<V8, HD>(p, f, at, there);
+  } while (at.next(2 * p.Hk));
 }
 
 // ---- attention --------------------------------------------------------------------------------------
@@ -710,8 +810,10 @@ hipError_t launch_cache4_attention(const Cache4Args& a, bool bf16, const Cache4P
 
 template <class V8, int HD>
 static hipError_t launch_write_t(const Cache4Args& a, bool read, hipStream_t s) {
-  const int per = 4 * (64 / (HD / 8));  // heads of a workgroup, keys' and values'
-  const dim3 grid(a.T, (2 * a.Hk + per - 1) / per);
+  const int per = 4 * FourLanes<HD>::kHeads;  // heads of a workgroup, keys' and values'
+  // all heads in one workgroup where the keys alone fill the GPU, else as many workgroups as there are heads for
+  const long long groups = four_groups(a.T, a.n);
+  const dim3 grid((unsigned)groups, groups >= 1024 ? 1 : (2 * a.Hk + per - 1) / per);
   if (read) {
     ESM_LAUNCH((cache4_read_kernel<V8, HD>), grid, dim3(256), 0, s, a);
   } else {

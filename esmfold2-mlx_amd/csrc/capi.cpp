@@ -1166,7 +1166,7 @@ int cache4_args(const char* fn, esm::Cache4Args& a, const void* data, const int*
     return fail(ESM_ERR_SHAPE, "%s: n=%d T=%d Hk=%d d=%d pages=%d width=%d", fn, n, T, Hk, d, pages, width);
   if (d % 8 != 0 || d > 128) return fail(ESM_ERR_UNSUPPORTED, "%s: d=%d (a multiple of 8 up to 128)", fn, d);
   if (dtype != ESM_F16 && dtype != ESM_BF16) return fail(ESM_ERR_UNSUPPORTED, "%s: dtype=%d", fn, dtype);
-  if (T >= (1 << 24) || n >= (1 << 24) || Hk > (1 << 16) || width >= (1 << 23) || (long long)T * Hk >= (1LL << 31))
+  if (T >= (1 << 24) || n >= (1 << 22) || Hk > (1 << 16) || width >= (1 << 23) || (long long)T * Hk >= (1LL << 31))
     return fail(ESM_ERR_SHAPE, "%s: n=%d T=%d Hk=%d width=%d too large", fn, n, T, Hk, width);
   if (n == 0 || T == 0) return ESM_OK;
   if (!cu || !lens || (width > 0 && !table) || (pages > 0 && !data)) return fail(ESM_ERR_NULL, "%s: NULL pointer", fn);
