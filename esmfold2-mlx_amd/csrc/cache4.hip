@@ -12,14 +12,15 @@
 // both by v_mfma_f32_16x16x32: a wave holds 16 rows of queries (or RT times 16), a row a lane (lane % 16) of every
 // accumulator, and takes 32 keys at a time. P is bf16 whatever the type (its range is p's times the values'); for fp16 it is
 // kept as the sum of two bf16 values, 16 bits of it. No operand passes through LDS: the cache lies in the order the matrix
-// cores take (Dp = 64 or 128, the head size filled up; a page and head's pieces behind one another):
-//   key codes   [4 blocks of 16 keys][64 lanes][Dp / 8 bytes]: lane 16 g + key % 16, dword t: dims 32 t + 8 g + {0 .. 7}, the
-//               dword's nibble i dim 2 i, nibble 4 + i dim 2 i + 1
-//   key steps   [4 blocks][Dp / 64 groups][16 keys] words s << 16 | 16 + z (in the type's own 16 bits)
-//   value codes [2 blocks of 32 keys][Dp / 64][64 lanes][16 bytes]: lane 16 g + dim % 16; a byte is one key's dims 32 p +
-//               lane % 16 (low) and 16 more (high), 8 bytes a pair p; key 16 b + 4 g + e of the block is slot 4 b + e, whose
-//               byte is {0, 2, 1, 3}[slot % 4] of the dword
-//   value steps [2 blocks][groups][32 slots] s (bf16), then the same of -(16 + z) (bf16), slot 8 g + 4 b + e
+// cores take (HD = 64 or 128, the head size filled up). A page's head is 8 chunks of 8 keys, one after the other, so that
+// whoever writes 8 keys writes whole lines of memory; key 4 b + e of chunk g is row 4 g + e of block b of the 32 keys' first
+// product, and slot 4 b + e of lane group g in the second:
+//   key codes    [2 b][4 lane groups][4 e][HD / 8 bytes]: lane group l's dword t: dims 32 t + 8 l + {0 .. 7}, the dword's nibble i
+//                dim 2 i, nibble 4 + i dim 2 i + 1
+//   value codes  [HD / 64][16 dims][16 bytes]: a byte is one key's dims 32 p + row (low) and 16 more (high), 8 bytes a pair p of
+//                the two; key 4 b + e is byte {0, 2, 1, 3}[e] of dword b
+//   key steps    [2 b][groups of 64 values][4 e] words s << 16 | 16 + z (in the type's own 16 bits)
+//   value steps  [groups][8 keys] s (bf16), then the same of -(16 + z) (bf16)
 #include <type_traits>
 
 #include "common.h"
@@ -32,68 +33,79 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
-// Bytes of a page and head, and of its parts.
+// Bytes of 8 keys of a page and head, and of their parts.
 template <int HD>
 struct Page {
-  static constexpr int kGroups = HD / 64;
-  static constexpr int kKeyCodes = 64 * HD / 2, kKeySteps = 64 * kGroups * 4;
-  static constexpr int kValCodes = kKeyCodes, kValSteps = kKeySteps;
-  static constexpr int kKeyStepsAt = kKeyCodes, kValCodesAt = kKeyStepsAt + kKeySteps, kValStepsAt = kValCodesAt + kValCodes;
-  static constexpr int kBytes = kValStepsAt + kValSteps;
+  static constexpr int kGroups = HD / 64, kCodes = 8 * HD / 2, kSteps = 8 * kGroups * 4;
+  static constexpr int kValCodesAt = kCodes, kKeyStepsAt = 2 * kCodes, kValStepsAt = kKeyStepsAt + kSteps;
+  static constexpr int kChunk = kValStepsAt + kSteps, kBytes = 8 * kChunk;
 };
 static_assert(Page<64>::kBytes == cache4_page_bytes(64) && Page<128>::kBytes == cache4_page_bytes(128), "a page's size");
 
 DEV uint32_t bf16_bits(float v) { return __builtin_bit_cast(uint32_t, v) >> 16; }  // (of values that bf16 holds)
 
 // ---- writing ------------------------------------------------------------------------------------
-// rint(x / s) from inv, about 1 / s: without a division, of which eight a lane bound the writing (26 us for 8,287 rows). x has at
-// most 11 binary places and s 8, so x / s lies on k + 1/2 or 2^-12 from it at least, and x inv is off by less than 2^-16: only
-// ties can go the wrong way, and those are told by x - t s = s / 2, which is exact, and go to the even one.
-DEV float whole_steps(float x, float s, float inv) {
-  float t = rintf(x * inv);
-  const float rest = fmaf(-t, s, x);
-  if (fabsf(rest) == 0.5f * s) t = 2.f * rintf(0.5f * (t + (rest > 0.f ? 0.5f : -0.5f)));
-  return t;
+// rint(x / s) without a division, of which eight a lane would bound the writing. x has at most 11 binary places and s 8, so x /
+// s lies on k + 1/2 or 2^-12 from it at least; x inv, off by 2^-22 of itself, |x / s| <= 120, is first rounded to 2^-13, which
+// leaves a tie a tie and nothing else one, then to the even whole number. Both roundings are those of an addition that leaves the
+// whole number in the low bits of its result.
+constexpr float kWhole = 12582912.f;  // 1.5 2^23
+DEV float whole_steps(float x, float inv13) {  // inv13: 2^13 / s; the number is the result's distance from kWhole
+  const float n = fmaf(x, inv13, kWhole) - kWhole;
+  return fmaf(n, 0x1p-13f, kWhole);
 }
-// Step and zero of a group from its least and largest value; bad: it holds a NaN or an infinity, s is NaN then.
-DEV void four_bit_step(float lo, float hi, bool bad, float& s, float& inv, float& z) {
+// Step and zero of a group from its least and largest value (apart by infinity where it holds a NaN or an infinity: s is NaN).
+DEV void four_bit_step(float lo, float hi, float& s, float& inv13, float& z) {
   const float far = fmaxf(fabsf(lo), fabsf(hi)), range = hi - lo;
-  const auto reaches = [&](float t) { return 15.f * t >= range && 120.f * t >= far && t >= 0x1p-96f; };
+  const auto reaches = [&](float t) { return (15.f * t >= range) & (120.f * t >= far) & (t >= 0x1p-96f); };
   uint32_t b = __builtin_bit_cast(uint32_t, fmaxf(fmaxf(range * (1.f / 15.f), far * (1.f / 120.f)), 0x1p-96f)) & 0xffff0000u;
-  if (reaches(__builtin_bit_cast(float, b - 0x10000u))) b -= 0x10000u;  // (the products may be off by a step of fp32 either way)
-  else if (!reaches(__builtin_bit_cast(float, b))) b += 0x10000u;
+  // (the products may be off by a step of fp32 either way)
+  const bool less = reaches(__builtin_bit_cast(float, b - 0x10000u)), enough = reaches(__builtin_bit_cast(float, b));
+  b = less ? b - 0x10000u : enough ? b : b + 0x10000u;
   s = __builtin_bit_cast(float, b);
-  inv = __builtin_amdgcn_rcpf(s);
-  z = whole_steps(-lo, s, inv);
-  if (bad) s = __builtin_bit_cast(float, 0x7fc00000u), z = 0.f;
+  inv13 = __builtin_amdgcn_rcpf(s) * 0x1p13f;
+  z = whole_steps(-lo, inv13) - kWhole;
+  if (!(range < INFINITY)) s = __builtin_bit_cast(float, 0x7fc00000u), inv13 = 0.f, z = 0.f;
+}
+// 8 values' codes, a byte each.
+DEV void eight_codes(const float (&v)[8], float inv13, float z, uint32_t (&bytes)[2]) {
+  const int zero = __builtin_bit_cast(int, kWhole), zi = (int)z;
+  int u[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) u[e] = min(max(__builtin_bit_cast(int, whole_steps(v[e], inv13)) + zi, zero), zero + 15);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {  // (the low bytes of four)
+    const uint32_t a = __builtin_amdgcn_perm(u[4 * i + 1], u[4 * i], 0x0c0c0400u), b = __builtin_amdgcn_perm(u[4 * i + 3], u[4 * i + 2], 0x04000c0cu);
+    bytes[i] = a | b;
+  }
 }
 
-// Four keys of a sequence that lie behind one another in a page, their slot a multiple of 4 (those at the ends of the call's
-// rows may be of other calls): key k's row is row + k for from <= k < to. page: -1 where it is none of the cache's, or the
-// rows stand before the sequence's first place or behind its table, or in no sequence.
-struct Four {
-  int row, from, to, page, key;
+// Eight keys of a sequence that make a chunk of a page (those at the ends of the call's rows may be of other calls): key k's
+// row is row + k for from <= k < to. page: -1 where it is none of the cache's, or the rows stand before the sequence's first
+// place or behind its table, or in no sequence.
+struct Eight {
+  int row, from, to, page, chunk;
 };
 // Groups there may be of T rows in n sequences: a sequence's first and last may be incomplete, so may those of no sequence.
-static long long four_groups(long long T, int n) { return T / 4 + 2LL * n + 4; }
-DEV bool find_four(const Cache4Args& p, int what, int lane, Four& f) {
+static long long eight_groups(long long T, int n) { return T / 8 + 2LL * n + 4; }
+DEV bool find_eight(const Cache4Args& p, int what, int lane, Eight& f) {
   int before = 0, end = 0, start = 0;
   for (int i0 = 0; i0 < p.n; i0 += 64) {
     const int i = min(i0 + lane, p.n - 1);
     const int a = min(max(p.cu[i], 0), p.T), nq = min(max(p.cu[i + 1], a), p.T) - a;
-    const long long first = (long long)p.lens[i] - nq, lead = first & 3;  // (may be negative)
-    const int groups = i0 + lane < p.n && nq > 0 ? (int)((lead + nq + 3) >> 2) : 0, sum = wave_scan(groups);
+    const long long first = (long long)p.lens[i] - nq, lead = first & 7;  // (may be negative)
+    const int groups = i0 + lane < p.n && nq > 0 ? (int)((lead + nq + 7) >> 3) : 0, sum = wave_scan(groups);
     const uint64_t hit = __ballot(what < before + sum);
     if (hit) {
       const int w = __builtin_ctzll(hit), seq = i0 + w;
       const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, w); };
       const int g = what - before - of(sum - groups), nqw = of(nq), leadw = of((int)lead);
-      const long long pos = (((long long)of((int)(first >> 32)) << 32) | (uint32_t)of((int)first)) - leadw + 4LL * g;
-      f.row = of(a) - leadw + 4 * g;
-      f.from = max(0, leadw - 4 * g);
-      f.to = min(4, leadw + nqw - 4 * g);
+      const long long pos = (((long long)of((int)(first >> 32)) << 32) | (uint32_t)of((int)first)) - leadw + 8LL * g;
+      f.row = of(a) - leadw + 8 * g;
+      f.from = max(0, leadw - 8 * g);
+      f.to = min(8, leadw + nqw - 8 * g);
       f.page = -1;
-      f.key = (int)(pos & 63);
+      f.chunk = (int)(pos & 63) >> 3;
       if (pos >= 0 && pos < (long long)p.width * kCache4Page) f.page = p.table[(size_t)seq * p.width + (pos >> 6)];
       if (f.page < 0 || f.page >= p.pages) f.page = -1;
       return g >= 0 && f.row + f.from >= 0 && f.row + f.to <= p.T;
@@ -104,22 +116,24 @@ DEV bool find_four(const Cache4Args& p, int what, int lane, Four& f) {
   }
   // rows of no sequence: behind the last, then before the first
   int g = what - before;
-  f.page = -1, f.key = 0, f.from = 0;
-  f.row = end + 4 * g;
-  f.to = min(4, p.T - f.row);
+  f.page = -1, f.chunk = 0, f.from = 0;
+  f.row = end + 8 * g;
+  f.to = min(8, p.T - f.row);
   if (f.to > 0) return g >= 0;
-  f.row = 4 * (g - (p.T - end + 3) / 4);
-  f.to = min(4, start - f.row);
+  f.row = 8 * (g - (p.T - end + 7) / 8);
+  f.to = min(8, start - f.row);
   return f.row >= 0 && f.to > 0;
 }
 
-// A wave takes four keys (or their values) of 64 / (HD / 2) heads: HD / 8 lanes a key, a lane 8 of its values.
+// A wave takes the eight keys (or their values) of 64 / (HD / 2) heads, four at a time: HD / 8 lanes a key, a lane 8 of its
+// values.
 template <int HD>
-struct FourLanes {
+struct EightLanes {
   static constexpr int kLanes = HD / 8, kHeads = 64 / (4 * kLanes);
-  int c, k, item;  // 8 values of key k of an item (the keys' heads, then the values')
-  DEV FourLanes(int lane) : c(lane % kLanes), k(lane / kLanes & 3), item((blockIdx.y * 4 + (threadIdx.x >> 6)) * kHeads + lane / (4 * kLanes)) {}
-  // The wave's next item, of those that the blocks of one group of keys deal among them; `first`: the item of its lane 0.
+  int c, k, item;  // 8 values of keys k and 4 + k of an item (the keys' heads, then the values')
+  DEV EightLanes(int lane) : c(lane % kLanes), k(lane / kLanes & 3), item((blockIdx.y * 4 + (threadIdx.x >> 6)) * kHeads + lane / (4 * kLanes)) {}
+  DEV bool in(const Eight& f, int b) const { return 4 * b + k >= f.from && 4 * b + k < f.to; }
+  // The wave's next item, of those that a group's workgroups deal among them.
   DEV bool next(int items) {
     item += 4 * gridDim.y * kHeads;
     return __builtin_amdgcn_readfirstlane(item) < items;
@@ -147,143 +161,193 @@ struct FourLanes {
     b = up ? n : v;
   }
 };
-DEV uint32_t two_lanes_on(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x102, 0xf, 0xf, false); }  // row_shl:2
-
-// One item of a wave: x, the lane's 8 values, to its place.
-template <class V8, int HD>
-DEV void hold_four(const Cache4Args& p, const Four& f, const FourLanes<HD>& at, V8 x, bool there) {
-  typedef Page<HD> P;
-  const int c = at.c;
-  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, mine = live && there, in = mine && 8 * c < p.d;
-  const int h = live ? at.item - (val ? p.Hk : 0) : 0, key = f.key + at.k;
-  float v[8], lo = INFINITY, hi = -INFINITY, none = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    v[e] = (float)x[e];
-    none = fmaf(v[e], 0.f, none);  // (NaN of a NaN or an infinity)
-    lo = fminf(lo, v[e]);
-    hi = fmaxf(hi, v[e]);
-  }
-  bool bad = !(none == 0.f);
-  if (!in) lo = INFINITY, hi = -INFINITY;
-  const auto over = [&](auto ctrl) {
-    const float a = dpp_f32<decltype(ctrl)::value>(lo), b = dpp_f32<decltype(ctrl)::value>(hi);
-    const int n = __builtin_amdgcn_update_dpp(0, (int)bad, decltype(ctrl)::value, 0xf, 0xf, false);
-    lo = fminf(lo, a), hi = fmaxf(hi, b), bad = bad || n;
-  };
-  over(std::integral_constant<int, 0xB1>{});   // quad_perm(1, 0, 3, 2)
-  over(std::integral_constant<int, 0x4E>{});   // quad_perm(2, 3, 0, 1)
-  over(std::integral_constant<int, 0x141>{});  // row_half_mirror: 8 lanes, a group
-  float s, inv, z;
-  if (lo > hi) lo = hi = 0.f;  // (a group past the head's values)
-  four_bit_step(lo, hi, bad, s, inv, z);
-  uint32_t code[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) code[e] = bad || !in ? 0 : (uint32_t)fminf(fmaxf(whole_steps(v[e], s, inv) + z, 0.f), 15.f);
-  char* page = (char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes;
-  const int g = c >> 3;  // group
-  // values: a lane of low nibbles (c / 2 even) joins the high ones of the lane two further, its bytes are 8 dims of a pair
-  uint32_t bytes[2] = {0, 0}, x4, y4;
-#pragma unroll
-  for (int e = 0; e < 8; e++) bytes[e >> 2] |= code[e] << (8 * (e & 3));
-  bytes[0] |= two_lanes_on(bytes[0]) << 4;
-  bytes[1] |= two_lanes_on(bytes[1]) << 4;
-  at.gather(bytes[0], bytes[1], x4, y4);
-  if (!live) return;
-  if (!val) {
-    if (!mine) return;
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) w |= code[e] << (4 * (e >> 1) + 16 * (e & 1));
-    const int blk = key >> 4, ln = 16 * (c & 3) + (key & 15), t = c >> 2;  // dims 8 c = 32 t + 8 (c % 4)
-    *reinterpret_cast<uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t) = w;
-    if ((c & 7) == 0) {
-      const uint32_t zb = std::is_same<V8, bf16x8>::value ? bf16_bits(16.f + z)
-                                                          : (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(16.f + z));
-      *reinterpret_cast<uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (key & 15)) * 4) =
-          (__builtin_bit_cast(uint32_t, s) & 0xffff0000u) | zb;
-    }
-  } else {
-    const int blk = key >> 5, k = key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);  // (slot % 4 is at.k)
-    if (!(c & 2)) {
-      const int pair = c >> 2, dim = 8 * (c & 1);  // of the pair's low 16
-      char* dst = page + P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + (slot & 4);
-      if (f.from == 0 && f.to == 4) {
-        *reinterpret_cast<uint32_t*>(dst + 16 * (2 * at.k)) = x4;
-        *reinterpret_cast<uint32_t*>(dst + 16 * (2 * at.k + 1)) = y4;
-      } else if (mine) {
-        const int byte = (0x3120 >> (4 * at.k)) & 3;
-#pragma unroll
-        for (int e = 0; e < 8; e++) dst[16 * e + byte] = (char)(bytes[e >> 2] >> (8 * (e & 3)));
-      }
-    }
-    if ((c & 7) == 0 && mine) {
-      uint16_t* st = reinterpret_cast<uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
-      st[0] = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
-      st[2 * P::kGroups * 32] = (uint16_t)bf16_bits(-(16.f + z));
-    }
-  }
+template <int N>
+DEV uint32_t lanes_on(uint32_t v) {  // of the lane N further in the 16
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + N, 0xf, 0xf, false);  // row_shl:N
 }
 
-// Bound by a wave's latencies (starts, table, rows): with rows enough to fill the GPU one workgroup takes all heads of its four
-// keys, the next one's values asked for before this one's work.
+// One item of a wave: x, the lane's 8 values of either key, to their places. Where all eight keys are new, lanes join what
+// lies together and write 8 and 16 bytes: as single dwords and bytes the stores bound the writing (8,287 rows 23 us).
+template <class V8, int HD>
+DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& at, const V8 (&x)[2]) {
+  typedef Page<HD> P;
+  const int c = at.c, g = c >> 3;  // group
+  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, all = f.from == 0 && f.to == 8;
+  const int h = live ? at.item - (val ? p.Hk : 0) : 0;
+  char* chunk = (char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes + f.chunk * P::kChunk;
+  uint32_t own[2][2], joined[2][2], x4[2], y4[2];
+  float s[2], z[2];
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    const bool in = live && at.in(f, b) && 8 * c < p.d;
+    float v[8], lo = INFINITY, hi = -INFINITY, none = 0.f, inv;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      v[e] = (float)x[b][e];
+      none = fmaf(v[e], 0.f, none);  // (NaN of a NaN or an infinity)
+      lo = fminf(lo, v[e]);
+      hi = fmaxf(hi, v[e]);
+    }
+    if (!in) lo = INFINITY, hi = -INFINITY;
+    if (!(none == 0.f)) hi = INFINITY;
+    const auto over = [&](auto ctrl) {
+      const auto other = [&](float t) {
+        const int i = __builtin_bit_cast(int, t);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, false));
+      };
+      lo = fminf(lo, other(lo)), hi = fmaxf(hi, other(hi));
+    };
+    over(std::integral_constant<int, 0xB1>{});   // quad_perm(1, 0, 3, 2)
+    over(std::integral_constant<int, 0x4E>{});   // quad_perm(2, 3, 0, 1)
+    over(std::integral_constant<int, 0x141>{});  // row_half_mirror: 8 lanes, a group
+    if (lo > hi) lo = hi = 0.f;  // (a group past the head's values)
+    four_bit_step(lo, hi, s[b], inv, z[b]);
+    eight_codes(v, inv, z[b], own[b]);
+  }
+  if (__any(val)) {  // a lane of low nibbles (c / 2 even) joins the high ones of the lane two further: 8 dims of a pair
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) joined[b][i] = own[b][i] | lanes_on<2>(own[b][i]) << 4;
+      if (all) at.gather(joined[b][0], joined[b][1], x4[b], y4[b]);
+    }
+  }
+  uint32_t xn[2], yn[2];  // the second pair's
+  if (all && __any(val)) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) xn[b] = lanes_on<4>(x4[b]), yn[b] = lanes_on<4>(y4[b]);
+  }
+  uint32_t w[2][HD / 32];
+#pragma unroll
+  for (int b = 0; b < 2; b++) {  // dims 0, 2, 4, 6 in the low half's nibbles, 1, 3, 5, 7 in the high half's
+    w[b][0] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[b][0] |= (own[b][e >> 2] >> (8 * (e & 3)) & 15) << (4 * (e >> 1) + 16 * (e & 1));
+    w[b][1] = lanes_on<4>(w[b][0]);
+    if constexpr (HD == 128) w[b][2] = lanes_on<8>(w[b][0]), w[b][3] = lanes_on<12>(w[b][0]);
+  }
+  if (!live) return;
+  if (!val) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      // dims 8 c = 32 (c / 4) + 8 (c % 4)
+      char* dst = chunk + ((b * 4 + (c & 3)) * 4 + at.k) * (HD / 8);
+      if (all) {
+        if (c < 4) {
+          if constexpr (HD == 128) {
+            *reinterpret_cast<u32x4*>(dst) = u32x4{w[b][0], w[b][1], w[b][2], w[b][3]};
+          } else {
+            *reinterpret_cast<u32x2*>(dst) = u32x2{w[b][0], w[b][1]};
+          }
+        }
+      } else if (at.in(f, b)) {
+        *reinterpret_cast<uint32_t*>(dst + 4 * (c >> 2)) = w[b][0];
+      }
+      if ((c & 7) == 0 && at.in(f, b)) {
+        const uint32_t zb = std::is_same<V8, bf16x8>::value ? bf16_bits(16.f + z[b])
+                                                            : (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(16.f + z[b]));
+        *reinterpret_cast<uint32_t*>(chunk + P::kKeyStepsAt + ((b * P::kGroups + g) * 4 + at.k) * 4) =
+            (__builtin_bit_cast(uint32_t, s[b]) & 0xffff0000u) | zb;
+      }
+    }
+    return;
+  }
+  if (!(c & 2)) {
+    const int pair = c >> 2, dim = 8 * (c & 1);  // of the pair's low 16
+    char* dst = chunk + P::kValCodesAt + ((pair >> 1) * 16 + dim) * 16 + 8 * (pair & 1);
+    if (all) {
+      if (!(pair & 1)) {
+        *reinterpret_cast<u32x4*>(dst + 16 * (2 * at.k)) = u32x4{x4[0], x4[1], xn[0], xn[1]};
+        *reinterpret_cast<u32x4*>(dst + 16 * (2 * at.k + 1)) = u32x4{y4[0], y4[1], yn[0], yn[1]};
+      }
+    } else {
+      const int byte = (0x3120 >> (4 * at.k)) & 3;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+        if (at.in(f, b))
+#pragma unroll
+          for (int e = 0; e < 8; e++) dst[16 * e + 4 * b + byte] = (char)(joined[b][e >> 2] >> (8 * (e & 3)));
+    }
+  }
+  if ((c & 7) == 0) {
+    uint16_t* st = reinterpret_cast<uint16_t*>(chunk + P::kValStepsAt) + 8 * g + at.k;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+      if (at.in(f, b)) {
+        st[4 * b] = (uint16_t)(__builtin_bit_cast(uint32_t, s[b]) >> 16);
+        st[8 * P::kGroups + 4 * b] = (uint16_t)bf16_bits(-(16.f + z[b]));
+      }
+  }
+}
+// With rows enough to fill the GPU one workgroup takes all heads of its eight keys, the next one's values asked for before this
+// one's work; single tokens are bound by a launch and the latencies of starts, table and rows.
 template <class V8, int HD>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
   const int lane = threadIdx.x & 63;
-  Four f;
-  if (!find_four(p, blockIdx.x, lane, f) || f.page < 0) return;
-  FourLanes<HD> at(lane);
-  const bool there = at.k >= f.from && at.k < f.to;
+  Eight f;
+  if (!find_eight(p, blockIdx.x, lane, f) || f.page < 0) return;
+  EightLanes<HD> at(lane);
+  if (__builtin_amdgcn_readfirstlane(at.item) >= 2 * p.Hk) return;
+  V8 x[2];
+  const char *kr[2], *vr[2];  // this lane's part of the rows' first heads
+  bool in[2];
+#pragma unroll
+  for (int b = 0; b < 2; b++) {
+    in[b] = at.in(f, b) && 8 * at.c < p.d;
+    const long long row = in[b] ? f.row + 4 * b + at.k : 0;
+    kr[b] = (const char*)p.k + 2 * (row * p.k_st + 8 * at.c);
+    vr[b] = (const char*)p.v + 2 * (row * p.v_st + 8 * at.c);
+  }
   const auto load = [&]() {
     const bool val = at.item >= p.Hk;
-    V8 x{};
-    if (there && at.item < 2 * p.Hk && 8 * at.c < p.d)
-      x = *reinterpret_cast<const V8*>((const uint16_t*)(val ? p.v : p.k) + (long long)(f.row + at.k) * (val ? p.v_st : p.k_st) +
-                                       (long long)(at.item - (val ? p.Hk : 0)) * (val ? p.v_sh : p.k_sh) + 8 * at.c);
-    return x;
+    const long long head = 2 * (long long)(at.item - (val ? p.Hk : 0)) * (val ? p.v_sh : p.k_sh);
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      x[b] = V8{};
+      if (in[b] && at.item < 2 * p.Hk) x[b] = *reinterpret_cast<const V8*>((val ? vr[b] : kr[b]) + head);
+    }
   };
-  V8 x = load();
+  load();
   for (bool more = true; more;) {
-    const FourLanes<HD> now = at;
-    const V8 y = x;
+    const EightLanes<HD> now = at;
+    const V8 y[2] = {x[0], x[1]};
     more = at.next(2 * p.Hk);
-    if (more) x = load();  // (the next item's, before this one's work)
-    hold_four<V8, HD>(p, f, now, y, there);
+    if (more) load();
+    hold_eight<V8, HD>(p, f, now, y);
   }
 }
 
+// What the rows' places hold, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
 template <class V8, int HD>
-DEV void give_four(const Cache4Args& p, const Four& f, const FourLanes<HD>& at, bool there) {
+DEV void give_four(const Cache4Args& p, const Eight& f, const EightLanes<HD>& at, int b) {
   typedef Page<HD> P;
-  const int c = at.c, g = c >> 3, key = f.key + at.k;
-  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, mine = live && there && 8 * c < p.d;
+  const int c = at.c, g = c >> 3;
+  const bool val = at.item >= p.Hk, live = at.item < 2 * p.Hk, mine = live && at.in(f, b) && 8 * c < p.d;
   const int h = live ? at.item - (val ? p.Hk : 0) : 0;
-  V8* dst = reinterpret_cast<V8*>((uint16_t*)(val ? p.vo : p.ko) + ((size_t)(mine ? f.row + at.k : 0) * p.Hk + h) * p.d + (mine ? 8 * c : 0));
+  V8* dst = reinterpret_cast<V8*>((uint16_t*)(val ? p.vo : p.ko) + ((size_t)(mine ? f.row + 4 * b + at.k : 0) * p.Hk + h) * p.d + (mine ? 8 * c : 0));
   if (f.page < 0) {
     if (mine) *dst = V8{};
     return;
   }
-  const char* page = (const char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes;
+  const char* chunk = (const char*)p.data + ((size_t)f.page * p.Hk + h) * P::kBytes + f.chunk * P::kChunk;
   float s, z;
   uint32_t code[8];
   if (val) {  // (a head's lanes exchange their bytes)
-    const int blk = key >> 5, k = key & 31, gk = (k & 15) >> 2, slot = 4 * (k >> 4) + (k & 3);
     const int pair = c >> 2, dim = 8 * (c & 1);
-    const char* src = page + P::kValCodesAt + ((blk * P::kGroups + (pair >> 1)) * 64 + 16 * gk + dim) * 16 + 8 * (pair & 1) + (slot & 4);
+    const char* src = chunk + P::kValCodesAt + ((pair >> 1) * 16 + dim) * 16 + 8 * (pair & 1) + 4 * b;
     uint32_t bytes[2];
     at.scatter(*reinterpret_cast<const uint32_t*>(src + 16 * (2 * at.k)), *reinterpret_cast<const uint32_t*>(src + 16 * (2 * at.k + 1)),
                bytes[0], bytes[1]);  // (the lanes of high nibbles read the same bytes)
 #pragma unroll
     for (int e = 0; e < 8; e++) code[e] = (bytes[e >> 2] >> (8 * (e & 3) + 2 * (c & 2))) & 15;
-    const uint16_t* st = reinterpret_cast<const uint16_t*>(page + P::kValStepsAt) + blk * P::kGroups * 32 + g * 32 + 8 * gk + slot;
+    const uint16_t* st = reinterpret_cast<const uint16_t*>(chunk + P::kValStepsAt) + 8 * g + 4 * b + at.k;
     s = __builtin_bit_cast(float, (uint32_t)st[0] << 16);
-    z = -__builtin_bit_cast(float, (uint32_t)st[2 * P::kGroups * 32] << 16) - 16.f;
+    z = -__builtin_bit_cast(float, (uint32_t)st[8 * P::kGroups] << 16) - 16.f;
   } else {
-    const int blk = key >> 4, ln = 16 * (c & 3) + (key & 15), t = c >> 2;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (blk * 64 + ln) * (HD / 8) + 4 * t);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(chunk + ((b * 4 + (c & 3)) * 4 + at.k) * (HD / 8) + 4 * (c >> 2));
 #pragma unroll
     for (int e = 0; e < 8; e++) code[e] = (w >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
-    const uint32_t st = *reinterpret_cast<const uint32_t*>(page + P::kKeyStepsAt + ((blk * P::kGroups + g) * 16 + (key & 15)) * 4);
+    const uint32_t st = *reinterpret_cast<const uint32_t*>(chunk + P::kKeyStepsAt + ((b * P::kGroups + g) * 4 + at.k) * 4);
     s = __builtin_bit_cast(float, st & 0xffff0000u);
     z = std::is_same<V8, bf16x8>::value ? __builtin_bit_cast(float, st << 16) - 16.f
                                         : (float)__builtin_bit_cast(half_t, (uint16_t)st) - 16.f;
@@ -294,17 +358,17 @@ DEV void give_four(const Cache4Args& p, const Four& f, const FourLanes<HD>& at, 
   for (int e = 0; e < 8; e++) y[e] = (decltype(+y[e]))(s * ((float)code[e] - z));
   *dst = y;
 }
-
-// What the rows' places hold, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
 template <class V8, int HD>
 __global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Args p) {
   const int lane = threadIdx.x & 63;
-  Four f;
-  if (!find_four(p, blockIdx.x, lane, f)) return;
-  FourLanes<HD> at(lane);
-  const bool there = at.k >= f.from && at.k < f.to;
+  Eight f;
+  if (!find_eight(p, blockIdx.x, lane, f)) return;
+  EightLanes<HD> at(lane);
+  if (__builtin_amdgcn_readfirstlane(at.item) >= 2 * p.Hk) return;
   do {
-    give_four<V8, HD>(p, f, at, there);
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+      if (4 * b < f.to && 4 * b + 4 > f.from) give_four<V8, HD>(p, f, at, b);
   } while (at.next(2 * p.Hk));
 }
 
@@ -444,34 +508,33 @@ struct Rows4 {
   };
   static DEV void load_keys(Keys& k, const char* page, int half, int lane) {
     typedef Page<HD> P;
-    const int g = lane >> 4;
+    const int g = lane >> 4, r = lane & 15;
+    const char* codes = page + (4 * half + (r >> 2)) * P::kChunk + (4 * g + (r & 3)) * (HD / 8);
+    const char* steps = page + (4 * half + g) * P::kChunk + P::kKeyStepsAt;
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-      const char* src = page + ((2 * half + b) * 64 + lane) * (HD / 8);
       if constexpr (HD == 128) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(src);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(codes + 2 * HD * b);
 #pragma unroll
         for (int t = 0; t < 4; t++) k.kc[b][t] = v[t];
       } else {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(src);
+        const u32x2 v = *reinterpret_cast<const u32x2*>(codes + 2 * HD * b);
         k.kc[b][0] = v[0], k.kc[b][1] = v[1];
       }
 #pragma unroll
-      for (int i = 0; i < G; i++)
-        k.ks[b][i] = *reinterpret_cast<const u32x4*>(page + P::kKeyStepsAt + (((2 * half + b) * G + i) * 16 + 4 * g) * 4);
+      for (int i = 0; i < G; i++) k.ks[b][i] = *reinterpret_cast<const u32x4*>(steps + (b * G + i) * 16);
     }
   }
   static DEV void load_values(Keys& k, const char* page, int half, int lane) {
     typedef Page<HD> P;
-    const int g = lane >> 4;
+    const char* chunk = page + (4 * half + (lane >> 4)) * P::kChunk;
 #pragma unroll
     for (int i = 0; i < G; i++) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(page + P::kValCodesAt + ((half * G + i) * 64 + lane) * 16);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(chunk + P::kValCodesAt + (16 * i + (lane & 15)) * 16);
 #pragma unroll
       for (int t = 0; t < 4; t++) k.vc[4 * i + t] = v[t];
-      const char* st = page + P::kValStepsAt + (half * G + i) * 64 + 16 * g;
-      k.vs[i] = *reinterpret_cast<const u32x4*>(st);
-      k.vz[i] = *reinterpret_cast<const u32x4*>(st + 128 * G);
+      k.vs[i] = *reinterpret_cast<const u32x4*>(chunk + P::kValStepsAt + 16 * i);
+      k.vz[i] = *reinterpret_cast<const u32x4*>(chunk + P::kValStepsAt + 16 * (G + i));
     }
   }
 
@@ -522,7 +585,7 @@ struct Rows4 {
       for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          s[r][j >> 2][j & 3] = key0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim[r] ? s[r][j >> 2][j & 3] : -INFINITY;
+          s[r][j >> 2][j & 3] = key0 + 8 * g + j <= lim[r] ? s[r][j >> 2][j & 3] : -INFINITY;
     }
     float p[RT][8];
 #pragma unroll
@@ -559,7 +622,7 @@ struct Rows4 {
           const uint32_t w = k.vs[i][j >> 1];
           const float st = __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16);
           float v = p[r][j] * st;
-          if (MASKED) v = key0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim[r] ? v : 0.f;
+          if (MASKED) v = key0 + 8 * g + j <= lim[r] ? v : 0.f;
           hi[r][j] = (__bf16)v;
           if (T::kSplit) lo[r][j] = (__bf16)(v - (float)hi[r][j]);
         }
@@ -810,9 +873,9 @@ hipError_t launch_cache4_attention(const Cache4Args& a, bool bf16, const Cache4P
 
 template <class V8, int HD>
 static hipError_t launch_write_t(const Cache4Args& a, bool read, hipStream_t s) {
-  const int per = 4 * FourLanes<HD>::kHeads;  // heads of a workgroup, keys' and values'
+  const int per = 4 * EightLanes<HD>::kHeads;  // heads of a workgroup, keys' and values'
   // all heads in one workgroup where the keys alone fill the GPU, else as many workgroups as there are heads for
-  const long long groups = four_groups(a.T, a.n);
+  const long long groups = eight_groups(a.T, a.n);
   const dim3 grid((unsigned)groups, groups >= 1024 ? 1 : (2 * a.Hk + per - 1) / per);
   if (read) {
     ESM_LAUNCH((cache4_read_kernel<V8, HD>), grid, dim3(256), 0, s, a);
