@@ -24,6 +24,7 @@ from torch import nn
 from torch.nn.modules.module import _has_any_global_hook
 
 from . import kernels
+from .f8 import F8Linear, F8Rows
 from .q8 import Q8Linear
 from .rotary import Rotary
 
@@ -47,17 +48,17 @@ HF_NORMS = {"ln1_w": "input_layernorm.weight", "ln1_b": "input_layernorm.bias", 
 _LAYER_KEY = re.compile(r"layers\.(\d+)\.([A-Za-z0-9_]+)")
 
 
-def hf_layer(tensors, i: int, device=None, linear=Q8Linear) -> tuple[dict, dict]:
+def hf_layer(tensors, i: int, device=None, linear=Q8Linear, fused: bool = False) -> tuple[dict, dict]:
     """One block from the published HF-named fp32 tensors (``tensors[f"esmc.layers.{i}.{name}"]``):
     (LayerNorm parameters by cache name, {linear: Q8Linear}), each linear quantised on the GPU
     from fp32 with MLX's affine 8-bit scheme (layer_params, mlx_esmc.py:53-75), or as ``linear``
-    (``F8Linear``) has it."""
+    (``F8Linear``) has it; ``fused``: w1 as a gated linear, whose end is the SwiGLU."""
     get = lambda name: tensors[f"esmc.layers.{i}.{name}"]  # noqa: E731
     ln = {n: get(h).detach().float() for n, h in HF_NORMS.items()}
     lin = {}
     for n, parts in HF_LINEARS.items():
         w = torch.cat([get(h).detach().float() for h in parts]) if len(parts) > 1 else get(parts[0]).detach().float()
-        lin[n] = linear.from_float(w, device=device)
+        lin[n] = linear.from_float(w, device=device, gated=True) if fused and n == "w1" else linear.from_float(w, device=device)
     return ln, lin
 
 
@@ -74,6 +75,8 @@ def _as_defined(m) -> bool:
 
 
 class EsmcBlock(nn.Module):
+    fused = False
+
     def __init__(self, ln1_w, ln1_b, q_ln, k_ln, ln2_w, ln2_b, wqkv: Q8Linear, wo: Q8Linear, w1: Q8Linear,
                  w2: Q8Linear, n_heads: int, device=None):
         super().__init__()
@@ -88,7 +91,9 @@ class EsmcBlock(nn.Module):
         self.D = wo.out_features
         self.F = w2.in_features
         self.n_heads = n_heads
-        if self.D != n_heads * 64 or wqkv.out_features != 3 * self.D or w1.out_features != 2 * self.F:
+        # a gated w1 ends with the SwiGLU itself, and the block takes its rows in e4m3 (``run_rows``)
+        self.fused = bool(getattr(w1, "gated", False))
+        if self.D != n_heads * 64 or wqkv.out_features != 3 * self.D or w1.out_features != (1 if self.fused else 2) * self.F:
             raise ValueError(f"ESMC block shapes: D={self.D}, heads={n_heads}, wqkv {wqkv.out_features}, "
                              f"w1 {w1.out_features}, w2 in {self.F}")
 
@@ -136,7 +141,10 @@ class EsmcBlock(nn.Module):
     def ffn(self, h2: torch.Tensor):
         """w2(silu(x1) * x2) with [x1 | x2] = w1(h2) (before the residual's / res_scale), as w2's
         split-K partials: (partials, splits) for ``esmc_layer_norm(..., y_parts=...)``."""
-        act = self.w1.swiglu(h2) if self.w1.pair_rows else kernels.esmc_swiglu(self.w1(h2))
+        if self.fused:
+            act = self.w1(h2, activation="silu")
+        else:
+            act = self.w1.swiglu(h2) if self.w1.pair_rows else kernels.esmc_swiglu(self.w1(h2))
         return self.w2.partials(act)
 
     def _native_linears(self):
@@ -186,6 +194,23 @@ class EsmcBlock(nn.Module):
         kernels.esmc_layer_norm(x_mid, next_w, next_b, EPS, y_parts=self.ffn(h2), alpha=1.0 / res_scale, x_out=x_out,
                                 out=out, fp32_out=out.dtype == torch.float32)
 
+    def takes_rows(self) -> bool:
+        """Whether ``run_rows`` is this block: e4m3 linears, a gated w1, and nothing put in the place of a part of it."""
+        return (self.fused and type(self) is EsmcBlock and not any(m in self.__dict__ for m in ("attention", "ffn", "run_packed"))
+                and (EsmcBlock.attention, EsmcBlock.ffn, EsmcBlock.run_packed) == _PACKED_METHODS
+                and all(type(getattr(self, m)) is F8Linear for m in LINEARS))
+
+    def run_rows(self, x: torch.Tensor, rows: F8Rows, cu: torch.Tensor, positions: torch.Tensor, rotary: Rotary,
+                 res_scale: float):
+        """``run_packed`` on e4m3 linears alone: ``rows`` = LN1(x) in e4m3, brought there by the norm itself, as are the
+        feed-forward's. (x after the attention, the feed-forward's part before / res_scale): the next norm adds them."""
+        T, D = x.shape
+        q, k, v = self.wqkv(rows).view(T, 3, self.n_heads, 64).unbind(1)
+        rotary(q, k, positions, norm="layer", over="row", q_w=self.q_ln, k_w=self.k_ln, eps=EPS, out=(q, k))
+        o = kernels.packed_attention(q, k, v, cu).view(T, D)
+        x_mid, h2 = _norm_rows(x, self.wo(o), self.ln2_w, self.ln2_b, 1.0 / res_scale)
+        return x_mid, self.w2(self.w1(h2, activation="silu"))
+
     def forward(self, x: torch.Tensor, sequence_id=None, res_scale: float = 1.0) -> torch.Tensor:
         """One block on an fp32 residual [B, L, D] (the reference's block_forward, mlx_esmc.py:84-102)."""
         x = x.to(torch.float32).contiguous()
@@ -198,6 +223,13 @@ class EsmcBlock(nn.Module):
 
 
 _BLOCK_METHODS = (EsmcBlock.attention, EsmcBlock.ffn)
+_PACKED_METHODS = (*_BLOCK_METHODS, EsmcBlock.run_packed)
+
+
+def _norm_rows(x, y, w, b, alpha: float, x_out=None):
+    """(x + alpha y, its LayerNorm in e4m3 as the linears take it)."""
+    x, h = kernels.add_norm_f8(x, y, w, b, alpha=alpha, norm="layer", eps=EPS, dtype=torch.float16, sum_out=x_out)
+    return x, F8Rows(*h, x.shape[:1], x.shape[1], torch.float16)
 
 
 def _chain_ids(sequence_id, B: int, L: int, device):
@@ -260,13 +292,17 @@ class HipEsmc(nn.Module):
 
     @classmethod
     def from_hf(cls, tensors, n_layers: int | None = None, n_heads: int = 40, cache=None,
-                device=None, linear=Q8Linear) -> "HipEsmc":
+                device=None, linear=Q8Linear, fused: bool = False) -> "HipEsmc":
         """From the published fp32 checkpoint's HF-named tensors (any mapping, e.g. a dict or a
         lazy shard reader: "esmc.embed_tokens.weight", "esmc.norm.weight",
         "esmc.layers.{i}.…"), every linear quantised to 8 bits on the GPU (the reference's
         from_shards, mlx_esmc.py:116-137). With ``cache`` (a path): load it when it exists,
         otherwise convert and write it there in the layout ``from_cache`` reads. ``linear``: the
-        class of the linears (``F8Linear`` for e4m3; the cache holds ``Q8Linear``'s arrays only)."""
+        class of the linears (``F8Linear`` for e4m3; the cache holds ``Q8Linear``'s arrays only). ``fused`` (``F8Linear``
+        only): the norms bring their rows to e4m3 themselves, from fp32, and the feed-forward's SwiGLU runs at the end of its
+        linear, on the products before their rounding: fewer roundings and launches in the packed form."""
+        if fused and linear is not F8Linear:
+            raise ValueError("fused norms and linears are F8Linear's")
         if cache is not None and linear is not Q8Linear:
             raise ValueError("the converted-weight cache holds Q8Linear's arrays")
         if cache is not None and os.path.exists(str(cache)):
@@ -277,7 +313,7 @@ class HipEsmc(nn.Module):
             n_layers = len(idx)
         layers = []
         for i in range(n_layers):
-            ln, lin = hf_layer(tensors, i, device=device, linear=linear)
+            ln, lin = hf_layer(tensors, i, device=device, linear=linear, fused=fused)
             layers.append(EsmcBlock(ln["ln1_w"], ln["ln1_b"], ln["q_ln"], ln["k_ln"], ln["ln2_w"], ln["ln2_b"],
                                     lin["wqkv"], lin["wo"], lin["w1"], lin["w2"], n_heads, device=device))
         esmc = cls(tensors["esmc.embed_tokens.weight"].detach().float(), layers,
@@ -350,9 +386,20 @@ class HipEsmc(nn.Module):
         hs[0] = self.embed[ids]
         if T == 0:
             return hs
+        states = hs.unbind(0)
+        if n and all(b.takes_rows() if isinstance(b, EsmcBlock) else False for b in self.layers):
+            first = self.layers[0]
+            _, rows = _norm_rows(states[0], None, first.ln1_w, first.ln1_b, 1.0)
+            for i, blk in enumerate(self.layers[:-1]):
+                nxt = self.layers[i + 1]
+                x_mid, y = blk.run_rows(states[i], rows, cu, positions, self._rotary, self.res_scale)
+                _, rows = _norm_rows(x_mid, y, nxt.ln1_w, nxt.ln1_b, 1.0 / self.res_scale, states[i + 1])
+            x_mid, y = self.layers[-1].run_rows(states[n - 1], rows, cu, positions, self._rotary, self.res_scale)
+            kernels.esmc_layer_norm(x_mid, self.norm_w, None, EPS, y=y, alpha=1.0 / self.res_scale, x_out=x_mid,
+                                    out=states[n], fp32_out=True)
+            return hs
         h = kernels.esmc_layer_norm(hs[0], self.layers[0].ln1_w, self.layers[0].ln1_b, EPS)
         x_last = torch.empty(T, D, dtype=torch.float32, device=dev)
-        states = hs.unbind(0)
         for i, blk in enumerate(self.layers):
             run = blk.run_packed if hasattr(blk, "run_packed") else partial(EsmcBlock.run_packed, blk)  # (refuses)
             last = i + 1 == n
