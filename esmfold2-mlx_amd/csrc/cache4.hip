@@ -2,7 +2,7 @@
 //
 // x ~ s (c - z) per key (or value) and group of 64 values of a head: s the least bf16 value, 2^-96 or more, of which 15 reach
 // over the group's range and 120 to its farthest value from zero; z = rint(-min / s), c = clamp(rint(x / s) + z, 0, 15). A
-// group that holds a NaN or an infinity reads as NaN (s is).
+// group that holds a NaN or an infinity, or whose range passes fp32, reads as NaN (s is).
 //
 // The matrix cores take codes as they are: in bf16 0x4180 | c << 3 is 16 + c, in fp16 0x4c00 | c << 6, one instruction for
 // two codes and a shift. Products with 16 + c and with -(16 + z) cancel in fp32, and s multiplies what comes out (keys) or the
@@ -167,7 +167,7 @@ DEV uint32_t lanes_on(uint32_t v) {  // of the lane N further in the 16
 }
 
 // One item of a wave: x, the lane's 8 values of either key, to their places. Where all eight keys are new, lanes join what
-// lies together and write 8 and 16 bytes: as single dwords and bytes the stores bound the writing (8,287 rows 23 us).
+// lies together and write 8 and 16 bytes.
 template <class V8, int HD>
 DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& at, const V8 (&x)[2]) {
   typedef Page<HD> P;
@@ -280,7 +280,9 @@ DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& a
   }
 }
 // With rows enough to fill the GPU one workgroup takes all heads of its eight keys, the next one's values asked for before this
-// one's work; single tokens are bound by a launch and the latencies of starts, table and rows.
+// one's work: 8,287 rows of 8 heads of 128 in 18.0 us, 43 MB, bound by its 30 vector instructions a value of a lane (with
+// divisions, and a branch for their ties, 23 us however the codes were stored). 64 single tokens 4.1 us: a launch and the
+// latencies of starts, table and rows.
 template <class V8, int HD>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
   const int lane = threadIdx.x & 63;
@@ -317,7 +319,8 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
   }
 }
 
-// What the rows' places hold, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0.
+// What the rows' places hold, as 16-bit values (rounded once): the inverse of the above. Rows without a place are 0. The
+// same 8,287 rows 10.9 us, 4 TB/s, bound by memory.
 template <class V8, int HD>
 DEV void give_four(const Cache4Args& p, const Eight& f, const EightLanes<HD>& at, int b) {
   typedef Page<HD> P;
@@ -649,7 +652,11 @@ struct Rows4 {
 };
 
 // A workgroup takes 16 RT rows (query, head of the group; row = query G + head) of a sequence and key head and one chunk of
-// its keys, a page a wave in turn, the next 32 keys' operands in flight; the waves' results are joined through LDS.
+// its keys, a page a wave in turn, the next 32 keys' operands in flight; the waves' results are joined through LDS. Bound by the
+// cache's bytes where contexts are long (32 of 8,000 to 24,400 keys, 8 key heads of 128, 597 MB in 122 us, 4.9 TB/s of a copy's
+// 5.1), else by a launch, latencies one after the other (lengths, table, first page) and 250 vector instructions a wave for 32
+// keys and 16 rows: 8 tokens, 38 MB 14.4 us; 16 x 5 tokens, 21 MB in three tiles a sequence 20.5. (64 keys in flight a wave took
+// all registers: 32 contexts 171 us, 8 tokens 23; more chunks than target's 256 a head cost more than they fill.)
 template <class T, int HD, int RT>
 __global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(Cache4Args p) {
   typedef Page<HD> P;
@@ -673,15 +680,6 @@ __global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(
       const int c = 32 * t + 8 * (lane >> 4);
       w.q[r][t] = typename T::v8{};
       if (ok && c < p.d) w.q[r][t] = *reinterpret_cast<const typename T::v8*>(src + 2 * c);
-    }
-#pragma unroll
-    for (int u = 0; u < R::G; u++) {
-      float t = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) t += (float)w.q[r][2 * u + j][e];
-      w.qs[r][u] = row_sum4(t);
     }
     w.m[r] = -INFINITY;
     w.l[r] = 0.f;
@@ -711,6 +709,18 @@ __global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(
     const char* page = at(id);
     R::load_keys(k, page, 0, lane);
     R::load_values(k, page, 0, lane);
+    __builtin_amdgcn_sched_barrier(0);  // (q's sums while the first keys are on their way)
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int i = 0; i < R::G; i++) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) t += (float)w.q[r][2 * i + j][e];
+        w.qs[r][i] = row_sum4(t);
+      }
     bool good = id >= 0 && id < p.pages;  // (a page of no cache: not seen)
     int u = 0, pg = page0;                // halves of pages
     // to the next half: what its step takes, and where the one behind it lies (behind the last page: that one again, not used)
@@ -786,7 +796,7 @@ __global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(
 }
 
 // The chunks of one (query, head) row: a thread takes one chunk's m and l, then groups of HD / 4 lanes sum O over every
-// 1024 / HD-th chunk, joined through LDS.
+// 1024 / HD-th chunk, joined through LDS. 4.2 to 5.3 us: a launch and three latencies.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args p, int rows) {
   __shared__ float weight[256], red[2][4];

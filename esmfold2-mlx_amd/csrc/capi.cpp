@@ -1208,7 +1208,8 @@ int cache4_read(void* k, void* v, const void* data, const int* cu, const int* le
   esm::Cache4Args a{};
   const int rc = cache4_args("cache4_read", a, data, cu, lens, table, n, T, Hk, d, pages, width, dtype);
   if (rc != ESM_OK) return rc;
-  if (n == 0 || T == 0) return ok();
+  if (T == 0) return ok();
+  a.T = T, a.Hk = Hk, a.d = d;  // (no sequence: rows without a place)
   if (!k || !v) return fail(ESM_ERR_NULL, "cache4_read: NULL pointer");
   if (!aligned16(k) || !aligned16(v)) return fail(ESM_ERR_ALIGN, "cache4_read: k and v must be 16-byte aligned");
   a.ko = k, a.vo = v;

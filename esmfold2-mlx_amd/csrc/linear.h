@@ -138,7 +138,8 @@ DEV void part16(float* part, long long row, int pieces, int ng, int g, const f32
   for (int j = 0; j < 4; j++) *reinterpret_cast<f32x4*>(dst + 4 * j) = v[j];
 }
 
-// The sum of the splits in their order and the end of the linear: a thread takes 16 packed columns of a row.
+// The sum of the splits in their order and the end of the linear: a thread takes 16 packed columns of a row. Bound by a launch
+// and two latencies: 238 rows of 2,560 4.8 us.
 template <class V8>
 __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ part, LinearEnd p, int M, int pieces, int splits) {
   const size_t each = (size_t)M * pieces * 4, step = each * 16;

@@ -223,6 +223,15 @@ def _rows8(pkg, x, y, w):
     return s, rows.codes.view(torch.uint8), rows.scales
 
 
+def test_rows_of_a_cache_without_sequences_read_as_zeros(gpu_lib, pkg):
+    cache = pkg.cache4.Cache4(2, 2, 64)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    for _ in range(2):  # (memory that held something else)
+        torch.full((2, 900, 2, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+        for t in cache.read(i32(0), none, none.view(0, 3), rows=900):
+            assert t.shape == (900, 2, 64) and not bool(t.any())
+
+
 def _calls(pkg):
     """Each call's ordinary forms, results as lists of tensors."""
     k = pkg.kernels
