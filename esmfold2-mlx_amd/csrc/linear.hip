@@ -266,10 +266,12 @@ __global__ __launch_bounds__(64 * WM * WN) void linear16_tiles_kernel(L16Args p)
 
 // ---- tiles of 256 x 256 ---------------------------------------------------------------------------
 // The same in steps of 32 k, of which LDS holds four where it holds two of 64. Rows of x land 64 bytes a row, 16-byte chunk c of
-// row r at c ^ (r / 4 % 4), so that a fragment's 16 rows cover the banks. A step's first fragments are read at the end of the step before
-// it, behind the products, as the barrier between them stands for the slot after the next: with the slot itself the
-// waves would leave each barrier only to wait for LDS. Bound by the matrix cores' power: 8,192 x 8,192 x 8,192 in 800 to 830 us, 1.37
-// PFLOP/s (a library's product 785); 3,481 x 2,560 x 7,680 128 us (121).
+// row r at c ^ (-(r / 4) % 4), so that the 16 lanes that LDS serves at a time, rows of two chunks, cover the banks (with c ^ (r /
+// 4 % 4) two of them met, a fifth of the cycles, which the clock made up for: the time was the same). A step's first fragments
+// are read at the end of the step before it, behind the products, as the barrier between them stands for the slot after the next:
+// with the slot itself the waves would leave each barrier only to wait for LDS. Bound by the matrix cores' power, 69% busy below
+// 1.6 GHz: 8,192 x 8,192 x 8,192 in 800 to 890 us by the box, up to 1.37 PFLOP/s (a library's product 785 on the fastest); 3,481 x
+// 2,560 x 7,680 128 to 135 us (121).
 template <class V8, int MB, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void linear16_large_kernel(L16Args p) {
   constexpr int NW = WM * WN, kX = 1024 * MB * WM, kW = 4096 * WN, kSlot = kX + kW;  // bytes a slot
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear16_large_kernel(L16Args p)
   const dma_src_t rw = dma_src((const char*)p.w + (size_t)ng0 * Ks * 4096, kBufRange);
   const uint32_t base = lds_address(lds);
   // where this lane reads x from: row lane / 4 of a load's 16, the chunk that lands at place lane % 4 of it
-  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  const int chunk = (lane & 3) ^ (-(lane >> 4) & 3);
   uint32_t xo[kLoadsX];
 #pragma unroll
   for (int i = 0; i < kLoadsX; i++) {
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear16_large_kernel(L16Args p)
   for (int i = 0; i < S - 1; i++)
 #pragma unroll
     for (int u = 0; u < kLoads; u++) load(min(k0 + i, k1 - 1), i, u);  // (past the last step: loaded again, not used)
-  const int mine = kX + 4096 * wn + 16 * lane, rows = 1024 * MB * wm + 64 * (lane & 15) + 16 * ((lane >> 4) ^ ((lane >> 2) & 3));
+  const int mine = kX + 4096 * wn + 16 * lane, rows = 1024 * MB * wm + 64 * (lane & 15) + 16 * ((lane >> 4) ^ (-(lane >> 2) & 3));
   const auto weight = [&](int slot, int j) { return *reinterpret_cast<const V8*>(lds + slot * kSlot + mine + 1024 * j); };
   const auto row = [&](int slot, int b) { return *reinterpret_cast<const V8*>(lds + slot * kSlot + rows + 1024 * b); };
   V8 wa[4], wb[4], x[R];
