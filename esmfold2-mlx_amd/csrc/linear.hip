@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_some_kernel(L16Args p
 // Workgroup tile of 16 MB WM rows of x by WN pieces of weights, WM x WN waves of 16 MB x 64 each. A step is 64 k: both
 // operands come by direct loads into a ring of S slots, S - 1 steps ahead. Rows of x land 128 bytes a row, 16-byte chunk c of row
 // r at c ^ (r % 8), so that a load takes whole lines of memory and a fragment's rows lie in different banks. Bound by what fills
-// LDS and by tiles too few for the CUs: 238 rows, 5,120 -> 2,560 in 64 x 128 18.1 us and 4.8 for its splits' sum (a library's
+// LDS and by tiles too few for the CUs: 238 rows, 5,120 -> 2,560 in 64 x 256, K in six, 18.1 us and 4.8 for its splits' sum (a library's
 // product 21.6), 1,000 rows, 2,560 -> 2,560 in 64 x 256 24.2 (23.7).
 template <class V8, int MB, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void linear16_tiles_kernel(L16Args p) {

@@ -7,7 +7,7 @@
 //
 // W waves take a row, a lane NIT pieces of 8 values, kept in registers between the sums and the output: every value
 // is read once. Bound by bytes: 16,384 rows of 8,192 in 215 us, 5.0 TB/s where a large copy runs 5.1; 3,481 rows of 2,560, fp32 to
-// e4m3, 23.7 us, 4.1 TB/s; small calls by a launch and two latencies, 8 rows of 2,560 4.0 us. Each wave's mean and squares about it are
+// e4m3, 23.7 us, 4.1 TB/s; small calls by a launch and two latencies, 8 rows of 4,096 4.0 us. Each wave's mean and squares about it are
 // joined as  mean = sum n_w mean_w / n,  M2 = sum M2_w + n_w (mean_w - mean)^2  with one barrier.
 #include <type_traits>
 

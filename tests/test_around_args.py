@@ -140,3 +140,34 @@ def test_gated_rows_are_a_permutation(pkg):
         for r in (0, 5, 17, 63):
             g, j, e = r // 16, r % 16 // 4, r % 4
             assert int(order[r]) == 8 * g + 4 * (j // 2) + e + (N // 2) * (j % 2)
+
+
+def test_the_norm_and_the_activations_restated(pkg):
+    import torch.nn.functional as F
+
+    from oracle import around as A
+    g = torch.Generator().manual_seed(1)
+    x, y, w, b = (torch.randn(*s, generator=g, dtype=torch.float64).float() for s in ((5, 40), (5, 40), (40,), (40,)))
+    s, _, h, bound = A.add_norm(x, y, 0.5, w, b, "layer", 1e-5)
+    assert torch.allclose(h, F.layer_norm(x.double() + 0.5 * y.double(), (40,), w.double(), b.double(), 1e-5), rtol=1e-12, atol=1e-12)
+    _, _, h, _ = A.add_norm(x, None, 1.0, w, None, "rms", 1e-6)
+    assert torch.allclose(h, F.rms_norm(x.double(), (40,), w.double(), 1e-6), rtol=1e-12, atol=1e-12) and bool((bound > 0).all())
+    z = torch.cat([torch.linspace(-30, 30, 601, dtype=torch.float64), torch.tensor([0.0, -0.0, 1e-30])])
+    for kind, ref in ((None, lambda t: t), ("relu", F.relu), ("gelu", F.gelu), ("gelu_tanh", lambda t: F.gelu(t, approximate="tanh")), ("silu", F.silu)):
+        assert torch.allclose(A.activate(z, kind)[0], ref(z), rtol=1e-9, atol=1e-12), kind
+    z, res = torch.randn(3, 8, generator=g, dtype=torch.float64), torch.randn(3, 4, generator=g).half()
+    y, _ = A.end(z, torch.zeros_like(z), w[:8], "silu", True, res, 2.0, torch.float16)
+    u = z + w[:8].double()
+    assert torch.allclose(y, res.double() + 2 * F.silu(u[:, :4]) * u[:, 4:], rtol=1e-9, atol=1e-12)
+
+
+def test_the_step_is_the_least_that_reaches(pkg):
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(200, 1, 64, generator=g) * torch.exp(4 * torch.randn(200, 1, 1, generator=g)) + 3 * torch.randn(200, 1, 1, generator=g)
+    x = x.bfloat16().double()
+    _, s, _ = C4.hold(x)
+    s = s[..., :1]
+    less = (s.float().view(torch.int32) - (1 << 16)).view(torch.float32).double()  # the bf16 value below
+    lo, hi, far = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True), x.abs().amax(-1, keepdim=True)
+    reaches = lambda t: (15 * t >= hi - lo) & (120 * t >= far)  # noqa: E731
+    assert bool(reaches(s).all()) and not bool(reaches(less).any())
