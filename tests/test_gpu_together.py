@@ -311,3 +311,60 @@ def test_both_ways_refuse_the_same(gpu_lib, pkg, monkeypatch):
     short = codes()
     monkeypatch.setattr(pkg.capi, "bind", pkg.capi._LongWay)
     assert short == codes() == [c for _, c in calls]
+
+
+def test_nothing_to_do(gpu_lib, pkg):
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    x = torch.zeros(0, 256, dtype=torch.bfloat16, device=DEV)
+    s, rows = pkg.norm.AddNorm(torch.ones(256))(x, x, f8=True)
+    assert s.shape == (0, 256) and rows.dequantized().shape == (0, 256) and rows.codes.shape == (0, 256)
+    w = torch.ones(128, 256, device=DEV)
+    for gated in (False, True):
+        lin, e8 = pkg.linear.Linear16.from_float(w, gated=gated, dtype=torch.bfloat16), pkg.f8.F8Linear.from_float(w, bias=w[:, 0], gated=gated)
+        for y in (lin(x, "silu"), e8(x, "gelu"), e8(rows), lin(x.view(3, 0, 256))):
+            assert y.shape[-1] == lin.out_features and not y.numel() and y.dtype is torch.bfloat16
+    cache = pkg.cache4.Cache4(2, 2, 64)
+    q, k = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=DEV)
+    for cu, lens, table in ((i32(0), none, none.view(0, 2)), (i32(0, 0), i32(5), i32(0).view(1, 1)), (i32(0, 0), i32(0), none.view(1, 0))):
+        cache.append(k, k, cu, lens, table)
+        assert cache.attend(q, cu, lens, table).shape == (0, 4, 64) and not bool(cache.data.any())
+        assert all(t.shape == (0, 2, 64) for t in cache.read(cu, lens, table))
+    # queries of sequences without keys or without a table: zeros; a cache without pages holds nothing
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=DEV)
+    empty = pkg.cache4.Cache4(0, 2, 64)
+    for c, lens, table in ((cache, i32(0, 0), i32(0, 1).view(2, 1)), (cache, i32(70, 9), none.view(2, 0)), (empty, i32(7, 1), i32(0, 0).view(2, 1))):
+        assert not bool(c.attend(q, i32(0, 2, 3), lens, table).any())
+        c.append(q[:, :2].contiguous(), q[:, :2].contiguous(), i32(0, 2, 3), lens, table if c is empty else none.view(2, 0))
+    assert not bool(cache.data.any())
+
+
+def test_offsets_past_32_bits(gpu_lib, pkg):
+    g = torch.Generator(device=DEV).manual_seed(5)
+    dt, D, T = torch.bfloat16, 8192, 270_000  # rows of 4.4 GB
+    x = torch.empty(T, D, dtype=dt, device=DEV)
+    x[-40:] = torch.randn(40, D, generator=g, device=DEV).to(dt)
+    x[:-40] = x[-1]
+    w = torch.ones(D, device=DEV)
+    s, h = pkg.kernels.add_norm(x, x, w)
+    few = pkg.kernels.add_norm(x[-40:].clone(), x[-40:].clone(), w)
+    # (few rows divide a row between more waves: sums in another order)
+    assert torch.equal(s[-40:], few[0]) and float((h[-40:].float() - few[1].float()).abs().max()) <= 2.0 ** -7 * float(few[1].abs().max())
+    assert torch.equal(h[0], h[-1]) and torch.equal(h[T // 2], h[-1])
+    del s, h
+    lin = pkg.linear.Linear16.from_float(torch.randn(D, 64, generator=g, device=DEV) / 8, dtype=dt)
+    y = lin(x[:, :64])
+    assert y.shape == (T, D)
+    check_linear16(y[-40:], x[-40:, :64].contiguous(), lin.weight, None, None, False, None, 1.0)
+    assert torch.equal(y[0], y[-1]) and torch.equal(y[T // 2], y[-1])
+    del x, y
+    # a cache of 4.5 GB: its first and last pages
+    cache = pkg.cache4.Cache4(62_000, 8, 128, dtype=dt)
+    table = i32(61_999, 1, 61_500, 30_000, 0).view(1, 5)
+    k, v = (torch.randn(300, 8, 128, generator=g, device=DEV).to(dt) for _ in range(2))
+    q = torch.randn(2, 16, 128, generator=g, device=DEV).to(dt)
+    cache.append(k, v, i32(0, 300), i32(300), table)
+    held = [C4.hold(t) for t in (k, v)]
+    for got, (c, s, z) in zip(cache.read(i32(0, 300), i32(300), table), held):
+        assert torch.equal(got, (s * (c - z)).to(dt))
+    ref, bound = C4.attention(q, *held, True, 128 ** -0.5)
+    assert bool(((cache.attend(q, i32(0, 2), i32(300), table).double() - ref).abs() <= bound).all())
