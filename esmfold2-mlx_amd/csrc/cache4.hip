@@ -163,7 +163,7 @@ struct EightLanes {
 };
 template <int N>
 DEV uint32_t lanes_on(uint32_t v) {  // of the lane N further in the 16
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x100 + N, 0xf, 0xf, false);  // row_shl:N
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x100 + N, 0xf, 0xf, true);  // row_shl:N (past the 16: 0)
 }
 
 // One item of a wave: x, the lane's 8 values of either key, to their places. Where all eight keys are new, lanes join what
@@ -180,22 +180,19 @@ DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& a
 #pragma unroll
   for (int b = 0; b < 2; b++) {
     const bool in = live && at.in(f, b) && 8 * c < p.d;
-    float v[8], lo = INFINITY, hi = -INFINITY, none = 0.f, inv;
+    float v[8], lo = INFINITY, hi = -INFINITY, inv;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < 8; e++) {  // (NaN stays)
       v[e] = (float)x[b][e];
-      none = fmaf(v[e], 0.f, none);  // (NaN of a NaN or an infinity)
-      lo = fminf(lo, v[e]);
-      hi = fmaxf(hi, v[e]);
+      lo = __builtin_elementwise_minimum(lo, v[e]);
+      hi = __builtin_elementwise_maximum(hi, v[e]);
     }
     if (!in) lo = INFINITY, hi = -INFINITY;
-    if (!(none == 0.f)) hi = INFINITY;
     const auto over = [&](auto ctrl) {
       const auto other = [&](float t) {
-        const int i = __builtin_bit_cast(int, t);
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, false));
+        return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, t), decltype(ctrl)::value, 0xf, 0xf, true));
       };
-      lo = fminf(lo, other(lo)), hi = fmaxf(hi, other(hi));
+      lo = __builtin_elementwise_minimum(lo, other(lo)), hi = __builtin_elementwise_maximum(hi, other(hi));
     };
     over(std::integral_constant<int, 0xB1>{});   // quad_perm(1, 0, 3, 2)
     over(std::integral_constant<int, 0x4E>{});   // quad_perm(2, 3, 0, 1)
@@ -220,9 +217,8 @@ DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& a
   uint32_t w[2][HD / 32];
 #pragma unroll
   for (int b = 0; b < 2; b++) {  // dims 0, 2, 4, 6 in the low half's nibbles, 1, 3, 5, 7 in the high half's
-    w[b][0] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) w[b][0] |= (own[b][e >> 2] >> (8 * (e & 3)) & 15) << (4 * (e >> 1) + 16 * (e & 1));
+    const uint32_t p0 = own[b][0] | own[b][0] >> 12, p1 = own[b][1] | own[b][1] >> 12;  // (bytes: 0 and 2, 1 and 3, ...)
+    w[b][0] = __builtin_amdgcn_perm(p1, p0, 0x05010400u);
     w[b][1] = lanes_on<4>(w[b][0]);
     if constexpr (HD == 128) w[b][2] = lanes_on<8>(w[b][0]), w[b][3] = lanes_on<12>(w[b][0]);
   }
@@ -280,8 +276,8 @@ DEV void hold_eight(const Cache4Args& p, const Eight& f, const EightLanes<HD>& a
   }
 }
 // With rows enough to fill the GPU one workgroup takes all heads of its eight keys, the next one's values asked for before this
-// one's work: 8,287 rows of 8 heads of 128 in 18.0 us, 43 MB, bound by its 30 vector instructions a value of a lane (with
-// divisions, and a branch for their ties, 23 us however the codes were stored). 64 single tokens 4.1 us: a launch and the
+// one's work: 8,287 rows of 8 heads of 128 in 16.5 us, 43 MB, bound by its 22 vector instructions a value of a lane (with 30 18.0,
+// with divisions, and a branch for their ties, 23 us however the codes were stored). 64 single tokens 4.1 us: a launch and the
 // latencies of starts, table and rows.
 template <class V8, int HD>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Args p) {
