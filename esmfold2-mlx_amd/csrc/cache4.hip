@@ -843,13 +843,16 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args p, int rows
 }
 
 // Rows of a tile by the mean rows of a sequence; keys divided unless the table holds few or the tiles alone fill the GPU
-// many times over.
+// many times over. Few: up to 4 passes the join costs more than they do (8 heads of 128, one token of 8 sequences on 1,000 keys
+// 12.2 us divided, 11.2 whole; on 1,500 12.8 and 13.4), up to 8 where a tile a sequence gives every CU one (64 on 2,000 keys 47.0
+// and 32.2, 64 on 0 to 2,000 30.6 and 25.0; on 0 to 4,000 51 and 49, but 32 on those 29 and 36).
 Cache4Plan cache4_plan(long long T, int n, int width, int Hk, int G, int cus) {
   Cache4Plan plan{};
   const long long per = T * G / n;
   plan.rt = per <= 64 ? 1 : 2;
   const long long tiles = T * G / (16 * plan.rt) + n;
-  plan.divide = width > 2 * kPass / kCache4Page && T * G / (16 * plan.rt) * Hk < 2LL * cus;
+  const long long each = T * G / (16 * plan.rt) > n ? T * G / (16 * plan.rt) : n;  // tiles of a key head, about
+  plan.divide = width > (each * Hk < cus ? 4 : 8) * (kPass / kCache4Page) && T * G / (16 * plan.rt) * Hk < 2LL * cus;
   plan.target = (int)((8LL * cus + Hk - 1) / Hk);
   if (plan.target > kCache4MaxChunks) plan.target = kCache4MaxChunks;
   plan.items = tiles + (plan.divide ? plan.target : 0);

@@ -155,6 +155,21 @@ def test_one_long_among_short(gpu_lib, pkg):
     c.check(c.attend())
 
 
+@pytest.mark.parametrize("longest", [1500, 3000])  # with a tile a sequence for every CU: whole, and divided
+def test_many_sequences_and_some_long(gpu_lib, pkg, longest):
+    nk = [longest if i in (7, 140) else (i * 53) % 300 for i in range(150)]
+    nq = [min(n, i % 3) for i, n in enumerate(nk)]
+    c = Case(pkg, nq, nk, 8, 2, 64, torch.bfloat16).fill()
+    c.check(c.attend())
+    # a page of no cache in the middle of a divided sequence: its keys are not seen
+    c.table[140, 11] = -7
+    c.table[7, 3] = 1 << 30
+    keep = torch.ones(c.ck[-1], dtype=torch.bool, device=DEV)
+    keep[c.ck[140] + 704:c.ck[140] + 768] = False
+    keep[c.ck[7] + 192:c.ck[7] + 256] = False
+    c.check(c.attend(), keep=keep)
+
+
 def test_pages_of_no_cache_and_shared_pages(gpu_lib, pkg):
     c = Case(pkg, [4, 4], [400, 400], 8, 2, 128, torch.bfloat16).fill()
     keep = torch.ones(800, dtype=torch.bool, device=DEV)
