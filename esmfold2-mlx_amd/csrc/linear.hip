@@ -37,7 +37,7 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_few_kernel(L16Args p)
   const int Kb = (p.K + 63) / 64, blocks = (Kb + 1) / 2;
   const int ng = blockIdx.x / (4 / NJ), j0 = blockIdx.x % (4 / NJ) * NJ;
   const int m = lane & 15;
-  const rsrc_t rw = make_rsrc_n((const char*)p.w + (size_t)ng * Kb * 8192, (uint32_t)Kb * 8192u);  // (past K: zeros)
+  const rsrc_t rw = make_rsrc((const char*)p.w + (size_t)ng * Kb * 8192);
   const rsrc_t rx = make_rsrc_n(p.x, (uint32_t)(2 * ((p.M - 1) * p.x_st + p.K)));
   const uint32_t xo = m < p.M ? (uint32_t)(2 * (m * p.x_st + 8 * (lane >> 4))) : kOOB;
   struct Block {
@@ -47,8 +47,10 @@ __global__ __launch_bounds__(64 * kL16Waves) void linear16_few_kernel(L16Args p)
     kb = min(kb, blocks - 1);  // (past the last: that one again, not used)
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
+      // (an odd count of 64s ends inside the block: zeros behind it, by the offset that the range is checked against)
+      const int wo = 2 * kb + i / 2 < Kb ? 16 * lane : (int)kOOB;
 #pragma unroll
-      for (int j = 0; j < NJ; j++) b.w[i][j] = bload8<V8>(rw, 16 * lane, kb * 16384 + 4096 * i + 1024 * (j0 + j));
+      for (int j = 0; j < NJ; j++) b.w[i][j] = bload8<V8>(rw, wo, kb * 16384 + 4096 * i + 1024 * (j0 + j));
       const int k = 128 * kb + 32 * i;
       b.x[i] = bload8<V8>(rx, (int)(k + 8 * (lane >> 4) < p.K ? xo + 2u * (uint32_t)k : kOOB), 0);
     }
