@@ -10,10 +10,11 @@
 //   S^T[key][row] = sum_g s_kg (sum_d (16 + c_kd) q_d - (16 + z_kg) Q_g),  Q_g = sum_d q_d
 //   O^T[d][row]  += sum_k (16 + c_kd) P_kg - (16 + z_kg) P_kg,             P_kg = p_k s_kg, rounded
 // both by v_mfma_f32_16x16x32: a wave holds 16 rows of queries (or RT times 16), a row a lane (lane % 16) of every
-// accumulator, and takes 32 keys at a time. P is bf16 whatever the type (its range is p's times the values'); for fp16 it is
-// kept as the sum of two bf16 values, 16 bits of it. No operand passes through LDS: the cache lies in the order the matrix
-// cores take (HD = 64 or 128, the head size filled up). A page's head is 8 chunks of 8 keys, one after the other, so that
-// whoever writes 8 keys writes whole lines of memory; key 4 b + e of chunk g is row 4 g + e of block b of the 32 keys' first
+// accumulator, and takes 32 keys at a time. P is bf16 whatever the type, as its range is p's times the values', and kept as the
+// sum of two bf16 values, 16 bits of it: with the first alone bf16's output was off by 0.0023 of itself on long contexts,
+// where its own rounding is 0.0017 (the second costs 5 to 9% of a token's time, 30% of a prompt's). No operand passes
+// through LDS: the cache lies in the order the matrix cores take (HD = 64 or 128, the head size filled up). A page's head is
+// 8 chunks of 8 keys, one after the other, so that whoever writes 8 keys writes whole lines of memory; key 4 b + e of chunk g is row 4 g + e of block b of the 32 keys' first
 // product, and slot 4 b + e of lane group g in the second:
 //   key codes    [2 b][4 lane groups][4 e][HD / 8 bytes]: lane group l's dword t: dims 32 t + 8 l + {0 .. 7}, the dword's nibble i
 //                dim 2 i, nibble 4 + i dim 2 i + 1
@@ -379,7 +380,6 @@ struct F16Keys {
   typedef half_t elem;
   static constexpr uint32_t kMask = 0x03c003c0u, kMagic = 0x4c004c00u;
   static constexpr int kUp = 6;      // a code's place in the 16 bits
-  static constexpr bool kSplit = true;
   static DEV f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static DEV float zero_of(uint32_t w) { return (float)__builtin_bit_cast(half_t, (uint16_t)w); }
 };
@@ -389,7 +389,6 @@ struct B16Keys {
   typedef __bf16 elem;
   static constexpr uint32_t kMask = 0x00780078u, kMagic = 0x41804180u;
   static constexpr int kUp = 3;
-  static constexpr bool kSplit = false;
   static DEV f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static DEV float zero_of(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 };
@@ -623,7 +622,7 @@ struct Rows4 {
           float v = p[r][j] * st;
           if (MASKED) v = key0 + 8 * g + j <= lim[r] ? v : 0.f;
           hi[r][j] = (__bf16)v;
-          if (T::kSplit) lo[r][j] = (__bf16)(v - (float)hi[r][j]);
+          lo[r][j] = (__bf16)(v - (float)hi[r][j]);
         }
       const bf16x8 z = __builtin_bit_cast(bf16x8, k.vz[i]);
 #pragma unroll
@@ -635,10 +634,8 @@ struct Rows4 {
           f32x4& acc = o[r][4 * i + u];
           acc = mfma_b16(v, hi[r], acc);
           acc = mfma_b16(z, hi[r], acc);
-          if (T::kSplit) {
-            acc = mfma_b16(v, lo[r], acc);
-            acc = mfma_b16(z, lo[r], acc);
-          }
+          acc = mfma_b16(v, lo[r], acc);
+          acc = mfma_b16(z, lo[r], acc);
         }
       }
     }

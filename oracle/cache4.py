@@ -30,15 +30,13 @@ def hold(x):
     return c, s, z
 
 
-def attention(q, k, v, causal, scale, keep=None):
+def attention(q, k, v, causal, scale, keep=None, u_p=2.0 ** -16):
     """(o, bound) of one sequence: q [nq, H, d] in its 16-bit type, k and v as ``hold`` gives them for its keys; ``keep`` [nk]:
     keys that may be seen at all.
 
-    u: o's rounding. P = p s is rounded by u_p: bf16's half step, in fp16 that of two bf16 values' sum; products are exact, each
-    sum over terms with 16 + c and 16 + z is off by a step (2^-23) of their magnitudes' sum per addition: dS of a score, and
-    the last term. e = 2 (dS + 2^-22 |score| + 2^-21 + (nk + 64) 2^-24) on numerator and sum, as packed attention's."""
-    u, u_p = HALF_STEP[q.dtype], 2.0 ** -16 if q.dtype is torch.float16 else 2.0 ** -8
-    tiny = SMALLEST[q.dtype]
+    u: o's rounding. P = p s is rounded by u_p, that of two bf16 values' sum; products are exact, each sum over terms with
+    16 + c and 16 + z is off by a step (2^-23) of their magnitudes' sum per addition: dS of a score, and the last term. e = 2 (dS + 2^-22 |score| + 2^-21 + (nk + 64) 2^-24) on numerator and sum, as packed attention's."""
+    u, tiny = HALF_STEP[q.dtype], SMALLEST[q.dtype]
     q = q.double()
     nq, H, d = q.shape
     (kc, ks, kz), (vc, vs, vz) = k, v

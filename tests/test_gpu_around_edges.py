@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+from oracle import around as A, cache4 as C4
+from test_gpu_cache4 import Case
 from test_gpu_linear16 import _inputs
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +31,28 @@ def test_weights_behind_a_piece_reach_nothing(gpu_lib, pkg, K, M, N, dtype):
     w[rows, 0], w[rows, K - 1] = float("inf"), float("nan")
     y = pkg.linear.Linear16.from_float(w, dtype=dtype)(x)
     assert torch.equal(y[:, ~rows], want[:, ~rows]) and bool(y[:, rows].isnan().all())
+
+
+@pytest.mark.parametrize("nq,nk,H,Hk,d", [([1], [9000], 32, 8, 128), ([1] * 8, [16385, 9002, 4097, 2501, 1025, 334, 77, 1], 32, 8, 128),
+                                          ([5, 40], [3000, 700], 16, 2, 64), ([200], [900], 10, 10, 80)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_probabilities_keep_16_bits(gpu_lib, pkg, nq, nk, H, Hk, d, dtype):
+    """The output's rounding is what there is to see. A kernel that holds o + e, |e| <= E, and rounds once is off by at most
+    the distance of o + e from the nearest value of the type, so by |round(o) - o| + 2 E at most; E is the oracle's bound
+    with probability times step kept to 2^-16, whatever the type, and without the rounding of o."""
+    c = Case(pkg, nq, nk, H, Hk, d, dtype, seed=3).fill()
+    o = c.attend().double()
+    held = [C4.hold(t) for t in (c.k, c.v)]
+    off = least = size = 0.0
+    for i in range(len(nq)):
+        rows, keys = slice(c.cq[i], c.cq[i + 1]), slice(c.ck[i], c.ck[i + 1])
+        ref, bound = C4.attention(c.q[rows], *([t[keys] for t in h] for h in held), True, d ** -0.5, u_p=2.0 ** -16)
+        E = bound - A.HALF_STEP[dtype] * ref.abs() - A.SMALLEST[dtype]
+        once = (ref.to(dtype).double() - ref).abs()
+        worst = float(((o[rows] - ref).abs() / (once + 2 * E + A.SMALLEST[dtype])).max())
+        assert worst <= 1.0, f"sequence {i}: {worst:.2f} of one rounding and 16 bits of the probabilities"
+        off, least, size = off + (o[rows] - ref).pow(2).sum(), least + once.pow(2).sum(), size + ref.pow(2).sum()
+    # As a whole: the scores' roundings, of magnitudes some 1,000 times a value of q, make p off by 2^-16 or so, P's own are
+    # 2^-17, independent from key to key; fp16's rounding of o is 2^-12.2, eleven times their sum, and 1.05 leaves room for
+    # 0.32 of it beside it in squares.
+    assert float(off) <= 1.05 ** 2 * float(least), f"{float((off / size) ** 0.5):.2e} off, one rounding {float((least / size) ** 0.5):.2e}"
