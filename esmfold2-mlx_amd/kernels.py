@@ -40,6 +40,57 @@ def _out(t: torch.Tensor, name: str, dtype, numel: int) -> torch.Tensor:
     return t
 
 
+def _memory(t):
+    """Where a tensor's values lie: (address, [(count, bytes from one to the next)] from the farthest apart on, bytes of the
+    innermost piece, address behind the last), or None for one of no values."""
+    at, n = t.data_ptr(), t.nbytes
+    if not n:
+        return None
+    if t.is_contiguous():
+        return at, [], n, at + n
+    size = t.element_size()
+    dims, width = sorted(((s * size, n) for n, s in zip(t.shape, t.stride()) if n > 1 and s)), size
+    while dims and dims[0][0] == width:  # (a run of whole pieces is one)
+        width *= dims.pop(0)[1]
+    dims = [(n, s) for s, n in reversed(dims)]
+    return at, dims, width, at + width + sum((n - 1) * s for n, s in dims)
+
+
+def _meet(pa: int, da, wa: int, pb: int, db, wb: int) -> bool:
+    ea, eb = (w + sum((n - 1) * s for n, s in d) for w, d in ((wa, da), (wb, db)))
+    if pa + ea <= pb or pb + eb <= pa:
+        return False
+    if not da and not db:
+        return True
+    if da and db and da[0][1] == db[0][1]:  # views of one wider row, say: row i of a and i + k of b, for the few k that are near
+        (na, s), nb = da[0], db[0][0]
+        ia, ib = ea - (na - 1) * s, eb - (nb - 1) * s
+        first, last = (pa - ib - pb) // s + 1, -((pb - pa - ia) // s) - 1
+        return any(_meet(pa, da[1:], wa, pb + k * s, db[1:], wb) for k in range(max(first, 1 - na), min(last, nb - 1) + 1))
+    if not da or (db and db[0][1] > da[0][1]):
+        pa, da, wa, ea, pb, db, wb, eb = pb, db, wb, eb, pa, da, wa, ea
+    n, s = da[0]
+    ia = ea - (n - 1) * s
+    return any(_meet(pa + i * s, da[1:], wa, pb, db, wb) for i in range(max((pb - pa - ia) // s + 1, 0), min(-((pa - pb - eb) // s), n)))
+
+
+def _apart(fn: str, name: str, out, *operands) -> None:
+    """Refuses an output that shares memory with an operand (None: none). Exact: views that lie between one another's rows
+    or heads are apart."""
+    at, a = out.data_ptr(), None
+    for t in operands:
+        if t is None or (t.data_ptr() + t.nbytes <= at if t.is_contiguous() else False):  # (ordinary ones: before it, or behind)
+            continue
+        a = a or _memory(out)
+        if a is None:
+            return
+        if t.data_ptr() >= a[3]:
+            continue
+        b = _memory(t)
+        if b is not None and _meet(*a[:3], *b[:3]):
+            raise capi.EsmError(-3, f"{fn}: {name} shares memory with an operand")
+
+
 def leading_dim(L: int) -> int:
     return capi.lib().tmu_leading_dim(L)
 
@@ -293,12 +344,15 @@ def qk_norm_rope(q, k, freq, positions=None, *, gain: float = 1.0, interleaved: 
             if not isinstance(t, torch.Tensor) or t.shape != like.shape:
                 raise capi.EsmError(-2, f"qk_norm_rope: {n} must be {tuple(like.shape)}")
             _distinct(t, n, dtype, index)
-        if T and (qo.data_ptr() == k.data_ptr() or ko.data_ptr() == q.data_ptr() or qo.data_ptr() == ko.data_ptr()):
-            raise capi.EsmError(-3, "qk_norm_rope: out may be (q, k), each in its own place")
         (_, qo_st, qo_sh), (_, ko_st, ko_sh) = _rows(qo, "out[0]"), _rows(ko, "out[1]")
-        for i, t, same in ((0, q, (qo_st, qo_sh) == (q_st, q_sh)), (1, k, (ko_st, ko_sh) == (k_st, k_sh))):
-            if T and out[i].data_ptr() == t.data_ptr() and not same:
-                raise capi.EsmError(-3, f"qk_norm_rope: out[{i}] over its input must have the input's strides")
+        # (each in its input's place or clear of both)
+        over_q = qo.data_ptr() == q.data_ptr() and (qo_st, qo_sh) == (q_st, q_sh)
+        over_k = ko.data_ptr() == k.data_ptr() and (ko_st, ko_sh) == (k_st, k_sh)
+        beside = (ko.data_ptr() - qo.data_ptr()) // 2
+        # (q and k of one row, in place: apart at a glance)
+        if not (over_q and over_k and q_st == k_st and (H - 1) * q_sh + d <= beside <= q_st - (Hk - 1) * k_sh - d):
+            _apart("qk_norm_rope", "out[0]", qo, ko, None if over_q else q, None if over_k else k)
+            _apart("qk_norm_rope", "out[1]", ko, None if over_q else q, None if over_k else k)
     capi.check(lib.qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh, qw,
         qwh, kw, kwh, float(eps), pos, pos64, freq.data_ptr(), float(gain), T, H, Hk, d, 2 * freq.numel(), _NORMS[norm], over == "row",
@@ -311,8 +365,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
     wider rows allowed; H a multiple of Hk) -> o [Tq, H, d]. ``cu_q``, ``cu_k`` int32 [n + 1] on the device: the first
     row of each sequence, then the end of the last (``cu_k`` None: the queries' own). ``causal``: query i of nq sees
     the keys 0 .. i + nk - nq of nk, so one new row sees a whole cache. Rows that see no key, or none whose score is
-    above -inf, are 0; rows of no sequence are not written. ``out`` may be q, and shares no other memory with the operands. The partial results of few rows
-    against many keys live in the shared scratch (``scratch.workspace``)."""
+    above -inf, are 0; rows of no sequence are not written. ``out`` may be q, and shares no other memory with the operands.
+    The partial results of few rows against many keys live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
         o = capi.bind.packed_attention(q, k, v, cu_q, cu_k, causal, scale, 0, 0)
@@ -349,10 +403,8 @@ def packed_attention(q, k, v, cu_q, cu_k=None, causal: bool = False, scale: floa
         oshape, o_st, o_sh = _distinct(o, "out", dtype, index)
         if oshape != q.shape:
             raise capi.EsmError(-2, f"packed_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
-        if Tq and Tk and o.data_ptr() in (k.data_ptr(), v.data_ptr()):
-            raise capi.EsmError(-3, "packed_attention: out may be q, not k or v")
-        if Tq and o.data_ptr() == q.data_ptr() and (o_st, o_sh) != (q_st, q_sh):
-            raise capi.EsmError(-3, "packed_attention: out over q must have its strides")
+        over = o.data_ptr() == q.data_ptr() and (o_st, o_sh) == (q_st, q_sh)
+        _apart("packed_attention", "out (which may be q)", o, None if over else q, k, v)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh,
             cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, H, Hk, d, bool(causal), d ** -0.5 if scale is None else float(scale),
             _DTYPES[dtype])
@@ -744,8 +796,7 @@ def f8_linear(x, codes, scales, N: int, out=None):
         y = _out(out, "out", x.dtype, M * N)
         if y.get_device() != index:
             raise capi.EsmError(-5, f"out must be on {x.device}")
-        if M and y.data_ptr() == x.data_ptr():
-            raise capi.EsmError(-3, "f8_linear: out may not be x")
+        _apart("f8_linear", "out", y, x, codes, scales)
     args = (x.data_ptr(), st, codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, K, N, _DTYPES[x.dtype])
     need = lib.f8_linear_workspace_bytes(M, K, N)
     if not need:
@@ -824,17 +875,17 @@ def _add_norm(fn, x, y, w, b, alpha, norm, eps, dtype, sum_out, out, f8):
         dtype = y.dtype if isinstance(y, torch.Tensor) else out.dtype if isinstance(out, torch.Tensor) else x.dtype
     if dtype not in _DTYPES or (x.dtype is not dtype and x.dtype is not torch.float32) or norm not in _NORM_KINDS:
         raise capi.EsmError(-4, f"{fn}: x in {x.dtype}, h in {dtype}, norm={norm!r} (x in fp32 or h's 16-bit type)")
+    wp, bp = _vector(w, "w", D, index), _vector(b, "b", D, index)
     y_st = s_st = h_st = 0
     s = x
     if y is not None:
         y_st, _ = _matrix(y, "y", (dtype,), index, x.shape)
         s = x.new_empty((T, D)) if sum_out is None else sum_out
         s_st, _ = _matrix(s, "sum_out", (x.dtype,), index, x.shape)
-        if T and (s.data_ptr() == y.data_ptr() or (s.data_ptr() == x.data_ptr() and s_st != x_st)):
-            raise capi.EsmError(-3, f"{fn}: sum_out may be x with its strides, and share no memory with y")
+        if sum_out is not None:
+            _apart(fn, "sum_out (which may be x)", s, None if s.data_ptr() == x.data_ptr() and s_st == x_st else x, y, w, b)
     elif sum_out is not None or alpha != 1.0:
         raise capi.EsmError(-2, f"{fn}: sum_out and alpha go with y")
-    wp, bp = _vector(w, "w", D, index), _vector(b, "b", D, index)
     hq = hs = None
     if f8:
         hq = torch.empty(int(lib.f8_rows_bytes(T, D)), dtype=torch.uint8, device=x.device)
@@ -843,8 +894,8 @@ def _add_norm(fn, x, y, w, b, alpha, norm, eps, dtype, sum_out, out, f8):
     else:
         h = torch.empty((T, D), dtype=dtype, device=x.device) if out is None else out
         h_st, _ = _matrix(h, "out", (dtype,), index, x.shape)
-        if T and any(t is not None and h.data_ptr() == t.data_ptr() for t in (x, y, s)):
-            raise capi.EsmError(-3, f"{fn}: out shares no memory with x, y or sum_out")
+        if out is not None:
+            _apart(fn, "out", h, x, y, sum_out, w, b)
     capi.check(lib.add_norm(x.data_ptr(), x.dtype is torch.float32, _ptr(y), float(alpha), None if y is None else s.data_ptr(),
                             None if f8 else h.data_ptr(), _ptr(hq), _ptr(hs), wp, bp, float(eps), _NORM_KINDS[norm], x_st,
                             y_st, s_st, h_st, T, D, _DTYPES[dtype], capi.stream_ptr()))
@@ -856,7 +907,7 @@ def add_norm(x, y=None, w=None, b=None, *, alpha: float = 1.0, norm: str = "rms"
     """(s, h): s = x + alpha * y (x itself without ``y``) and h = the norm of s, "rms" or "layer", times ``w``, plus ``b``
     (fp32 [D]; None: 1 and 0), one pass. x [T, D] in fp32 or in h's type, y and h fp16 or bf16 (``dtype``: h's, else y's or
     x's); rows may lie apart. fp32 throughout, the norm of s as it is before its rounding to x's type. ``sum_out`` may be
-    x; ``out`` shares no memory with the operands. D a multiple of 8 up to 32768."""
+    x and shares no other memory with the operands; ``out`` shares no memory with the operands. D a multiple of 8 up to 32768."""
     return _add_norm("add_norm", x, y, w, b, alpha, norm, eps, dtype, sum_out, out, False)
 
 
@@ -867,8 +918,8 @@ def add_norm_f8(x, y=None, w=None, b=None, *, alpha: float = 1.0, norm: str = "r
     return _add_norm("add_norm_f8", x, y, w, b, alpha, norm, eps, dtype, sum_out, None, True)
 
 
-def _linear_end(fn, M: int, No: int, Nb: int, bias, activation, residual, out, dtype, index: int, x):
-    """The checks of a linear's end: (bias, residual, its stride, activation, y)."""
+def _linear_end(fn, M: int, No: int, Nb: int, bias, activation, residual, out, dtype, index: int, *operands):
+    """The checks of a linear's end: (bias, residual, its stride, activation, y); ``operands``: what else out is clear of."""
     if activation not in _ACTIVATIONS:
         raise capi.EsmError(-4, f"{fn}: activation={activation!r}")
     bp = _vector(bias, "bias", Nb, index)
@@ -881,10 +932,8 @@ def _linear_end(fn, M: int, No: int, Nb: int, bias, activation, residual, out, d
         y = _out(out, "out", dtype, M * No)
         if y.get_device() != index:
             raise capi.EsmError(-5, f"out must be on cuda:{index}")
-        if M and x is not None and y.data_ptr() == x.data_ptr():
-            raise capi.EsmError(-3, f"{fn}: out may be the residual, not x")
-        if M > 1 and residual is not None and y.data_ptr() == residual.data_ptr() and r_st != No:
-            raise capi.EsmError(-3, f"{fn}: out over the residual must have its strides")
+        over = residual is not None and y.data_ptr() == residual.data_ptr() and (M <= 1 or r_st == No)
+        _apart(fn, "out (which may be the residual)", y, None if over else residual, bias, *operands)
     return bp, _ptr(residual), r_st, _ACTIVATIONS[activation], y
 
 
@@ -906,7 +955,8 @@ def linear16(x, packed, N: int, bias=None, *, gated: bool = False, activation: s
     """y = residual + alpha * act(x . W^T + bias), or with ``gated`` residual + alpha * act(g) u of the two halves of the
     N outputs: x [M, K] fp16 or bf16 (rows may lie apart), W [N, K] of its type as ``linear16_pack`` has it, ``bias`` [N]
     fp32, ``activation`` None, "relu", "gelu", "gelu_tanh" or "silu", ``residual`` of y's type. fp32 sums, one rounding.
-    ``out`` (contiguous) may be the residual. Split-K partials live in the shared scratch (``scratch.workspace``)."""
+    ``out`` (contiguous) may be the residual, and shares no other memory with the operands. Split-K partials live in the
+    shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     act = _ACTIVATIONS.get(activation)
     if out is None and act is not None:
@@ -925,7 +975,8 @@ def linear16(x, packed, N: int, bias=None, *, gated: bool = False, activation: s
     _aux(packed, "packed", _UINT8, index)
     if not packed.numel() or packed.numel() != lib.linear16_packed_bytes(N, K, gated):
         raise capi.EsmError(-2, f"linear16: {packed.numel()} packed bytes for [{N}, {K}]")
-    bp, rp, r_st, act, y = _linear_end("linear16", M, N // 2 if gated else N, N, bias, activation, residual, out, x.dtype, index, x)
+    bp, rp, r_st, act, y = _linear_end("linear16", M, N // 2 if gated else N, N, bias, activation, residual, out, x.dtype, index, x,
+                                    packed)
     args = (x.data_ptr(), x_st, packed.data_ptr(), bp, rp, r_st, float(alpha), act, gated, y.data_ptr(), M, K, N, _DTYPES[x.dtype])
     need = lib.linear16_workspace_bytes(M, K, N, gated)
     if not need:
@@ -971,7 +1022,8 @@ def f8_linear_end(x, codes, scales, N: int, bias=None, *, gated: bool = False, a
         with torch.cuda.device(index):
             return f8_linear_end(x, codes, scales, N, bias, gated=gated, activation=activation, residual=residual, alpha=alpha,
                                  rows=rows, dtype=dtype, out=out)
-    bp, rp, r_st, act, y = _linear_end("f8_linear_end", M, N // 2 if gated else N, N, bias, activation, residual, out, dtype, index, x)
+    bp, rp, r_st, act, y = _linear_end("f8_linear_end", M, N // 2 if gated else N, N, bias, activation, residual, out, dtype, index, x,
+                                       xq, sx, codes, scales)
     args = (_ptr(x), x_st, _ptr(xq), _ptr(sx), codes.data_ptr(), scales.data_ptr(), bp, rp, r_st, float(alpha), act, gated,
             y.data_ptr(), M, K, N, _DTYPES[dtype])
     need = lib.f8_linear_end_workspace_bytes(M, K, N, gated, xq is not None)
@@ -1048,8 +1100,8 @@ def cache4_attention(data, q, heads: int, cu, lens, table, causal: bool = True, 
     """softmax(q k^T * scale) v over keys and values held in 4 bits (``cache4.Cache4`` of q's type, ``heads`` key heads): q [T,
     H, d] -> o [T, H, d]. Sequence i has the query rows cu[i] .. cu[i + 1] - 1 and the first lens[i] keys of its pages
     table[i]; ``causal``: its last row sees the last key. Rows that see no key are 0, rows of no sequence are not written,
-    keys in pages outside the cache are not seen. ``out`` may be q. Where keys are divided between workgroups the partial
-    results live in the shared scratch (``scratch.workspace``)."""
+    keys in pages outside the cache are not seen. ``out`` may be q, and shares no other memory with the operands. Where keys
+    are divided between workgroups the partial results live in the shared scratch (``scratch.workspace``)."""
     lib = capi.lib()
     if out is None:
         o = capi.bind.cache4_attention(data, q, heads, cu, lens, table, causal, scale, 0, 0)
@@ -1074,8 +1126,8 @@ def cache4_attention(data, q, heads: int, cu, lens, table, causal: bool = True, 
         oshape, o_st, o_sh = _distinct(o, "out", dtype, index)
         if oshape != q.shape:
             raise capi.EsmError(-2, f"cache4_attention: out {tuple(o.shape)}, writes {tuple(q.shape)}")
-        if T and o.data_ptr() == q.data_ptr() and (o_st, o_sh) != (q_st, q_sh):
-            raise capi.EsmError(-3, "cache4_attention: out over q must have its strides")
+        over = o.data_ptr() == q.data_ptr() and (o_st, o_sh) == (q_st, q_sh)
+        _apart("cache4_attention", "out (which may be q)", o, None if over else q, data, cu, lens, table)
     args = (q.data_ptr(), o.data_ptr(), q_st, q_sh, o_st, o_sh, data.data_ptr(), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), n,
             T, H, heads, d, pages, width, bool(causal), d ** -0.5 if scale is None else float(scale), _DTYPES[dtype])
     need = lib.cache4_attention_workspace_bytes(n, T, width, H, heads, d)

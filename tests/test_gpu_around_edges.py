@@ -56,3 +56,64 @@ def test_probabilities_keep_16_bits(gpu_lib, pkg, nq, nk, H, Hk, d, dtype):
     # 2^-17, independent from key to key; fp16's rounding of o is 2^-12.2, eleven times their sum, and 1.05 leaves room for
     # 0.32 of it beside it in squares.
     assert float(off) <= 1.05 ** 2 * float(least), f"{float((off / size) ** 0.5):.2e} off, one rounding {float((least / size) ** 0.5):.2e}"
+
+
+def test_outputs_that_lie_on_an_operand_elsewhere_than_at_its_start(gpu_lib, pkg):
+    K, E = pkg.kernels, pkg.capi.EsmError
+    for T in (5, 1100):
+        buf = torch.randn(T + 9, 192, device=DEV).half()
+        x, y, w = buf[:T, :64], torch.randn(T, 64, device=DEV).half(), torch.ones(64, device=DEV)
+        ybuf = torch.zeros(T + 1, 64, dtype=torch.float16, device=DEV)
+        wide = torch.zeros(T + 1, 64, dtype=torch.float32, device=DEV)
+        for kw in (dict(sum_out=buf[1:T + 1, :64]), dict(sum_out=buf[:T, 8:72]), dict(out=buf[1:T + 1, :64]), dict(out=buf[:T, 56:120]),
+                   dict(sum_out=buf[:T, 64:128], out=buf[2:T + 2, 64:128])):
+            with pytest.raises(E) as e:
+                K.add_norm(x, y, w, **kw)
+            assert e.value.code == -3, kw
+        with pytest.raises(E):
+            K.add_norm(x, ybuf[:T], w, out=ybuf[1:])
+        with pytest.raises(E):
+            K.add_norm(wide[:T], y, wide[T], sum_out=wide[1:])  # over the weight
+        s, h = K.add_norm(x.clone(), y, w)
+        s1, h1 = K.add_norm(x, y, w, sum_out=buf[:T, 64:128], out=buf[:T, 128:])  # beside x in its rows
+        assert torch.equal(s, s1) and torch.equal(h, h1)
+        s1, h1 = K.add_norm(x, y, w, sum_out=x, out=buf[:T, 128:])
+        assert torch.equal(s, s1) and torch.equal(h, h1)
+    x = torch.randn(40, 64, device=DEV).half()
+    lin = pkg.linear.Linear16.from_float(torch.randn(64, 64, device=DEV), torch.randn(64, device=DEV))
+    r = torch.randn(41, 64, device=DEV).half()
+    e8 = pkg.f8.F8Linear.from_float(torch.randn(64, 64, device=DEV))
+    for call in (lambda: lin(x[:32], out=x[8:]), lambda: lin(x[:39], residual=r[:39], out=r[1:40]), lambda: lin(x[8:], out=x.view(-1)[504:504 + 2048]),
+                 lambda: K.f8_linear_end(x[:32], e8.codes_packed, e8.scales, 64, out=x[8:]), lambda: K.f8_linear(x[:32], e8.codes_packed, e8.scales, 64, out=x[8:])):
+        with pytest.raises(E) as e:
+            call()
+        assert e.value.code == -3
+    want = lin(x[:39], residual=r[:39])
+    assert torch.equal(lin(x[:39], residual=r[:39], out=r[:39]), want)
+    both = torch.randn(80, 64, device=DEV).half()
+    assert torch.equal(lin(both[:40], out=both[40:]), lin(both[:40].clone()))
+    c = Case(pkg, [5, 60], [200, 100], 8, 2, 64, torch.bfloat16).fill()
+    want, wide = c.attend(), torch.zeros(66, 24, 64, dtype=torch.bfloat16, device=DEV)
+    wide[:65, :8] = c.q
+    q = wide[:65, :8]
+    for out in (wide[1:, :8], wide[:65, 4:12], wide[:65, 7:15]):
+        with pytest.raises(E) as e:
+            c.cache.attend(q, c.cu, c.lens, c.table, out=out)
+        assert e.value.code == -3
+    assert torch.equal(c.cache.attend(q, c.cu, c.lens, c.table, out=wide[:65, 8:16]), want)
+    cu = torch.tensor([0, 65], dtype=torch.int32, device=DEV)
+    q, k, v = wide[:65, :8], wide[:65, 8:16], wide[:65, 16:]
+    for out in (wide[1:, :8], wide[1:, 8:16], wide[:65, 12:20], wide[1:, 16:]):
+        with pytest.raises(E) as e:
+            K.packed_attention(q, k, v, cu, out=out)
+        assert e.value.code == -3
+    freq = torch.ones(32, dtype=torch.float64, device=DEV)
+    for out in ((wide[1:, :8], k), (q, wide[1:, 8:16]), (k, q), (wide[:65, 4:12], wide[:65, 16:])):
+        with pytest.raises(E) as e:
+            K.qk_norm_rope(q, k, freq, out=out)
+        assert e.value.code == -3
+    one = wide[:65, 0, :].contiguous().view(-1)  # a head each, the second half a head further
+    with pytest.raises(E):
+        K.qk_norm_rope(one[:4096].view(64, 1, 64), one[32:4128].view(64, 1, 64), freq, out=(one[:4096].view(64, 1, 64), one[32:4128].view(64, 1, 64)))
+    want = K.qk_norm_rope(q, k, freq)
+    assert all(torch.equal(a, b) for a, b in zip(want, K.qk_norm_rope(q, k, freq, out=(q, k))))
