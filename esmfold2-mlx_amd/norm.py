@@ -38,6 +38,9 @@ class AddNorm(nn.Module):
             raise ValueError("AddNorm: rows in e4m3 have no out")
         flat = len(shape) == 2
         if not flat:  # (views of whole rows; a copy would lose what is written to it)
+            for name, t in (("y", y), ("sum_out", sum_out), ("out", out)):
+                if t is not None and t.shape != shape:
+                    raise ValueError(f"AddNorm: {name} {tuple(t.shape)}, x is {tuple(shape)}")
             view = lambda t: None if t is None else t.view(-1, D)  # noqa: E731
             x, y, sum_out, out = x.reshape(-1, D), None if y is None else y.reshape(-1, D), view(sum_out), view(out)
         s, h = kernels._add_norm("add_norm", x, y, w, b, alpha, self.norm, self.eps, dtype, sum_out, out, f8)

@@ -117,3 +117,15 @@ def test_outputs_that_lie_on_an_operand_elsewhere_than_at_its_start(gpu_lib, pkg
         K.qk_norm_rope(one[:4096].view(64, 1, 64), one[32:4128].view(64, 1, 64), freq, out=(one[:4096].view(64, 1, 64), one[32:4128].view(64, 1, 64)))
     want = K.qk_norm_rope(q, k, freq)
     assert all(torch.equal(a, b) for a, b in zip(want, K.qk_norm_rope(q, k, freq, out=(q, k))))
+
+
+def test_leading_dimensions_of_the_norms_operands_agree(gpu_lib, pkg):
+    n = pkg.norm.AddNorm(torch.ones(64))
+    x, y = torch.randn(2, 3, 64, device=DEV), torch.randn(2, 3, 64, device=DEV).half()
+    h = torch.empty_like(y)
+    for call in (lambda: n(x, y.view(3, 2, 64)), lambda: n(x, y.view(6, 64)), lambda: n(x, y, out=h.view(3, 2, 64)), lambda: n(x, y, sum_out=torch.empty(6, 64, device=DEV)),
+                 lambda: n(x, y.view(3, 2, 64), f8=True)):
+        with pytest.raises(ValueError):
+            call()
+    s, got = n(x, y, sum_out=x, out=h)
+    assert got.data_ptr() == h.data_ptr() and s.data_ptr() == x.data_ptr() and s.shape == got.shape == (2, 3, 64)
