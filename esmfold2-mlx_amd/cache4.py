@@ -49,6 +49,7 @@ class Cache4:
 
     def attend(self, q: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, causal: bool = True,
                scale: float | None = None, out=None) -> torch.Tensor:
-        """softmax(q k^T scale) v of q [T, H, head_dim] over each sequence's keys; ``causal``: its last row sees the last."""
+        """softmax(q k^T scale) v of q [T, H, head_dim] over each sequence's keys; ``causal``: its last row sees the last. Sums
+        are fp32: values below 2^96."""
         self._check(q, "q")
         return kernels.cache4_attention(self.data, q, self.heads, cu, lens, table, causal, scale, out)

@@ -531,7 +531,8 @@ int f8_linear_end(const void* x, int64_t x_st, const uint8_t* xq, const float* s
  * cache4_attention: o = softmax(scale q k^T) v over the sequence's keys, q and o [T, H, d], query head h with key head h / (H /
  *   Hk); causal: row i of nq sees the keys 0 .. i + nk - nq of nk. lens beyond the table are brought inside; keys in pages
  *   outside 0 .. pages - 1 are not seen. Rows that see no key are 0, rows of no sequence are not written, what unseen places
- *   hold reaches no output. Scores and sums are fp32; probability times step is rounded to 16 bits for the second product. |q| < 2^110.
+ *   hold reaches no output. Scores and sums are fp32; probability times step is rounded to 16 bits for the second product.
+ *   |q| < 2^110, |v| < 2^96 (larger values are held and read, but sums of them with 16 + c may pass fp32 on the way).
  * d % 8 == 0, d <= 128; strides as packed_attention's. Workspace 256-byte aligned (0: none).
  */
 size_t cache4_bytes(int pages, int Hk, int d);

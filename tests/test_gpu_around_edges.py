@@ -129,3 +129,22 @@ def test_leading_dimensions_of_the_norms_operands_agree(gpu_lib, pkg):
             call()
     s, got = n(x, y, sum_out=x, out=h)
     assert got.data_ptr() == h.data_ptr() and s.data_ptr() == x.data_ptr() and s.shape == got.shape == (2, 3, 64)
+
+
+def test_values_up_to_the_limit(gpu_lib, pkg):
+    c = Case(pkg, [2, 30], [900, 200], 8, 2, 128, torch.bfloat16)
+    c.v = (c.v.float().clamp(-4, 4) * 2.0 ** 93.9).to(torch.bfloat16)  # below 2^96
+    # a row whose first key is the least, so that what it is made relative to lags behind: p up to 2^8
+    c.q[0], c.k[:, :] = 1.0, c.k * 0.01
+    c.k[1:900] += 0.04
+    c.fill()
+    o = c.attend()
+    assert bool(torch.isfinite(o).all())
+    c.check(o)
+    rk, rv = c.cache.read(c.whole, c.lens, c.table)
+    assert bool(torch.isfinite(rv).all())
+    c.v *= 2.0 ** 30  # held and read as any other
+    c.fill()
+    for got, x in zip(c.cache.read(c.whole, c.lens, c.table), (c.k, c.v)):
+        code, s, z = C4.hold(x)
+        assert torch.equal(got, (s * (code - z)).to(torch.bfloat16))
