@@ -71,6 +71,8 @@ SIGNATURES = {
     "linear16_pack": (_int, [_vp, _vp, _int, _int, _int, _vp]),
     "linear16_workspace_bytes": (_sz, [_int] * 4),
     "linear16": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
+    "linear16_tile": (_int, [_int] * 4 + [_vp]),
+    "f8_linear_tile": (_int, [_int] * 4 + [_vp]),
     "f8_linear_end_workspace_bytes": (_sz, [_int] * 5),
     "f8_linear_end": (_int, [_vp, _i64] + [_vp] * 6 + [_i64, _f32, _int, _int, _vp] + [_int] * 4 + [_vp, _sz, _vp]),
     "cache4_bytes": (_sz, [_int] * 3),

@@ -1300,6 +1300,20 @@ size_t f8_rows_scales_bytes(int M, int K) {
   return M > 0 && K > 0 ? (size_t)round_up(M, 16) * ((K + 127) / 128) * 4 + 1024 : 0;  // (1 KB that a tile's last rows read past)
 }
 
+namespace {
+int tile_code(int form_rows, int weight_rows, int splits, int* out) {
+  if (out) *out = splits;
+  return 1000 * form_rows + weight_rows;
+}
+}  // namespace
+
+int f8_linear_tile(int M, int K, int N, int gated, int* splits) {
+  if (!linear_shape(M, K, N, gated, 16) || M == 0) return tile_code(0, 0, 0, splits);
+  const esm::F8Plan p = esm::f8_plan(M, K, 64 * esm::linear_pieces(N, gated), cu_count(), gated);
+  if (p.form == esm::kF8Few) return tile_code(0, 16 * p.mb, 1, splits);
+  return p.form == esm::kF8Some ? tile_code(16 * p.mb, 64, 1, splits) : tile_code(32 * p.mb, 256, p.splits, splits);
+}
+
 size_t f8_linear_end_workspace_bytes(int M, int K, int N, int gated, int coded) {
   return linear_shape(M, K, N, gated, 16) && M > 0 ? f8_end_layout(M, K, N, gated, coded).total : 0;
 }
@@ -1348,6 +1362,15 @@ size_t linear16_workspace_bytes(int M, int K, int N, int gated) {
   if (!linear_shape(M, K, N, gated, 8) || M == 0) return 0;
   const esm::L16Plan plan = esm::linear16_plan(M, K, N, gated != 0, cu_count());
   return plan.splits > 1 ? (size_t)plan.splits * M * esm::linear_pieces(N, gated) * 256 : 0;
+}
+
+int linear16_tile(int M, int K, int N, int gated, int* splits) {
+  if (!linear_shape(M, K, N, gated, 8) || M == 0) return tile_code(0, 0, 0, splits);
+  const esm::L16Plan p = esm::linear16_plan(M, K, N, gated != 0, cu_count());
+  if (p.form == esm::kL16Few) return tile_code(0, 16 * p.mb, 1, splits);
+  if (p.form == esm::kL16Some) return tile_code(16 * p.mb, 64, 1, splits);
+  const esm::L16Size t = esm::linear16_size(p.mb);
+  return tile_code(t.rows, t.weights, p.splits, splits);
 }
 
 int linear16(const void* x, int64_t x_st, const void* wp, const float* bias, const void* residual, int64_t r_st, float alpha,

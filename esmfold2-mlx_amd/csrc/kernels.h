@@ -383,6 +383,10 @@ AttnPlan packed_attention_plan(long long Tq, long long Tk, int n, int Hk, int G,
 hipError_t launch_packed_attention(const PackedAttnArgs& a, bool bf16, bool many, hipStream_t s);
 hipError_t launch_linear16_pack(const void* w, void* out, int N, int K, bool gated, hipStream_t s);
 L16Plan linear16_plan(int M, int K, int N, bool gated, int cus);
+struct L16Size {
+  int rows, weights;      // of x, of the packed weights
+};
+L16Size linear16_size(int tile);
 hipError_t launch_linear16(const L16Args& a, bool bf16, const L16Plan& plan, hipStream_t s);
 constexpr int linear_pieces(int N, bool gated) { return gated ? (N / 2 + 31) / 32 : (N + 63) / 64; }
 hipError_t launch_add_norm(const AddNormArgs& a, bool bf16, bool x32, hipStream_t s);

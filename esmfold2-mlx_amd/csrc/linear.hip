@@ -437,6 +437,8 @@ static hipError_t launch_some16(L16Args a, hipStream_t s) {
 static const struct L16Tile { int rows, pieces, per_cu; double start, step; } kL16Tile[] = {
     {64, 2, 2, 2.5, 0.41}, {64, 4, 1, 2.5, 0.58}, {128, 2, 1, 2.5, 0.60}, {128, 4, 1, 3.5, 0.76}, {192, 4, 1, 4.0, 1.15}, {256, 4, 1, 4.5, 1.47}};
 
+L16Size linear16_size(int tile) { return L16Size{kL16Tile[tile].rows, 64 * kL16Tile[tile].pieces}; }
+
 template <class V8>
 static hipError_t launch_linear16_t(const L16Args& a, int form, int mb, hipStream_t s) {
   if (form == kL16Few) {

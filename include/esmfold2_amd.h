@@ -493,6 +493,9 @@ int packed_attention(const void* q, const void* k, const void* v, void* o, int64
  *   r_st apart, may be y where r_st is the outputs), y contiguous. K % 8 == 0, N % 8 == 0 (gated: 16), x_st <= 2^21.
  * f8_linear_end: the same on e4m3 weights (f8_pack_codes; gated: rows in linear16's order, see F8Linear, N % 64 == 0) with
  *   x [M, K] in 16 bits brought to e4m3 as f8_linear does, or (x NULL) add_norm's codes and scales of M rows.
+ * linear16_tile, f8_linear_tile: which form the launch plan picks for a shape on the current device (tests, tuning): 1000 x
+ *   the rows of x + the packed weight rows that a workgroup takes, no rows where it takes all, up to 16; *splits (unless
+ *   NULL) between how many workgroups K is divided. 0 where the shape is none.
  * Workspaces as their sizes say, 256-byte aligned (0: none).
  */
 #define ESM_ACT_NONE 0
@@ -508,6 +511,8 @@ size_t f8_rows_scales_bytes(int M, int K);
 size_t linear16_packed_bytes(int N, int K, int gated);
 int linear16_pack(const void* w, void* wp, int N, int K, int gated, void* stream);
 size_t linear16_workspace_bytes(int M, int K, int N, int gated);
+int linear16_tile(int M, int K, int N, int gated, int* splits);
+int f8_linear_tile(int M, int K, int N, int gated, int* splits);
 int linear16(const void* x, int64_t x_st, const void* wp, const float* bias, const void* residual, int64_t r_st, float alpha,
              int activation, int gated, void* y, int M, int K, int N, int dtype, void* workspace, size_t workspace_bytes,
              void* stream);
