@@ -44,3 +44,49 @@ def test_workspaces_are_what_the_splits_write(lib):
                 want += -(-(rows * kb * 132 + 1024) // 256) * 256
             assert lib.f8_linear_end_workspace_bytes(M, K, N, gated, 0) == want
     assert divided > 1000
+
+
+def _divided(n, T, width, H, Hk):
+    """Whether keys are divided, at 256 CUs: tables of more than 16 pages, or 32 where the tiles alone give every CU one, and
+    tiles below two a CU."""
+    G = H // Hk
+    rt = 1 if T * G // n <= 64 else 2
+    tiles = T * G // (16 * rt)
+    return rt, width > (16 if max(tiles, n) * Hk < 256 else 32) and tiles * Hk < 512
+
+
+def _f32(v):
+    return ctypes.c_float(v).value
+
+
+def test_the_caches_workspace_holds_every_item(lib):
+    """What the kernels number on the device, (sequence, tile, chunk of keys), restated: chunks of whole passes of 256 keys, two
+    at least and a 256th of the table at least, as spread all over 2,048 / Hk workgroups (256 at most) of a key head."""
+    rng = random.Random(5)
+    spread = lambda hi: int(hi ** rng.random())  # noqa: E731
+    seen = 0
+    for _ in range(4000):
+        n, Hk, G, d = spread(300), spread(40), spread(32), 8 * rng.randint(1, 16)
+        nq = [spread(rng.choice((1, 2, 8, 300))) if rng.random() < 0.9 else 0 for _ in range(n)]
+        width = spread(rng.choice((8, 40, 600, 40000)))
+        nk = [rng.choice((0, 64 * width, rng.randrange(64 * width + 1), spread(64 * width))) for _ in range(n)]
+        T = sum(nq) + rng.choice((0, 0, 5))
+        if T == 0:
+            continue
+        need = lib.cache4_attention_workspace_bytes(n, T, width, Hk * G, Hk, d)
+        rt, divided = _divided(n, T, width, Hk * G, Hk)
+        assert (need > 0) == divided
+        if not divided:
+            continue
+        seen += 1
+        each = Hk * 16 * rt * (8 + 4 * (64 if d <= 64 else 128))
+        assert need % each == 0
+        items, target = need // each, min(-(-2048 // Hk), 256)
+        tiles = [-(-q * G // (16 * rt)) for q in nq]
+        passes = 0.0
+        for t, k in zip(tiles, nk):
+            passes = _f32(passes + _f32(t * -(-k // 256)))
+        keys = 256 * max(2, math.ceil(_f32(passes / target)), -(-64 * width // 65536))
+        chunks = [max(1, -(-k // keys)) for k in nk]
+        assert sum(t * c for t, c in zip(tiles, chunks)) <= items and max(chunks) <= 256
+    assert seen > 500
