@@ -60,7 +60,8 @@ def product8(xd, codes, scales):
 
 def activate(z, kind):
     """(act(z), bound of the kernel's own arithmetic on exact z). An exponential's argument is off by 2^-23 of itself and the
-    result by a few steps; gelu's polynomial by 0.75e-7 of z, absolute."""
+    result by a few steps; gelu's polynomial by 0.75e-7 of z, absolute, in exact arithmetic, and by up to 8 steps (2^-23) of its
+    own result in fp32, half of the 16 that the bound counts."""
     if kind is None:
         return z, torch.zeros_like(z)
     if kind == "relu":
