@@ -6,6 +6,7 @@ import torch
 from oracle import around as A, cache4 as C4
 from test_gpu_cache4 import Case
 from test_gpu_linear16 import _inputs
+from test_gpu_norm import _check as check_norm, _check8 as check_norm8, _inputs as norm_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -148,3 +149,40 @@ def test_values_up_to_the_limit(gpu_lib, pkg):
     for got, x in zip(c.cache.read(c.whole, c.lens, c.table), (c.k, c.v)):
         code, s, z = C4.hold(x)
         assert torch.equal(got, (s * (code - z)).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("T", [1, 5, 17, 1023, 1030])  # a row a workgroup, and several
+@pytest.mark.parametrize("D", [144, 2560])
+def test_what_lies_behind_the_norms_last_row_stays(gpu_lib, pkg, T, D):
+    x, y, w, _ = norm_inputs(T, D, torch.float32, torch.bfloat16, seed=T)
+    s, h = torch.full((T + 40, D), 7.0, device=DEV), torch.full((T + 40, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    pkg.kernels.add_norm(x, y, w, sum_out=s[20:T + 20], out=h[20:T + 20])
+    for t in (s, h):
+        assert bool((t[:20] == 7).all() and (t[T + 20:] == 7).all())
+    check_norm(s[20:T + 20], h[20:T + 20], x, y, 1.0, w, None, "rms", 1e-6)
+    # e4m3: blocks of 16 rows, of which the last is not whole
+    mp, kb = -(-T // 16) * 16, -(-D // 128)
+    n, m = gpu_lib.f8_rows_bytes(T, D), gpu_lib.f8_rows_scales_bytes(T, D)
+    assert n == mp * kb * 128 and m == mp * kb * 4 + 1024
+    hq, hs = torch.full((n + 4096,), 165, dtype=torch.uint8, device=DEV), torch.full((m // 4 + 1024,), -3.0, device=DEV)
+    assert gpu_lib.add_norm(x.data_ptr(), 1, y.data_ptr(), 1.0, s[20:].data_ptr(), None, hq.data_ptr(), hs.data_ptr(), w.data_ptr(), None, 1e-6, 1, D, D, D,
+                            0, T, D, 1, pkg.capi.stream_ptr()) == 0
+    assert bool((hq[n:] == 165).all() and (hs[kb * mp:] == -3).all())
+    behind = hq[:n].view(mp // 16, kb, 2, 4, 16, 16).permute(0, 4, 1, 3, 2, 5).reshape(mp, -1)[T:]
+    assert bool((behind == 165).all() and (hs[:kb * mp].view(kb, mp)[:, T:] == -3).all())
+    rows = pkg.f8.F8Rows(hq[:n], hs[:m // 4], (T,), D, torch.bfloat16)
+    check_norm8(rows, x, y, 1.0, w, None, "rms", 1e-6)
+    assert bool((s[:20] == 7).all() and (s[T + 20:] == 7).all())
+
+
+@pytest.mark.parametrize("D", [8200, 12800, 16904, 20000, 24576, 32768])  # 3 to 11 waves a row, 3 to 8 pieces a lane
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_many_long_rows(gpu_lib, pkg, D, norm):
+    for T, stream, dtype in ((1024, torch.float32, torch.float16), (1500, torch.bfloat16, torch.bfloat16)):
+        x, y, w, b = norm_inputs(T, D, stream, dtype, seed=D)
+        b = b if norm == "layer" else None
+        s, h = pkg.kernels.add_norm(x, y, w, b, norm=norm, eps=1e-5)
+        check_norm(s, h, x, y, 1.0, w, b, norm, 1e-5)
+        if D % 16 == 0:
+            _, rows = pkg.norm.AddNorm(w, b, norm=norm, eps=1e-5)(x, y, f8=True)
+            check_norm8(rows, x, y, 1.0, w, b, norm, 1e-5)
