@@ -365,7 +365,7 @@ PyObject* lin8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &codes = aux(a[5], at::kByte, device), &scales = aux(a[6], at::kFloat, device);
     const int64_t kb = ((int64_t)K + 127) / 128;
     need(M > 0 && codes.numel() == ((int64_t)N + 63) / 64 * kb * 8192 && scales.numel() == ((int64_t)N + 127) / 128 * kb);
-    need((size_t)q.numel() >= entry.rows(M, K) && (size_t)sx.numel() * 4 >= entry.rows_scales(M, K));
+    need((size_t)q.numel() == entry.rows(M, K) && (size_t)sx.numel() * 4 == entry.rows_scales(M, K));
     const at::ScalarType type = bf16 ? at::kBFloat16 : at::kHalf;
     const End e(a + 8, M, N, type, device);
     void* stream = stream_on(device);

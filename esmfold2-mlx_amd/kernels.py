@@ -1015,8 +1015,9 @@ def f8_linear_end(x, codes, scales, N: int, bias=None, *, gated: bool = False, a
             _aux(t, n, kinds, index)
         if dtype not in _DTYPES:
             raise capi.EsmError(-2, f"f8_linear_end: dtype={dtype}")
-        if (xq.numel() < lib.f8_rows_bytes(M, K) or 4 * sx.numel() < lib.f8_rows_scales_bytes(M, K)
-                or codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128)):
+        if xq.numel() != lib.f8_rows_bytes(M, K) or 4 * sx.numel() != lib.f8_rows_scales_bytes(M, K):
+            raise capi.EsmError(-2, f"f8_linear_end: {xq.numel()} bytes of codes and {sx.numel()} scales for rows [{M}, {K}]")
+        if codes.numel() != -(-N // 64) * -(-K // 128) * 8192 or scales.numel() != -(-N // 128) * -(-K // 128):
             raise capi.EsmError(-2, f"f8_linear_end: {codes.numel()} packed codes and {scales.numel()} scales for [{N}, {K}]")
     if index != _current():
         with torch.cuda.device(index):

@@ -186,3 +186,19 @@ def test_many_long_rows(gpu_lib, pkg, D, norm):
         if D % 16 == 0:
             _, rows = pkg.norm.AddNorm(w, b, norm=norm, eps=1e-5)(x, y, f8=True)
             check_norm8(rows, x, y, 1.0, w, b, norm, 1e-5)
+
+
+def test_rows_in_e4m3_of_another_count_are_refused(gpu_lib, pkg, monkeypatch):
+    """The scales of a block of columns lie a whole count of 16 rows behind one another: of another, others' would be read."""
+    K, lin = pkg.kernels, pkg.f8.F8Linear.from_float(torch.randn(64, 640, device=DEV))
+    x = torch.randn(40, 640, device=DEV).half()
+    q, s = K.add_norm_f8(x)[1]
+    call = lambda M, K_=640: K.f8_linear_end(None, lin.codes_packed, lin.scales, 64, rows=(q, s, M, K_), dtype=torch.float16)  # noqa: E731
+    want = call(40)
+    for _ in range(2):
+        for M, K_ in ((30, 640), (49, 640), (16, 640), (0, 640), (-1, 640), (40, 512)):
+            with pytest.raises(pkg.capi.EsmError) as e:
+                call(M, K_)
+            assert e.value.code == -2, (M, K_)
+        assert torch.equal(call(33), want[:33]) and torch.equal(call(40), want)
+        monkeypatch.setattr(pkg.capi, "bind", pkg.capi._LongWay)
