@@ -198,7 +198,8 @@ class EsmcBlock(nn.Module):
         """Whether ``run_rows`` is this block: e4m3 linears, a gated w1, and nothing put in the place of a part of it."""
         return (self.fused and type(self) is EsmcBlock and not any(m in self.__dict__ for m in ("attention", "ffn", "run_packed"))
                 and (EsmcBlock.attention, EsmcBlock.ffn, EsmcBlock.run_packed) == _PACKED_METHODS
-                and all(type(getattr(self, m)) is F8Linear for m in LINEARS))
+                and F8Linear.forward is _F8_FORWARD
+                and all(type(m) is F8Linear and "forward" not in m.__dict__ for m in (self.wqkv, self.wo, self.w1, self.w2)))
 
     def run_rows(self, x: torch.Tensor, rows: F8Rows, cu: torch.Tensor, positions: torch.Tensor, rotary: Rotary,
                  res_scale: float):
@@ -224,6 +225,7 @@ class EsmcBlock(nn.Module):
 
 _BLOCK_METHODS = (EsmcBlock.attention, EsmcBlock.ffn)
 _PACKED_METHODS = (*_BLOCK_METHODS, EsmcBlock.run_packed)
+_F8_FORWARD = F8Linear.forward
 
 
 def _norm_rows(x, y, w, b, alpha: float, x_out=None):

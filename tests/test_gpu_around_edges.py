@@ -5,8 +5,10 @@ import torch
 
 from oracle import around as A, cache4 as C4
 from test_gpu_cache4 import Case
+from test_gpu_esmc_packed import _gen
 from test_gpu_linear16 import _inputs
 from test_gpu_norm import _check as check_norm, _check8 as check_norm8, _inputs as norm_inputs
+from test_gpu_together import _hf
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -202,3 +204,24 @@ def test_rows_in_e4m3_of_another_count_are_refused(gpu_lib, pkg, monkeypatch):
             assert e.value.code == -2, (M, K_)
         assert torch.equal(call(33), want[:33]) and torch.equal(call(40), want)
         monkeypatch.setattr(pkg.capi, "bind", pkg.capi._LongWay)
+
+
+def test_a_linear_with_another_forward_takes_16_bit_rows(gpu_lib, pkg, monkeypatch):
+    """A forward put in the place of a linear's own is written for tensors: the block then runs its separate calls."""
+    F8 = pkg.f8.F8Linear
+    model = pkg.esmc.HipEsmc.from_hf(_hf(256, 384, 2, 5), n_heads=4, linear=F8, fused=True)
+    ids, cu = torch.randint(0, 33, (150,), generator=_gen(3)).to(DEV), torch.tensor([0, 100, 150], dtype=torch.int32, device=DEV)
+    want = model.packed_hidden_states(ids, cu)
+    blk, seen = model.layers[1], []
+    own = blk.wqkv.forward
+    blk.wqkv.forward = lambda x: seen.append(x.dtype) or own(x)  # (x.dtype of a tensor)
+    assert not blk.takes_rows()
+    other = model.packed_hidden_states(ids, cu)
+    assert seen == [torch.float16] and float((other[-1] - want[-1]).pow(2).mean().sqrt()) <= 0.15  # (e4m3's error of both)
+    del blk.wqkv.forward
+    assert blk.takes_rows() and torch.equal(model.packed_hidden_states(ids, cu), want)
+    kinds, forward = [], F8.forward
+    monkeypatch.setattr(F8, "forward", lambda self, x, *a, **k: kinds.append(type(x)) or forward(self, x, *a, **k))
+    assert not blk.takes_rows()
+    model.packed_hidden_states(ids, cu)
+    assert kinds and all(k is torch.Tensor for k in kinds)
