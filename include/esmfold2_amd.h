@@ -526,8 +526,10 @@ int f8_linear_end(const void* x, int64_t x_st, const uint8_t* xq, const float* s
  *
  * A value stands as s (c - z), c in 0 .. 15, with s and z per key (or value), head and 64 values: s the least bf16 value, 2^-96
  * or more, of which 15 reach over the 64 values' range and 120 to the farthest from zero, z = rint(-min / s), c = clamp(rint(x
- * / s) + z, 0, 15); 64 values with a NaN or an infinity among them, or apart by 2^128 or more, read as NaN. data: cache4_bytes(pages, Hk, d) bytes, 16-byte
- * aligned, zeroed or written before they are read. The layout is the kernels' own and depends on dtype.
+ * / s) + z, 0, 15): off by s / 2 at most, so values that near the type's largest may read as infinity. 64 values with a NaN or
+ * an infinity among them, or apart by 2^128 or more, read as NaN. data: cache4_bytes(pages, Hk, d) bytes, 16-byte aligned,
+ * zeroed or written before they are read. The layout is the kernels' own and depends on dtype; heads are filled up to 64 or
+ * 128 values.
  * Sequence i has the rows cu[i] .. cu[i + 1] - 1 of a call (int32 [n + 1], ascending; brought inside 0 .. T), which are the
  * last of its lens[i] keys (int32 [n]); its key j lies in page table[i][j / 64] (int32 [n, width]). All of them on the device.
  *

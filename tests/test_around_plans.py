@@ -90,3 +90,8 @@ def test_the_caches_workspace_holds_every_item(lib):
         chunks = [max(1, -(-k // keys)) for k in nk]
         assert sum(t * c for t, c in zip(tiles, chunks)) <= items and max(chunks) <= 256
     assert seen > 500
+
+
+def test_the_caches_memory_beside_16_bits(lib):
+    for d, share in ((128, 0.28125), (120, 0.3), (96, 0.375), (80, 0.45), (72, 0.5), (64, 0.28125), (32, 0.5625), (24, 0.75), (16, 1.125), (8, 2.25)):
+        assert lib.cache4_bytes(5, 3, d) == share * 5 * 64 * 3 * 2 * d * 2

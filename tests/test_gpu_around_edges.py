@@ -225,3 +225,15 @@ def test_a_linear_with_another_forward_takes_16_bit_rows(gpu_lib, pkg, monkeypat
     assert not blk.takes_rows()
     model.packed_hidden_states(ids, cu)
     assert kinds and all(k is torch.Tensor for k in kinds)
+
+
+def test_values_next_to_the_types_largest(gpu_lib, pkg):
+    c = Case(pkg, [1], [70], 1, 1, 64, torch.float16)
+    c.k[5] = torch.linspace(0, 65504, 64, device=DEV).half()  # 15 steps are 65760
+    c.v[9] = torch.linspace(-65504, 65504, 64, device=DEV).half()
+    c.fill()
+    for got, x in zip(c.cache.read(c.whole, c.lens, c.table), (c.k, c.v)):
+        code, s, z = C4.hold(x)
+        held = s * (code - z)
+        assert torch.equal(got, held.half()) and float(((held - x.double()).abs() / s).max()) <= 0.5
+    assert bool(c.cache.read(c.whole, c.lens, c.table)[0][5].isinf().any())
