@@ -32,6 +32,7 @@ namespace esm {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // Bytes of 8 keys of a page and head, and of their parts.
@@ -614,16 +615,25 @@ struct Rows4 {
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 hi[RT], lo[RT];
 #pragma unroll
-      for (int r = 0; r < RT; r++)
+      for (int r = 0; r < RT; r++) {
+        u32x4 h4, l4;  // (two values a conversion)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 8; j += 2) {
           const uint32_t w = k.vs[i][j >> 1];
-          const float st = __builtin_bit_cast(float, j & 1 ? w & 0xffff0000u : w << 16);
-          float v = p[r][j] * st;
-          if (MASKED) v = key0 + 8 * g + j <= lim[r] ? v : 0.f;
-          hi[r][j] = (__bf16)v;
-          lo[r][j] = (__bf16)(v - (float)hi[r][j]);
+          f32x2 v = {p[r][j] * __builtin_bit_cast(float, w << 16), p[r][j + 1] * __builtin_bit_cast(float, w & 0xffff0000u)};
+          if (MASKED) {
+            v[0] = key0 + 8 * g + j <= lim[r] ? v[0] : 0.f;
+            v[1] = key0 + 8 * g + j + 1 <= lim[r] ? v[1] : 0.f;
+          }
+          const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+          v[0] -= __builtin_bit_cast(float, h << 16);
+          v[1] -= __builtin_bit_cast(float, h & 0xffff0000u);
+          h4[j >> 1] = h;
+          l4[j >> 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
         }
+        hi[r] = __builtin_bit_cast(bf16x8, h4);
+        lo[r] = __builtin_bit_cast(bf16x8, l4);
+      }
       const bf16x8 z = __builtin_bit_cast(bf16x8, k.vz[i]);
 #pragma unroll
       for (int u = 0; u < 4; u++) {
