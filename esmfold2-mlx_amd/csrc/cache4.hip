@@ -12,7 +12,7 @@
 // both by v_mfma_f32_16x16x32: a wave holds 16 rows of queries (or RT times 16), a row a lane (lane % 16) of every
 // accumulator, and takes 32 keys at a time. P is bf16 whatever the type, as its range is p's times the values', and kept as the
 // sum of two bf16 values, 16 bits of it: with the first alone bf16's output was off by 0.0023 of itself on long contexts,
-// where its own rounding is 0.0017 (the second costs 5 to 9% of a token's time, 30% of a prompt's). No operand passes
+// where its own rounding is 0.0017 (the second costs 4 to 8% of a token's time, 24 to 31% of a prompt's). No operand passes
 // through LDS: the cache lies in the order the matrix cores take (HD = 64 or 128, the head size filled up). A page's head is
 // 8 chunks of 8 keys, one after the other, so that whoever writes 8 keys writes whole lines of memory; key 4 b + e of chunk g is row 4 g + e of block b of the 32 keys' first
 // product, and slot 4 b + e of lane group g in the second:
@@ -656,10 +656,11 @@ struct Rows4 {
 
 // A workgroup takes 16 RT rows (query, head of the group; row = query G + head) of a sequence and key head and one chunk of
 // its keys, a page a wave in turn, the next 32 keys' operands in flight; the waves' results are joined through LDS. Bound by the
-// cache's bytes where contexts are long (32 of 8,000 to 24,400 keys, 8 key heads of 128, 597 MB in 122 us, 4.9 TB/s of a copy's
-// 5.1), else by a launch, latencies one after the other (lengths, table, first page) and 250 vector instructions a wave for 32
-// keys and 16 rows: 8 tokens, 38 MB 14.4 us; 16 x 5 tokens, 21 MB in three tiles a sequence 20.5. (64 keys in flight a wave took
-// all registers: 32 contexts 171 us, 8 tokens 23; more chunks than target's 256 a head cost more than they fill.)
+// cache's bytes, of which a wave has 32 keys' in flight, where contexts are long (32 of 8,000 to 24,400 keys, 8 key heads of 128,
+// 597 MB in 126 us, 4.7 TB/s of a copy's 5.1), else by a launch, latencies one after the other (lengths, table, first page) and 355
+// vector and 40 matrix instructions a wave for 32 keys and 16 rows: 8 tokens, 38 MB 16.6 us; 16 x 5 tokens, 21 MB in three tiles a
+// sequence 20.7; 2,048 causal rows on 16,384 keys 1.28 ms, 0.45 PFLOP/s. (64 keys in flight a wave took all registers: 32 contexts
+// 40% slower, 8 tokens 60%; more chunks than target's 256 a head cost more than they fill.)
 template <class T, int HD, int RT>
 __global__ __launch_bounds__(256, RT == 2 ? 2 : 3) void cache4_attention_kernel(Cache4Args p) {
   typedef Page<HD> P;
@@ -851,8 +852,8 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args p, int rows
 
 // Rows of a tile by the mean rows of a sequence; keys divided unless the table holds few or the tiles alone fill the GPU
 // many times over. Few: up to 4 passes the join costs more than they do (8 heads of 128, one token of 8 sequences on 1,000 keys
-// 12.2 us divided, 11.2 whole; on 1,500 12.8 and 13.4), up to 8 where a tile a sequence gives every CU one (64 on 2,000 keys 47.0
-// and 32.2, 64 on 0 to 2,000 30.6 and 25.0; on 0 to 4,000 51 and 49, but 32 on those 29 and 36).
+// 13.6 us divided, 12.7 whole; on 1,500 13.5 and 17.6), up to 8 where a tile a sequence gives every CU one (64 on 2,000 keys 48.0
+// and 36.6, 64 on 0 to 2,000 31.9 and 31.5; on 0 to 4,000 56.4 and 56.4, but 32 on those 27.6 and 38.4).
 Cache4Plan cache4_plan(long long T, int n, int width, int Hk, int G, int cus) {
   Cache4Plan plan{};
   const long long per = T * G / n;
